@@ -287,8 +287,7 @@ def _call(case, s):
         return {"q": q.detach(), "k": k.detach(), "dq": dq, "dk": dk}
     # every step brings its own lengths and pages: its plan is part of the pass
     plan = paged.plan(s["query_starts"], s["context_lengths"], s["page_table"], s["key_pages"],
-                      tokens=s["q"].shape[0], query_heads=case["heads"],
-                      max_query_tokens=case["new_high"] if case["chunks"] else 1)
+                      tokens=s["q"].shape[0], query_heads=case["heads"])
     res, q = {}, s["q"]
     if case["kind"] != "attend":
         q = paged.append(s["k"], s["v"], s["key_pages"], s["value_pages"], plan, query=q,
