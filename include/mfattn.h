@@ -248,6 +248,89 @@ int mf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_gain,
 int mf_segment_positions(const int32_t* segment_ids, int batch, int seq_len,
                          int32_t* positions, void* stream);
 
+/* Rotary embeddings in their general form (kernels/rotary.py:7-39 rotates
+ * whole heads in the half layout): pair i of the first rotary_dim dims of each
+ * head -- dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved --
+ * turns by position * frequencies[i] and is multiplied by magnitude; the other
+ * dims are copied.  fp32 arithmetic (angles exact at any position), one
+ * rounding.  backward != 0 turns the other way (the transpose): q and k are
+ * then the gradients of q_out and k_out.
+ * q [tokens] x [q_heads, head_dim] with q_stride elements between tokens (each
+ * head dense), k likewise; q_out and k_out are dense and may be q and k where
+ * those are dense.  q or k is null with 0 heads.  positions [tokens] int32, or
+ * NULL: token % seq_len.  frequencies: rotary_dim / 2 radians per position, in
+ * HOST memory, read before the call returns.  head_dim even, up to 1024;
+ * rotary_dim even, up to 256. */
+int mf_rotate(const void* q, long long q_stride, const void* k,
+              long long k_stride, const int32_t* positions,
+              const double* frequencies, int dtype, int tokens, int seq_len,
+              int q_heads, int kv_heads, int head_dim, int rotary_dim,
+              int interleaved, float magnitude, int backward, void* q_out,
+              void* k_out, void* stream);
+
+/* The plan of a paged serving step.  `sequences` (up to 4096) ragged sequences
+ * bring new tokens query_starts[r] .. query_starts[r + 1] - 1 (int32
+ * [sequences + 1], ascending) of a [tokens, heads, 64] batch; tokens past the
+ * last sequence belong to nobody.  context_lengths[r] counts the tokens of
+ * sequence r, the new ones included; token position p is slot p % page_size of
+ * page page_table[r * table_stride + p / page_size], max_pages entries a row.
+ * Page sizes are multiples of 8.  An entry outside [0, pages) holds no keys:
+ * tokens there are not written, and not attended to.  A context beyond the
+ * table's reach is read as that reach; new tokens that exceed their context
+ * have negative positions: not written, and attending to nothing.
+ * The plan serves every layer of the step, on any stream ordered after it; it
+ * depends on the batch's shapes, and on the table's entries while it is used:
+ * the table must not change between the plan and the calls that take both. */
+size_t mf_paged_plan_bytes(int sequences, int tokens, int q_heads,
+                           int kv_heads, int dtype);
+int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
+                  const int32_t* page_table, long long table_stride,
+                  int sequences, int tokens, int max_pages, int page_size,
+                  int pages, int q_heads, int kv_heads, int dtype, void* plan,
+                  size_t plan_bytes, void* stream);
+
+/* The step's new keys and values into their pages (the cache write of
+ * layers/attention.py:309-317 for many ragged tokens), with the prologue of
+ * layers/attention.py:62-97 on the way: optional RMS norm of each query and
+ * key head with its gain ([64] in the tensor dtype, NULL: none), then optional
+ * rotation at the token's position (frequencies NULL: none; otherwise as
+ * mf_rotate).  fp32 arithmetic, one rounding.  q [tokens, q_heads, 64] is
+ * written to q_out (dense; may be q where that is dense); q and q_out NULL: no
+ * queries.  k, v [tokens, kv_heads, 64]; token strides in elements.
+ * k_pages, v_pages: [pages][page_size][kv_heads][64] with strides
+ * {page, slot, head} in elements (HOST arrays of 3), the last dimension dense.
+ * Where two tokens have the same page and slot, either remains. */
+int mf_paged_append(const void* q, long long q_stride, const void* k,
+                    long long k_stride, const void* v, long long v_stride,
+                    const void* q_gain, const void* k_gain, float eps,
+                    const double* frequencies, int rotary_dim, int interleaved,
+                    float magnitude, int dtype, int tokens, int sequences,
+                    int q_heads, int kv_heads, int head_dim, int page_size,
+                    int pages, const void* plan, size_t plan_bytes,
+                    void* k_pages, void* v_pages, const long long* k_strides,
+                    const long long* v_strides, void* q_out, void* stream);
+
+/* Causal attention of a step's new tokens over their pages: a query at
+ * position p sees slots 0 .. p of its sequence (what mf_decode computes for
+ * one new token a row, kernels/attention.py:264-282, over pages and for any
+ * number of new tokens; a query that sees no key yields zeros).  q
+ * [tokens, q_heads, 64] with q_stride elements between tokens, out dense.
+ * k_pages, v_pages and their strides as mf_paged_append, 16-byte aligned rows;
+ * a page within 2 GiB.  Rows of out past the last sequence are zeroed when
+ * zero_rest != 0 and left as they are otherwise.  Deterministic.  `workspace`
+ * holds the partial results of keys split over workgroups
+ * (mf_paged_attn_workspace_bytes); it is this call's alone while it runs. */
+size_t mf_paged_attn_workspace_bytes(int sequences, int tokens, int q_heads,
+                                     int kv_heads, int dtype);
+int mf_paged_attn(const void* q, long long q_stride, const void* k_pages,
+                  const void* v_pages, const long long* k_strides,
+                  const long long* v_strides, const int32_t* page_table,
+                  long long table_stride, int dtype, int tokens, int sequences,
+                  int max_pages, int page_size, int pages, int q_heads,
+                  int kv_heads, int head_dim, float scale, const void* plan,
+                  size_t plan_bytes, int zero_rest, void* out, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 /* Segmented short (depthwise) convolution of the packed conv layers, gates
  * fused:  out = c_gate * conv(b_gate * values)  over [B, T, C] (C a multiple
  * of 8), taps [C, kernel_size] (kernel_size <= 8) in the tensor dtype.  A tap

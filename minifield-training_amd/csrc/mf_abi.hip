@@ -10,6 +10,7 @@
 
 #include "../../include/mfattn.h"
 #include "mf_common.h"
+#include "mf_paged.h"
 
 namespace mf {
 hipError_t launch_block_map(const int32_t* seg, const void* mask, int mask_u8, int mode, int batch,
@@ -58,6 +59,30 @@ hipError_t launch_segmented_conv_bwd(const void* b, const void* c, const void* v
                                      const int32_t* seg, const void* g, bool centered, bool f32,
                                      int B, int T, int C, int K, void* db, void* dc, void* dv,
                                      float* dw, void* workspace, hipStream_t stream);
+hipError_t launch_rotate(const void* q, long long q_stride, const void* k, long long k_stride,
+                         const int32_t* positions, const double* frequencies, bool f32, int tokens,
+                         int seq_len, int Hq, int Hkv, int D, int rotary_dim, int interleaved,
+                         float magnitude, bool backward, void* q_out, void* k_out,
+                         hipStream_t stream);
+hipError_t launch_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
+                             const int32_t* page_table, long long table_stride, int sequences,
+                             int tokens, int max_pages, int page_size, int pages, int Hq, int Hkv,
+                             bool f32, void* plan, hipStream_t stream);
+hipError_t launch_paged_append(const void* q, long long q_stride, const void* k,
+                               long long k_stride, const void* v, long long v_stride,
+                               const void* q_gain, const void* k_gain, float eps,
+                               const double* frequencies, int rotary_dim, int interleaved,
+                               float magnitude, bool f32, int tokens, int Hq, int Hkv,
+                               int page_size, int pages, const PagedToken* records, void* k_pages,
+                               void* v_pages, const PagedStrides& k_strides,
+                               const PagedStrides& v_strides, void* q_out, hipStream_t stream);
+hipError_t launch_paged_attn(const void* q, long long q_stride, const void* k_pages,
+                             const void* v_pages, const PagedStrides& k_strides,
+                             const PagedStrides& v_strides, const int32_t* page_table,
+                             long long table_stride, bool f32, int tokens, int sequences,
+                             int page_size, int pages, int Hq, int Hkv, float scale,
+                             const void* plan, bool zero_rest, void* out, void* workspace,
+                             hipStream_t stream);
 }  // namespace mf
 
 namespace {
@@ -510,6 +535,228 @@ int mf_segmented_conv_bwd(const void* b_gate, const void* c_gate, const void* va
                                                  d_c_gate, d_values, d_taps, workspace,
                                                  static_cast<hipStream_t>(stream)),
                    "mf_segmented_conv_bwd launch");
+}
+
+namespace {
+
+// Frequencies and their layout; head_dim and the dtype are checked by the callers.
+int check_rotation(const double* frequencies, int rotary_dim, int head_dim, float magnitude) {
+  if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || rotary_dim > 256)
+    return fail(MF_ERR_SHAPE, "rotary_dim must be even and in [2, min(head_dim, 256)] (got %d of %d)",
+                rotary_dim, head_dim);
+  for (int i = 0; i < rotary_dim / 2; ++i)
+    if (!std::isfinite(frequencies[i]))
+      return fail(MF_ERR_INVALID_ARGUMENT, "frequencies must be finite (number %d is %g)", i,
+                  frequencies[i]);
+  if (!std::isfinite(magnitude))
+    return fail(MF_ERR_INVALID_ARGUMENT, "magnitude must be finite (got %g)", (double)magnitude);
+  return MF_OK;
+}
+
+// Elements between the tokens of a [tokens, heads, dim] operand.
+int check_token_stride(const char* what, long long stride, int heads, int dim) {
+  if (stride < (long long)heads * dim)
+    return fail(MF_ERR_SHAPE, "%s: %lld elements between tokens, rows have %lld", what, stride,
+                (long long)heads * dim);
+  return MF_OK;
+}
+
+int check_paged(int dtype, int sequences, int tokens, int q_heads, int kv_heads) {
+  if (dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16)
+    return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
+  if (sequences < 1 || tokens < 1 || q_heads < 1 || kv_heads < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "Sizes must be positive (sequences=%d tokens=%d q_heads=%d kv_heads=%d)", sequences,
+                tokens, q_heads, kv_heads);
+  if (sequences > mf::kMaxSequences)
+    return fail(MF_ERR_SHAPE, "at most %d sequences a step (got %d)", mf::kMaxSequences, sequences);
+  if (q_heads % kv_heads) return fail(MF_ERR_HEADS, "Query heads must be divisible by KV heads");
+  // one launch's workgroups of 256 threads stay below 2^32 threads
+  if ((long long)tokens * q_heads > (1ll << 28) || kv_heads > 1024)
+    return fail(MF_ERR_SHAPE, "tokens * q_heads must not exceed 2^28, nor kv_heads 1024");
+  return MF_OK;
+}
+
+int check_pool(int page_size, int pages) {
+  if (page_size < 1 || pages < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT, "Sizes must be positive (page_size=%d pages=%d)", page_size,
+                pages);
+  if (page_size % 8)
+    return fail(MF_ERR_SHAPE, "page_size must be a multiple of 8 (got %d)", page_size);
+  return MF_OK;
+}
+
+int check_plan(int sequences, int tokens, int q_heads, int kv_heads, int dtype, const void* plan,
+               size_t plan_bytes) {
+  if (!plan) return fail(MF_ERR_INVALID_ARGUMENT, "plan must be non-null");
+  if (reinterpret_cast<uintptr_t>(plan) % 16)
+    return fail(MF_ERR_INVALID_ARGUMENT, "plan must be 16-byte aligned");
+  const size_t need = mf_paged_plan_bytes(sequences, tokens, q_heads, kv_heads, dtype);
+  if (plan_bytes < need)
+    return fail(MF_ERR_WORKSPACE, "plan holds %zu bytes, %zu needed", plan_bytes, need);
+  return MF_OK;
+}
+
+int check_page_strides(const char* what, const long long* s, int page_size, int kv_heads,
+                       mf::PagedStrides* out) {
+  if (!s) return fail(MF_ERR_INVALID_ARGUMENT, "%s strides must be non-null", what);
+  if (s[0] < 0 || s[1] < 0 || s[2] < 0 || (page_size > 1 && s[1] < mf::kD) ||
+      (kv_heads > 1 && s[2] < mf::kD))
+    return fail(MF_ERR_SHAPE, "%s: strides {%lld, %lld, %lld} of page, slot and head overlap", what,
+                s[0], s[1], s[2]);
+  // rows of eight slots are addressed with 32-bit offsets from their first
+  if (s[1] > (1ll << 31) / (4ll * 8))
+    return fail(MF_ERR_SHAPE, "%s: %lld elements between slots (at most 2^26)", what, s[1]);
+  *out = {s[0], s[1], s[2]};
+  return MF_OK;
+}
+
+}  // namespace
+
+int mf_rotate(const void* q, long long q_stride, const void* k, long long k_stride,
+              const int32_t* positions, const double* frequencies, int dtype, int tokens,
+              int seq_len, int q_heads, int kv_heads, int head_dim, int rotary_dim,
+              int interleaved, float magnitude, int backward, void* q_out, void* k_out,
+              void* stream) {
+  if (dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16)
+    return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
+  if (tokens < 1 || seq_len < 1 || q_heads < 0 || kv_heads < 0 || q_heads + kv_heads < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "Sizes must be positive (tokens=%d seq_len=%d q_heads=%d kv_heads=%d)", tokens,
+                seq_len, q_heads, kv_heads);
+  if (head_dim < 2 || head_dim % 2 || head_dim > 1024)
+    return fail(MF_ERR_HEAD_DIM, "head_dim must be even and in [2, 1024] (got %d)", head_dim);
+  if ((long long)q_heads + kv_heads > 65535)
+    return fail(MF_ERR_SHAPE, "at most 65535 heads (got %d and %d)", q_heads, kv_heads);
+  if ((q_heads > 0) != (q && q_out) || (q_heads == 0 && (q || q_out)) ||
+      (kv_heads > 0) != (k && k_out) || (kv_heads == 0 && (k || k_out)))
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "q and q_out must be non-null with heads and null without, k and k_out likewise");
+  if (!frequencies) return fail(MF_ERR_INVALID_ARGUMENT, "frequencies must be non-null");
+  if (int rc = check_rotation(frequencies, rotary_dim, head_dim, magnitude)) return rc;
+  if (q)
+    if (int rc = check_token_stride("q", q_stride, q_heads, head_dim)) return rc;
+  if (k)
+    if (int rc = check_token_stride("k", k_stride, kv_heads, head_dim)) return rc;
+  return check_hip(mf::launch_rotate(q, q ? q_stride : 0, k, k ? k_stride : 0, positions, frequencies,
+                                     dtype == MF_DTYPE_F32, tokens, seq_len, q_heads, kv_heads,
+                                     head_dim, rotary_dim, interleaved != 0, magnitude,
+                                     backward != 0, q_out, k_out, static_cast<hipStream_t>(stream)),
+                   "mf_rotate launch");
+}
+
+size_t mf_paged_plan_bytes(int sequences, int tokens, int q_heads, int kv_heads, int dtype) {
+  if (sequences < 1 || tokens < 1 || q_heads < 1 || kv_heads < 1) return 0;
+  return mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32).total;
+}
+
+int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
+                  const int32_t* page_table, long long table_stride, int sequences, int tokens,
+                  int max_pages, int page_size, int pages, int q_heads, int kv_heads, int dtype,
+                  void* plan, size_t plan_bytes, void* stream) {
+  if (int rc = check_paged(dtype, sequences, tokens, q_heads, kv_heads)) return rc;
+  if (int rc = check_pool(page_size, pages)) return rc;
+  if (max_pages < 1 || table_stride < max_pages)
+    return fail(MF_ERR_SHAPE, "page_table rows hold %lld entries, max_pages is %d (at least 1)",
+                table_stride, max_pages);
+  if ((long long)max_pages * page_size > (1ll << 30))
+    return fail(MF_ERR_SHAPE, "max_pages * page_size must not exceed 2^30");
+  if (!query_starts || !context_lengths || !page_table)
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "query_starts, context_lengths and page_table must be non-null");
+  if (int rc = check_plan(sequences, tokens, q_heads, kv_heads, dtype, plan, plan_bytes)) return rc;
+  return check_hip(mf::launch_paged_plan(query_starts, context_lengths, page_table, table_stride,
+                                         sequences, tokens, max_pages, page_size, pages, q_heads,
+                                         kv_heads, dtype == MF_DTYPE_F32, plan,
+                                         static_cast<hipStream_t>(stream)),
+                   "mf_paged_plan launch");
+}
+
+int mf_paged_append(const void* q, long long q_stride, const void* k, long long k_stride,
+                    const void* v, long long v_stride, const void* q_gain, const void* k_gain,
+                    float eps, const double* frequencies, int rotary_dim, int interleaved,
+                    float magnitude, int dtype, int tokens, int sequences, int q_heads,
+                    int kv_heads, int head_dim, int page_size, int pages, const void* plan,
+                    size_t plan_bytes, void* k_pages, void* v_pages, const long long* k_strides,
+                    const long long* v_strides, void* q_out, void* stream) {
+  if (int rc = check_paged(dtype, sequences, tokens, q_heads, kv_heads)) return rc;
+  if (int rc = check_pool(page_size, pages)) return rc;
+  if (head_dim != mf::kD)
+    return fail(MF_ERR_HEAD_DIM, "head_dim must be %d (got %d)", mf::kD, head_dim);
+  if (int rc = check_plan(sequences, tokens, q_heads, kv_heads, dtype, plan, plan_bytes)) return rc;
+  if (!k || !v || !k_pages || !v_pages || (q == nullptr) != (q_out == nullptr) || (q_gain && !q))
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "k, v and the pages must be non-null, q and q_out both given or both null");
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(MF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative (got %g)", (double)eps);
+  if (frequencies)
+    if (int rc = check_rotation(frequencies, rotary_dim, head_dim, magnitude)) return rc;
+  if (q)
+    if (int rc = check_token_stride("q", q_stride, q_heads, head_dim)) return rc;
+  if (int rc = check_token_stride("k", k_stride, kv_heads, head_dim)) return rc;
+  if (int rc = check_token_stride("v", v_stride, kv_heads, head_dim)) return rc;
+  mf::PagedStrides ks, vs;
+  if (int rc = check_page_strides("k_pages", k_strides, page_size, kv_heads, &ks)) return rc;
+  if (int rc = check_page_strides("v_pages", v_strides, page_size, kv_heads, &vs)) return rc;
+  const mf::PagedLayout lay =
+      mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32);
+  const mf::PagedToken* records = reinterpret_cast<const mf::PagedToken*>(
+      static_cast<const char*>(plan) + lay.tokens);
+  return check_hip(mf::launch_paged_append(q, q ? q_stride : 0, k, k_stride, v, v_stride, q_gain,
+                                           k_gain, eps, frequencies, rotary_dim, interleaved != 0,
+                                           frequencies ? magnitude : 1.f, dtype == MF_DTYPE_F32,
+                                           tokens, q ? q_heads : 0, kv_heads, page_size, pages,
+                                           records, k_pages, v_pages, ks, vs, q_out,
+                                           static_cast<hipStream_t>(stream)),
+                   "mf_paged_append launch");
+}
+
+size_t mf_paged_attn_workspace_bytes(int sequences, int tokens, int q_heads, int kv_heads,
+                                     int dtype) {
+  if (sequences < 1 || tokens < 1 || q_heads < 1 || kv_heads < 1) return 0;
+  return mf::paged_workspace_bytes(
+      mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32),
+      kv_heads);
+}
+
+int mf_paged_attn(const void* q, long long q_stride, const void* k_pages, const void* v_pages,
+                  const long long* k_strides, const long long* v_strides,
+                  const int32_t* page_table, long long table_stride, int dtype, int tokens,
+                  int sequences, int max_pages, int page_size, int pages, int q_heads,
+                  int kv_heads, int head_dim, float scale, const void* plan, size_t plan_bytes,
+                  int zero_rest, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_paged(dtype, sequences, tokens, q_heads, kv_heads)) return rc;
+  if (int rc = check_pool(page_size, pages)) return rc;
+  if (head_dim != mf::kD)
+    return fail(MF_ERR_HEAD_DIM, "head_dim must be %d (got %d)", mf::kD, head_dim);
+  if (max_pages < 1 || table_stride < max_pages)
+    return fail(MF_ERR_SHAPE, "page_table rows hold %lld entries, max_pages is %d (at least 1)",
+                table_stride, max_pages);
+  if (int rc = check_scale(scale)) return rc;
+  if (int rc = check_plan(sequences, tokens, q_heads, kv_heads, dtype, plan, plan_bytes)) return rc;
+  if (!q || !k_pages || !v_pages || !page_table || !out || !workspace)
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "q, the pages, page_table, out and the workspace must be non-null");
+  if (int rc = check_token_stride("q", q_stride, q_heads, head_dim)) return rc;
+  mf::PagedStrides ks, vs;
+  if (int rc = check_page_strides("k_pages", k_strides, page_size, kv_heads, &ks)) return rc;
+  if (int rc = check_page_strides("v_pages", v_strides, page_size, kv_heads, &vs)) return rc;
+  const long long unit = dtype == MF_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  const long long all = ks.page | ks.slot | ks.head | vs.page | vs.slot | vs.head | q_stride;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) |
+                       reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(out) |
+                       reinterpret_cast<uintptr_t>(workspace);
+  if (all % unit || at % 16)
+    return fail(MF_ERR_SHAPE, "rows of q, out, the pages and the workspace must be 16-byte aligned");
+  const size_t need = mf_paged_attn_workspace_bytes(sequences, tokens, q_heads, kv_heads, dtype);
+  if (workspace_bytes < need)
+    return fail(MF_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+  return check_hip(mf::launch_paged_attn(q, q_stride, k_pages, v_pages, ks, vs, page_table,
+                                         table_stride, dtype == MF_DTYPE_F32, tokens, sequences,
+                                         page_size, pages, q_heads, kv_heads, scale, plan,
+                                         zero_rest != 0, out, workspace,
+                                         static_cast<hipStream_t>(stream)),
+                   "mf_paged_attn launch");
 }
 
 const char* mf_last_error(void) { return g_last_error.c_str(); }

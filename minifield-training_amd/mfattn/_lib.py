@@ -41,6 +41,8 @@ CONV_CENTERED = 1
 
 TILE = 128
 HEAD_DIM = 64
+ROTATE_MAX_DIM = 256        # rotated dims of a head
+ROTATE_MAX_HEAD_DIM = 1024
 
 EXPORTS = (
     "mf_plan_layout",
@@ -62,6 +64,12 @@ EXPORTS = (
     "mf_qk_norm_rope_bwd_workspace_bytes",
     "mf_qk_norm_rope_bwd",
     "mf_segment_positions",
+    "mf_rotate",
+    "mf_paged_plan_bytes",
+    "mf_paged_plan",
+    "mf_paged_append",
+    "mf_paged_attn_workspace_bytes",
+    "mf_paged_attn",
     "mf_segmented_conv",
     "mf_segmented_conv_bwd_workspace_bytes",
     "mf_segmented_conv_bwd",
@@ -142,6 +150,24 @@ def _load() -> ctypes.CDLL:
     lib.mf_segmented_conv_bwd.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
                                           vp, vp, vp, vp, vp, sz, vp]
     lib.mf_segmented_conv_bwd.restype = i32
+    i64 = ctypes.c_longlong
+    lib.mf_rotate.argtypes = [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32,
+                              f32, i32, vp, vp, vp]
+    lib.mf_rotate.restype = i32
+    lib.mf_paged_plan_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.mf_paged_plan_bytes.restype = sz
+    lib.mf_paged_plan.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, vp, sz,
+                                  vp]
+    lib.mf_paged_plan.restype = i32
+    lib.mf_paged_append.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, i32, i32, f32,
+                                    i32, i32, i32, i32, i32, i32, i32, i32, vp, sz, vp, vp, vp,
+                                    vp, vp, vp]
+    lib.mf_paged_append.restype = i32
+    lib.mf_paged_attn_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.mf_paged_attn_workspace_bytes.restype = sz
+    lib.mf_paged_attn.argtypes = [vp, i64, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32,
+                                  i32, i32, i32, f32, vp, sz, i32, vp, vp, sz, vp]
+    lib.mf_paged_attn.restype = i32
     lib.mf_segment_positions.argtypes = [vp, i32, i32, vp, vp]
     lib.mf_segment_positions.restype = i32
     lib.mf_block_map_placements.argtypes = [vp, i32, i32, i32, i32, vp, sz, vp, vp, vp]

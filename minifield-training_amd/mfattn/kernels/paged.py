@@ -1,0 +1,241 @@
+"""Serving over a paged key/value cache: plan, append and causal attention.
+
+The cached attention of ``kernels/attention.py:264-282, :591-610`` and the
+cache write of ``layers/attention.py:309-317`` for a batch of ragged
+sequences, each with any number of new tokens (one: decode; several: drafted
+tokens; many: a chunk of a prompt), whose keys and values live in pages of a
+pool that all sequences share::
+
+    step = paged.plan(query_starts, context_lengths, page_table, key_pages,
+                      tokens=n, query_heads=hq)              # once a step
+    q = paged.append(k, v, key_pages, value_pages, step, query=q, rotary=rot,
+                     query_gain=qg, key_gain=kg, eps=1e-5)    # every layer
+    out = paged.attention(q, key_pages, value_pages, step)
+
+Pools are ``[pages, page_size, Hkv, 64]`` tensors or views of one (heads before
+slots, keys and values in one tensor, a contiguous cache through
+:func:`cache_pages`): only the last dimension has to be dense.  New tokens are
+``[tokens, heads, 64]``, sequence after sequence.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from .. import _lib
+from ..ops import _ptr, _raw_stream, dtype_code, on_device, require_device, token_rows
+from .rotary import Rotary
+
+
+class Plan:
+    """One step's new tokens and work items on the device, for every layer of the step."""
+
+    def __init__(self, buf, page_table, sequences, tokens, query_heads, pool, code):
+        self.buf, self.page_table = buf, page_table
+        self.sequences, self.tokens, self.query_heads = sequences, tokens, query_heads
+        self.pages, self.page_size, self.kv_heads, _ = pool
+        self.pool, self.code = pool, code
+        self.nbytes = buf.numel()
+
+    def token_records(self) -> torch.Tensor:
+        """``[tokens, 4]`` int32: position, page (negative: none), slot and sequence of each."""
+        return self.buf[512:512 + 16 * self.tokens].view(torch.int32).view(-1, 4)
+
+
+@functools.lru_cache(maxsize=256)
+def _strides(page: int, slot: int, head: int):
+    return (ctypes.c_longlong * 3)(page, slot, head)
+
+
+def _pool_strides(pages: torch.Tensor):
+    page, slot, head, last = pages.stride()
+    p, s, h, d = pages.shape
+    # a dimension of one is never stepped over
+    if last != 1 and d > 1:
+        raise ValueError("the pages' last dimension must be dense")
+    return _strides(page if p > 1 else 0, slot if s > 1 else 0, head if h > 1 else 0)
+
+
+def _check_pool(key_pages: torch.Tensor, value_pages: torch.Tensor, plan: Plan) -> None:
+    if key_pages.shape != plan.pool or value_pages.shape != plan.pool:
+        raise ValueError(f"the plan is for pages {list(plan.pool)}, the call has "
+                         f"{list(key_pages.shape)} and {list(value_pages.shape)}")
+
+
+def _int32(x: torch.Tensor, shape: tuple[int, ...], what: str) -> torch.Tensor:
+    if x.shape != shape:
+        raise ValueError(f"{what} must be {list(shape)}, got {list(x.shape)}")
+    if x.dtype is not torch.int32:
+        if x.is_floating_point() or x.is_complex() or x.dtype is torch.bool:
+            raise ValueError(f"{what} must hold integers, got {x.dtype}")
+        x = x.to(torch.int32)
+    return x.contiguous()
+
+
+def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: torch.Tensor,
+         key_pages: torch.Tensor, *, tokens: int, query_heads: int) -> Plan:
+    """Plan one step of ``R`` sequences over the pool ``key_pages`` (values have its shape).
+
+    ``query_starts [R + 1]`` (ascending) delimits the sequences' new tokens in a
+    batch of ``tokens``; those past the last belong to nobody.
+    ``context_lengths [R]`` counts each sequence's tokens, the new ones
+    included.  Token position ``p`` of sequence ``r`` is slot ``p % page_size``
+    of page ``page_table[r, p // page_size]``; entries outside the pool (-1, say,
+    behind a context or for a page that was given up) hold no keys.  Nothing is
+    read back to the host.  The table must stay as it is while the plan is used.
+    """
+    if key_pages.dim() != 4:
+        raise ValueError("pages must be [pages, page_size, heads, head_dim]")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    code = dtype_code(key_pages)
+    pool = key_pages.shape
+    pages, page_size, kv_heads, d = pool
+    if d != _lib.HEAD_DIM:
+        raise ValueError(f"paged attention serves head_dim {_lib.HEAD_DIM} (got {d})")
+    r, width = page_table.shape
+    starts = _int32(query_starts, (r + 1,), "query_starts")
+    contexts = _int32(context_lengths, (r,), "context_lengths")
+    table = page_table
+    if table.dtype is not torch.int32 or (width > 1 and table.stride(1) != 1) or (
+            r > 1 and table.stride(0) < width):
+        table = _int32(table, (r, width), "page_table")
+    device = require_device(key_pages, starts, contexts, table)
+    lib = _lib.LIB
+    nbytes = lib.mf_paged_plan_bytes(r, tokens, query_heads, kv_heads, code)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with on_device(device):
+        _lib.check(lib.mf_paged_plan(
+            starts.data_ptr(), contexts.data_ptr(), table.data_ptr(),
+            table.stride(0) if r > 1 else width, r, tokens, width, page_size, pages, query_heads,
+            kv_heads, code, buf.data_ptr(), nbytes, _raw_stream(device.index)))
+    return Plan(buf, table, r, tokens, query_heads, pool, code)
+
+
+def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
+           value_pages: torch.Tensor, plan: Plan, *, query: torch.Tensor | None = None,
+           rotary: Rotary | None = None, query_gain: torch.Tensor | None = None,
+           key_gain: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor | None:
+    """Write the step's keys and values into their pages, in place; returns the query.
+
+    Keys and the query (where given) are RMS-normalised over each head with
+    their gain, if they have one, then rotated at their token's position, if
+    ``rotary`` is given; values are copied.  Tokens without a page are left out
+    (their query is still returned).  float32 arithmetic, one rounding.  Pages
+    that several sequences share must not be appended to.  Forward only.
+    """
+    tensors = [t for t in (key, value, key_pages, value_pages, query, query_gain, key_gain)
+               if t is not None]
+    code = plan.code
+    dtype = key_pages.dtype
+    for t in tensors[:4 if query is None else 5]:
+        if t.dtype is not dtype:
+            raise ValueError(f"queries, keys, values and pages must share one dtype (got {dtype} "
+                             f"and {t.dtype})")
+    if dtype_code(key_pages) != code:
+        raise ValueError("the plan is for pages of another dtype")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("paged.append has no backward; call it under torch.no_grad()")
+    _check_pool(key_pages, value_pages, plan)
+    n, d = plan.tokens, _lib.HEAD_DIM
+    if key.shape != (n, plan.kv_heads, d) or value.shape != key.shape:
+        raise ValueError(f"keys and values must be {[n, plan.kv_heads, d]}, got "
+                         f"{list(key.shape)} and {list(value.shape)}")
+    if query is not None and query.shape != (n, plan.query_heads, d):
+        raise ValueError(f"the query must be {[n, plan.query_heads, d]}, got {list(query.shape)}")
+    if query is None and query_gain is not None:
+        raise ValueError("query_gain needs a query")
+    for gain in (query_gain, key_gain):
+        if gain is not None and gain.shape != (d,):
+            raise ValueError(f"gains must be [{d}], got {list(gain.shape)}")
+    if rotary is not None and (not isinstance(rotary, Rotary) or rotary.head_dim != d):
+        raise ValueError(f"rotary must be a Rotary of heads of {d}")
+    if key_pages.data_ptr() == value_pages.data_ptr():
+        raise ValueError("keys and values need pages of their own")
+    device = require_device(key_pages, plan.buf, *tensors)
+    kg = None if key_gain is None else key_gain.to(dtype).contiguous()
+    qg = None if query_gain is None else query_gain.to(dtype).contiguous()
+    key, k_step = token_rows(key)
+    value, v_step = token_rows(value)
+    out, q_step = None, 0
+    if query is not None:
+        query, q_step = token_rows(query)
+        out = torch.empty((n, plan.query_heads, d), dtype=dtype, device=device)
+    if rotary is None:
+        turn = (None, 0, 0, 1.0)
+    else:
+        turn = (rotary._array, rotary.rotary_dim, rotary.interleaved, rotary.magnitude)
+    with on_device(device):
+        _lib.check(_lib.LIB.mf_paged_append(
+            _ptr(query), q_step, key.data_ptr(), k_step, value.data_ptr(), v_step, _ptr(qg),
+            _ptr(kg), eps, *turn, code, n, plan.sequences, plan.query_heads, plan.kv_heads, d,
+            plan.page_size, plan.pages, plan.buf.data_ptr(), plan.nbytes, key_pages.data_ptr(),
+            value_pages.data_ptr(), _pool_strides(key_pages), _pool_strides(value_pages),
+            _ptr(out), _raw_stream(device.index)))
+    return out
+
+
+def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, plan: Plan,
+              *, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the step's new tokens over their sequences' pages.
+
+    ``query [tokens, Hq, 64]``: the query at position ``p`` of its sequence sees
+    the keys at positions ``0 .. p`` (the step's own keys must be in their pages:
+    :func:`append`).  A query that sees no key yields zeros.  ``scale`` defaults
+    to ``64 ** -0.5``.  Rows behind the last sequence are zeros, or left as they
+    are in an ``out`` that is given.  Slots behind a context may hold anything.
+    Forward only; the same inputs give the same bits.
+    """
+    n, hq, d = plan.tokens, plan.query_heads, _lib.HEAD_DIM
+    if query.shape != (n, hq, d):
+        raise ValueError(f"the query must be {[n, hq, d]}, got {list(query.shape)}")
+    dtype = query.dtype
+    if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
+        raise ValueError(f"query and pages must share one dtype (got {dtype}, {key_pages.dtype} "
+                         f"and {value_pages.dtype})")
+    code = dtype_code(query)
+    if code != plan.code:
+        raise ValueError("the plan is for pages of another dtype")
+    _check_pool(key_pages, value_pages, plan)
+    if torch.is_grad_enabled() and (query.requires_grad or key_pages.requires_grad
+                                    or value_pages.requires_grad):
+        raise ValueError("paged.attention has no backward; call it under torch.no_grad()")
+    device = require_device(query, key_pages, value_pages, plan.buf)
+    query, q_step = token_rows(query)
+    zero_rest = out is None
+    if zero_rest:
+        out = torch.empty((n, hq, d), dtype=dtype, device=device)
+    elif (out.shape != (n, hq, d) or out.dtype is not dtype or not out.is_contiguous()
+          or out.device != device):
+        raise ValueError(f"out must be a contiguous {dtype} {[n, hq, d]} on {device}")
+    lib = _lib.LIB
+    ws_bytes = lib.mf_paged_attn_workspace_bytes(plan.sequences, n, hq, plan.kv_heads, code)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    table = plan.page_table
+    with on_device(device):
+        _lib.check(lib.mf_paged_attn(
+            query.data_ptr(), q_step, key_pages.data_ptr(), value_pages.data_ptr(),
+            _pool_strides(key_pages), _pool_strides(value_pages), table.data_ptr(),
+            table.stride(0) if plan.sequences > 1 else table.shape[1], code, n, plan.sequences,
+            table.shape[1], plan.page_size, plan.pages, hq, plan.kv_heads, d,
+            d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes, zero_rest,
+            out.data_ptr(), ws.data_ptr(), ws_bytes, _raw_stream(device.index)))
+    return out
+
+
+def cache_pages(cache: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """A contiguous ``[B, capacity, Hkv, 64]`` cache as pages, without a copy.
+
+    Returns the pages and the page table ``[B, capacity / page_size]`` of its rows.
+    """
+    if cache.dim() != 4 or not cache.is_contiguous():
+        raise ValueError("the cache must be a contiguous [B, capacity, heads, head_dim] tensor")
+    b, cap, h, d = cache.shape
+    if page_size < 1 or cap % page_size:
+        raise ValueError(f"the capacity {cap} must be whole pages of {page_size}")
+    per = cap // page_size
+    table = torch.arange(b * per, dtype=torch.int32, device=cache.device).view(b, per)
+    return cache.view(b * per, page_size, h, d), table

@@ -1,0 +1,178 @@
+"""Rotary position embeddings: half and interleaved layouts, part of the head, long contexts.
+
+The general form of ``apply_rotary`` (``kernels/rotary.py:7-39`` of the
+reference, which rotates whole heads in the half layout): pair ``i`` of the
+``rotary_dim`` rotated dims turns by ``position * frequencies[i]`` and the
+other dims pass.  Arithmetic is float32 (angles exact at any position), rounded
+once to the tensors' dtype; :func:`prologue.qk_norm_rope` rounds every step, as
+the reference's declared types do, so its results differ in the last bit.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+from ..ops import (_ptr, _raw_stream, dtype_code, on_device, require_device, token_rows)
+from .prologue import _positions
+
+_SCALINGS = ("none", "linear", "base", "bands", "ramp")
+
+
+class Rotary:
+    """The frequencies of a rotary embedding, made once from a model's configuration.
+
+    ``head_dim`` is the width of a head, of which the first ``rotary_dim``
+    (default: all) rotate; ``interleaved`` pairs dims ``(2i, 2i + 1)`` instead
+    of ``(i, i + rotary_dim / 2)``.  ``frequencies[i] = theta ** (-2i /
+    rotary_dim)`` radians per position, stretched for contexts ``factor`` times
+    longer than the model was trained on by ``scaling``:
+
+    * ``none``
+    * ``linear``: every frequency divided by ``factor``;
+    * ``base``: ``theta`` multiplied by ``factor ** (rotary_dim / (rotary_dim - 2))``,
+      which keeps the first frequency and divides the last by ``factor``;
+    * ``bands``: by the turns a pair makes in ``original_length`` positions: kept
+      above ``fast`` (default 4), divided by ``factor`` below ``slow`` (default 1),
+      blended linearly in the turns between;
+    * ``ramp``: by the pair's index: kept up to the index whose pair makes ``fast``
+      (default 32) turns in ``original_length``, divided by ``factor`` from the one
+      with ``slow`` (default 1) on, blended linearly in the index between; the
+      rotated dims are also multiplied by ``magnitude`` (default ``0.1 ln(factor) + 1``).
+
+    Given ``frequencies`` (``rotary_dim / 2`` numbers) replace all of this.
+    """
+
+    def __init__(self, head_dim: int, *, theta: float = 10000.0, rotary_dim: int | None = None,
+                 interleaved: bool = False, scaling: str | None = None, factor: float = 1.0,
+                 original_length: int | None = None, fast: float | None = None,
+                 slow: float = 1.0, magnitude: float | None = None, frequencies=None):
+        r = head_dim if rotary_dim is None else rotary_dim
+        scaling = "none" if scaling is None else scaling
+        if head_dim < 2 or head_dim % 2 or head_dim > _lib.ROTATE_MAX_HEAD_DIM:
+            raise ValueError(f"head_dim must be even and in [2, {_lib.ROTATE_MAX_HEAD_DIM}] "
+                             f"(got {head_dim})")
+        if r < 2 or r % 2 or r > min(head_dim, _lib.ROTATE_MAX_DIM):
+            raise ValueError(f"rotary_dim must be even and in [2, min(head_dim, "
+                             f"{_lib.ROTATE_MAX_DIM})] (got {r} of {head_dim})")
+        if scaling not in _SCALINGS:
+            raise ValueError(f"Unsupported rotary scaling: {scaling}")
+        if not (theta > 1 and math.isfinite(theta)):
+            raise ValueError("theta must be finite and above 1")
+        if not (factor >= 1 and math.isfinite(factor)):
+            raise ValueError("factor must be finite and at least 1")
+        if scaling in ("bands", "ramp"):
+            fast = (4.0 if scaling == "bands" else 32.0) if fast is None else fast
+            if not original_length or original_length < 1:
+                raise ValueError(f"{scaling} scaling needs original_length")
+            if not 0 < slow < fast:
+                raise ValueError("scaling needs 0 < slow < fast turns")
+        if frequencies is not None:
+            freqs = [float(f) for f in frequencies]
+            if len(freqs) != r // 2:
+                raise ValueError(f"frequencies must hold rotary_dim / 2 = {r // 2} numbers")
+        else:
+            freqs = _scaled(r, theta, scaling, factor, original_length, fast, slow)
+        if magnitude is None:
+            magnitude = 1.0 + 0.1 * math.log(factor) if scaling == "ramp" else 1.0
+        if not all(math.isfinite(f) for f in (*freqs, magnitude)):
+            raise ValueError("frequencies and magnitude must be finite")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, r, bool(interleaved)
+        self.frequencies, self.magnitude = tuple(freqs), float(magnitude)
+        self._array = (ctypes.c_double * len(freqs))(*freqs)  # the C ABI's host array
+
+    def __repr__(self) -> str:
+        return (f"Rotary(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, "
+                f"interleaved={self.interleaved}, magnitude={self.magnitude:g})")
+
+
+def _scaled(r, theta, scaling, factor, length, fast, slow) -> list[float]:
+    if scaling == "base":
+        # of a single pair there is no last frequency to slow
+        theta = theta * factor ** (r / (r - 2)) if r > 2 else theta
+    freqs = [theta ** (-2 * i / r) for i in range(r // 2)]
+    if scaling == "linear":
+        return [f / factor for f in freqs]
+    if scaling == "bands":
+        keep = [(length * f / (2 * math.pi) - slow) / (fast - slow) for f in freqs]
+        keep = [min(max(x, 0.0), 1.0) for x in keep]
+        return [f * (x + (1 - x) / factor) for f, x in zip(freqs, keep)]
+    if scaling == "ramp":
+        # index whose pair makes n turns in `length` positions
+        lo, hi = (r * math.log(length / (2 * math.pi * n)) / (2 * math.log(theta))
+                  for n in (fast, slow))
+        lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), r - 1)
+        drop = [min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0) for i in range(r // 2)]
+        return [f * (1 - x + x / factor) for f, x in zip(freqs, drop)]
+    return freqs
+
+
+def _launch(q, k, positions, rotary, backward):
+    """Rotates q and k ([B, T, H, D] or [N, H, D], either None) into new dense tensors."""
+    one = q if q is not None else k
+    shape, device = one.shape, one.device
+    tokens, seq_len = (shape[0] * shape[1], shape[1]) if one.dim() == 4 else (shape[0], shape[0])
+    q, q_stride = (None, 0) if q is None else token_rows(q)
+    k, k_stride = (None, 0) if k is None else token_rows(k)
+    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    with on_device(device):
+        _lib.check(_lib.LIB.mf_rotate(
+            _ptr(q), q_stride, _ptr(k), k_stride, _ptr(positions), rotary._array, dtype_code(one),
+            tokens, seq_len, 0 if q is None else q.shape[-2], 0 if k is None else k.shape[-2],
+            rotary.head_dim, rotary.rotary_dim, rotary.interleaved, rotary.magnitude, backward,
+            _ptr(q_out), _ptr(k_out), _raw_stream(device.index)))
+    return q_out, k_out
+
+
+class Rotate(torch.autograd.Function):
+    """Rotation of queries and keys in one launch; the backward turns the gradients back."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, rotary):
+        ctx.save_for_backward(positions)
+        ctx.rotary = rotary
+        ctx.set_materialize_grads(False)
+        return _launch(q, k, positions, rotary, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        if dq is None and dk is None:
+            return None, None, None, None
+        dq, dk = _launch(dq, dk, ctx.saved_tensors[0], ctx.rotary, True)
+        return dq, dk, None, None
+
+
+def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positions=None
+           ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotate ``query [B, T, Hq, D]`` and ``key [B, T, Hkv, D]`` (or ``[N, H, D]`` both).
+
+    ``positions`` are integers: a scalar, ``[T]`` or ``[B, T]`` (``[N]`` for
+    three dimensions); ``None`` means ``0 .. T-1`` on every row.  ``key`` may be
+    ``None``.  Slices of one projection are read where they are as long as each
+    head is dense and tokens are evenly spaced.  Differentiable in both, once.
+    """
+    if not isinstance(rotary, Rotary):
+        raise ValueError("rotary must be a Rotary")
+    if query.dim() not in (3, 4):
+        raise ValueError("query must be [B, T, H, D] or [N, H, D]")
+    if query.shape[-1] != rotary.head_dim:
+        raise ValueError(f"the rotary embedding is for heads of {rotary.head_dim}, "
+                         f"the query has {query.shape[-1]}")
+    if key is not None and (key.shape[:-2] != query.shape[:-2] or key.shape[-1] != query.shape[-1]
+                            or key.dtype != query.dtype):
+        raise ValueError("query and key must share batch, length, head_dim and dtype")
+    dtype_code(query)
+    device = require_device(query) if key is None else require_device(query, key)
+    if query.dim() == 4:
+        pos = _positions(positions, query.shape[0], query.shape[1], device)
+    else:
+        pos = _positions(positions, 1, query.shape[0], device)
+    if not torch.is_grad_enabled() or not (query.requires_grad
+                                           or (key is not None and key.requires_grad)):
+        return _launch(query, key, pos, rotary, False)
+    return Rotate.apply(query, key, pos, rotary)

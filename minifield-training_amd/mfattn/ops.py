@@ -10,6 +10,7 @@ calls the HIP backward once.
 from __future__ import annotations
 
 import collections
+import contextlib
 import threading
 import weakref
 
@@ -83,6 +84,44 @@ def require_contiguous(what: str, *tensors: torch.Tensor) -> None:
         if t is not None and not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous (got a strided view of shape "
                              f"{list(t.shape)}); pass .contiguous()")
+
+
+class _OtherDevice:
+    """Makes a tensor's device the current one around a launch (streams belong to devices)."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        torch.cuda.set_device(self.before)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context of a launch on ``device``: nothing to do where it is the current one."""
+    if torch.cuda.current_device() == device.index:
+        return _SAME_DEVICE
+    return _OtherDevice(device.index)
+
+
+def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``x [..., H, D]`` and the elements between its tokens, copied only where its
+    heads are not dense, its tokens not evenly spaced or its rows not aligned: the
+    parts of one projection, for example, are read where they are."""
+    *lead, h, d = x.shape
+    st = x.stride()
+    step = st[-3] if lead[-1] > 1 else st[0] if len(lead) == 2 and lead[0] > 1 else h * d
+    if (st[-1] == 1 and (h == 1 or st[-2] == d) and step >= h * d
+            and (len(lead) < 2 or lead[0] == 1 or st[0] == lead[1] * step)
+            and step * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0):
+        return x, step
+    return x.contiguous(), h * d
 
 
 def _require_lse(lse: torch.Tensor, b: int, hq: int, t: int) -> None:
