@@ -298,7 +298,8 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
  * written to q_out (dense; may be q where that is dense); q and q_out NULL: no
  * queries.  k, v [tokens, kv_heads, 64]; token strides in elements.
  * k_pages, v_pages: [pages][page_size][kv_heads][64] with strides
- * {page, slot, head} in elements (HOST arrays of 3), the last dimension dense.
+ * {page, slot, head} in elements (HOST arrays of 3; at most 2^26 between slots
+ * and 2^29 between heads), the last dimension dense.
  * Where two tokens have the same page and slot, either remains. */
 int mf_paged_append(const void* q, long long q_stride, const void* k,
                     long long k_stride, const void* v, long long v_stride,
@@ -315,8 +316,8 @@ int mf_paged_append(const void* q, long long q_stride, const void* k,
  * one new token a row, kernels/attention.py:264-282, over pages and for any
  * number of new tokens; a query that sees no key yields zeros).  q
  * [tokens, q_heads, 64] with q_stride elements between tokens, out dense.
- * k_pages, v_pages and their strides as mf_paged_append, 16-byte aligned rows;
- * a page within 2 GiB.  Rows of out past the last sequence are zeroed when
+ * k_pages, v_pages and their strides as mf_paged_append, with 16-byte aligned
+ * rows.  Rows of out past the last sequence are zeroed when
  * zero_rest != 0 and left as they are otherwise.  Deterministic.  `workspace`
  * holds the partial results of keys split over workgroups
  * (mf_paged_attn_workspace_bytes); it is this call's alone while it runs. */

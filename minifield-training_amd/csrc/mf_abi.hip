@@ -572,8 +572,8 @@ int check_paged(int dtype, int sequences, int tokens, int q_heads, int kv_heads)
     return fail(MF_ERR_SHAPE, "at most %d sequences a step (got %d)", mf::kMaxSequences, sequences);
   if (q_heads % kv_heads) return fail(MF_ERR_HEADS, "Query heads must be divisible by KV heads");
   // one launch's workgroups of 256 threads stay below 2^32 threads
-  if ((long long)tokens * q_heads > (1ll << 28) || kv_heads > 1024)
-    return fail(MF_ERR_SHAPE, "tokens * q_heads must not exceed 2^28, nor kv_heads 1024");
+  if ((long long)tokens * q_heads > (1ll << 26) || kv_heads > 1024)
+    return fail(MF_ERR_SHAPE, "tokens * q_heads must not exceed 2^26, nor kv_heads 1024");
   return MF_OK;
 }
 
@@ -607,6 +607,9 @@ int check_page_strides(const char* what, const long long* s, int page_size, int 
   // rows of eight slots are addressed with 32-bit offsets from their first
   if (s[1] > (1ll << 31) / (4ll * 8))
     return fail(MF_ERR_SHAPE, "%s: %lld elements between slots (at most 2^26)", what, s[1]);
+  // and two neighbouring heads' rows with them
+  if (s[2] > (1ll << 29))
+    return fail(MF_ERR_SHAPE, "%s: %lld elements between heads (at most 2^29)", what, s[2]);
   *out = {s[0], s[1], s[2]};
   return MF_OK;
 }
@@ -661,6 +664,11 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
                 table_stride, max_pages);
   if ((long long)max_pages * page_size > (1ll << 30))
     return fail(MF_ERR_SHAPE, "max_pages * page_size must not exceed 2^30");
+  // units of keys over all tiles are counted in 32 bits
+  if (mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32).cap_tiles *
+          ((long long)max_pages * page_size) > (1ll << 36))
+    return fail(MF_ERR_SHAPE, "%d sequences of %d tokens over %d x %d slots are too many for one step",
+                sequences, tokens, max_pages, page_size);
   if (!query_starts || !context_lengths || !page_table)
     return fail(MF_ERR_INVALID_ARGUMENT,
                 "query_starts, context_lengths and page_table must be non-null");

@@ -8,22 +8,30 @@
 // position p lives in page page_table[r][p / page_size], slot p % page_size.
 // The attention of KV head h works on rows: row i * G + g of a sequence is
 // query token i and head h * G + g (G query heads per KV head).  Rows are cut
-// into tiles, a tile's visible keys into items; one workgroup takes an item of
-// one KV head.  Everything is derived on the device: the host never reads a
-// length back.
+// into tiles and a tile's visible keys into items.  There are two kinds: tiles
+// of few rows (a sequence of up to 32, or in fp32 every 32 rows), whose items are
+// bound by the keys they read, and tiles of many (up to 256), bound by their
+// products.  Everything is derived on the device: the host never reads a length
+// back.
 #pragma once
 
 #include "mf_common.h"
 
 namespace mf {
 
-constexpr int kFewRows = 32;     // rows up to which a sequence's waves split the keys
-constexpr int kManyRows = 128;   // rows of a tile whose waves split the rows (bf16)
-constexpr int kUnitKeys = 128;   // an item's keys come in units of this many
+constexpr int kFewRows = 32;
+constexpr int kManyRows = 256;
 constexpr int kMaxSequences = 4096;
-// Items per KV head times KV heads that the splitting aims at: the workgroups
-// the chip holds at once (four per CU).
-constexpr int kTargetItems = 1024;
+constexpr int kKeyWaves = 4;                // waves of a workgroup, which share a few-rows item's keys
+constexpr int kFewKeys = 32 * kKeyWaves;    // keys come in units of this many there
+constexpr int kManyKeys = 64;               // and of this many here
+// Shares times workgroups of a share: what is resident at once, two per CU.
+constexpr int kFewGroups = 512;
+constexpr int kManyGroups = 512;
+// A tile of many rows writes up to 66 KB of partial results per item and KV head:
+// its shares have at least this many units.
+constexpr int kManyUnits = 4;
+constexpr int kJoinRows = 8;  // rows of a split tile that one workgroup joins
 
 // One new token: where it is and where its key and value go (page < 0: nowhere).
 struct PagedToken {
@@ -40,42 +48,55 @@ struct PagedItem {
   int sequence;
 };
 
-// One tile that was split: its items' partial results are joined.
-struct PagedTile {
-  int start, row0, nrows, partial, splits, pad[3];
+// Up to kJoinRows rows of a tile that was split, whose items' partial results are
+// joined: item i's are rows partial + i * step.
+struct PagedJoin {
+  int start, row0, nrows, partial, splits, step, pad[2];
 };
+
+// Kinds of tiles.
+constexpr int kFew = 0, kMany = 1;
 
 struct PagedLayout {
-  size_t zeros, tokens, items, tiles, total;
-  int tile_rows;      // rows of the largest tile
-  int cap_items, cap_tiles;
-  size_t cap_rows;    // rows of partial results
-  int target;         // items per KV head aimed at
+  size_t zeros, tokens, shares[2], items[2], joins, total;
+  int head_pair;       // KV heads a wave of a few-rows item takes (bf16: 2 where they are even)
+  int target[2];       // shares of each kind at most
+  int cap_tiles, cap_items[2], cap_joins;
+  size_t cap_rows;     // rows of partial results
 };
 
-// header (ints): 0 items, 1 split tiles, 2 end of the last sequence's tokens
-constexpr int kHeadItems = 0, kHeadTiles = 1, kHeadEnd = 2;
+// header (ints)
+constexpr int kHeadShares = 0, kHeadJoins = 2, kHeadEnd = 3;  // shares of each kind: 0 and 1
 
-// Bounds: a sequence of M rows has one tile (M <= 32) or ceil(M / 128), so at
-// most sequences + tokens G / 128 in all.  With W units of keys over all tiles
-// and items of C = max(1, ceil(W / target)) units, the items are at most
-// sum ceil(w / C) <= W / C + tiles <= target + tiles, and the partial rows
-// sum n ceil(w / C) <= rows of a tile * target + sum n.
+// Bounds: a sequence of M rows has one tile (M <= 32) or ceil(M / 256), so at
+// most sequences + tokens G / 256 in all.  Every boundary between shares adds an
+// item, so there are at most shares + tiles of each kind, and rows of a tile * shares
+// + sum n partial rows.
 __host__ __device__ inline PagedLayout paged_layout(int sequences, int tokens, int G, int Hkv,
                                                     bool f32) {
   PagedLayout p;
   const long long rows = (long long)tokens * G;
-  p.tile_rows = f32 ? kFewRows : kManyRows;
-  p.target = kTargetItems / Hkv < 1 ? 1 : kTargetItems / Hkv;
-  p.cap_tiles = (int)(sequences + rows / p.tile_rows);
-  p.cap_items = p.target + p.cap_tiles;
-  const long long most = rows < p.tile_rows ? rows : p.tile_rows;
-  p.cap_rows = (size_t)(most * p.target + rows);
+  p.head_pair = !f32 && Hkv % 2 == 0 ? 2 : 1;
+  const int pairs = Hkv / p.head_pair;
+  const bool many = !f32 && rows > kFewRows;
+  p.target[kFew] = kFewGroups / pairs < 1 ? 1 : kFewGroups / pairs;
+  p.target[kMany] = !many ? 0 : kManyGroups / Hkv < 1 ? 1 : kManyGroups / Hkv;
+  p.cap_tiles = (int)(sequences + rows / (f32 ? kFewRows : kManyRows));
+  p.cap_items[kFew] = p.target[kFew] + (f32 ? p.cap_tiles : sequences);
+  p.cap_items[kMany] = many ? p.target[kMany] + p.cap_tiles : 0;
+  p.cap_joins = (int)(p.cap_tiles + rows / kJoinRows);
+  p.cap_rows = (size_t)((rows < kFewRows ? rows : kFewRows) * p.target[kFew] +
+                        (rows < kManyRows ? rows : kManyRows) * p.target[kMany] + rows);
   size_t off = 256;
   p.zeros = off;  off += 256;
   p.tokens = off; off = align256(off + sizeof(PagedToken) * (size_t)tokens);
-  p.items = off;  off = align256(off + sizeof(PagedItem) * (size_t)p.cap_items);
-  p.tiles = off;  off = align256(off + sizeof(PagedTile) * (size_t)p.cap_tiles);
+  for (int k = 0; k < 2; ++k) {
+    p.shares[k] = off;
+    off = align256(off + sizeof(int) * (size_t)(p.target[k] + 1));
+    p.items[k] = off;
+    off = align256(off + sizeof(PagedItem) * (size_t)p.cap_items[k]);
+  }
+  p.joins = off;  off = align256(off + sizeof(PagedJoin) * (size_t)p.cap_joins);
   p.total = off;
   return p;
 }

@@ -2,15 +2,16 @@
 //
 // For each KV head the rows of a sequence are its (token, head of the group)
 // pairs; row i * G + g at position p sees keys 0 .. p.  The plan (mf_paged.h)
-// cut rows into tiles and a tile's keys into items; one workgroup of four waves
-// takes an item of one KV head, in one of two ways:
+// cut rows into tiles and a tile's keys into items; a workgroup of four waves
+// takes an item in one of two ways:
 //
-//   up to 32 rows (decode, drafts): every wave holds all rows and takes every
-//     fourth 32-key block, with a K and a V buffer of its own in LDS: no barrier
-//     until the waves' softmax states are merged.  Bound: HBM, each cached key
-//     and value is read once for all rows of its head.
-//   up to 128 rows (chunks): every wave holds 32 rows, all share 64-key stages in
-//     a ring of two.  Bound: MFMA and the LDS reads that feed it.
+//   up to 32 rows (decode, drafts): every wave holds all rows of one or two KV
+//     heads and takes 32-key blocks of its own, through a K and a V buffer of its
+//     own in LDS: no barrier until the states of waves that share an item are
+//     merged.  Bound: HBM, each cached key and value is read once for all rows of
+//     its head.
+//   up to 256 rows (chunks), one KV head: every wave holds 64 rows, all share
+//     64-key stages in a ring of four.  Bound: MFMA and the softmax between.
 //
 // Both use S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: an accumulator
 // column is a row of the batch, so its maximum and sum are in-lane reductions and
@@ -24,10 +25,10 @@
 //
 // Pages.  Page sizes are multiples of 8 and blocks start at multiples of 32, so
 // eight keys of a block lie in one page: their page number is a scalar load, and
-// their rows are moved by one LDS DMA from a scalar base.  Keys that are not
-// there (behind the context, in a page outside the pool) are read from a row of
-// zeros in the plan, so that nothing a masked slot holds, infinities and NaN
-// included, meets a product.
+// their rows are moved by LDS DMAs from a scalar base.  Keys that are not there
+// (behind the context, in a page outside the pool) are read from a row of zeros
+// in the plan, so that nothing a masked slot holds, infinities and NaN included,
+// meets a product.
 #include "mf_f32.h"
 #include "mf_lds.h"
 #include "mf_paged.h"
@@ -41,26 +42,30 @@ struct PagedArgs {
   const int* table;
   const int* head;
   const char* zeros;
-  const int* items;
-  const int* tiles;
+  const int* shares[2];     // by kind
+  const int* items[2];
+  const int* joins;
   char* out;
-  float2* ml;               // partial results: (max in log2 units, sum) per row and KV head
+  float2* ml;               // partial results: (max in log2 units, sum) per KV head and row
   float* acc;               // and 64 outputs
   long long q_stride;       // bytes between tokens
   PagedStrides ks, vs;      // bytes
   long long table_stride;
   long long out_bytes;
-  int page_size, pages, Hq, Hkv, G, zero_rest, tile_blocks;
+  long long cap_rows;       // partial rows of a KV head
+  int page_size, pages, Hq, Hkv, G;
+  int few_turns, many_turns;  // 256 workgroups each
+  int join_blocks, head_pairs;
   float scale_log2;
-  FastDiv div_g, div_page, div_hkv;
+  FastDiv div_g, div_page, div_hkv, div_pairs;
 };
 
 struct ItemView {
   int start, row0, nrows, base, key0, key1, partial, sequence;
 };
 
-__device__ __forceinline__ ItemView load_item(const PagedArgs& a, int item) {
-  const i32x8u r = ld_const8(a.items, 8 * item);
+__device__ __forceinline__ ItemView load_item(const int* items, int item) {
+  const i32x8u r = ld_const8(items, 8 * item);
   return {r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};
 }
 
@@ -78,7 +83,13 @@ __device__ __forceinline__ long long row_offset(const PagedArgs& a, const PagedS
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// dma16 with a 64-bit address per lane.
+// LDS DMAs of 16 bytes a lane (mf_lds.h) that are not kept in cache: a few-rows
+// item's keys and values are read once.
+__device__ __forceinline__ void dma16_once(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :: "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+}
+// With a 64-bit address per lane.
 __device__ __forceinline__ void dma16_lane(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                :: "v"(src), "s"(lds) : "memory", "m0");
@@ -90,23 +101,6 @@ __device__ __forceinline__ void wait_vm_lds() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-// Rows of keys key0 .. key0 + 7 (one page, `page` already checked or -1) into
-// rows r0 .. r0 + 7 of an LDS tile; rows of keys from `end` on, and of no page,
-// are zeros.  lane_off: the lane's byte offset from the first row.
-__device__ __forceinline__ void dma_keys8(const PagedArgs& a, const char* pool,
-                                          const PagedStrides& s, uint32_t lane_off, int chunk_off16,
-                                          int page, int key0, int end, int kvh, char* tile, int r0) {
-  const uint32_t dst = uniform((int)lds_offset(tile + r0 * kRowBytes));
-  const char* base = pool + row_offset(a, s, max(page, 0), key0, kvh);
-  if (page >= 0 && key0 + 8 <= end) {
-    dma16(base, lane_off, dst);
-  } else {
-    const int row = __lane_id() >> 3;
-    const char* src = page >= 0 && key0 + row < end ? base + lane_off : a.zeros + chunk_off16;
-    dma16_lane(src, dst);
-  }
-}
 
 // One row's running softmax: probabilities are 2^(s c - shift); shift is the
 // running maximum in log2 units once a key was seen, and moves only when a new
@@ -134,13 +128,13 @@ __device__ __forceinline__ void grow(RowState& st, float mx, f32x16 (&acc)[2]) {
   }
 }
 
-// Probabilities, their sums, and O += P V of one 32-key block whose V rows are
-// rows v0 .. v0 + 31 of an LDS tile.
-__device__ __forceinline__ void block_pv(f32x16& s, RowState& st, float c, const char* vt, int v0,
-                                         int lane, f32x16 (&acc)[2]) {
+// Probabilities of one 32-key block in bf16 (the operands of its two 16-key
+// steps), and their sums.
+__device__ __forceinline__ void block_probs(f32x16& s, RowState& st, float c, bf16x8& p0, bf16x8& p1) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], c, -st.shift));
-  const bf16x8 p0 = pack8(s, 0), p1 = pack8(s, 8);
+  p0 = pack8(s, 0);
+  p1 = pack8(s, 8);
   const u32x4 w0 = __builtin_bit_cast(u32x4, p0), w1 = __builtin_bit_cast(u32x4, p1);
   const bf16x2 ones = __builtin_bit_cast(bf16x2, 0x3F803F80u);
 #pragma unroll
@@ -149,41 +143,25 @@ __device__ __forceinline__ void block_pv(f32x16& s, RowState& st, float c, const
     st.l0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a0), ones, st.l0, false);
     st.l1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a1), ones, st.l1, false);
   }
-  const int tr_row = tr_row_of(lane), tr_col = tr_col_of(lane);
-#pragma unroll
-  for (int db = 0; db < 2; ++db) {
-    const bf16x8 va = tile_tr_operand(vt, v0 + tr_row, db * 32 + tr_col);
-    const bf16x8 vb = tile_tr_operand(vt, v0 + 16 + tr_row, db * 32 + tr_col);
-    acc[db] = mfma32x32x16(va, p0, acc[db]);
-    acc[db] = mfma32x32x16(vb, p1, acc[db]);
-  }
-}
-
-__device__ __forceinline__ f32x16 block_scores(const char* kt, int k0, int lane,
-                                               const bf16x8 (&qf)[4]) {
-  f32x16 s = zero16();
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-    s = mfma32x32x16(tile_chunk(kt, k0 + (lane & 31), 2 * ks + (lane >> 5)), qf[ks], s);
-  return s;
 }
 
 // Scores of keys from the lane's limit on (block of 32 keys from kb) and of the
-// 8-key groups in `gone` become -inf; returns the column's maximum in the lane.
-__device__ __forceinline__ float mask_scores(f32x16& s, int kb, int lim, bool diag, int gone,
-                                             int lane) {
-  if (diag) {
+// 8-key groups in `gone` become -inf.
+__device__ __forceinline__ void mask_scores(f32x16& s, int kb, int lim, int gone, int lane) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = kb + acc_row(r, lane) < lim ? s[r] : kNegInf;
-  }
-  if (gone) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (gone >> g & 1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * g + i] = kNegInf;
-      }
-  }
+  for (int r = 0; r < 16; ++r)
+    s[r] = kb + acc_row(r, lane) < lim && !(gone >> (r >> 2) & 1) ? s[r] : kNegInf;
+}
+
+// A value the compiler cannot see through: what is computed from it stays in the
+// branch it is made in.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
+// Maximum of a column's scores in the lane.
+__device__ __forceinline__ float column_max(const f32x16& s) {
   float mx = fmaxf(s[0], s[1]);
 #pragma unroll
   for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
@@ -212,271 +190,507 @@ __device__ __forceinline__ int row_limit(const PagedArgs& a, const ItemView& it,
 }
 
 // --------------------------------------------------------------------------
-// Up to 32 rows: the waves split the keys.
+// Up to 32 rows of HW (1 or 2) adjacent KV heads a wave.
+//
+// A wave's K (and V) block in LDS is 32 tokens of HW 128-byte rows; a DMA moves
+// 8 / HW tokens, HW * 128 consecutive bytes of each where heads lie next to each
+// other.  (Two heads: 256-byte pieces of a token's row instead of 128.)  The
+// 16-byte pieces of a token are permuted by XOR with few_swz(token), so that the
+// 16 tokens that an operand read covers fall on all banks, and the transposing
+// reads of eight tokens too.
 // --------------------------------------------------------------------------
-constexpr int kWaveLds = 2 * 32 * kRowBytes;  // a wave's K and V block
+template <int HW>
+__device__ __forceinline__ int few_swz(int t) {
+  return HW == 1 ? swz(t) : ((t & 7) << 1) | ((t >> 3) & 1);
+}
 
-__device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
-                                         float (*lm)[kFewRows], float (*ll)[kFewRows]) {
+template <int HW>
+struct FewLds {
+  static constexpr int kTok = HW * kRowBytes;      // bytes of a token
+  static constexpr int kBlock = 32 * kTok;         // a K or V block
+  static constexpr int kWave = 2 * kBlock;
+};
+
+// Keys of block kb .. kb + 31 of a pool into a wave's LDS block.  off: the lane's
+// byte offsets from the first token of a DMA, by the DMA's number (mod 4 for two
+// heads, where the permutation depends on it).
+template <int HW>
+__device__ __forceinline__ void few_fetch(const PagedArgs& a, const char* pool,
+                                          const PagedStrides& s, const uint32_t (&off)[2 * HW],
+                                          const int (&page)[4], int kb, int end, int head0,
+                                          char* block) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int key = kb + 8 * g;
+    const char* base = pool + row_offset(a, s, max(page[g], 0), key, head0);
+    if (page[g] >= 0 && key + 8 <= end) {
+#pragma unroll
+      for (int j = 0; j < HW; ++j)
+        dma16_once(base + j * 4 * s.slot, off[HW == 1 ? 0 : (2 * g + j) & 3],
+                   uniform((int)lds_offset(block + (HW * g + j) * 1024)));
+    } else {
+      const int lane = __lane_id();
+#pragma unroll
+      for (int j = 0; j < HW; ++j) {
+        const bool there = page[g] >= 0 && key + j * 4 + lane / (8 * HW) < end;
+        const char* src = there ? base + j * 4 * s.slot + off[HW == 1 ? 0 : (2 * g + j) & 3]
+                                : a.zeros + 16 * (lane & 7);
+        dma16_lane(src, uniform((int)lds_offset(block + (HW * g + j) * 1024)));
+      }
+    }
+  }
+}
+
+template <int HW>
+__device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it, int pair,
+                                         int key_wave, char* wave_lds, float* lm, float* ll) {
+  typedef FewLds<HW> L;
   const int lane = fresh_lane_id();  // (not kept alive across the other path's loop)
-  const int wave = uniform(threadIdx.x >> 6);
-  char* kt = lds + wave * kWaveLds;
-  char* vt = kt + 32 * kRowBytes;
+  const int half = lane >> 5;
+  const int head0 = HW * pair;
+  char* kt = wave_lds;
+  char* vt = wave_lds + L::kBlock;
   const int row = min(lane & 31, it.nrows - 1);
-  bf16x8 qf[4];
-  load_query(a, row_of(a, it, row, kvh), lane, qf);
+  bf16x8 qf[HW][4];
+#pragma unroll
+  for (int h = 0; h < HW; ++h) load_query(a, row_of(a, it, row, head0 + h), lane, qf[h]);
   const int lim = row_limit(a, it, row);
   const int least = uniform(row_limit(a, it, 0));
   drain_memory();
 
-  const int chunk16 = ((lane & 7) ^ swz(lane >> 3)) * 16;
-  const uint32_t k_off = (uint32_t)((lane >> 3) * a.ks.slot) + chunk16;
-  const uint32_t v_off = (uint32_t)((lane >> 3) * a.vs.slot) + chunk16;
+  // the lane's piece of a DMA: token tok, and the piece whose place is the lane's
+  uint32_t k_off[2 * HW], v_off[2 * HW];
+#pragma unroll
+  for (int i = 0; i < 2 * HW; ++i) {
+    const int tok = lane / (8 * HW);
+    const int piece = (lane & (8 * HW - 1)) ^ few_swz<HW>(HW == 1 ? tok : 4 * i + tok);
+    k_off[i] = (uint32_t)(tok * a.ks.slot) + (uint32_t)((piece >> 3) * a.ks.head) + 16 * (piece & 7);
+    v_off[i] = (uint32_t)(tok * a.vs.slot) + (uint32_t)((piece >> 3) * a.vs.head) + 16 * (piece & 7);
+  }
+  // operand addresses: piece 8 h + 2 ks + half of token lane & 31, and for the
+  // transposing reads piece 8 h + 4 db + tr_col / 8 of token tr_row (+ 8, + 16)
+  const int tr_row = tr_row_of(lane), tr_col = tr_col_of(lane);
+  const int k_at = (lane & 31) * L::kTok + ((half ^ few_swz<HW>(lane & 31)) << 4);
+  const int v_at = tr_row * L::kTok + (((tr_col >> 3) ^ few_swz<HW>(tr_row)) << 4) + 2 * (tr_col & 7);
+
   const int* trow = a.table + it.sequence * a.table_stride;
   const int blocks = (it.key1 - it.key0 + 31) >> 5;
-
-  f32x16 acc[2] = {zero16(), zero16()};
-  RowState st = {0.f, kNegInf, 0.f, 0.f};
-  const float c = a.scale_log2;
-  int page[4];  // of the block that is fetched next
-  auto pages_of = [&](int b) {
+  f32x16 acc[HW][2];
+  RowState st[HW];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int id = page_of(a, trow, min(it.key0 + 32 * b + 8 * g, it.key1 - 1));
-      page[g] = (unsigned)id < (unsigned)a.pages ? id : -1;
-    }
-  };
-  auto fetch = [&](const char* pool, const PagedStrides& s, uint32_t off, int b, char* tile) {
+  for (int h = 0; h < HW; ++h) {
+    acc[h][0] = acc[h][1] = zero16();
+    st[h] = {0.f, kNegInf, 0.f, 0.f};
+  }
+  const float c = a.scale_log2;
+  // Pages of the block that is fetched next: the table's entries, checked only when
+  // they are used (a check is a wait for the load).
+  int entry[4], page[4];
+  int gone = 0, gone_next = 0;
+  auto load_entries = [&](int b) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      dma_keys8(a, pool, s, off, chunk16, page[g], it.key0 + 32 * b + 8 * g, it.key1, kvh, tile,
-                8 * g);
+      entry[g] = page_of(a, trow, min(it.key0 + 32 * b + 8 * g, it.key1 - 1));
   };
-  int gone = 0, gone_next = 0;
-  auto gone_of = [&]() {
-    int m = 0;
+  auto check_entries = [&]() {
+    gone_next = 0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) m |= page[g] < 0 ? 1 << g : 0;
-    return m;
+    for (int g = 0; g < 4; ++g) {
+      page[g] = (unsigned)entry[g] < (unsigned)a.pages ? entry[g] : -1;
+      gone_next |= page[g] < 0 ? 1 << g : 0;
+    }
   };
-  int b = wave;
+  int b = key_wave;
   if (b < blocks) {
-    pages_of(b);
-    gone_next = gone_of();
-    fetch(a.k, a.ks, k_off, b, kt);
-    fetch(a.v, a.vs, v_off, b, vt);
+    load_entries(b);
+    check_entries();
+    few_fetch<HW>(a, a.k, a.ks, k_off, page, it.key0 + 32 * b, it.key1, head0, kt);
+    few_fetch<HW>(a, a.v, a.vs, v_off, page, it.key0 + 32 * b, it.key1, head0, vt);
   }
-  for (; b < blocks; b += 4) {
-    const int kb = it.key0 + 32 * b;
-    const bool more = b + 4 < blocks;
+  for (; b < blocks; b += kKeyWaves) {
+    const int kb = it.key0 + 32 * b, next = b + kKeyWaves;
+    const bool more = next < blocks;
     gone = gone_next;
+    if (more) load_entries(next);
+    wait_vm_lds<4 * HW>();  // K is there; V's DMAs may be on their way
+    f32x16 s[HW];
+#pragma unroll
+    for (int h = 0; h < HW; ++h) {
+      s[h] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        s[h] = mfma32x32x16(ld_bf16x8(kt + (k_at ^ ((8 * h + 2 * ks) << 4))), qf[h][ks], s[h]);
+    }
+    wait_lds();
+    __builtin_amdgcn_sched_barrier(0);
     if (more) {
-      pages_of(b + 4);
-      gone_next = gone_of();
+      check_entries();
+      few_fetch<HW>(a, a.k, a.ks, k_off, page, it.key0 + 32 * next, it.key1, head0, kt);
     }
-    wait_vm_lds<4>();  // K is there; V's four may be on their way
-    f32x16 s = block_scores(kt, 0, lane, qf);
+    const bool masked = kb + 32 > least || gone;
+    bf16x8 p[HW][2];
+#pragma unroll
+    for (int h = 0; h < HW; ++h) {
+      if (masked) mask_scores(s[h], opaque(kb), lim, gone, lane);
+      grow(st[h], fmaf(halves_max(column_max(s[h])), c, -st[h].shift), acc[h]);
+      block_probs(s[h], st[h], c, p[h][0], p[h][1]);
+    }
+    if (more) wait_vm_lds<4 * HW>(); else wait_vm_lds<0>();
+#pragma unroll
+    for (int h = 0; h < HW; ++h)
+#pragma unroll
+      for (int db = 0; db < 2; ++db)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const char* at = vt + 16 * j * L::kTok;
+          const int x = v_at ^ ((8 * h + 4 * db) << 4);
+          const u32x2 lo = lds_read_tr16(at + x);
+          // token + 8: the permutation of two heads differs in its lowest bit
+          const u32x2 hi = lds_read_tr16(at + 8 * L::kTok + (HW == 1 ? x : x ^ 16));
+          const u32x4 w = {lo[0], lo[1], hi[0], hi[1]};
+          acc[h][db] = mfma32x32x16(__builtin_bit_cast(bf16x8, w), p[h][j], acc[h][db]);
+        }
     wait_lds();
     __builtin_amdgcn_sched_barrier(0);
-    if (more) fetch(a.k, a.ks, k_off, b + 4, kt);
-    const float mx = mask_scores(s, kb, lim, kb + 32 > least, gone, lane);
-    grow(st, fmaf(halves_max(mx), c, -st.shift), acc);
-    if (more) wait_vm_lds<4>(); else wait_vm_lds<0>();
-    block_pv(s, st, c, vt, 0, lane, acc);
-    wait_lds();
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) fetch(a.v, a.vs, v_off, b + 4, vt);
+    if (more) few_fetch<HW>(a, a.v, a.vs, v_off, page, it.key0 + 32 * next, it.key1, head0, vt);
   }
-  wait_vm_lds<0>();
+  wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS
 
-  // merge the waves: states to LDS (16-byte pieces of a row swizzled by the row)
-  const float l = halves_sum(st.l0 + st.l1);
-  if (lane < 32) {
-    lm[wave][lane] = st.lag > 0.f ? st.shift : kNegInf;
-    ll[wave][lane] = l;
-  }
-  if ((lane & 31) < it.nrows) {
+  // the wave's states to LDS: row r of head h at (32 h + r) * 256 bytes, 16-byte
+  // pieces permuted by the row
 #pragma unroll
-    for (int db = 0; db < 2; ++db)
+  for (int h = 0; h < HW; ++h) {
+    const float l = halves_sum(st[h].l0 + st[h].l1);
+    if (lane < 32) {
+      lm[32 * h + lane] = st[h].lag > 0.f ? st[h].shift : kNegInf;
+      ll[32 * h + lane] = l;
+    }
+    if ((lane & 31) < it.nrows) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int piece = 8 * db + 2 * g + (lane >> 5);
-        f32x4 x;
+      for (int db = 0; db < 2; ++db)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = acc[db][4 * g + i];
-        *reinterpret_cast<f32x4*>(kt + (lane & 31) * 256 + ((piece ^ (lane & 15)) << 4)) = x;
-      }
-  }
-  __syncthreads();
-  const int r = threadIdx.x >> 3, d8 = threadIdx.x & 7;
-  if (r >= it.nrows) return;
-  float top = lm[0][r];
+        for (int g = 0; g < 4; ++g) {
+          const int piece = 8 * db + 2 * g + half;
+          f32x4 x;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, lm[w][r]);
-  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float wt = lm[w][r] == kNegInf ? 0.f : fast_exp2(lm[w][r] - top);
-    sum = fmaf(wt, ll[w][r], sum);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(lds + w * kWaveLds + r * 256 +
-                                                      (((2 * d8 + h) ^ (r & 15)) << 4));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[4 * h + i] = fmaf(wt, x[i], o[4 * h + i]);
+          for (int i = 0; i < 4; ++i) x[i] = acc[h][db][4 * g + i];
+          *reinterpret_cast<f32x4*>(wave_lds + (32 * h + (lane & 31)) * 256 +
+                                    ((piece ^ (lane & 15)) << 4)) = x;
+        }
     }
   }
-  if (it.partial < 0) {
-    const RowOf ro = row_of(a, it, r, kvh);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    bf16x8 y;
+}
+
+// Merges the waves' states of an item and writes rows or partial results; eight
+// threads a row.
+template <int HW>
+__device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it, int pair,
+                                          const char* lds, const float (*lm)[64],
+                                          const float (*ll)[64]) {
+  const int d8 = threadIdx.x & 7;
+  for (int x = threadIdx.x >> 3; x < HW * it.nrows; x += 8 * kKeyWaves) {
+    const int h = x >= it.nrows ? 1 : 0, r = x - h * it.nrows, at = 32 * h + r;
+    const int kvh = HW * pair + h;
+    float top = kNegInf;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (bf16)(sum > 0.f ? o[i] * inv : 0.f);
-    *reinterpret_cast<bf16x8*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2) + 16 * d8) = y;
-  } else {
-    const size_t at = ((size_t)it.partial + r) * a.Hkv + kvh;
-    f32x4 x, y;
+    for (int w = 0; w < kKeyWaves; ++w) top = fmaxf(top, lm[w][at]);
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = o[i], y[i] = o[4 + i];
-    *reinterpret_cast<f32x4*>(a.acc + at * kD + 8 * d8) = x;
-    *reinterpret_cast<f32x4*>(a.acc + at * kD + 8 * d8 + 4) = y;
-    if (d8 == 0) a.ml[at] = make_float2(top, sum);
+    for (int w = 0; w < kKeyWaves; ++w) {
+      const float m = lm[w][at];
+      const float wt = m == kNegInf ? 0.f : fast_exp2(m - top);
+      sum = fmaf(wt, ll[w][at], sum);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(lds + w * FewLds<HW>::kWave + at * 256 +
+                                                        (((2 * d8 + q) ^ (r & 15)) << 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[4 * q + i] = fmaf(wt, y[i], o[4 * q + i]);
+      }
+    }
+    if (it.partial < 0) {
+      const RowOf ro = row_of(a, it, r, kvh);
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      bf16x8 y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (bf16)(sum > 0.f ? o[i] * inv : 0.f);
+      *reinterpret_cast<bf16x8*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2) + 16 * d8) = y;
+    } else {
+      const size_t to = (size_t)(kvh * a.cap_rows) + it.partial + r;
+      f32x4 y, z;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = o[i], z[i] = o[4 + i];
+      *reinterpret_cast<f32x4*>(a.acc + to * kD + 8 * d8) = y;
+      *reinterpret_cast<f32x4*>(a.acc + to * kD + 8 * d8 + 4) = z;
+      if (d8 == 0) a.ml[to] = make_float2(top, sum);
+    }
   }
 }
 
 // --------------------------------------------------------------------------
-// Up to 128 rows: the waves split the rows.
+// Up to 256 rows: the waves split the rows, 64 (two 32-row blocks) each, so that
+// every K and V operand read from LDS feeds two MFMAs.
 // --------------------------------------------------------------------------
 constexpr int kSlotBytes = 2 * kTileBytes;  // 64 keys of K and of V
+constexpr int kSlots = 4;
 
-__device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it, int kvh,
-                                          char* lds, int (*lost)[4]) {
+__device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
+                                          int (*lost)[4]) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  const bool idle = 32 * wave >= it.nrows;
-  const int row = min(32 * wave + (lane & 31), it.nrows - 1);
-  bf16x8 qf[4];
-  load_query(a, row_of(a, it, row, kvh), lane, qf);
-  const int lim = idle ? 0 : row_limit(a, it, row);
-  // the rows' limits ascend
-  const int least = uniform(__builtin_amdgcn_readlane(lim, 0));
-  const int most = uniform(__builtin_amdgcn_readlane(lim, 31));
+  bf16x8 qf[2][4];
+  int lim[2], least = 0, most = 0;
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int row0 = 64 * wave + 32 * rb;
+    const int row = min(row0 + (lane & 31), it.nrows - 1);
+    load_query(a, row_of(a, it, row, kvh), lane, qf[rb]);
+    lim[rb] = row_limit(a, it, row);
+    // the rows' limits ascend
+    if (rb == 0) least = uniform(__builtin_amdgcn_readlane(lim[0], 0));
+    if (row0 < it.nrows) most = uniform(__builtin_amdgcn_readlane(lim[rb], 31));
+  }
   drain_memory();
 
-  const int chunk16 = ((lane & 7) ^ swz(lane >> 3)) * 16;
-  const uint32_t k_off = (uint32_t)((lane >> 3) * a.ks.slot) + chunk16;
-  const uint32_t v_off = (uint32_t)((lane >> 3) * a.vs.slot) + chunk16;
+  const int piece16 = ((lane & 7) ^ swz(lane >> 3)) * 16;
+  const uint32_t k_off = (uint32_t)((lane >> 3) * a.ks.slot) + piece16;
+  const uint32_t v_off = (uint32_t)((lane >> 3) * a.vs.slot) + piece16;
   const int* trow = a.table + it.sequence * a.table_stride;
   const int stages = (it.key1 - it.key0 + 63) >> 6;
-
-  f32x16 acc[2] = {zero16(), zero16()};
-  RowState st = {0.f, kNegInf, 0.f, 0.f};
-  const float c = a.scale_log2;
-  int page[2];  // of this wave's two groups of the stage that is fetched next
-  auto pages_of = [&](int s) {
+  f32x16 acc[2][2];
+  RowState st[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int id = page_of(a, trow, min(it.key0 + 64 * s + 8 * (wave + 4 * j), it.key1 - 1));
-      page[j] = (unsigned)id < (unsigned)a.pages ? id : -1;
-    }
+  for (int rb = 0; rb < 2; ++rb) {
+    acc[rb][0] = acc[rb][1] = zero16();
+    st[rb] = {0.f, kNegInf, 0.f, 0.f};
+  }
+  const float c = a.scale_log2, inv_c = 1.f / c;
+  float top[2] = {kNegInf, kNegInf};  // scores from which a row's shift moves
+
+  // the table's entries of this wave's two 8-key groups of the stage that is fetched
+  // next, checked when they are used (a check is a wait for the load)
+  int entry[2];
+  auto load_entries = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      entry[j] = page_of(a, trow, min(it.key0 + 64 * s + 8 * (wave + 4 * j), it.key1 - 1));
   };
   auto fetch = [&](int s) {
-    char* slot = lds + (s & 1) * kSlotBytes;
+    char* slot = lds + (s & (kSlots - 1)) * kSlotBytes;
+    int page[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      page[j] = (unsigned)entry[j] < (unsigned)a.pages ? entry[j] : -1;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int g = wave + 4 * j, key = it.key0 + 64 * s + 8 * g;
-      dma_keys8(a, a.k, a.ks, k_off, chunk16, page[j], key, it.key1, kvh, slot, 8 * g);
-      dma_keys8(a, a.v, a.vs, v_off, chunk16, page[j], key, it.key1, kvh, slot + kTileBytes, 8 * g);
+      const int pg = max(page[j], 0);
+      const char* kp = a.k + row_offset(a, a.ks, pg, key, kvh);
+      const char* vp = a.v + row_offset(a, a.vs, pg, key, kvh);
+      const uint32_t dst = uniform((int)lds_offset(slot + 8 * g * kRowBytes));
+      if (page[j] >= 0 && key + 8 <= it.key1) {
+        dma16(kp, k_off, dst);
+        dma16(vp, v_off, dst + kTileBytes);
+      } else {
+        const bool there = page[j] >= 0 && key + (lane >> 3) < it.key1;
+        const char* none = a.zeros + 16 * (lane & 7);
+        dma16_lane(there ? kp + k_off : none, dst);
+        dma16_lane(there ? vp + v_off : none, dst + kTileBytes);
+      }
     }
     // groups of this wave without a page: bit wave + 4 j
-    lost[s & 1][wave] = (page[0] < 0 ? 1 << wave : 0) | (page[1] < 0 ? 16 << wave : 0);
+    lost[s & (kSlots - 1)][wave] = (page[0] < 0 ? 1 << wave : 0) | (page[1] < 0 ? 16 << wave : 0);
   };
-  if (stages > 0) {
-    pages_of(0);
-    fetch(0);
-    if (stages > 1) pages_of(1);
-  }
-  for (int s = 0; s < stages; ++s) {
-    wait_vm_lds<0>();
-    barrier();
-    if (s + 1 < stages) {
-      fetch(s + 1);
-      if (s + 2 < stages) pages_of(s + 2);
+#pragma unroll
+  for (int s = 0; s < kSlots - 1; ++s)
+    if (s < stages) {
+      load_entries(s);
+      fetch(s);
     }
-    const int4 lo = *reinterpret_cast<const int4*>(lost[s & 1]);
+  if (kSlots - 1 < stages) load_entries(kSlots - 1);
+
+  const int tr_row = tr_row_of(lane), tr_col = tr_col_of(lane);
+  auto read_keys = [&](const char* kt, int k0, bf16x8 (&k)[4]) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) k[ks] = tile_chunk(kt, k0 + (lane & 31), 2 * ks + (lane >> 5));
+  };
+  // scores of one 32-key block for both row blocks
+  auto scores = [&](const bf16x8 (&k)[4], f32x16 (&out)[2]) {
+    out[0] = out[1] = zero16();
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      out[0] = mfma32x32x16(k[ks], qf[0][ks], out[0]);
+      out[1] = mfma32x32x16(k[ks], qf[1][ks], out[1]);
+    }
+  };
+  // One 32-key block: cur are its scores and mx their maxima; next and mx become
+  // those of the block whose keys are rows k0 .. of kn.  The next block's first
+  // product runs under this one's exponentials, its maxima under this one's second
+  // product: a wave alone keeps both pipes in use.  The operands of both are read
+  // first, under the check of the maxima.
+  auto step = [&](int kb, int gone, f32x16 (&cur)[2], f32x16 (&next)[2], float (&mx)[2],
+                  const char* kn, int k0, const char* vt, int v0) {
+    bf16x8 k[4], v[2][2];
+    read_keys(kn, k0, k);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < 2; ++db)
+        v[j][db] = tile_tr_operand(vt, v0 + 16 * j + tr_row, db * 32 + tr_col);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kb + 32 > least || gone) {
+      const int at = opaque(kb);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        mask_scores(cur[rb], at, lim[rb], gone, lane);
+        mx[rb] = column_max(cur[rb]);
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+      if (__any(mx[rb] > top[rb])) {
+        grow(st[rb], fmaf(halves_max(mx[rb]), c, -st[rb].shift), acc[rb]);
+        top[rb] = (st[rb].shift + st[rb].lag) * inv_c;
+      }
+    scores(k, next);
+    bf16x8 p[2][2];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) block_probs(cur[rb], st[rb], c, p[rb][0], p[rb][1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        acc[0][db] = mfma32x32x16(v[j][db], p[0][j], acc[0][db]);
+        acc[1][db] = mfma32x32x16(v[j][db], p[1][j], acc[1][db]);
+      }
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) mx[rb] = column_max(next[rb]);
+  };
+
+  f32x16 sa[2], sb[2];
+  float mx[2];
+  for (int s = 0; s < stages; ++s) {
+    // this wave's parts of stages s and s + 1 are there; the one behind may be on its way
+    if (s + 2 < stages) wait_vm_lds<4>(); else wait_vm_lds<0>();
+    barrier();
+    if (s + kSlots - 1 < stages) {
+      fetch(s + kSlots - 1);
+      if (s + kSlots < stages) load_entries(s + kSlots);
+    }
+    const int4 lo = *reinterpret_cast<const int4*>(lost[s & (kSlots - 1)]);
     const int gone = uniform(lo.x | lo.y | lo.z | lo.w);
-    const char* kt = lds + (s & 1) * kSlotBytes;
+    const char* kt = lds + (s & (kSlots - 1)) * kSlotBytes;
     const char* vt = kt + kTileBytes;
+    const char* kn = lds + ((s + 1) & (kSlots - 1)) * kSlotBytes;
     const int kb = it.key0 + 64 * s;
-    const bool run0 = kb < most, run1 = kb + 32 < most;
-    if (!run0) continue;
-    f32x16 s0 = block_scores(kt, 0, lane, qf), s1;
-    if (run1) s1 = block_scores(kt, 32, lane, qf);
-    float mx = mask_scores(s0, kb, lim, kb + 32 > least, gone & 15, lane);
-    if (run1) mx = fmaxf(mx, mask_scores(s1, kb + 32, lim, kb + 64 > least, gone >> 4, lane));
-    grow(st, fmaf(halves_max(mx), c, -st.shift), acc);
-    block_pv(s0, st, c, vt, 0, lane, acc);
-    if (run1) block_pv(s1, st, c, vt, 32, lane, acc);
+    if (kb >= most) continue;
+    if (s == 0) {
+      bf16x8 k[4];
+      read_keys(kt, 0, k);
+      scores(k, sa);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) mx[rb] = column_max(sa[rb]);
+    }
+    step(kb, gone & 15, sa, sb, mx, kt, 32, vt, 0);
+    // (behind the last stage the next block's scores are of whatever lies there, unused)
+    step(kb + 32, gone >> 4, sb, sa, mx, kn, 0, vt, 32);
   }
-  wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS at exit
+  wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS
 
   const int elane = fresh_lane_id();
-  const int half = elane >> 5, erow = 32 * wave + (elane & 31);
-  const float l = halves_sum(st.l0 + st.l1);
-  if (erow >= it.nrows) return;
+  const int half = elane >> 5;
   if (it.partial < 0) {
-    const RowOf ro = row_of(a, it, erow, kvh);
-    const bool has = l > 0.f;
-    store_bf16_rows(reinterpret_cast<bf16*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2)),
-                    acc, has ? 1.f / l : 0.f, has, half);
-  } else {
-    const size_t at = ((size_t)it.partial + erow) * a.Hkv + kvh;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      const int row = 64 * wave + 32 * rb + (elane & 31);
+      const float l = halves_sum(st[rb].l0 + st[rb].l1);
+      if (row >= it.nrows) continue;
+      const RowOf ro = row_of(a, it, row, kvh);
+      const bool has = l > 0.f;
+      store_bf16_rows(reinterpret_cast<bf16*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2)),
+                      acc[rb], has ? 1.f / l : 0.f, has, half);
+    }
+    return;
+  }
+  // Partial results go through LDS (16 KB of the ring a wave, 16-byte pieces of a row
+  // permuted by the row), so that a store covers four whole rows.
+  __syncthreads();  // every wave is done with the ring
+  char* rows = lds + wave * kSlotBytes;
+  const size_t first = (size_t)(kvh * a.cap_rows) + it.partial + 64 * wave;
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int r = 32 * rb + (elane & 31);
+    const float l = halves_sum(st[rb].l0 + st[rb].l1);
+    if (half == 0 && 64 * wave + r < it.nrows)
+      a.ml[first + r] = make_float2(st[rb].lag > 0.f ? st[rb].shift : kNegInf, l);
 #pragma unroll
     for (int db = 0; db < 2; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         f32x4 x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = acc[db][4 * g + i];
-        *reinterpret_cast<f32x4*>(a.acc + at * kD + 32 * db + 8 * g + 4 * half) = x;
+        for (int i = 0; i < 4; ++i) x[i] = acc[rb][db][4 * g + i];
+        *reinterpret_cast<f32x4*>(rows + r * 256 + (((8 * db + 2 * g + half) ^ (r & 15)) << 4)) = x;
       }
-    if (half == 0) a.ml[at] = make_float2(st.lag > 0.f ? st.shift : kNegInf, l);
+  }
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 4 * i + (elane >> 4), piece = elane & 15;
+    if (64 * wave + r < it.nrows)
+      *reinterpret_cast<f32x4*>(a.acc + (first + r) * kD + 4 * piece) =
+          *reinterpret_cast<const f32x4*>(rows + r * 256 + ((piece ^ (r & 15)) << 4));
   }
 }
 
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
+// Workgroups: the few-rows shares' (head pairs fastest) and the many-rows shares'
+// (KV heads fastest, so that with 8 of them each XCD's L2 holds one head's keys), in
+// turn 256 of each while there are both: one for every CU, so that a CU's two
+// workgroups are one that waits for memory and one that computes.
+template <int HW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_attn_bf16_kernel(PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * kSlotBytes];
-  __shared__ __attribute__((aligned(16))) float small[2][4][kFewRows];
-  static_assert(4 * kWaveLds <= sizeof(lds), "the waves' blocks fit the ring");
-  const int item = uniform(fast_div(blockIdx.x, a.div_hkv));
-  if (item >= ld_const(a.head, kHeadItems)) return;
-  const int kvh = uniform(blockIdx.x - item * a.Hkv);
-  const ItemView it = load_item(a, item);
-  if (it.nrows < 1) return;
-  if (it.nrows <= kFewRows)
-    few_rows(a, it, kvh, lds, small[0], small[1]);
-  else
-    many_rows(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(small));
+  __shared__ __attribute__((aligned(16))) char lds[kSlots * kSlotBytes];
+  __shared__ __attribute__((aligned(16))) float lm[4][64], ll[4][64];
+  static_assert(4 * FewLds<HW>::kWave <= sizeof(lds), "the waves' blocks fit the ring");
+  const int turn = blockIdx.x >> 8, both = 2 * min(a.few_turns, a.many_turns);
+  const bool few = turn < both ? !(turn & 1) : a.few_turns > a.many_turns;
+  const int block = (turn < both ? turn >> 1 : turn - both / 2) * 256 + (blockIdx.x & 255);
+  if (few) {
+    const int share = uniform(fast_div(block, a.div_pairs));
+    if (share >= ld_const(a.head, kHeadShares + kFew)) return;
+    const int pair = uniform(block - share * a.head_pairs);
+    const int wave = uniform(threadIdx.x >> 6);
+    const int end = ld_const(a.shares[kFew], share + 1);
+    for (int item = ld_const(a.shares[kFew], share); item < end; ++item) {
+      const ItemView it = load_item(a.items[kFew], item);
+      if (it.nrows < 1) continue;
+      few_rows<HW>(a, it, pair, wave, lds + wave * FewLds<HW>::kWave, lm[wave], ll[wave]);
+      __syncthreads();
+      few_merge<HW>(a, it, pair, lds, lm, ll);
+      __syncthreads();
+    }
+    return;
+  }
+  const int share = uniform(fast_div(block, a.div_hkv));
+  if (share >= ld_const(a.head, kHeadShares + kMany)) return;
+  const int kvh = uniform(block - share * a.Hkv);
+  const int end = ld_const(a.shares[kMany], share + 1);
+  for (int item = ld_const(a.shares[kMany], share); item < end; ++item) {
+    const ItemView it = load_item(a.items[kMany], item);
+    if (it.nrows < 1) continue;
+    many_rows(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(lm));
+    __syncthreads();
+  }
 }
 
 // --------------------------------------------------------------------------
 // fp32: always up to 32 rows; the waves split the keys (32x32x2 MFMAs, rows staged
 // through registers, as the packed fp32 forward).
 // --------------------------------------------------------------------------
-struct F32Keys {
-  f32x4 x[8];
-};
-
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-void paged_attn_f32_kernel(PagedArgs a) {
-  __shared__ F32Tile kt[4], vt[4], qt;
-  __shared__ float lm[4][32], ll[4][32];
-  const int item = uniform(fast_div(blockIdx.x, a.div_hkv));
-  if (item >= ld_const(a.head, kHeadItems)) return;
-  const int kvh = uniform(blockIdx.x - item * a.Hkv);
-  const ItemView it = load_item(a, item);
-  if (it.nrows < 1) return;
+__device__ __forceinline__ void f32_item(const PagedArgs& a, const ItemView& it, int kvh,
+                                         F32Tile (&kt)[4], F32Tile (&vt)[4], F32Tile& qt,
+                                         float (&lm)[4][32], float (&ll)[4][32]) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
   const int row = min(lane & 31, it.nrows - 1);
@@ -549,7 +763,8 @@ void paged_attn_f32_kernel(PagedArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = mfma32x32x2(kr[e], qr[e], s);
     }
-    const float mx = halves_max(mask_scores(s, kb, lim, kb + 32 > least, gone, lane));
+    if (kb + 32 > least || gone) mask_scores(s, kb, lim, gone, lane);
+    const float mx = halves_max(column_max(s));
     if (__any(mx > m)) {
       const float mnew = fmaxf(m, mx);
       const float alpha = mnew == kNegInf ? 1.f : fast_exp2((m - mnew) * c);
@@ -592,7 +807,7 @@ void paged_attn_f32_kernel(PagedArgs a) {
     wt[w] = lm[w][r] == kNegInf ? 0.f : fast_exp2(lm[w][r] - top);
     sum = fmaf(wt[w], ll[w][r], sum);
   }
-  const size_t at = ((size_t)max(it.partial, 0) + r) * a.Hkv + kvh;
+  const size_t at = (size_t)(kvh * a.cap_rows) + max(it.partial, 0) + r;
   const RowOf ro = row_of(a, it, r, kvh);
   const float inv = it.partial >= 0 ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
   float* dst = it.partial >= 0 ? a.acc + at * kD + d0
@@ -610,90 +825,119 @@ void paged_attn_f32_kernel(PagedArgs a) {
   if (it.partial >= 0 && d0 == 0) a.ml[at] = make_float2(top, sum);
 }
 
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void paged_attn_f32_kernel(PagedArgs a) {
+  __shared__ F32Tile kt[4], vt[4], qt;
+  __shared__ float lm[4][32], ll[4][32];
+  const int share = uniform(fast_div(blockIdx.x, a.div_hkv));
+  if (share >= ld_const(a.head, kHeadShares + kFew)) return;
+  const int kvh = uniform(blockIdx.x - share * a.Hkv);
+  const int end = ld_const(a.shares[kFew], share + 1);
+  for (int item = ld_const(a.shares[kFew], share); item < end; ++item) {
+    const ItemView it = load_item(a.items[kFew], item);
+    if (it.nrows < 1) continue;
+    f32_item(a, it, kvh, kt, vt, qt, lm, ll);
+    __syncthreads();
+  }
+}
+
 // --------------------------------------------------------------------------
 // Joins the items of split tiles, in item order: o = sum_i 2^(m_i - M) acc_i / sum_i
-// 2^(m_i - M) l_i.  A workgroup takes a tile of one KV head; eight threads of a
-// row take eight dims each, and where there are few rows, the rest of the
-// threads share the items.  Workgroups past the tiles zero the output rows that
-// belong to no sequence, where that is asked for.
+// 2^(m_i - M) l_i.  A workgroup takes up to eight rows of a tile for one KV head:
+// eight threads of a row take eight dims each, and the threads that are left
+// share the items, four at a time in flight.  Workgroups past the rows zero the
+// output rows that belong to no sequence, where that is asked for.
 // --------------------------------------------------------------------------
 template <bool F32>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  __shared__ float part[32][64];
+  __shared__ float part[32][68];
   __shared__ float2 pml[32];
-  if ((int)blockIdx.x >= a.tile_blocks) {
+  if ((int)blockIdx.x >= a.join_blocks) {
     const long long row = (long long)a.Hq * kD * (F32 ? 4 : 2);
     const long long end = ld_const(a.head, kHeadEnd) * row;
-    const long long at = (long long)(blockIdx.x - a.tile_blocks) * 16384;
+    const long long at = (long long)(blockIdx.x - a.join_blocks) * 16384;
     for (long long x = at + 16 * threadIdx.x; x < min(at + 16384, a.out_bytes); x += 16 * 256)
       if (x >= end) st_u32x4(a.out + x, u32x4{0, 0, 0, 0});
     return;
   }
   const int t = uniform(fast_div(blockIdx.x, a.div_hkv));
-  if (t >= ld_const(a.head, kHeadTiles)) return;
+  if (t >= ld_const(a.head, kHeadJoins)) return;
   const int kvh = uniform(blockIdx.x - t * a.Hkv);
-  const i32x8u tr = ld_const8(a.tiles, 8 * t);
+  const i32x8u j = ld_const8(a.joins, 8 * t);
   ItemView it = {};
-  it.start = tr[0];
-  it.row0 = tr[1];
-  it.nrows = tr[2];
-  const int partial = tr[3], splits = tr[4];
-  int rp = 1;  // rows a round takes
-  while (rp < it.nrows && rp < 32) rp <<= 1;
-  const int sp = 32 / rp;  // threads' groups that share a row's items
+  it.start = j[0];
+  it.row0 = j[1];
+  it.nrows = j[2];
+  const int partial = j[3], splits = j[4], step = j[5];
+  const int log_rp = it.nrows > 4 ? 3 : it.nrows > 2 ? 2 : it.nrows > 1 ? 1 : 0;
+  const int sp = 32 >> log_rp;  // threads' groups that share a row's items
   const int slot = threadIdx.x >> 3, d0 = 8 * (threadIdx.x & 7);
-  const int r = slot & (rp - 1), share = slot / rp;
-  for (int row0 = 0; row0 < it.nrows; row0 += rp) {
-    const int row = min(row0 + r, it.nrows - 1);
-    float m = kNegInf, l = 0.f, o[8];
+  const int r = slot & ((1 << log_rp) - 1), share = slot >> log_rp;
+  const int row = min(r, it.nrows - 1);
+  const size_t base = (size_t)(kvh * a.cap_rows) + partial + row;
+  float m = kNegInf, l = 0.f, o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = 0.f;
-    for (int s = share; s < splits; s += sp) {
-      const size_t at = ((size_t)partial + (size_t)s * it.nrows + row) * a.Hkv + kvh;
-      const float2 ml = a.ml[at];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.acc + at * kD + d0);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(a.acc + at * kD + d0 + 4);
-      const float top = fmaxf(m, ml.x);
-      const float wa = m == kNegInf ? 0.f : fast_exp2(m - top);
-      const float wb = ml.x == kNegInf ? 0.f : fast_exp2(ml.x - top);
-      l = l * wa + ml.y * wb;
+  for (int i = 0; i < 8; ++i) o[i] = 0.f;
+  for (int s0 = share; s0 < splits; s0 += 4 * sp) {
+    float2 ml[4];
+    f32x4 x[4], y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i] = o[i] * wa + x[i] * wb;
-        o[4 + i] = o[4 + i] * wa + y[i] * wb;
-      }
-      m = top;
+    for (int i = 0; i < 4; ++i) {
+      // (past the last item its results again, with no weight)
+      const size_t at = base + (size_t)min(s0 + i * sp, splits - 1) * step;
+      ml[i] = a.ml[at];
+      x[i] = *reinterpret_cast<const f32x4*>(a.acc + at * kD + d0);
+      y[i] = *reinterpret_cast<const f32x4*>(a.acc + at * kD + d0 + 4);
     }
-    __syncthreads();  // the previous round's readers are done
+    float top = m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) part[slot][d0 + i] = o[i];
-    if (d0 == 0) pml[slot] = make_float2(m, l);
-    __syncthreads();
-    if (share == 0 && row0 + r < it.nrows) {
-      float top = m;
-      for (int x = 1; x < sp; ++x) top = fmaxf(top, pml[x * rp + r].x);
-      float sum = 0.f, z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int x = 0; x < sp; ++x) {
-        const float2 ml = pml[x * rp + r];
-        const float w = ml.x == kNegInf ? 0.f : fast_exp2(ml.x - top);
-        sum = fmaf(w, ml.y, sum);
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i * sp >= splits) ml[i] = make_float2(kNegInf, 0.f);
+      top = fmaxf(top, ml[i].x);
+    }
+    const float wa = m == kNegInf ? 0.f : fast_exp2(m - top);
+    l *= wa;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = fmaf(w, part[x * rp + r][d0 + i], z[i]);
-      }
-      const RowOf ro = row_of(a, it, row, kvh);
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      const long long at = ((long long)ro.token * a.Hq + ro.head) * kD + d0;
-      if constexpr (F32) {
-        float* dst = reinterpret_cast<float*>(a.out) + at;
+    for (int i = 0; i < 8; ++i) o[i] *= wa;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = sum > 0.f ? z[i] * inv : 0.f;
-      } else {
-        bf16x8 y;
+    for (int i = 0; i < 4; ++i) {
+      const float w = ml[i].x == kNegInf ? 0.f : fast_exp2(ml[i].x - top);
+      l = fmaf(w, ml[i].y, l);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (bf16)(sum > 0.f ? z[i] * inv : 0.f);
-        *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(a.out) + at) = y;
+      for (int e = 0; e < 4; ++e) {
+        o[e] = fmaf(w, x[i][e], o[e]);
+        o[4 + e] = fmaf(w, y[i][e], o[4 + e]);
       }
     }
+    m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[slot][d0 + i] = o[i];
+  if (d0 == 0) pml[slot] = make_float2(m, l);
+  __syncthreads();
+  // thread = (row, two dims): the shares in order
+  const int er = threadIdx.x >> 5, e0 = 2 * (threadIdx.x & 31);
+  if (er >= it.nrows) return;
+  float top = kNegInf;
+  for (int x = 0; x < sp; ++x) top = fmaxf(top, pml[(x << log_rp) + er].x);
+  float sum = 0.f, z0 = 0.f, z1 = 0.f;
+  for (int x = 0; x < sp; ++x) {
+    const float2 ml = pml[(x << log_rp) + er];
+    const float w = ml.x == kNegInf ? 0.f : fast_exp2(ml.x - top);
+    sum = fmaf(w, ml.y, sum);
+    z0 = fmaf(w, part[(x << log_rp) + er][e0], z0);
+    z1 = fmaf(w, part[(x << log_rp) + er][e0 + 1], z1);
+  }
+  const RowOf ro = row_of(a, it, er, kvh);
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  z0 = sum > 0.f ? z0 * inv : 0.f;
+  z1 = sum > 0.f ? z1 * inv : 0.f;
+  const long long at = ((long long)ro.token * a.Hq + ro.head) * kD + e0;
+  if constexpr (F32) {
+    *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(z0, z1);
+  } else {
+    const bf16x2 y = {(bf16)z0, (bf16)z1};
+    *reinterpret_cast<bf16x2*>(reinterpret_cast<bf16*>(a.out) + at) = y;
   }
 }
 
@@ -714,8 +958,11 @@ hipError_t launch_paged_attn(const void* q, long long q_stride, const void* k_pa
   a.table = page_table;
   a.head = reinterpret_cast<const int*>(p);
   a.zeros = p + lay.zeros;
-  a.items = reinterpret_cast<const int*>(p + lay.items);
-  a.tiles = reinterpret_cast<const int*>(p + lay.tiles);
+  a.joins = reinterpret_cast<const int*>(p + lay.joins);
+  for (int k = 0; k < 2; ++k) {
+    a.shares[k] = reinterpret_cast<const int*>(p + lay.shares[k]);
+    a.items[k] = reinterpret_cast<const int*>(p + lay.items[k]);
+  }
   a.out = reinterpret_cast<char*>(out);
   a.ml = reinterpret_cast<float2*>(workspace);
   a.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) +
@@ -730,22 +977,30 @@ hipError_t launch_paged_attn(const void* q, long long q_stride, const void* k_pa
   a.Hq = Hq;
   a.Hkv = Hkv;
   a.G = Hq / Hkv;
-  a.zero_rest = zero_rest;
-  a.tile_blocks = lay.cap_tiles * Hkv;
+  a.cap_rows = (long long)lay.cap_rows;
+  a.head_pairs = Hkv / lay.head_pair;
+  const int few_blocks = lay.target[kFew] * a.head_pairs;
+  a.few_turns = (few_blocks + 255) / 256;
+  a.many_turns = (lay.target[kMany] * Hkv + 255) / 256;
+  a.join_blocks = lay.cap_joins * Hkv;
+  a.div_pairs = make_fastdiv(a.head_pairs);
   a.scale_log2 = scale * kLog2e;
   a.div_g = make_fastdiv(a.G);
   a.div_page = make_fastdiv(page_size);
   a.div_hkv = make_fastdiv(Hkv);
-  const dim3 grid((unsigned)lay.cap_items * Hkv);
   const long long rest = zero_rest ? (a.out_bytes + 16383) / 16384 : 0;
-  const dim3 join((unsigned)(a.tile_blocks + rest));
+  const dim3 join((unsigned)(a.join_blocks + rest));
   if (f32) {
-    hipLaunchKernelGGL(paged_attn_f32_kernel, grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(paged_attn_f32_kernel, dim3((unsigned)few_blocks), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(paged_join_kernel<true>, join, dim3(256), 0, stream, a);
-  } else {
-    hipLaunchKernelGGL(paged_attn_bf16_kernel, grid, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(paged_join_kernel<false>, join, dim3(256), 0, stream, a);
+    return hipGetLastError();
   }
+  const dim3 grid(256u * (unsigned)(a.few_turns + a.many_turns));
+  if (lay.head_pair == 2)
+    hipLaunchKernelGGL(paged_attn_bf16_kernel<2>, grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(paged_attn_bf16_kernel<1>, grid, dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(paged_join_kernel<false>, join, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -23,29 +23,35 @@ struct PlanArgs {
 };
 
 constexpr int kPlanThreads = 256;
-// A tile of many rows writes 33 KB of partial results per item and KV head:
-// its items are at least this many units.
-constexpr int kManyUnits = 4;
 
-// Inclusive prefix sum over the workgroup; `sum` gets the total.
-__device__ __forceinline__ int block_prefix(int x, int* lds, int& sum) {
+// Two counters that are summed together.
+struct Two {
+  int a, b;
+};
+
+// Exclusive prefix sums over the workgroup; `sum` gets the totals.
+__device__ __forceinline__ Two block_prefix(Two x, Two* lds, Two& sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Two y = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off);
-    if (lane >= off) x += y;
+    const int a = __shfl_up(y.a, off), b = __shfl_up(y.b, off);
+    if (lane >= off) y.a += a, y.b += b;
   }
-  __syncthreads();  // the previous round's readers are done
-  if (lane == 63) lds[wave] = x;
+  __syncthreads();  // the previous call's readers are done
+  if (lane == 63) lds[wave] = y;
   __syncthreads();
-  int before = 0;
-  sum = 0;
+  y.a -= x.a;
+  y.b -= x.b;
+  sum = {0, 0};
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) before += lds[w];
-    sum += lds[w];
+    const Two t = lds[w];
+    if (w < wave) y.a += t.a, y.b += t.b;
+    sum.a += t.a;
+    sum.b += t.b;
   }
-  return x + before;
+  return y;
 }
 
 struct Span {
@@ -54,39 +60,61 @@ struct Span {
 
 __device__ __forceinline__ Span span_of(const PlanArgs& a, int r) {
   Span s;
-  s.start = min(max(a.starts[r], 0), a.N);
-  s.count = max(min(max(a.starts[r + 1], 0), a.N) - s.start, 0);
-  const long long reach = (long long)a.width * a.page_size;
-  s.context = (int)min((long long)max(a.contexts[r], 0), min(reach, (long long)INT32_MAX));
+  const int start = a.starts[r], next = a.starts[r + 1], context = a.contexts[r];
+  s.start = min(max(start, 0), a.N);
+  s.count = max(min(max(next, 0), a.N) - s.start, 0);
+  s.context = min(max(context, 0), a.width * a.page_size);  // (at most 2^30)
   return s;
 }
 
-__device__ __forceinline__ int tile_rows_of(const PlanArgs& a, long long rows) {
-  return a.f32 || rows <= kFewRows ? kFewRows : kManyRows;
-}
-
-// Tile `t` of sequence r: its rows and the keys that its last row sees.
-struct TileSpan {
-  Span s;
-  int r, row0, nrows, keys, units;
+// A tile: its rows, the keys that its last row sees and those in units; where its
+// kind's units stand before it; its items (the first one's place, their number) and
+// its first partial row.
+struct Tile {
+  int sequence, start, row0, nrows, base, keys, units, kind;
+  int unit0, item0, items, row;
 };
 
-__device__ __forceinline__ TileSpan tile_of(const PlanArgs& a, const int* pre, int t) {
-  TileSpan x;
-  int lo = 0, hi = a.R - 1;  // last r with pre[r] <= t
+// Workgroup 0's sequences, so that each is read once, and a round's tiles.
+struct PlanLds {
+  int tiles[kMaxSequences];  // tiles before each sequence
+  int start[kMaxSequences], count[kMaxSequences], context[kMaxSequences];
+  Two sums[kPlanThreads / 64];
+  unsigned long long work[2];
+  int item_at[kPlanThreads], join_at[kPlanThreads];  // before each tile of the round
+  Tile tile[kPlanThreads];
+};
+
+// The last of `n` ascending entries that is at most x.
+__device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= t) lo = mid; else hi = mid - 1;
+    if (at[mid] <= x) lo = mid; else hi = mid - 1;
   }
-  x.r = lo;
-  x.s = span_of(a, lo);
-  const long long rows = (long long)x.s.count * a.G;
-  const int tr = tile_rows_of(a, rows);
-  x.row0 = (t - pre[lo]) * tr;
+  return lo;
+}
+
+__device__ __forceinline__ bool is_few(const PlanArgs& a, long long rows) {
+  return a.f32 || rows <= kFewRows;
+}
+
+__device__ __forceinline__ Tile tile_of(const PlanArgs& a, const PlanLds& l, int t) {
+  Tile x = {};
+  const int r = last_not_above(l.tiles, a.R, t);
+  x.sequence = r;
+  x.start = l.start[r];
+  const int count = l.count[r], context = l.context[r];
+  const long long rows = (long long)count * a.G;
+  x.kind = is_few(a, rows) ? kFew : kMany;
+  const int tr = x.kind == kFew ? kFewRows : kManyRows;
+  x.row0 = (t - l.tiles[r]) * tr;
   x.nrows = (int)max(min((long long)tr, rows - x.row0), 0ll);
   const int last = fast_div(x.row0 + max(x.nrows, 1) - 1, a.div_g);  // token of the last row
-  x.keys = max(min(x.s.context - x.s.count + last + 1, x.s.context), 0);
-  x.units = (x.keys + kUnitKeys - 1) / kUnitKeys;
+  x.base = context - count;
+  x.keys = max(min(x.base + last + 1, context), 0);
+  const int unit = x.kind == kFew ? kFewKeys : kManyKeys;
+  x.units = (x.keys + unit - 1) / unit;
   return x;
 }
 
@@ -95,99 +123,146 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     const int t = (blockIdx.x - 1) * kPlanThreads + threadIdx.x;
     if (t >= a.N) return;
     PagedToken rec = {0, -1, 0, -1};
-    int lo = 0, hi = a.R - 1;  // last r with starts[r] <= t
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.starts[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    const Span s = span_of(a, lo);
+    const int r = last_not_above(a.starts, a.R, t);
+    const Span s = span_of(a, r);
     if (t >= s.start && t < s.start + s.count) {
       rec.position = s.context - s.count + (t - s.start);
-      rec.sequence = lo;
+      rec.sequence = r;
       if (rec.position >= 0) {
         const int p = fast_div(rec.position, a.div_page);
         rec.slot = rec.position - p * a.page_size;
-        const int page = a.table[(long long)lo * a.table_stride + p];
+        const int page = a.table[(long long)r * a.table_stride + p];
         rec.page = page >= 0 && page < a.pages ? page : -1;
       }
     }
     reinterpret_cast<PagedToken*>(a.plan + a.lay.tokens)[t] = rec;
     return;
   }
-  __shared__ int pre[kMaxSequences + 1];
-  __shared__ int sums[kPlanThreads / 64];
-  __shared__ unsigned long long work;
-  if (threadIdx.x < 64) reinterpret_cast<int*>(a.plan + a.lay.zeros)[threadIdx.x] = 0;
-  if (threadIdx.x == 0) work = 0;
+  __shared__ PlanLds l;
+  const int tid = threadIdx.x;
+  if (tid < 64) reinterpret_cast<int*>(a.plan + a.lay.zeros)[tid] = 0;
+  if (tid < 2) l.work[tid] = 0;
   // tiles before every sequence
-  int carry = 0;
+  int ntiles = 0;
   for (int r0 = 0; r0 < a.R; r0 += kPlanThreads) {
-    const int r = r0 + threadIdx.x;
+    const int r = r0 + tid;
     int tiles = 0;
     if (r < a.R) {
-      const long long rows = (long long)span_of(a, r).count * a.G;
-      const int tr = tile_rows_of(a, rows);
+      const Span s = span_of(a, r);
+      const long long rows = (long long)s.count * a.G;
+      const int tr = is_few(a, rows) ? kFewRows : kManyRows;
       tiles = (int)((rows + tr - 1) / tr);
+      l.start[r] = s.start;
+      l.count[r] = s.count;
+      l.context[r] = s.context;
     }
-    int sum;
-    const int incl = block_prefix(tiles, sums, sum);
-    if (r < a.R) pre[r] = carry + incl - tiles;
-    carry += sum;
+    Two sum;
+    const Two before = block_prefix({tiles, 0}, l.sums, sum);
+    if (r < a.R) l.tiles[r] = ntiles + before.a;
+    ntiles += sum.a;
   }
-  const int ntiles = min(carry, a.lay.cap_tiles);
+  ntiles = min(ntiles, a.lay.cap_tiles);
   __syncthreads();
-  // units of keys over all tiles
-  unsigned long long mine = 0;
-  for (int t = threadIdx.x; t < ntiles; t += kPlanThreads) mine += tile_of(a, pre, t).units;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off);
-  if ((threadIdx.x & 63) == 0) atomicAdd(&work, mine);  // (integers: any order)
-  __syncthreads();
-  const int target = a.lay.target;
-  const int chunk = (int)max((work + target - 1) / target, 1ull);
-  int items = 0, split_tiles = 0, rows = 0;
-  PagedItem* item = reinterpret_cast<PagedItem*>(a.plan + a.lay.items);
-  PagedTile* tile = reinterpret_cast<PagedTile*>(a.plan + a.lay.tiles);
-  for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
-    const int t = t0 + threadIdx.x;
-    TileSpan x = {};
-    int splits = 0;
+  // units of keys over the tiles of each kind (below 2^31: the entry point checks
+  // tiles times the table's reach)
+  unsigned long long mine[2] = {0, 0};
+  Tile x = {};  // the thread's tile of the round (of the first round before it starts)
+  for (int t = (ntiles - 1) / kPlanThreads * kPlanThreads + tid; t >= 0; t -= kPlanThreads)
     if (t < ntiles) {
-      x = tile_of(a, pre, t);
-      const int c = !a.f32 && x.nrows > kFewRows ? max(chunk, kManyUnits) : chunk;
-      splits = max((x.units + c - 1) / c, 1);
+      x = tile_of(a, l, t);
+      mine[0] += x.kind == kFew ? x.units : 0;
+      mine[1] += x.kind == kMany ? x.units : 0;
     }
-    int sum_items, sum_tiles, sum_rows;
-    const int at = items + block_prefix(splits, sums, sum_items) - splits;
-    const int split = splits > 1;
-    const int at_tile = split_tiles + block_prefix(split, sums, sum_tiles) - split;
-    const int need = split ? splits * x.nrows : 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mine[k] += __shfl_xor(mine[k], off);
+    if ((tid & 63) == 0 && mine[k]) atomicAdd(&l.work[k], mine[k]);  // (integers: any order)
+  }
+  __syncthreads();
+  // units of a share
+  const int target[2] = {a.lay.target[0], max(a.lay.target[1], 1)};
+  const int share[2] = {max((int)((l.work[0] + target[0] - 1) / target[0]), 1),
+                        max((int)((l.work[1] + target[1] - 1) / target[1]), kManyUnits)};
+  int* shares[2] = {reinterpret_cast<int*>(a.plan + a.lay.shares[0]),
+                    reinterpret_cast<int*>(a.plan + a.lay.shares[1])};
+  PagedItem* items[2] = {reinterpret_cast<PagedItem*>(a.plan + a.lay.items[0]),
+                         reinterpret_cast<PagedItem*>(a.plan + a.lay.items[1])};
+  PagedJoin* joins = reinterpret_cast<PagedJoin*>(a.plan + a.lay.joins);
+  Two units = {0, 0}, nitems = {0, 0}, nrest = {0, 0};  // by kind; by kind; joins and partial rows
+  for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
+    if (t0 > 0) x = t0 + tid < ntiles ? tile_of(a, l, t0 + tid) : Tile{};
+    const bool live = t0 + tid < ntiles, few = x.kind == kFew;
+    const int c = few ? share[0] : share[1];
+    Two sum, before;
+    before = block_prefix({live && few ? x.units : 0, live && !few ? x.units : 0}, l.sums, sum);
+    x.unit0 = few ? units.a + before.a : units.b + before.b;
+    units.a += sum.a;
+    units.b += sum.b;
+    x.items = !live ? 0 : x.units == 0 ? 1 : (x.unit0 + x.units - 1) / c - x.unit0 / c + 1;
+    before = block_prefix({few ? x.items : 0, few ? 0 : x.items}, l.sums, sum);
+    const int round_items = sum.a + sum.b;
+    l.item_at[tid] = before.a + before.b;
+    x.item0 = few ? nitems.a + before.a : nitems.b + before.b;
+    nitems.a += sum.a;
+    nitems.b += sum.b;
+    const bool split = x.items > 1;
+    before = block_prefix({split ? (x.nrows + kJoinRows - 1) / kJoinRows : 0,
+                           split ? x.items * x.nrows : 0}, l.sums, sum);
+    const int round_joins = sum.a;
+    l.join_at[tid] = before.a;
     // (overlapping sequences, which no caller should make, could need more rows
     // than there are: they share the first ones)
-    int at_rows = rows + block_prefix(need, sums, sum_rows) - need;
-    if ((size_t)at_rows + need > a.lay.cap_rows) at_rows = 0;
-    for (int i = 0; i < splits; ++i) {
-      if (at + i >= a.lay.cap_items) break;
+    x.row = nrest.b + before.b;
+    if ((size_t)x.row + (size_t)x.items * x.nrows > a.lay.cap_rows) x.row = 0;
+    l.tile[tid] = x;
+    __syncthreads();
+    const int round = min(ntiles - t0, kPlanThreads);
+    for (int i = tid; i < round_items; i += kPlanThreads) {
+      const int j = last_not_above(l.item_at, round, i);
+      const Tile y = l.tile[j];
+      const int k = i - l.item_at[j], per = y.kind == kFew ? share[0] : share[1];
+      const int unit = y.kind == kFew ? kFewKeys : kManyKeys;
+      // (a tile without keys goes with the unit before it)
+      const int s = y.units > 0 ? y.unit0 / per + k : max(y.unit0 - 1, 0) / per;
       PagedItem it;
-      it.start = x.s.start;
-      it.row0 = x.row0;
-      it.nrows = x.nrows;
-      it.base = x.s.context - x.s.count;
-      it.key0 = (int)((long long)x.units * i / splits) * kUnitKeys;
-      it.key1 = min((int)((long long)x.units * (i + 1) / splits) * kUnitKeys, x.keys);
-      it.partial = split ? at_rows + i * x.nrows : -1;
-      it.sequence = x.r;
-      item[at + i] = it;
+      it.start = y.start;
+      it.row0 = y.row0;
+      it.nrows = y.nrows;
+      it.base = y.base;
+      it.key0 = k == 0 ? 0 : (s * per - y.unit0) * unit;
+      it.key1 = k == y.items - 1 ? y.keys : ((s + 1) * per - y.unit0) * unit;
+      it.partial = y.items > 1 ? y.row + k * y.nrows : -1;
+      it.sequence = y.sequence;
+      const int at = y.item0 + k;
+      if (at < a.lay.cap_items[y.kind]) items[y.kind][at] = it;
+      // is it the first item of its share?
+      if (k > 0 || at == 0 || (y.units > 0 && y.unit0 > 0 && (y.unit0 - 1) / per != s))
+        if (s < a.lay.target[y.kind]) shares[y.kind][s] = at;
     }
-    if (split) tile[at_tile] = PagedTile{x.s.start, x.row0, x.nrows, at_rows, splits, {0, 0, 0}};
-    items += sum_items;
-    split_tiles += sum_tiles;
-    rows += sum_rows;
+    for (int i = tid; i < round_joins; i += kPlanThreads) {
+      const int j = last_not_above(l.join_at, round, i);
+      const Tile y = l.tile[j];
+      const int r0 = (i - l.join_at[j]) * kJoinRows;
+      if (nrest.a + i < a.lay.cap_joins)
+        joins[nrest.a + i] = PagedJoin{y.start, y.row0 + r0, min(y.nrows - r0, kJoinRows),
+                                       y.row + r0, y.items, y.nrows, {0, 0}};
+    }
+    __syncthreads();
+    nrest.a += sum.a;
+    nrest.b += sum.b;
   }
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     int* head = reinterpret_cast<int*>(a.plan);
-    head[kHeadItems] = min(items, a.lay.cap_items);
-    head[kHeadTiles] = split_tiles;
+    const int all_units[2] = {units.a, units.b}, all_items[2] = {nitems.a, nitems.b};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int used = min(all_units[k] > 0 ? (all_units[k] - 1) / share[k] + 1 : all_items[k] > 0,
+                           a.lay.target[k]);
+      head[kHeadShares + k] = used;
+      shares[k][used] = min(all_items[k], a.lay.cap_items[k]);
+    }
+    head[kHeadJoins] = min(nrest.a, a.lay.cap_joins);
     head[kHeadEnd] = min(max(a.starts[a.R], 0), a.N);
   }
 }

@@ -33,12 +33,17 @@ from .rotary import Rotary
 class Plan:
     """One step's new tokens and work items on the device, for every layer of the step."""
 
+    __slots__ = ("buf", "page_table", "sequences", "tokens", "query_heads", "kv_heads", "pages",
+                 "page_size", "pool", "code", "nbytes", "q_shape", "k_shape", "table_stride", "width")
+
     def __init__(self, buf, page_table, sequences, tokens, query_heads, pool, code):
         self.buf, self.page_table = buf, page_table
         self.sequences, self.tokens, self.query_heads = sequences, tokens, query_heads
-        self.pages, self.page_size, self.kv_heads, _ = pool
-        self.pool, self.code = pool, code
-        self.nbytes = buf.numel()
+        self.pages, self.page_size, self.kv_heads, d = pool
+        self.pool, self.code, self.nbytes = pool, code, buf.numel()
+        self.q_shape, self.k_shape = (tokens, query_heads, d), (tokens, self.kv_heads, d)
+        self.width = page_table.shape[1]
+        self.table_stride = page_table.stride(0) if sequences > 1 else self.width
 
     def token_records(self) -> torch.Tensor:
         """``[tokens, 4]`` int32: position, page (negative: none), slot and sequence of each."""
@@ -46,23 +51,32 @@ class Plan:
 
 
 @functools.lru_cache(maxsize=256)
-def _strides(page: int, slot: int, head: int):
-    return (ctypes.c_longlong * 3)(page, slot, head)
-
-
-def _pool_strides(pages: torch.Tensor):
-    page, slot, head, last = pages.stride()
-    p, s, h, d = pages.shape
-    # a dimension of one is never stepped over
-    if last != 1 and d > 1:
+def _pool_strides(strides: tuple[int, ...], shape: tuple[int, ...]):
+    """The C ABI's (page, slot, head) strides; a dimension of one is never stepped over."""
+    if strides[3] != 1 and shape[3] > 1:
         raise ValueError("the pages' last dimension must be dense")
-    return _strides(page if p > 1 else 0, slot if s > 1 else 0, head if h > 1 else 0)
+    return (ctypes.c_longlong * 3)(*(s if n > 1 else 0 for s, n in zip(strides[:3], shape)))
 
 
 def _check_pool(key_pages: torch.Tensor, value_pages: torch.Tensor, plan: Plan) -> None:
     if key_pages.shape != plan.pool or value_pages.shape != plan.pool:
         raise ValueError(f"the plan is for pages {list(plan.pool)}, the call has "
                          f"{list(key_pages.shape)} and {list(value_pages.shape)}")
+
+
+def _records_grad(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _gain(gain: torch.Tensor | None, dtype: torch.dtype, d: int) -> torch.Tensor | None:
+    if gain is None:
+        return None
+    if gain.shape != (d,):
+        raise ValueError(f"gains must be [{d}], got {list(gain.shape)}")
+    return gain if gain.dtype is dtype and gain.is_contiguous() else gain.to(dtype).contiguous()
 
 
 def _int32(x: torch.Tensor, shape: tuple[int, ...], what: str) -> torch.Tensor:
@@ -127,54 +141,51 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     (their query is still returned).  float32 arithmetic, one rounding.  Pages
     that several sequences share must not be appended to.  Forward only.
     """
-    tensors = [t for t in (key, value, key_pages, value_pages, query, query_gain, key_gain)
-               if t is not None]
-    code = plan.code
     dtype = key_pages.dtype
-    for t in tensors[:4 if query is None else 5]:
+    for t in (key, value, value_pages) if query is None else (query, key, value, value_pages):
         if t.dtype is not dtype:
             raise ValueError(f"queries, keys, values and pages must share one dtype (got {dtype} "
                              f"and {t.dtype})")
-    if dtype_code(key_pages) != code:
+    code = dtype_code(key_pages)
+    if code != plan.code:
         raise ValueError("the plan is for pages of another dtype")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and _records_grad(key, value, key_pages, value_pages, query,
+                                                 query_gain, key_gain):
         raise ValueError("paged.append has no backward; call it under torch.no_grad()")
     _check_pool(key_pages, value_pages, plan)
-    n, d = plan.tokens, _lib.HEAD_DIM
-    if key.shape != (n, plan.kv_heads, d) or value.shape != key.shape:
-        raise ValueError(f"keys and values must be {[n, plan.kv_heads, d]}, got "
+    if key.shape != plan.k_shape or value.shape != plan.k_shape:
+        raise ValueError(f"keys and values must be {list(plan.k_shape)}, got "
                          f"{list(key.shape)} and {list(value.shape)}")
-    if query is not None and query.shape != (n, plan.query_heads, d):
-        raise ValueError(f"the query must be {[n, plan.query_heads, d]}, got {list(query.shape)}")
-    if query is None and query_gain is not None:
-        raise ValueError("query_gain needs a query")
-    for gain in (query_gain, key_gain):
-        if gain is not None and gain.shape != (d,):
-            raise ValueError(f"gains must be [{d}], got {list(gain.shape)}")
-    if rotary is not None and (not isinstance(rotary, Rotary) or rotary.head_dim != d):
+    if query is None:
+        if query_gain is not None:
+            raise ValueError("query_gain needs a query")
+    elif query.shape != plan.q_shape:
+        raise ValueError(f"the query must be {list(plan.q_shape)}, got {list(query.shape)}")
+    n, _, d = plan.k_shape
+    qg, kg = _gain(query_gain, dtype, d), _gain(key_gain, dtype, d)
+    if rotary is None:
+        turn = (None, 0, 0, 1.0)
+    elif not isinstance(rotary, Rotary) or rotary.head_dim != d:
         raise ValueError(f"rotary must be a Rotary of heads of {d}")
+    else:
+        turn = rotary._turn
     if key_pages.data_ptr() == value_pages.data_ptr():
         raise ValueError("keys and values need pages of their own")
-    device = require_device(key_pages, plan.buf, *tensors)
-    kg = None if key_gain is None else key_gain.to(dtype).contiguous()
-    qg = None if query_gain is None else query_gain.to(dtype).contiguous()
+    device = require_device(key_pages, plan.buf, key, value, value_pages,
+                            *(t for t in (query, qg, kg) if t is not None))
     key, k_step = token_rows(key)
     value, v_step = token_rows(value)
     out, q_step = None, 0
     if query is not None:
         query, q_step = token_rows(query)
-        out = torch.empty((n, plan.query_heads, d), dtype=dtype, device=device)
-    if rotary is None:
-        turn = (None, 0, 0, 1.0)
-    else:
-        turn = (rotary._array, rotary.rotary_dim, rotary.interleaved, rotary.magnitude)
+        out = torch.empty(plan.q_shape, dtype=dtype, device=device)
     with on_device(device):
         _lib.check(_lib.LIB.mf_paged_append(
             _ptr(query), q_step, key.data_ptr(), k_step, value.data_ptr(), v_step, _ptr(qg),
             _ptr(kg), eps, *turn, code, n, plan.sequences, plan.query_heads, plan.kv_heads, d,
             plan.page_size, plan.pages, plan.buf.data_ptr(), plan.nbytes, key_pages.data_ptr(),
-            value_pages.data_ptr(), _pool_strides(key_pages), _pool_strides(value_pages),
-            _ptr(out), _raw_stream(device.index)))
+            value_pages.data_ptr(), _pool_strides(key_pages.stride(), plan.pool),
+            _pool_strides(value_pages.stride(), plan.pool), _ptr(out), _raw_stream(device.index)))
     return out
 
 
@@ -189,10 +200,9 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     are in an ``out`` that is given.  Slots behind a context may hold anything.
     Forward only; the same inputs give the same bits.
     """
-    n, hq, d = plan.tokens, plan.query_heads, _lib.HEAD_DIM
-    if query.shape != (n, hq, d):
-        raise ValueError(f"the query must be {[n, hq, d]}, got {list(query.shape)}")
-    dtype = query.dtype
+    shape, dtype = plan.q_shape, query.dtype
+    if query.shape != shape:
+        raise ValueError(f"the query must be {list(shape)}, got {list(query.shape)}")
     if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
         raise ValueError(f"query and pages must share one dtype (got {dtype}, {key_pages.dtype} "
                          f"and {value_pages.dtype})")
@@ -200,29 +210,29 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     if code != plan.code:
         raise ValueError("the plan is for pages of another dtype")
     _check_pool(key_pages, value_pages, plan)
-    if torch.is_grad_enabled() and (query.requires_grad or key_pages.requires_grad
-                                    or value_pages.requires_grad):
+    if torch.is_grad_enabled() and _records_grad(query, key_pages, value_pages):
         raise ValueError("paged.attention has no backward; call it under torch.no_grad()")
     device = require_device(query, key_pages, value_pages, plan.buf)
     query, q_step = token_rows(query)
     zero_rest = out is None
     if zero_rest:
-        out = torch.empty((n, hq, d), dtype=dtype, device=device)
-    elif (out.shape != (n, hq, d) or out.dtype is not dtype or not out.is_contiguous()
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif (out.shape != shape or out.dtype is not dtype or not out.is_contiguous()
           or out.device != device):
-        raise ValueError(f"out must be a contiguous {dtype} {[n, hq, d]} on {device}")
+        raise ValueError(f"out must be a contiguous {dtype} {list(shape)} on {device}")
+    n, hq, d = shape
     lib = _lib.LIB
     ws_bytes = lib.mf_paged_attn_workspace_bytes(plan.sequences, n, hq, plan.kv_heads, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    table = plan.page_table
     with on_device(device):
         _lib.check(lib.mf_paged_attn(
             query.data_ptr(), q_step, key_pages.data_ptr(), value_pages.data_ptr(),
-            _pool_strides(key_pages), _pool_strides(value_pages), table.data_ptr(),
-            table.stride(0) if plan.sequences > 1 else table.shape[1], code, n, plan.sequences,
-            table.shape[1], plan.page_size, plan.pages, hq, plan.kv_heads, d,
-            d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes, zero_rest,
-            out.data_ptr(), ws.data_ptr(), ws_bytes, _raw_stream(device.index)))
+            _pool_strides(key_pages.stride(), plan.pool),
+            _pool_strides(value_pages.stride(), plan.pool), plan.page_table.data_ptr(),
+            plan.table_stride, code, n, plan.sequences, plan.width, plan.page_size, plan.pages, hq,
+            plan.kv_heads, d, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(),
+            plan.nbytes, zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes,
+            _raw_stream(device.index)))
     return out
 
 

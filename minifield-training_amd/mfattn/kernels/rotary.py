@@ -82,7 +82,8 @@ class Rotary:
             raise ValueError("frequencies and magnitude must be finite")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, r, bool(interleaved)
         self.frequencies, self.magnitude = tuple(freqs), float(magnitude)
-        self._array = (ctypes.c_double * len(freqs))(*freqs)  # the C ABI's host array
+        # the C ABI's arguments: host array, rotary_dim, interleaved, magnitude
+        self._turn = ((ctypes.c_double * len(freqs))(*freqs), r, int(self.interleaved), self.magnitude)
 
     def __repr__(self) -> str:
         return (f"Rotary(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, "
@@ -113,18 +114,24 @@ def _scaled(r, theta, scaling, factor, length, fast, slow) -> list[float]:
 def _launch(q, k, positions, rotary, backward):
     """Rotates q and k ([B, T, H, D] or [N, H, D], either None) into new dense tensors."""
     one = q if q is not None else k
-    shape, device = one.shape, one.device
-    tokens, seq_len = (shape[0] * shape[1], shape[1]) if one.dim() == 4 else (shape[0], shape[0])
-    q, q_stride = (None, 0) if q is None else token_rows(q)
-    k, k_stride = (None, 0) if k is None else token_rows(k)
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    shape, dtype, device = one.shape, one.dtype, one.device
+    tokens, seq_len = (shape[0] * shape[1], shape[1]) if len(shape) == 4 else (shape[0], shape[0])
+    qp = kp = qo = ko = q_out = k_out = None
+    hq = hkv = q_stride = k_stride = 0
+    if q is not None:
+        q, q_stride = token_rows(q)
+        q_out = torch.empty(q.shape, dtype=dtype, device=device)
+        hq, qp, qo = q.shape[-2], q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        k, k_stride = token_rows(k)
+        k_out = torch.empty(k.shape, dtype=dtype, device=device)
+        hkv, kp, ko = k.shape[-2], k.data_ptr(), k_out.data_ptr()
+    array, rotary_dim, interleaved, magnitude = rotary._turn
     with on_device(device):
         _lib.check(_lib.LIB.mf_rotate(
-            _ptr(q), q_stride, _ptr(k), k_stride, _ptr(positions), rotary._array, dtype_code(one),
-            tokens, seq_len, 0 if q is None else q.shape[-2], 0 if k is None else k.shape[-2],
-            rotary.head_dim, rotary.rotary_dim, rotary.interleaved, rotary.magnitude, backward,
-            _ptr(q_out), _ptr(k_out), _raw_stream(device.index)))
+            qp, q_stride, kp, k_stride, _ptr(positions), array, dtype_code(one), tokens, seq_len, hq,
+            hkv, rotary.head_dim, rotary_dim, interleaved, magnitude, backward, qo, ko,
+            _raw_stream(device.index)))
     return q_out, k_out
 
 

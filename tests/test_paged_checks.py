@@ -225,7 +225,7 @@ PAGED = [
     (dict(n=0), _lib.ERR_INVALID_ARGUMENT, "positive"),
     (dict(r=5000), _lib.ERR_SHAPE, "4096 sequences"),
     (dict(hq=3), _lib.ERR_HEADS, "divisible"),
-    (dict(n=1 << 27, hq=4), _lib.ERR_SHAPE, "2^28"),
+    (dict(n=1 << 25, hq=4), _lib.ERR_SHAPE, "2^26"),
     (dict(hq=2048, hkv=2048), _lib.ERR_SHAPE, "1024"),
     (dict(ps=12), _lib.ERR_SHAPE, "multiple of 8"),
     (dict(ps=0), _lib.ERR_INVALID_ARGUMENT, "positive"),
@@ -240,6 +240,7 @@ PAGED = [
     (dict(width=0), _lib.ERR_SHAPE, "max_pages"),
     (dict(stride=7), _lib.ERR_SHAPE, "max_pages"),
     (dict(width=1 << 27, stride=1 << 27), _lib.ERR_SHAPE, "2^30"),
+    (dict(r=4096, width=1 << 24, stride=1 << 24, ps=64), _lib.ERR_SHAPE, "too many for one step"),
     (dict(starts=None), _lib.ERR_INVALID_ARGUMENT, "non-null"),
     (dict(table=None), _lib.ERR_INVALID_ARGUMENT, "non-null"),
 ])
@@ -271,6 +272,7 @@ def _append(**kw):
     (dict(vst=_strides(2048, 128, 0)), _lib.ERR_SHAPE, "overlap"),
     (dict(vst=_strides(-2048, 128, 64)), _lib.ERR_SHAPE, "overlap"),
     (dict(vst=_strides(2048, 1 << 27, 64)), _lib.ERR_SHAPE, "2^26"),
+    (dict(kst=_strides(2048, 128, 1 << 30)), _lib.ERR_SHAPE, "2^29"),
 ])
 def test_append_abi_refuses(kw, code, text):
     assert _append(**kw) == code
