@@ -467,39 +467,51 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
   const float c = a.scale_log2, inv_c = 1.f / c;
   float top[2] = {kNegInf, kNegInf};  // scores from which a row's shift moves
 
-  // the table's entries of this wave's two 8-key groups of the stage that is fetched
-  // next, checked when they are used (a check is a wait for the load)
+  // A wave fetches keys 16 wave .. + 15 of a stage: two groups of eight, in one page
+  // where the page size is a multiple of 16.  The table's entries of the stage that is
+  // fetched next are loaded a stage ahead and checked when they are used (a check is
+  // a wait for the load).
+  const char* kbase = a.k + kvh * a.ks.head;
+  const char* vbase = a.v + kvh * a.vs.head;
+  const bool one_page = a.page_size % 16 == 0;
+  const bool alike = a.ks.page == a.vs.page && a.ks.slot == a.vs.slot;
   int entry[2];
   auto load_entries = [&](int s) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      entry[j] = page_of(a, trow, min(it.key0 + 64 * s + 8 * (wave + 4 * j), it.key1 - 1));
+    const int key = it.key0 + 64 * s + 16 * wave;
+    entry[0] = page_of(a, trow, min(key, it.key1 - 1));
+    if (!one_page) entry[1] = page_of(a, trow, min(key + 8, it.key1 - 1));
   };
   auto fetch = [&](int s) {
     char* slot = lds + (s & (kSlots - 1)) * kSlotBytes;
-    int page[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      page[j] = (unsigned)entry[j] < (unsigned)a.pages ? entry[j] : -1;
+    const int key = it.key0 + 64 * s + 16 * wave;
+    const int at = key - fast_div(key, a.div_page) * a.page_size;
+    const uint32_t dst = uniform((int)lds_offset(slot + 16 * wave * kRowBytes));
+    const bool whole = one_page && (unsigned)entry[0] < (unsigned)a.pages && key + 16 <= it.key1;
+    if (whole) {
+      const long long off = entry[0] * a.ks.page + at * a.ks.slot;
+      const long long voff = alike ? off : entry[0] * a.vs.page + at * a.vs.slot;
+      dma16(kbase + off, k_off, dst);
+      dma16(kbase + off + 8 * a.ks.slot, k_off, dst + 8 * kRowBytes);
+      dma16(vbase + voff, v_off, dst + kTileBytes);
+      dma16(vbase + voff + 8 * a.vs.slot, v_off, dst + kTileBytes + 8 * kRowBytes);
+      lost[s & (kSlots - 1)][wave] = 0;
+      return;
+    }
+    int gone = 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int g = wave + 4 * j, key = it.key0 + 64 * s + 8 * g;
-      const int pg = max(page[j], 0);
-      const char* kp = a.k + row_offset(a, a.ks, pg, key, kvh);
-      const char* vp = a.v + row_offset(a, a.vs, pg, key, kvh);
-      const uint32_t dst = uniform((int)lds_offset(slot + 8 * g * kRowBytes));
-      if (page[j] >= 0 && key + 8 <= it.key1) {
-        dma16(kp, k_off, dst);
-        dma16(vp, v_off, dst + kTileBytes);
-      } else {
-        const bool there = page[j] >= 0 && key + (lane >> 3) < it.key1;
-        const char* none = a.zeros + 16 * (lane & 7);
-        dma16_lane(there ? kp + k_off : none, dst);
-        dma16_lane(there ? vp + v_off : none, dst + kTileBytes);
-      }
+      const int first = key + 8 * j;
+      const int id = one_page ? entry[0] : entry[j];
+      const bool page = (unsigned)id < (unsigned)a.pages;
+      const bool there = page && first + (lane >> 3) < it.key1;
+      const char* none = a.zeros + 16 * (lane & 7);
+      dma16_lane(there ? a.k + row_offset(a, a.ks, page ? id : 0, first, kvh) + k_off : none,
+                 dst + 8 * j * kRowBytes);
+      dma16_lane(there ? a.v + row_offset(a, a.vs, page ? id : 0, first, kvh) + v_off : none,
+                 dst + kTileBytes + 8 * j * kRowBytes);
+      gone |= page ? 0 : 1 << (2 * wave + j);
     }
-    // groups of this wave without a page: bit wave + 4 j
-    lost[s & (kSlots - 1)][wave] = (page[0] < 0 ? 1 << wave : 0) | (page[1] < 0 ? 16 << wave : 0);
+    lost[s & (kSlots - 1)][wave] = gone;  // bit g: keys 8 g .. of the stage have no page
   };
 #pragma unroll
   for (int s = 0; s < kSlots - 1; ++s)
@@ -654,7 +666,7 @@ void paged_attn_bf16_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) float lm[4][64], ll[4][64];
   static_assert(4 * FewLds<HW>::kWave <= sizeof(lds), "the waves' blocks fit the ring");
   const int turn = blockIdx.x >> 8, both = 2 * min(a.few_turns, a.many_turns);
-  const bool few = turn < both ? !(turn & 1) : a.few_turns > a.many_turns;
+  const bool few = turn < both ? turn & 1 : a.few_turns > a.many_turns;
   const int block = (turn < both ? turn >> 1 : turn - both / 2) * 256 + (blockIdx.x & 255);
   if (few) {
     const int share = uniform(fast_div(block, a.div_pairs));
