@@ -248,22 +248,27 @@ int mf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_gain,
 int mf_segment_positions(const int32_t* segment_ids, int batch, int seq_len,
                          int32_t* positions, void* stream);
 
+/* Frequencies of a rotary embedding (radians per position, `pairs` finite
+ * numbers) as turns per position, in 2^-64ths of a turn: what mf_rotate and
+ * mf_paged_append take.  Both arrays in HOST memory. */
+int mf_rotary_turns(const double* frequencies, int pairs, uint64_t* turns);
+
 /* Rotary embeddings in their general form (kernels/rotary.py:7-39 rotates
  * whole heads in the half layout): pair i of the first rotary_dim dims of each
  * head -- dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved --
- * turns by position * frequencies[i] and is multiplied by magnitude; the other
+ * turns by position * turns[i] and is multiplied by magnitude; the other
  * dims are copied.  fp32 arithmetic (angles exact at any position), one
  * rounding.  backward != 0 turns the other way (the transpose): q and k are
  * then the gradients of q_out and k_out.
  * q [tokens] x [q_heads, head_dim] with q_stride elements between tokens (each
  * head dense), k likewise; q_out and k_out are dense and may be q and k where
  * those are dense.  q or k is null with 0 heads.  positions [tokens] int32, or
- * NULL: token % seq_len.  frequencies: rotary_dim / 2 radians per position, in
+ * NULL: token % seq_len.  turns: rotary_dim / 2 numbers of mf_rotary_turns, in
  * HOST memory, read before the call returns.  head_dim even, up to 1024;
  * rotary_dim even, up to 256. */
 int mf_rotate(const void* q, long long q_stride, const void* k,
               long long k_stride, const int32_t* positions,
-              const double* frequencies, int dtype, int tokens, int seq_len,
+              const uint64_t* turns, int dtype, int tokens, int seq_len,
               int q_heads, int kv_heads, int head_dim, int rotary_dim,
               int interleaved, float magnitude, int backward, void* q_out,
               void* k_out, void* stream);
@@ -293,7 +298,7 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
  * layers/attention.py:309-317 for many ragged tokens), with the prologue of
  * layers/attention.py:62-97 on the way: optional RMS norm of each query and
  * key head with its gain ([64] in the tensor dtype, NULL: none), then optional
- * rotation at the token's position (frequencies NULL: none; otherwise as
+ * rotation at the token's position (turns NULL: none; otherwise as
  * mf_rotate).  fp32 arithmetic, one rounding.  q [tokens, q_heads, 64] is
  * written to q_out (dense; may be q where that is dense); q and q_out NULL: no
  * queries.  k, v [tokens, kv_heads, 64]; token strides in elements.
@@ -304,7 +309,7 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
 int mf_paged_append(const void* q, long long q_stride, const void* k,
                     long long k_stride, const void* v, long long v_stride,
                     const void* q_gain, const void* k_gain, float eps,
-                    const double* frequencies, int rotary_dim, int interleaved,
+                    const uint64_t* turns, int rotary_dim, int interleaved,
                     float magnitude, int dtype, int tokens, int sequences,
                     int q_heads, int kv_heads, int head_dim, int page_size,
                     int pages, const void* plan, size_t plan_bytes,

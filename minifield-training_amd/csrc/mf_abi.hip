@@ -60,7 +60,7 @@ hipError_t launch_segmented_conv_bwd(const void* b, const void* c, const void* v
                                      int B, int T, int C, int K, void* db, void* dc, void* dv,
                                      float* dw, void* workspace, hipStream_t stream);
 hipError_t launch_rotate(const void* q, long long q_stride, const void* k, long long k_stride,
-                         const int32_t* positions, const double* frequencies, bool f32, int tokens,
+                         const int32_t* positions, const uint64_t* turns, bool f32, int tokens,
                          int seq_len, int Hq, int Hkv, int D, int rotary_dim, int interleaved,
                          float magnitude, bool backward, void* q_out, void* k_out,
                          hipStream_t stream);
@@ -71,7 +71,7 @@ hipError_t launch_paged_plan(const int32_t* query_starts, const int32_t* context
 hipError_t launch_paged_append(const void* q, long long q_stride, const void* k,
                                long long k_stride, const void* v, long long v_stride,
                                const void* q_gain, const void* k_gain, float eps,
-                               const double* frequencies, int rotary_dim, int interleaved,
+                               const uint64_t* turns, int rotary_dim, int interleaved,
                                float magnitude, bool f32, int tokens, int Hq, int Hkv,
                                int page_size, int pages, const PagedToken* records, void* k_pages,
                                void* v_pages, const PagedStrides& k_strides,
@@ -539,15 +539,11 @@ int mf_segmented_conv_bwd(const void* b_gate, const void* c_gate, const void* va
 
 namespace {
 
-// Frequencies and their layout; head_dim and the dtype are checked by the callers.
-int check_rotation(const double* frequencies, int rotary_dim, int head_dim, float magnitude) {
+// The rotated part of a head; head_dim and the dtype are checked by the callers.
+int check_rotation(int rotary_dim, int head_dim, float magnitude) {
   if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || rotary_dim > 256)
     return fail(MF_ERR_SHAPE, "rotary_dim must be even and in [2, min(head_dim, 256)] (got %d of %d)",
                 rotary_dim, head_dim);
-  for (int i = 0; i < rotary_dim / 2; ++i)
-    if (!std::isfinite(frequencies[i]))
-      return fail(MF_ERR_INVALID_ARGUMENT, "frequencies must be finite (number %d is %g)", i,
-                  frequencies[i]);
   if (!std::isfinite(magnitude))
     return fail(MF_ERR_INVALID_ARGUMENT, "magnitude must be finite (got %g)", (double)magnitude);
   return MF_OK;
@@ -616,8 +612,24 @@ int check_page_strides(const char* what, const long long* s, int page_size, int 
 
 }  // namespace
 
+int mf_rotary_turns(const double* frequencies, int pairs, uint64_t* turns) {
+  if (!frequencies || !turns || pairs < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT, "frequencies and turns must be non-null, pairs positive");
+  const long double two_pi = 6.283185307179586476925286766559005768L;
+  for (int i = 0; i < pairs; ++i) {
+    if (!std::isfinite(frequencies[i]))
+      return fail(MF_ERR_INVALID_ARGUMENT, "frequencies must be finite (number %d is %g)", i,
+                  frequencies[i]);
+    long double t = (long double)frequencies[i] / two_pi;
+    t -= std::floor(t);
+    const long double x = std::floor(t * 18446744073709551616.0L + 0.5L);
+    turns[i] = x >= 18446744073709551616.0L ? 0 : (uint64_t)x;  // (a whole turn is none)
+  }
+  return ok();
+}
+
 int mf_rotate(const void* q, long long q_stride, const void* k, long long k_stride,
-              const int32_t* positions, const double* frequencies, int dtype, int tokens,
+              const int32_t* positions, const uint64_t* turns, int dtype, int tokens,
               int seq_len, int q_heads, int kv_heads, int head_dim, int rotary_dim,
               int interleaved, float magnitude, int backward, void* q_out, void* k_out,
               void* stream) {
@@ -635,13 +647,13 @@ int mf_rotate(const void* q, long long q_stride, const void* k, long long k_stri
       (kv_heads > 0) != (k && k_out) || (kv_heads == 0 && (k || k_out)))
     return fail(MF_ERR_INVALID_ARGUMENT,
                 "q and q_out must be non-null with heads and null without, k and k_out likewise");
-  if (!frequencies) return fail(MF_ERR_INVALID_ARGUMENT, "frequencies must be non-null");
-  if (int rc = check_rotation(frequencies, rotary_dim, head_dim, magnitude)) return rc;
+  if (!turns) return fail(MF_ERR_INVALID_ARGUMENT, "turns must be non-null");
+  if (int rc = check_rotation(rotary_dim, head_dim, magnitude)) return rc;
   if (q)
     if (int rc = check_token_stride("q", q_stride, q_heads, head_dim)) return rc;
   if (k)
     if (int rc = check_token_stride("k", k_stride, kv_heads, head_dim)) return rc;
-  return check_hip(mf::launch_rotate(q, q ? q_stride : 0, k, k ? k_stride : 0, positions, frequencies,
+  return check_hip(mf::launch_rotate(q, q ? q_stride : 0, k, k ? k_stride : 0, positions, turns,
                                      dtype == MF_DTYPE_F32, tokens, seq_len, q_heads, kv_heads,
                                      head_dim, rotary_dim, interleaved != 0, magnitude,
                                      backward != 0, q_out, k_out, static_cast<hipStream_t>(stream)),
@@ -682,7 +694,7 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
 
 int mf_paged_append(const void* q, long long q_stride, const void* k, long long k_stride,
                     const void* v, long long v_stride, const void* q_gain, const void* k_gain,
-                    float eps, const double* frequencies, int rotary_dim, int interleaved,
+                    float eps, const uint64_t* turns, int rotary_dim, int interleaved,
                     float magnitude, int dtype, int tokens, int sequences, int q_heads,
                     int kv_heads, int head_dim, int page_size, int pages, const void* plan,
                     size_t plan_bytes, void* k_pages, void* v_pages, const long long* k_strides,
@@ -697,8 +709,8 @@ int mf_paged_append(const void* q, long long q_stride, const void* k, long long 
                 "k, v and the pages must be non-null, q and q_out both given or both null");
   if (!(eps >= 0.f) || !std::isfinite(eps))
     return fail(MF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative (got %g)", (double)eps);
-  if (frequencies)
-    if (int rc = check_rotation(frequencies, rotary_dim, head_dim, magnitude)) return rc;
+  if (turns)
+    if (int rc = check_rotation(rotary_dim, head_dim, magnitude)) return rc;
   if (q)
     if (int rc = check_token_stride("q", q_stride, q_heads, head_dim)) return rc;
   if (int rc = check_token_stride("k", k_stride, kv_heads, head_dim)) return rc;
@@ -711,8 +723,8 @@ int mf_paged_append(const void* q, long long q_stride, const void* k, long long 
   const mf::PagedToken* records = reinterpret_cast<const mf::PagedToken*>(
       static_cast<const char*>(plan) + lay.tokens);
   return check_hip(mf::launch_paged_append(q, q ? q_stride : 0, k, k_stride, v, v_stride, q_gain,
-                                           k_gain, eps, frequencies, rotary_dim, interleaved != 0,
-                                           frequencies ? magnitude : 1.f, dtype == MF_DTYPE_F32,
+                                           k_gain, eps, turns, rotary_dim, interleaved != 0,
+                                           turns ? magnitude : 1.f, dtype == MF_DTYPE_F32,
                                            tokens, q ? q_heads : 0, kv_heads, page_size, pages,
                                            records, k_pages, v_pages, ks, vs, q_out,
                                            static_cast<hipStream_t>(stream)),

@@ -29,15 +29,22 @@ struct Two {
   int a, b;
 };
 
+// Inclusive prefix sum over a wave, with DPP row shifts and broadcasts (a shuffle
+// goes through LDS: six of them took 0.2 us).
+__device__ __forceinline__ int wave_prefix_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2, 3
+  return x;
+}
+
 // Exclusive prefix sums over the workgroup; `sum` gets the totals.
 __device__ __forceinline__ Two block_prefix(Two x, Two* lds, Two& sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Two y = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int a = __shfl_up(y.a, off), b = __shfl_up(y.b, off);
-    if (lane >= off) y.a += a, y.b += b;
-  }
+  Two y = {wave_prefix_sum(x.a), wave_prefix_sum(x.b)};
   __syncthreads();  // the previous call's readers are done
   if (lane == 63) lds[wave] = y;
   __syncthreads();
@@ -80,7 +87,6 @@ struct PlanLds {
   int tiles[kMaxSequences];  // tiles before each sequence
   int start[kMaxSequences], count[kMaxSequences], context[kMaxSequences];
   Two sums[kPlanThreads / 64];
-  unsigned long long work[2];
   int item_at[kPlanThreads], join_at[kPlanThreads];  // before each tile of the round
   Tile tile[kPlanThreads];
 };
@@ -119,11 +125,16 @@ __device__ __forceinline__ Tile tile_of(const PlanArgs& a, const PlanLds& l, int
 }
 
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
+  __shared__ PlanLds l;
+  const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
-    const int t = (blockIdx.x - 1) * kPlanThreads + threadIdx.x;
+    // (the search in LDS: in memory each of its steps is a round trip)
+    for (int r = tid; r < a.R; r += kPlanThreads) l.start[r] = a.starts[r];
+    __syncthreads();
+    const int t = (blockIdx.x - 1) * kPlanThreads + tid;
     if (t >= a.N) return;
     PagedToken rec = {0, -1, 0, -1};
-    const int r = last_not_above(a.starts, a.R, t);
+    const int r = last_not_above(l.start, a.R, t);
     const Span s = span_of(a, r);
     if (t >= s.start && t < s.start + s.count) {
       rec.position = s.context - s.count + (t - s.start);
@@ -138,10 +149,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     reinterpret_cast<PagedToken*>(a.plan + a.lay.tokens)[t] = rec;
     return;
   }
-  __shared__ PlanLds l;
-  const int tid = threadIdx.x;
   if (tid < 64) reinterpret_cast<int*>(a.plan + a.lay.zeros)[tid] = 0;
-  if (tid < 2) l.work[tid] = 0;
   // tiles before every sequence
   int ntiles = 0;
   for (int r0 = 0; r0 < a.R; r0 += kPlanThreads) {
@@ -156,34 +164,28 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       l.count[r] = s.count;
       l.context[r] = s.context;
     }
-    Two sum;
-    const Two before = block_prefix({tiles, 0}, l.sums, sum);
-    if (r < a.R) l.tiles[r] = ntiles + before.a;
-    ntiles += sum.a;
+    Two total;
+    const Two ahead = block_prefix({tiles, 0}, l.sums, total);
+    if (r < a.R) l.tiles[r] = ntiles + ahead.a;
+    ntiles += total.a;
   }
   ntiles = min(ntiles, a.lay.cap_tiles);
   __syncthreads();
   // units of keys over the tiles of each kind (below 2^31: the entry point checks
-  // tiles times the table's reach)
-  unsigned long long mine[2] = {0, 0};
-  Tile x = {};  // the thread's tile of the round (of the first round before it starts)
-  for (int t = (ntiles - 1) / kPlanThreads * kPlanThreads + tid; t >= 0; t -= kPlanThreads)
-    if (t < ntiles) {
-      x = tile_of(a, l, t);
-      mine[0] += x.kind == kFew ? x.units : 0;
-      mine[1] += x.kind == kMany ? x.units : 0;
-    }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mine[k] += __shfl_xor(mine[k], off);
-    if ((tid & 63) == 0 && mine[k]) atomicAdd(&l.work[k], mine[k]);  // (integers: any order)
+  // tiles times the table's reach); the first round's are summed again in its turn
+  Tile x = tid < ntiles ? tile_of(a, l, tid) : Tile{};
+  Two work = {0, 0}, sum, before;
+  for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
+    const Tile y = t0 == 0 ? x : t0 + tid < ntiles ? tile_of(a, l, t0 + tid) : Tile{};
+    before = block_prefix({y.kind == kFew ? y.units : 0, y.kind == kFew ? 0 : y.units}, l.sums, sum);
+    if (t0 == 0) x.unit0 = y.kind == kFew ? before.a : before.b;
+    work.a += sum.a;
+    work.b += sum.b;
   }
-  __syncthreads();
   // units of a share
   const int target[2] = {a.lay.target[0], max(a.lay.target[1], 1)};
-  const int share[2] = {max((int)((l.work[0] + target[0] - 1) / target[0]), 1),
-                        max((int)((l.work[1] + target[1] - 1) / target[1]), kManyUnits)};
+  const int share[2] = {max((work.a + target[0] - 1) / target[0], 1),
+                        max((work.b + target[1] - 1) / target[1], kManyUnits)};
   int* shares[2] = {reinterpret_cast<int*>(a.plan + a.lay.shares[0]),
                     reinterpret_cast<int*>(a.plan + a.lay.shares[1])};
   PagedItem* items[2] = {reinterpret_cast<PagedItem*>(a.plan + a.lay.items[0]),
@@ -191,14 +193,18 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   PagedJoin* joins = reinterpret_cast<PagedJoin*>(a.plan + a.lay.joins);
   Two units = {0, 0}, nitems = {0, 0}, nrest = {0, 0};  // by kind; by kind; joins and partial rows
   for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
-    if (t0 > 0) x = t0 + tid < ntiles ? tile_of(a, l, t0 + tid) : Tile{};
-    const bool live = t0 + tid < ntiles, few = x.kind == kFew;
+    const bool live = t0 + tid < ntiles;
+    if (ntiles > kPlanThreads) {
+      if (t0 > 0) x = live ? tile_of(a, l, t0 + tid) : Tile{};
+      before = block_prefix({x.kind == kFew ? x.units : 0, x.kind == kFew ? 0 : x.units}, l.sums, sum);
+      x.unit0 = x.kind == kFew ? units.a + before.a : units.b + before.b;
+      units.a += sum.a;
+      units.b += sum.b;
+    } else {
+      units = work;
+    }
+    const bool few = x.kind == kFew;
     const int c = few ? share[0] : share[1];
-    Two sum, before;
-    before = block_prefix({live && few ? x.units : 0, live && !few ? x.units : 0}, l.sums, sum);
-    x.unit0 = few ? units.a + before.a : units.b + before.b;
-    units.a += sum.a;
-    units.b += sum.b;
     x.items = !live ? 0 : x.units == 0 ? 1 : (x.unit0 + x.units - 1) / c - x.unit0 / c + 1;
     before = block_prefix({few ? x.items : 0, few ? 0 : x.items}, l.sums, sum);
     const int round_items = sum.a + sum.b;

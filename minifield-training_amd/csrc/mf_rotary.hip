@@ -10,8 +10,8 @@
 // mf_prologue.hip rounds every step to the tensor dtype, as the reference's
 // declared types do: kernels/rotary.py:7-39.)
 //
-// Angles.  f_i / 2 pi modulo one turn is a 64-bit fraction made on the host in
-// extended precision; position * fraction modulo 2^64 drops whole turns exactly,
+// Angles.  f_i / 2 pi modulo one turn is a 64-bit fraction, made on the host in
+// extended precision (mf_rotary_turns); position * fraction modulo 2^64 drops whole turns exactly,
 // so the angle is good to 2^-32 turns plus position * 2^-65 at any int32 position.
 // (An fp32 product is off by position * 2^-24 radians: 0.008 at 131072, twice a
 // bf16 rounding.)
@@ -225,15 +225,6 @@ __global__ __launch_bounds__(256) void turn_rows_kernel(TurnArgs a) {
   }
 }
 
-// Turns per position of pair i as a 64-bit fraction of a turn.
-static uint64_t turn_fraction(double f) {
-  const long double two_pi = 6.283185307179586476925286766559005768L;
-  long double t = (long double)f / two_pi;
-  t -= __builtin_floorl(t);
-  const long double x = __builtin_floorl(t * 18446744073709551616.0L + 0.5L);
-  return x >= 18446744073709551616.0L ? 0 : (uint64_t)x;
-}
-
 template <typename T, int V, bool PAGED>
 static hipError_t launch_turn_v(TurnArgs& a, hipStream_t stream) {
   a.uph = a.D / (2 * V);
@@ -268,16 +259,16 @@ static hipError_t launch_turn(TurnArgs& a, bool f32, uint64_t addresses, uint64_
                    : launch_turn_v<bf16, 1, PAGED>(a, stream);
 }
 
-static void set_turns(TurnArgs& a, const double* frequencies, int rotary_dim, int interleaved,
+static void set_turns(TurnArgs& a, const uint64_t* turns, int rotary_dim, int interleaved,
                       float magnitude) {
-  a.half = frequencies ? rotary_dim / 2 : 0;
+  a.half = turns ? rotary_dim / 2 : 0;
   a.interleaved = interleaved;
   a.magnitude = magnitude;
-  for (int i = 0; i < a.half; ++i) a.turn[i] = turn_fraction(frequencies[i]);
+  for (int i = 0; i < a.half; ++i) a.turn[i] = turns[i];
 }
 
 hipError_t launch_rotate(const void* q, long long q_stride, const void* k, long long k_stride,
-                         const int32_t* positions, const double* frequencies, bool f32, int tokens,
+                         const int32_t* positions, const uint64_t* turns, bool f32, int tokens,
                          int seq_len, int Hq, int Hkv, int D, int rotary_dim, int interleaved,
                          float magnitude, bool backward, void* q_out, void* k_out,
                          hipStream_t stream) {
@@ -295,7 +286,7 @@ hipError_t launch_rotate(const void* q, long long q_stride, const void* k, long 
   a.heads[1] = Hkv;
   a.sign = backward ? -1.f : 1.f;
   a.div_len = make_fastdiv(seq_len);
-  set_turns(a, frequencies, rotary_dim, interleaved, magnitude);
+  set_turns(a, turns, rotary_dim, interleaved, magnitude);
   return launch_turn<false>(a, f32, (uint64_t)q | (uint64_t)k | (uint64_t)q_out | (uint64_t)k_out,
                             (uint64_t)(q_stride | k_stride), stream);
 }
@@ -303,7 +294,7 @@ hipError_t launch_rotate(const void* q, long long q_stride, const void* k, long 
 hipError_t launch_paged_append(const void* q, long long q_stride, const void* k,
                                long long k_stride, const void* v, long long v_stride,
                                const void* q_gain, const void* k_gain, float eps,
-                               const double* frequencies, int rotary_dim, int interleaved,
+                               const uint64_t* turns, int rotary_dim, int interleaved,
                                float magnitude, bool f32, int tokens, int Hq, int Hkv,
                                int page_size, int pages, const PagedToken* records, void* k_pages,
                                void* v_pages, const PagedStrides& k_strides,
@@ -333,7 +324,7 @@ hipError_t launch_paged_append(const void* q, long long q_stride, const void* k,
   a.heads[2] = Hkv;
   a.sign = 1.f;
   a.div_len = make_fastdiv(1);
-  set_turns(a, frequencies, rotary_dim, interleaved, magnitude);
+  set_turns(a, turns, rotary_dim, interleaved, magnitude);
   const uint64_t addresses = (uint64_t)q | (uint64_t)k | (uint64_t)v | (uint64_t)q_out |
                              (uint64_t)k_pages | (uint64_t)v_pages | (uint64_t)q_gain |
                              (uint64_t)k_gain;

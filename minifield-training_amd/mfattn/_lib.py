@@ -64,6 +64,7 @@ EXPORTS = (
     "mf_qk_norm_rope_bwd_workspace_bytes",
     "mf_qk_norm_rope_bwd",
     "mf_segment_positions",
+    "mf_rotary_turns",
     "mf_rotate",
     "mf_paged_plan_bytes",
     "mf_paged_plan",
@@ -151,6 +152,8 @@ def _load() -> ctypes.CDLL:
                                           vp, vp, vp, vp, vp, sz, vp]
     lib.mf_segmented_conv_bwd.restype = i32
     i64 = ctypes.c_longlong
+    lib.mf_rotary_turns.argtypes = [vp, i32, vp]
+    lib.mf_rotary_turns.restype = i32
     lib.mf_rotate.argtypes = [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32,
                               f32, i32, vp, vp, vp]
     lib.mf_rotate.restype = i32

@@ -26,7 +26,7 @@ import functools
 import torch
 
 from .. import _lib
-from ..ops import _ptr, _raw_stream, dtype_code, on_device, require_device, token_rows
+from ..ops import _ptr, _raw_stream, dtype_code, launch, require_device, token_rows
 from .rotary import Rotary
 
 
@@ -56,6 +56,14 @@ def _pool_strides(strides: tuple[int, ...], shape: tuple[int, ...]):
     if strides[3] != 1 and shape[3] > 1:
         raise ValueError("the pages' last dimension must be dense")
     return (ctypes.c_longlong * 3)(*(s if n > 1 else 0 for s, n in zip(strides[:3], shape)))
+
+
+@functools.lru_cache(maxsize=256)
+def _sizes(sequences: int, tokens: int, query_heads: int, kv_heads: int, code: int):
+    """Bytes of a plan and of an attention's workspace."""
+    lib = _lib.LIB
+    return (lib.mf_paged_plan_bytes(sequences, tokens, query_heads, kv_heads, code),
+            lib.mf_paged_attn_workspace_bytes(sequences, tokens, query_heads, kv_heads, code))
 
 
 def _check_pool(key_pages: torch.Tensor, value_pages: torch.Tensor, plan: Plan) -> None:
@@ -118,14 +126,11 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
             r > 1 and table.stride(0) < width):
         table = _int32(table, (r, width), "page_table")
     device = require_device(key_pages, starts, contexts, table)
-    lib = _lib.LIB
-    nbytes = lib.mf_paged_plan_bytes(r, tokens, query_heads, kv_heads, code)
+    nbytes, _ = _sizes(r, tokens, query_heads, kv_heads, code)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with on_device(device):
-        _lib.check(lib.mf_paged_plan(
-            starts.data_ptr(), contexts.data_ptr(), table.data_ptr(),
-            table.stride(0) if r > 1 else width, r, tokens, width, page_size, pages, query_heads,
-            kv_heads, code, buf.data_ptr(), nbytes, _raw_stream(device.index)))
+    launch(device, _lib.LIB.mf_paged_plan, starts.data_ptr(), contexts.data_ptr(), table.data_ptr(),
+           table.stride(0) if r > 1 else width, r, tokens, width, page_size, pages, query_heads,
+           kv_heads, code, buf.data_ptr(), nbytes, _raw_stream(device.index))
     return Plan(buf, table, r, tokens, query_heads, pool, code)
 
 
@@ -168,7 +173,7 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     elif not isinstance(rotary, Rotary) or rotary.head_dim != d:
         raise ValueError(f"rotary must be a Rotary of heads of {d}")
     else:
-        turn = rotary._turn
+        turn = rotary._args
     if key_pages.data_ptr() == value_pages.data_ptr():
         raise ValueError("keys and values need pages of their own")
     device = require_device(key_pages, plan.buf, key, value, value_pages,
@@ -179,13 +184,12 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     if query is not None:
         query, q_step = token_rows(query)
         out = torch.empty(plan.q_shape, dtype=dtype, device=device)
-    with on_device(device):
-        _lib.check(_lib.LIB.mf_paged_append(
-            _ptr(query), q_step, key.data_ptr(), k_step, value.data_ptr(), v_step, _ptr(qg),
-            _ptr(kg), eps, *turn, code, n, plan.sequences, plan.query_heads, plan.kv_heads, d,
-            plan.page_size, plan.pages, plan.buf.data_ptr(), plan.nbytes, key_pages.data_ptr(),
-            value_pages.data_ptr(), _pool_strides(key_pages.stride(), plan.pool),
-            _pool_strides(value_pages.stride(), plan.pool), _ptr(out), _raw_stream(device.index)))
+    launch(device, _lib.LIB.mf_paged_append, _ptr(query), q_step, key.data_ptr(), k_step,
+           value.data_ptr(), v_step, _ptr(qg), _ptr(kg), eps, *turn, code, n, plan.sequences,
+           plan.query_heads, plan.kv_heads, d, plan.page_size, plan.pages, plan.buf.data_ptr(),
+           plan.nbytes, key_pages.data_ptr(), value_pages.data_ptr(),
+           _pool_strides(key_pages.stride(), plan.pool),
+           _pool_strides(value_pages.stride(), plan.pool), _ptr(out), _raw_stream(device.index))
     return out
 
 
@@ -221,18 +225,14 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
           or out.device != device):
         raise ValueError(f"out must be a contiguous {dtype} {list(shape)} on {device}")
     n, hq, d = shape
-    lib = _lib.LIB
-    ws_bytes = lib.mf_paged_attn_workspace_bytes(plan.sequences, n, hq, plan.kv_heads, code)
+    _, ws_bytes = _sizes(plan.sequences, n, hq, plan.kv_heads, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    with on_device(device):
-        _lib.check(lib.mf_paged_attn(
-            query.data_ptr(), q_step, key_pages.data_ptr(), value_pages.data_ptr(),
-            _pool_strides(key_pages.stride(), plan.pool),
-            _pool_strides(value_pages.stride(), plan.pool), plan.page_table.data_ptr(),
-            plan.table_stride, code, n, plan.sequences, plan.width, plan.page_size, plan.pages, hq,
-            plan.kv_heads, d, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(),
-            plan.nbytes, zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes,
-            _raw_stream(device.index)))
+    launch(device, _lib.LIB.mf_paged_attn, query.data_ptr(), q_step, key_pages.data_ptr(),
+           value_pages.data_ptr(), _pool_strides(key_pages.stride(), plan.pool),
+           _pool_strides(value_pages.stride(), plan.pool), plan.page_table.data_ptr(),
+           plan.table_stride, code, n, plan.sequences, plan.width, plan.page_size, plan.pages, hq,
+           plan.kv_heads, d, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes,
+           zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes, _raw_stream(device.index))
     return out
 
 

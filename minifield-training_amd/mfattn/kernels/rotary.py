@@ -16,7 +16,7 @@ import math
 import torch
 
 from .. import _lib
-from ..ops import (_ptr, _raw_stream, dtype_code, on_device, require_device, token_rows)
+from ..ops import _ptr, _raw_stream, dtype_code, launch, require_device, token_rows
 from .prologue import _positions
 
 _SCALINGS = ("none", "linear", "base", "bands", "ramp")
@@ -82,8 +82,11 @@ class Rotary:
             raise ValueError("frequencies and magnitude must be finite")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, r, bool(interleaved)
         self.frequencies, self.magnitude = tuple(freqs), float(magnitude)
+        self._turns = (ctypes.c_uint64 * len(freqs))()
+        _lib.check(_lib.LIB.mf_rotary_turns((ctypes.c_double * len(freqs))(*freqs), len(freqs),
+                                            self._turns))
         # the C ABI's arguments: host array, rotary_dim, interleaved, magnitude
-        self._turn = ((ctypes.c_double * len(freqs))(*freqs), r, int(self.interleaved), self.magnitude)
+        self._args = (ctypes.addressof(self._turns), r, int(self.interleaved), self.magnitude)
 
     def __repr__(self) -> str:
         return (f"Rotary(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, "
@@ -126,12 +129,10 @@ def _launch(q, k, positions, rotary, backward):
         k, k_stride = token_rows(k)
         k_out = torch.empty(k.shape, dtype=dtype, device=device)
         hkv, kp, ko = k.shape[-2], k.data_ptr(), k_out.data_ptr()
-    array, rotary_dim, interleaved, magnitude = rotary._turn
-    with on_device(device):
-        _lib.check(_lib.LIB.mf_rotate(
-            qp, q_stride, kp, k_stride, _ptr(positions), array, dtype_code(one), tokens, seq_len, hq,
-            hkv, rotary.head_dim, rotary_dim, interleaved, magnitude, backward, qo, ko,
-            _raw_stream(device.index)))
+    turns, rotary_dim, interleaved, magnitude = rotary._args
+    launch(device, _lib.LIB.mf_rotate, qp, q_stride, kp, k_stride, _ptr(positions), turns,
+           dtype_code(one), tokens, seq_len, hq, hkv, rotary.head_dim, rotary_dim, interleaved,
+           magnitude, backward, qo, ko, _raw_stream(device.index))
     return q_out, k_out
 
 

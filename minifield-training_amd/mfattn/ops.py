@@ -10,7 +10,6 @@ calls the HIP backward once.
 from __future__ import annotations
 
 import collections
-import contextlib
 import threading
 import weakref
 
@@ -105,14 +104,16 @@ class _OtherDevice:
         torch.cuda.set_device(self.before)
 
 
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context of a launch on ``device``: nothing to do where it is the current one."""
+def launch(device: torch.device, function, *args) -> None:
+    """Calls an entry point that launches on ``device``, making it the current one where it
+    is not, and raises for a nonzero status."""
     if _current_device() == device.index:
-        return _SAME_DEVICE
-    return _OtherDevice(device.index)
+        rc = function(*args)
+    else:
+        with _OtherDevice(device.index):
+            rc = function(*args)
+    if rc:
+        _lib.check(rc)
 
 
 def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:

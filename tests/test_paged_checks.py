@@ -178,7 +178,7 @@ def test_cache_pages_refuses():
 
 
 def _rotate(**kw):
-    a = dict(q=PTR, qs=256, k=PTR, ks=128, pos=None, freq=(ctypes.c_double * 32)(*[1.0] * 32),
+    a = dict(q=PTR, qs=256, k=PTR, ks=128, pos=None, turns=(ctypes.c_uint64 * 32)(*[1] * 32),
              dtype=1, tokens=3, seq=3, hq=4, hkv=2, d=64, r=64, inter=0, mu=1.0, back=0, qo=PTR,
              ko=PTR)
     a.update(kw)
@@ -197,8 +197,7 @@ def _rotate(**kw):
     (dict(q=None), _lib.ERR_INVALID_ARGUMENT, "null"),
     (dict(hkv=0), _lib.ERR_INVALID_ARGUMENT, "null"),
     (dict(hkv=65535), _lib.ERR_SHAPE, "65535"),
-    (dict(freq=None), _lib.ERR_INVALID_ARGUMENT, "frequencies"),
-    (dict(freq=(ctypes.c_double * 32)(*[float("nan")] * 32)), _lib.ERR_INVALID_ARGUMENT, "finite"),
+    (dict(turns=None), _lib.ERR_INVALID_ARGUMENT, "turns"),
     (dict(mu=float("inf")), _lib.ERR_INVALID_ARGUMENT, "magnitude"),
     (dict(qs=255), _lib.ERR_SHAPE, "between tokens"),
     (dict(ks=-128), _lib.ERR_SHAPE, "between tokens"),
@@ -206,6 +205,21 @@ def _rotate(**kw):
 def test_rotate_abi_refuses(kw, code, text):
     assert _rotate(**kw) == code
     assert text in _msg()
+
+
+def test_turns_of_frequencies():
+    freqs = [1.0, 2 * math.pi, -1.0, 0.0, 1e-9, 2 * math.pi * 5.25, 1e6]
+    turns = (ctypes.c_uint64 * 7)()
+    assert L.mf_rotary_turns((ctypes.c_double * 7)(*freqs), 7, turns) == _lib.OK
+    # 2^-64ths of a turn; a double holds f / 2 pi to 2^-53 of it, modulo whole turns
+    for f, t in zip(freqs, turns):
+        exact = f / (2 * math.pi) % 1.0
+        off = abs(t / 2.0 ** 64 - exact)
+        assert min(off, 1 - off) <= 2.0 ** -52 * max(1.0, abs(f)), (f, t)
+    assert L.mf_rotary_turns((ctypes.c_double * 1)(float("nan")), 1, turns) == _lib.ERR_INVALID_ARGUMENT
+    assert "finite" in _msg()
+    assert L.mf_rotary_turns(None, 1, turns) == _lib.ERR_INVALID_ARGUMENT
+    assert L.mf_rotary_turns((ctypes.c_double * 1)(1.0), 0, turns) == _lib.ERR_INVALID_ARGUMENT
 
 
 def _strides(*s):
@@ -251,7 +265,7 @@ def test_plan_abi_refuses(kw, code, text):
 
 def _append(**kw):
     a = dict(q=PTR, qs=256, k=PTR, ks=128, v=PTR, vs=128, qg=PTR, kg=PTR, eps=1e-5,
-             freq=(ctypes.c_double * 32)(*[1.0] * 32), rd=64, inter=0, mu=1.0, dtype=1, n=4, r=2, hq=4,
+             turns=(ctypes.c_uint64 * 32)(*[1] * 32), rd=64, inter=0, mu=1.0, dtype=1, n=4, r=2, hq=4,
              hkv=2, d=64, ps=16, pages=9, plan=PTR, nbytes=1 << 30, kp=PTR, vp=PTR,
              kst=_strides(2048, 128, 64), vst=_strides(2048, 128, 64), qo=PTR)
     a.update(kw)
