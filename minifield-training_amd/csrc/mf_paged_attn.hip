@@ -211,29 +211,29 @@ struct FewLds {
   static constexpr int kWave = 2 * kBlock;
 };
 
-// Keys of block kb .. kb + 31 of a pool into a wave's LDS block.  off: the lane's
-// byte offsets from the first token of a DMA, by the DMA's number (mod 4 for two
-// heads, where the permutation depends on it).
+// Keys of block kb .. kb + 31 of a pool into a wave's LDS block.  at: byte offsets of
+// the first rows of its four groups; off: the lane's byte offsets from the first
+// token of a DMA, by the DMA's number (mod 4 for two heads, where the permutation
+// depends on it).
 template <int HW>
-__device__ __forceinline__ void few_fetch(const PagedArgs& a, const char* pool,
-                                          const PagedStrides& s, const uint32_t (&off)[2 * HW],
-                                          const int (&page)[4], int kb, int end, int head0,
-                                          char* block) {
+__device__ __forceinline__ void few_fetch(const PagedArgs& a, const char* pool, long long slot,
+                                          const long long (&at)[4], const uint32_t (&off)[2 * HW],
+                                          int gone, int kb, int end, char* block) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int key = kb + 8 * g;
-    const char* base = pool + row_offset(a, s, max(page[g], 0), key, head0);
-    if (page[g] >= 0 && key + 8 <= end) {
+    const char* base = pool + at[g];
+    if (!(gone >> g & 1) && key + 8 <= end) {
 #pragma unroll
       for (int j = 0; j < HW; ++j)
-        dma16_once(base + j * 4 * s.slot, off[HW == 1 ? 0 : (2 * g + j) & 3],
+        dma16_once(base + j * 4 * slot, off[HW == 1 ? 0 : (2 * g + j) & 3],
                    uniform((int)lds_offset(block + (HW * g + j) * 1024)));
     } else {
       const int lane = __lane_id();
 #pragma unroll
       for (int j = 0; j < HW; ++j) {
-        const bool there = page[g] >= 0 && key + j * 4 + lane / (8 * HW) < end;
-        const char* src = there ? base + j * 4 * s.slot + off[HW == 1 ? 0 : (2 * g + j) & 3]
+        const bool there = !(gone >> g & 1) && key + j * 4 + lane / (8 * HW) < end;
+        const char* src = there ? base + j * 4 * slot + off[HW == 1 ? 0 : (2 * g + j) & 3]
                                 : a.zeros + 16 * (lane & 7);
         dma16_lane(src, uniform((int)lds_offset(block + (HW * g + j) * 1024)));
       }
@@ -241,7 +241,7 @@ __device__ __forceinline__ void few_fetch(const PagedArgs& a, const char* pool,
   }
 }
 
-template <int HW>
+template <int HW, bool ALIKE>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it, int pair,
                                          int key_wave, char* wave_lds, float* lm, float* ll) {
   typedef FewLds<HW> L;
@@ -265,7 +265,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
     const int tok = lane / (8 * HW);
     const int piece = (lane & (8 * HW - 1)) ^ few_swz<HW>(HW == 1 ? tok : 4 * i + tok);
     k_off[i] = (uint32_t)(tok * a.ks.slot) + (uint32_t)((piece >> 3) * a.ks.head) + 16 * (piece & 7);
-    v_off[i] = (uint32_t)(tok * a.vs.slot) + (uint32_t)((piece >> 3) * a.vs.head) + 16 * (piece & 7);
+    v_off[i] = ALIKE ? k_off[i] : (uint32_t)(tok * a.vs.slot) +
+                                      (uint32_t)((piece >> 3) * a.vs.head) + 16 * (piece & 7);
   }
   // operand addresses: piece 8 h + 2 ks + half of token lane & 31, and for the
   // transposing reads piece 8 h + 4 db + tr_col / 8 of token tr_row (+ 8, + 16)
@@ -283,29 +284,38 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
     st[h] = {0.f, kNegInf, 0.f, 0.f};
   }
   const float c = a.scale_log2;
-  // Pages of the block that is fetched next: the table's entries, checked only when
-  // they are used (a check is a wait for the load).
-  int entry[4], page[4];
-  int gone = 0, gone_next = 0;
+  // The table's entries of the block that is fetched next, checked only when they are
+  // used (a check is a wait for the load); where its rows are; the groups of eight
+  // keys without a page.
+  int entry[4], gone = 0, gone_next = 0;
+  long long at[4];
   auto load_entries = [&](int b) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       entry[g] = page_of(a, trow, min(it.key0 + 32 * b + 8 * g, it.key1 - 1));
   };
-  auto check_entries = [&]() {
+  auto place = [&](const PagedStrides& s, int b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at[g] = row_offset(a, s, gone_next >> g & 1 ? 0 : entry[g], it.key0 + 32 * b + 8 * g, head0);
+  };
+  auto fetch_keys = [&](int b) {
     gone_next = 0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      page[g] = (unsigned)entry[g] < (unsigned)a.pages ? entry[g] : -1;
-      gone_next |= page[g] < 0 ? 1 << g : 0;
-    }
+    for (int g = 0; g < 4; ++g) gone_next |= (unsigned)entry[g] < (unsigned)a.pages ? 0 : 1 << g;
+    place(a.ks, b);
+    few_fetch<HW>(a, a.k, a.ks.slot, at, k_off, gone_next, it.key0 + 32 * b, it.key1, kt);
+  };
+  auto fetch_values = [&](int b) {
+    if (!ALIKE) place(a.vs, b);
+    few_fetch<HW>(a, a.v, ALIKE ? a.ks.slot : a.vs.slot, at, v_off, gone_next, it.key0 + 32 * b,
+                  it.key1, vt);
   };
   int b = key_wave;
   if (b < blocks) {
     load_entries(b);
-    check_entries();
-    few_fetch<HW>(a, a.k, a.ks, k_off, page, it.key0 + 32 * b, it.key1, head0, kt);
-    few_fetch<HW>(a, a.v, a.vs, v_off, page, it.key0 + 32 * b, it.key1, head0, vt);
+    fetch_keys(b);
+    fetch_values(b);
   }
   for (; b < blocks; b += kKeyWaves) {
     const int kb = it.key0 + 32 * b, next = b + kKeyWaves;
@@ -323,10 +333,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
     }
     wait_lds();
     __builtin_amdgcn_sched_barrier(0);
-    if (more) {
-      check_entries();
-      few_fetch<HW>(a, a.k, a.ks, k_off, page, it.key0 + 32 * next, it.key1, head0, kt);
-    }
+    if (more) fetch_keys(next);
     const bool masked = kb + 32 > least || gone;
     bf16x8 p[HW][2];
 #pragma unroll
@@ -352,7 +359,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
         }
     wait_lds();
     __builtin_amdgcn_sched_barrier(0);
-    if (more) few_fetch<HW>(a, a.v, a.vs, v_off, page, it.key0 + 32 * next, it.key1, head0, vt);
+    if (more) fetch_values(next);
   }
   wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS
 
@@ -434,6 +441,7 @@ __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it
 constexpr int kSlotBytes = 2 * kTileBytes;  // 64 keys of K and of V
 constexpr int kSlots = 4;
 
+template <bool ALIKE>
 __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
                                           int (*lost)[4]) {
   const int lane = threadIdx.x & 63;
@@ -454,7 +462,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
 
   const int piece16 = ((lane & 7) ^ swz(lane >> 3)) * 16;
   const uint32_t k_off = (uint32_t)((lane >> 3) * a.ks.slot) + piece16;
-  const uint32_t v_off = (uint32_t)((lane >> 3) * a.vs.slot) + piece16;
+  const uint32_t v_off = ALIKE ? k_off : (uint32_t)((lane >> 3) * a.vs.slot) + piece16;
   const int* trow = a.table + it.sequence * a.table_stride;
   const int stages = (it.key1 - it.key0 + 63) >> 6;
   f32x16 acc[2][2];
@@ -472,9 +480,9 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
   // fetched next are loaded a stage ahead and checked when they are used (a check is
   // a wait for the load).
   const char* kbase = a.k + kvh * a.ks.head;
-  const char* vbase = a.v + kvh * a.vs.head;
+  const char* vbase = a.v + kvh * (ALIKE ? a.ks.head : a.vs.head);
   const bool one_page = a.page_size % 16 == 0;
-  const bool alike = a.ks.page == a.vs.page && a.ks.slot == a.vs.slot;
+  const PagedStrides& vs = ALIKE ? a.ks : a.vs;
   int entry[2];
   auto load_entries = [&](int s) {
     const int key = it.key0 + 64 * s + 16 * wave;
@@ -489,11 +497,11 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
     const bool whole = one_page && (unsigned)entry[0] < (unsigned)a.pages && key + 16 <= it.key1;
     if (whole) {
       const long long off = entry[0] * a.ks.page + at * a.ks.slot;
-      const long long voff = alike ? off : entry[0] * a.vs.page + at * a.vs.slot;
+      const long long voff = ALIKE ? off : entry[0] * vs.page + at * vs.slot;
       dma16(kbase + off, k_off, dst);
       dma16(kbase + off + 8 * a.ks.slot, k_off, dst + 8 * kRowBytes);
       dma16(vbase + voff, v_off, dst + kTileBytes);
-      dma16(vbase + voff + 8 * a.vs.slot, v_off, dst + kTileBytes + 8 * kRowBytes);
+      dma16(vbase + voff + 8 * vs.slot, v_off, dst + kTileBytes + 8 * kRowBytes);
       lost[s & (kSlots - 1)][wave] = 0;
       return;
     }
@@ -507,7 +515,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
       const char* none = a.zeros + 16 * (lane & 7);
       dma16_lane(there ? a.k + row_offset(a, a.ks, page ? id : 0, first, kvh) + k_off : none,
                  dst + 8 * j * kRowBytes);
-      dma16_lane(there ? a.v + row_offset(a, a.vs, page ? id : 0, first, kvh) + v_off : none,
+      dma16_lane(there ? a.v + row_offset(a, vs, page ? id : 0, first, kvh) + v_off : none,
                  dst + kTileBytes + 8 * j * kRowBytes);
       gone |= page ? 0 : 1 << (2 * wave + j);
     }
@@ -659,7 +667,8 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
 // (KV heads fastest, so that with 8 of them each XCD's L2 holds one head's keys), in
 // turn 256 of each while there are both: one for every CU, so that a CU's two
 // workgroups are one that waits for memory and one that computes.
-template <int HW>
+// ALIKE: the pools of keys and values have the same strides.
+template <int HW, bool ALIKE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_attn_bf16_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[kSlots * kSlotBytes];
@@ -677,7 +686,7 @@ void paged_attn_bf16_kernel(PagedArgs a) {
     for (int item = ld_const(a.shares[kFew], share); item < end; ++item) {
       const ItemView it = load_item(a.items[kFew], item);
       if (it.nrows < 1) continue;
-      few_rows<HW>(a, it, pair, wave, lds + wave * FewLds<HW>::kWave, lm[wave], ll[wave]);
+      few_rows<HW, ALIKE>(a, it, pair, wave, lds + wave * FewLds<HW>::kWave, lm[wave], ll[wave]);
       __syncthreads();
       few_merge<HW>(a, it, pair, lds, lm, ll);
       __syncthreads();
@@ -691,7 +700,7 @@ void paged_attn_bf16_kernel(PagedArgs a) {
   for (int item = ld_const(a.shares[kMany], share); item < end; ++item) {
     const ItemView it = load_item(a.items[kMany], item);
     if (it.nrows < 1) continue;
-    many_rows(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(lm));
+    many_rows<ALIKE>(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(lm));
     __syncthreads();
   }
 }
@@ -1008,10 +1017,15 @@ hipError_t launch_paged_attn(const void* q, long long q_stride, const void* k_pa
     return hipGetLastError();
   }
   const dim3 grid(256u * (unsigned)(a.few_turns + a.many_turns));
-  if (lay.head_pair == 2)
-    hipLaunchKernelGGL(paged_attn_bf16_kernel<2>, grid, dim3(256), 0, stream, a);
+  const bool alike = a.ks.page == a.vs.page && a.ks.slot == a.vs.slot && a.ks.head == a.vs.head;
+  if (lay.head_pair == 2 && alike)
+    hipLaunchKernelGGL((paged_attn_bf16_kernel<2, true>), grid, dim3(256), 0, stream, a);
+  else if (lay.head_pair == 2)
+    hipLaunchKernelGGL((paged_attn_bf16_kernel<2, false>), grid, dim3(256), 0, stream, a);
+  else if (alike)
+    hipLaunchKernelGGL((paged_attn_bf16_kernel<1, true>), grid, dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL(paged_attn_bf16_kernel<1>, grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_attn_bf16_kernel<1, false>), grid, dim3(256), 0, stream, a);
   hipLaunchKernelGGL(paged_join_kernel<false>, join, dim3(256), 0, stream, a);
   return hipGetLastError();
 }

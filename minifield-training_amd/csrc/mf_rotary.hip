@@ -229,15 +229,19 @@ template <typename T, int V, bool PAGED>
 static hipError_t launch_turn_v(TurnArgs& a, hipStream_t stream) {
   a.uph = a.D / (2 * V);
   a.units = (a.heads[0] + a.heads[1] + a.heads[2]) * a.uph;
-  const bool wide = (long long)a.tokens * a.units >= 256 * 4 * 1024;
-  const int per = 256 * (wide ? 4 : 1);
+  // One unit a thread, two where a token has more units than a workgroup has threads:
+  // the rows in flight come from many workgroups, not from deep loops.  us for one,
+  // two and four units: 8 x 4096 tokens of 16/8 heads 35.6, 35.7 and 40.8 (5.7 TB/s;
+  // a copy of 1 GiB runs at 5.2), the append of 20912 tokens 34.1, 35.9 and 40.2;
+  // 8 x 2048 of 24 heads of 96, 24 rotated (288 units) 34.7, 30.3 and 31.1.
+  const int per = a.units > 256 ? 512 : 256;
   a.tpb = per / a.units < 1 ? 1 : per / a.units > kTurnTokens ? kTurnTokens : per / a.units;
   a.div_units = make_fastdiv(a.units);
   a.div_uph = make_fastdiv(a.uph);
   a.div_half = make_fastdiv(a.half < 1 ? 1 : a.half);
   const unsigned grid = (unsigned)((a.tokens + a.tpb - 1) / a.tpb);
-  if (wide)
-    hipLaunchKernelGGL((turn_rows_kernel<T, V, 4, PAGED>), dim3(grid), dim3(256), 0, stream, a);
+  if (per > 256)
+    hipLaunchKernelGGL((turn_rows_kernel<T, V, 2, PAGED>), dim3(grid), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((turn_rows_kernel<T, V, 1, PAGED>), dim3(grid), dim3(256), 0, stream, a);
   return hipGetLastError();

@@ -49,6 +49,9 @@ class Batch:
             pool = normal(2, pages, hkv, page_size, 64).transpose(2, 3)
         elif layout == "together":  # keys and values of a slot side by side
             pool = normal(pages, page_size, 2, hkv, 64).permute(2, 0, 1, 3, 4)
+        elif layout == "apart":     # keys by slots, values by heads
+            pool = (normal(pages, page_size, hkv, 64),
+                    normal(pages, hkv, page_size, 64).transpose(1, 2))
         else:
             raise KeyError(layout)
         self.key_pages, self.value_pages = pool[0], pool[1]

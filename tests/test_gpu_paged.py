@@ -44,7 +44,7 @@ def test_plan_of_many_sequences(device):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("layout", ["slots", "heads", "together"])
+@pytest.mark.parametrize("layout", ["slots", "heads", "together", "apart"])
 @pytest.mark.parametrize("form", ["norm+turn", "turn", "norm", "copy", "part", "odd"])
 def test_append_writes_its_slots_and_nothing_else(form, layout, dtype, device):
     say("append", form, layout, dtype)
@@ -118,6 +118,10 @@ SHAPES = [
     ([(2, 90)], 5, 5, 48, "heads"),
     ([(1, 20000)], 4, 4, 64, "heads"),                                   # many items
     ([(70, 3000)] * 3 + [(1, 2500)] * 20, 8, 4, 16, "slots"),            # both paths, split
+    ([(90, 400), (1, 333), (2, 60)], 8, 4, 16, "apart"),                 # strides of their own
+    ([(90, 400), (1, 333), (2, 60)], 9, 3, 24, "apart"),
+    ([(1, 3000)] * 300, 2, 2, 16, "slots"),                              # more tiles than a round
+    ([(20, 90)] * 290 + [(40, 50)], 2, 1, 8, "heads"),
 ]
 
 
