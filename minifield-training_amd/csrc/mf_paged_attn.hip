@@ -29,6 +29,8 @@
 // (behind the context, in a page outside the pool) are read from a row of zeros
 // in the plan, so that nothing a masked slot holds, infinities and NaN included,
 // meets a product.
+#include <type_traits>
+
 #include "mf_f32.h"
 #include "mf_lds.h"
 #include "mf_paged.h"
@@ -168,6 +170,75 @@ __device__ __forceinline__ float column_max(const f32x16& s) {
   return mx;
 }
 
+// Infinities and NaN among values that some rows of an item do not see.  Their
+// probability is 0 there, and 0 times such a value is NaN.  Any leaves its mark in the
+// sums, so the loops do not look for them: an item with causally masked keys whose
+// sums are not all finite is done once more (Careful, 32 rows at a time), now with
+// these values taken out of the operands of masked blocks (drop_wild) and added by
+// themselves to the rows that do see them (add_wild, key by key).  Rows that see none
+// come out with the same bits as without them.  (A check of every masked block as it
+// comes cost chunks 4 %, in registers.)
+typedef std::false_type Plain;
+typedef std::true_type Careful;
+
+// Bits 15 and 31 of the result: whether the low and the high half of a word are
+// such values (an exponent of all ones carries into them).
+__device__ __forceinline__ uint32_t wild_bits(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+// Bit 31: whether one of the floats is one.
+__device__ __forceinline__ uint32_t wild_bits(const f32x16& v) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) any |= (__float_as_uint(v[r]) & 0x7f800000u) + 0x00800000u;
+  return any & 0x80000000u;
+}
+__device__ __forceinline__ uint32_t wild_bits(const bf16x8& v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  return wild_bits(w[0]) | wild_bits(w[1]) | wild_bits(w[2]) | wild_bits(w[3]);
+}
+__device__ __forceinline__ void drop_wild(bf16x8& v) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = w[i];
+    w[i] = x & ~((wild_bits(x) >> 15) * 0xffffu);
+  }
+  v = __builtin_bit_cast(bf16x8, w);
+}
+// The same of a float, as all ones or zero.  (Integers throughout: the file is compiled
+// as if no value were NaN, and a comparison of floats may be simplified by that.)
+__device__ __forceinline__ uint32_t wild_mask(float x) {
+  return 0u - (((__float_as_uint(x) & 0x7f800000u) + 0x00800000u) >> 31);
+}
+// acc += x, whatever x is.
+__device__ __forceinline__ float add_any(float acc, float x) {
+  asm("v_add_f32 %0, %0, %1" : "+v"(acc) : "v"(x));
+  return acc;
+}
+// quad(key, 4 db + g): dims 32 db + 8 g + 4 half .. + 3 of a key of the block; `seen`
+// keys of it are the lane's row's.
+template <typename Quad>
+__device__ __forceinline__ void add_wild(f32x16 (&acc)[2], int seen, Quad quad) {
+#pragma unroll 1
+  for (int key = 0; key < 32; ++key) {
+    const uint32_t mine = key < seen ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x2 w = quad(key, 4 * db + g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x = w[i];
+          const uint32_t y = x & ((wild_bits(x) >> 15) * 0xffffu) & mine;
+          acc[db][4 * g + 2 * i] = add_any(acc[db][4 * g + 2 * i], bf16_lo(y));
+          acc[db][4 * g + 2 * i + 1] = add_any(acc[db][4 * g + 2 * i + 1], bf16_hi(y));
+        }
+      }
+  }
+}
+
 // The lane's row of an item, and its output row.
 struct RowOf {
   int token, head;
@@ -241,7 +312,9 @@ __device__ __forceinline__ void few_fetch(const PagedArgs& a, const char* pool, 
   }
 }
 
-template <int HW, bool ALIKE>
+// ALONE: the wave takes all keys of its rows, carefully, with the many-rows path's
+// arithmetic (rows that do not see an infinity or NaN get that path's very bits).
+template <int HW, bool ALIKE, bool ALONE>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it, int pair,
                                          int key_wave, char* wave_lds, float* lm, float* ll) {
   typedef FewLds<HW> L;
@@ -278,11 +351,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
   const int blocks = (it.key1 - it.key0 + 31) >> 5;
   f32x16 acc[HW][2];
   RowState st[HW];
-#pragma unroll
-  for (int h = 0; h < HW; ++h) {
-    acc[h][0] = acc[h][1] = zero16();
-    st[h] = {0.f, kNegInf, 0.f, 0.f};
-  }
+  float top[HW];
   const float c = a.scale_log2;
   // The table's entries of the block that is fetched next, checked only when they are
   // used (a check is a wait for the load); where its rows are; the groups of eight
@@ -311,56 +380,98 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
     few_fetch<HW>(a, a.v, ALIKE ? a.ks.slot : a.vs.slot, at, v_off, gone_next, it.key0 + 32 * b,
                   it.key1, vt);
   };
-  int b = key_wave;
-  if (b < blocks) {
-    load_entries(b);
-    fetch_keys(b);
-    fetch_values(b);
-  }
-  for (; b < blocks; b += kKeyWaves) {
-    const int kb = it.key0 + 32 * b, next = b + kKeyWaves;
-    const bool more = next < blocks;
-    gone = gone_next;
-    if (more) load_entries(next);
-    wait_vm_lds<4 * HW>();  // K is there; V's DMAs may be on their way
-    f32x16 s[HW];
+  auto run = [&](auto how) {
+    constexpr bool careful = decltype(how)::value;
 #pragma unroll
     for (int h = 0; h < HW; ++h) {
-      s[h] = zero16();
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        s[h] = mfma32x32x16(ld_bf16x8(kt + (k_at ^ ((8 * h + 2 * ks) << 4))), qf[h][ks], s[h]);
+      acc[h][0] = acc[h][1] = zero16();
+      st[h] = {0.f, kNegInf, 0.f, 0.f};
+      top[h] = kNegInf;
     }
-    wait_lds();
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) fetch_keys(next);
-    const bool masked = kb + 32 > least || gone;
-    bf16x8 p[HW][2];
-#pragma unroll
-    for (int h = 0; h < HW; ++h) {
-      if (masked) mask_scores(s[h], opaque(kb), lim, gone, lane);
-      grow(st[h], fmaf(halves_max(column_max(s[h])), c, -st[h].shift), acc[h]);
-      block_probs(s[h], st[h], c, p[h][0], p[h][1]);
+    int b = ALONE ? 0 : key_wave;
+    if (b < blocks) {
+      load_entries(b);
+      fetch_keys(b);
+      fetch_values(b);
     }
-    if (more) wait_vm_lds<4 * HW>(); else wait_vm_lds<0>();
+    constexpr int kStep = ALONE ? 1 : kKeyWaves;
+    for (; b < blocks; b += kStep) {
+      const int kb = it.key0 + 32 * b, next = b + kStep;
+      const bool more = next < blocks;
+      gone = gone_next;
+      if (more) load_entries(next);
+      wait_vm_lds<4 * HW>();  // K is there; V's DMAs may be on their way
+      f32x16 s[HW];
 #pragma unroll
-    for (int h = 0; h < HW; ++h)
+      for (int h = 0; h < HW; ++h) {
+        s[h] = zero16();
 #pragma unroll
-      for (int db = 0; db < 2; ++db)
+        for (int ks = 0; ks < 4; ++ks)
+          s[h] = mfma32x32x16(ld_bf16x8(kt + (k_at ^ ((8 * h + 2 * ks) << 4))), qf[h][ks], s[h]);
+      }
+      wait_lds();
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) fetch_keys(next);
+      const bool masked = kb + 32 > least || gone;
+      bf16x8 p[HW][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const char* at = vt + 16 * j * L::kTok;
-          const int x = v_at ^ ((8 * h + 4 * db) << 4);
-          const u32x2 lo = lds_read_tr16(at + x);
-          // token + 8: the permutation of two heads differs in its lowest bit
-          const u32x2 hi = lds_read_tr16(at + 8 * L::kTok + (HW == 1 ? x : x ^ 16));
-          const u32x4 w = {lo[0], lo[1], hi[0], hi[1]};
-          acc[h][db] = mfma32x32x16(__builtin_bit_cast(bf16x8, w), p[h][j], acc[h][db]);
+      for (int h = 0; h < HW; ++h) {
+        if (masked) mask_scores(s[h], opaque(kb), lim, gone, lane);
+        const float mx = column_max(s[h]);
+        if (!ALONE || __any(mx > top[h])) {
+          grow(st[h], fmaf(halves_max(mx), c, -st[h].shift), acc[h]);
+          if (ALONE) top[h] = (st[h].shift + st[h].lag) * (1.f / c);
         }
-    wait_lds();
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) fetch_values(next);
+        block_probs(s[h], st[h], c, p[h][0], p[h][1]);
+      }
+      if (more) wait_vm_lds<4 * HW>(); else wait_vm_lds<0>();
+#pragma unroll
+      for (int h = 0; h < HW; ++h) {
+        bf16x8 v[2][2];
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const char* from = vt + 16 * j * L::kTok;
+            const int x = v_at ^ ((8 * h + 4 * db) << 4);
+            const u32x2 lo = lds_read_tr16(from + x);
+            // token + 8: the permutation of two heads differs in its lowest bit
+            const u32x2 hi = lds_read_tr16(from + 8 * L::kTok + (HW == 1 ? x : x ^ 16));
+            const u32x4 w = {lo[0], lo[1], hi[0], hi[1]};
+            v[db][j] = __builtin_bit_cast(bf16x8, w);
+          }
+        if (careful && masked) {
+          add_wild(acc[h], lim - kb, [&](int key, int piece) {
+            return *reinterpret_cast<const u32x2*>(
+                vt + key * L::kTok + (((8 * h + piece) ^ few_swz<HW>(key)) << 4) + 8 * half);
+          });
+#pragma unroll
+          for (int db = 0; db < 2; ++db) {
+            drop_wild(v[db][0]);
+            drop_wild(v[db][1]);
+          }
+        }
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[h][db] = mfma32x32x16(v[db][j], p[h][j], acc[h][db]);
+      }
+      wait_lds();
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) fetch_values(next);
+    }
+  };
+  bool careful = ALONE;
+  if constexpr (!ALONE) {
+    run(Plain{});
+    if (it.key1 > least) {
+      uint32_t wild = 0;
+#pragma unroll
+      for (int h = 0; h < HW; ++h) wild |= wild_bits(acc[h][0]) | wild_bits(acc[h][1]);
+      careful = __any(wild != 0);
+    }
   }
+  if (careful) run(Careful{});
   wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS
 
   // the wave's states to LDS: row r of head h at (32 h + r) * 256 bytes, 16-byte
@@ -388,29 +499,29 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
   }
 }
 
-// Merges the waves' states of an item and writes rows or partial results; eight
-// threads a row.
-template <int HW>
+// Merges the states of an item that waves first .. first + WAVES - 1 hold, and writes
+// rows or partial results; eight threads of these waves a row.
+template <int HW, int WAVES>
 __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it, int pair,
-                                          const char* lds, const float (*lm)[64],
-                                          const float (*ll)[64]) {
-  const int d8 = threadIdx.x & 7;
-  for (int x = threadIdx.x >> 3; x < HW * it.nrows; x += 8 * kKeyWaves) {
+                                          int first, int thread, const char* lds,
+                                          const float (*lm)[64], const float (*ll)[64]) {
+  const int d8 = thread & 7;
+  for (int x = thread >> 3; x < HW * it.nrows; x += 8 * WAVES) {
     const int h = x >= it.nrows ? 1 : 0, r = x - h * it.nrows, at = 32 * h + r;
     const int kvh = HW * pair + h;
     float top = kNegInf;
 #pragma unroll
-    for (int w = 0; w < kKeyWaves; ++w) top = fmaxf(top, lm[w][at]);
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lm[first + w][at]);
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKeyWaves; ++w) {
-      const float m = lm[w][at];
+    for (int w = 0; w < WAVES; ++w) {
+      const float m = lm[first + w][at];
       const float wt = m == kNegInf ? 0.f : fast_exp2(m - top);
-      sum = fmaf(wt, ll[w][at], sum);
+      sum = fmaf(wt, ll[first + w][at], sum);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(lds + w * FewLds<HW>::kWave + at * 256 +
-                                                        (((2 * d8 + q) ^ (r & 15)) << 4));
+        const f32x4 y = *reinterpret_cast<const f32x4*>(
+            lds + (first + w) * FewLds<HW>::kWave + at * 256 + (((2 * d8 + q) ^ (r & 15)) << 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[4 * q + i] = fmaf(wt, y[i], o[4 * q + i]);
       }
@@ -434,6 +545,23 @@ __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it
   }
 }
 
+// A many-rows item again: every wave its own 64 rows, 32 at a time.
+template <bool ALIKE>
+__device__ __forceinline__ void many_again(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
+                                           float (&lm)[4][64], float (&ll)[4][64]) {
+  const int wave = uniform(threadIdx.x >> 6);
+  __syncthreads();  // the waves are done with what LDS held
+#pragma unroll 1
+  for (int row = 64 * wave; row < min(64 * wave + 64, it.nrows); row += 32) {
+    const ItemView part = {it.start, it.row0 + row, min(32, it.nrows - row), it.base, it.key0,
+                           it.key1,  it.partial < 0 ? -1 : it.partial + row, it.sequence};
+    few_rows<1, ALIKE, true>(a, part, kvh, wave, lds + wave * FewLds<1>::kWave, lm[wave], ll[wave]);
+    wave_lds_fence();
+    few_merge<1, 1>(a, part, kvh, wave, threadIdx.x & 63, lds, lm, ll);
+    wave_lds_fence();
+  }
+}
+
 // --------------------------------------------------------------------------
 // Up to 256 rows: the waves split the rows, 64 (two 32-row blocks) each, so that
 // every K and V operand read from LDS feeds two MFMAs.
@@ -441,9 +569,10 @@ __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it
 constexpr int kSlotBytes = 2 * kTileBytes;  // 64 keys of K and of V
 constexpr int kSlots = 4;
 
+// False if the item has to be done again, carefully.
 template <bool ALIKE>
-__device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
-                                          int (*lost)[4]) {
+__device__ __forceinline__ bool many_rows(const PagedArgs& a, const ItemView& it, int kvh, char* lds,
+                                          int (*lost)[4], int* flags) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
   bf16x8 qf[2][4];
@@ -467,13 +596,8 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
   const int stages = (it.key1 - it.key0 + 63) >> 6;
   f32x16 acc[2][2];
   RowState st[2];
-#pragma unroll
-  for (int rb = 0; rb < 2; ++rb) {
-    acc[rb][0] = acc[rb][1] = zero16();
-    st[rb] = {0.f, kNegInf, 0.f, 0.f};
-  }
   const float c = a.scale_log2, inv_c = 1.f / c;
-  float top[2] = {kNegInf, kNegInf};  // scores from which a row's shift moves
+  float top[2];  // scores from which a row's shift moves
 
   // A wave fetches keys 16 wave .. + 15 of a stage: two groups of eight, in one page
   // where the page size is a multiple of 16.  The table's entries of the stage that is
@@ -521,14 +645,6 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
     }
     lost[s & (kSlots - 1)][wave] = gone;  // bit g: keys 8 g .. of the stage have no page
   };
-#pragma unroll
-  for (int s = 0; s < kSlots - 1; ++s)
-    if (s < stages) {
-      load_entries(s);
-      fetch(s);
-    }
-  if (kSlots - 1 < stages) load_entries(kSlots - 1);
-
   const int tr_row = tr_row_of(lane), tr_col = tr_col_of(lane);
   auto read_keys = [&](const char* kt, int k0, bf16x8 (&k)[4]) {
 #pragma unroll
@@ -587,6 +703,19 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
     for (int rb = 0; rb < 2; ++rb) mx[rb] = column_max(next[rb]);
   };
 
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    acc[rb][0] = acc[rb][1] = zero16();
+    st[rb] = {0.f, kNegInf, 0.f, 0.f};
+    top[rb] = kNegInf;
+  }
+#pragma unroll
+  for (int s = 0; s < kSlots - 1; ++s)
+    if (s < stages) {
+      load_entries(s);
+      fetch(s);
+    }
+  if (kSlots - 1 < stages) load_entries(kSlots - 1);
   f32x16 sa[2], sb[2];
   float mx[2];
   for (int s = 0; s < stages; ++s) {
@@ -611,11 +740,21 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb) mx[rb] = column_max(sa[rb]);
     }
-    step(kb, gone & 15, sa, sb, mx, kt, 32, vt, 0);
     // (behind the last stage the next block's scores are of whatever lies there, unused)
+    step(kb, gone & 15, sa, sb, mx, kt, 32, vt, 0);
     step(kb + 32, gone >> 4, sb, sa, mx, kn, 0, vt, 32);
   }
   wait_vm_lds<0>();  // no DMA may still target this workgroup's LDS
+  if (it.key1 > row_limit(a, it, 0)) {
+    uint32_t wild = 0;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) wild |= wild_bits(acc[rb][0]) | wild_bits(acc[rb][1]);
+    const bool mine = __any(wild != 0);
+    flags[wave] = mine;
+    __syncthreads();
+    const int4 any = *reinterpret_cast<const int4*>(flags);
+    if (uniform(any.x | any.y | any.z | any.w)) return false;
+  }
 
   const int elane = fresh_lane_id();
   const int half = elane >> 5;
@@ -630,7 +769,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
       store_bf16_rows(reinterpret_cast<bf16*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2)),
                       acc[rb], has ? 1.f / l : 0.f, has, half);
     }
-    return;
+    return true;
   }
   // Partial results go through LDS (16 KB of the ring a wave, 16-byte pieces of a row
   // permuted by the row), so that a store covers four whole rows.
@@ -661,6 +800,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const ItemView& it
       *reinterpret_cast<f32x4*>(a.acc + (first + r) * kD + 4 * piece) =
           *reinterpret_cast<const f32x4*>(rows + r * 256 + ((piece ^ (r & 15)) << 4));
   }
+  return true;
 }
 
 // Workgroups: the few-rows shares' (head pairs fastest) and the many-rows shares'
@@ -686,9 +826,9 @@ void paged_attn_bf16_kernel(PagedArgs a) {
     for (int item = ld_const(a.shares[kFew], share); item < end; ++item) {
       const ItemView it = load_item(a.items[kFew], item);
       if (it.nrows < 1) continue;
-      few_rows<HW, ALIKE>(a, it, pair, wave, lds + wave * FewLds<HW>::kWave, lm[wave], ll[wave]);
+      few_rows<HW, ALIKE, false>(a, it, pair, wave, lds + wave * FewLds<HW>::kWave, lm[wave], ll[wave]);
       __syncthreads();
-      few_merge<HW>(a, it, pair, lds, lm, ll);
+      few_merge<HW, kKeyWaves>(a, it, pair, 0, threadIdx.x, lds, lm, ll);
       __syncthreads();
     }
     return;
@@ -700,7 +840,9 @@ void paged_attn_bf16_kernel(PagedArgs a) {
   for (int item = ld_const(a.shares[kMany], share); item < end; ++item) {
     const ItemView it = load_item(a.items[kMany], item);
     if (it.nrows < 1) continue;
-    many_rows<ALIKE>(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(lm));
+    if (!many_rows<ALIKE>(a, it, kvh, lds, reinterpret_cast<int(*)[4]>(lm),
+                          reinterpret_cast<int*>(ll)))
+      many_again<ALIKE>(a, it, kvh, lds, lm, ll);
     __syncthreads();
   }
 }
@@ -759,56 +901,83 @@ __device__ __forceinline__ void f32_item(const PagedArgs& a, const ItemView& it,
       if (gone >> g & 1) x[2 * g] = x[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
 
-  f32x16 acc[2] = {zero16(), zero16()};
-  float m = kNegInf, l = 0.f;
+  f32x16 acc[2];
+  float m, l;
   const float c = a.scale_log2;
-  int b = wave;
-  if (b < blocks) fetch(b);
-  __syncthreads();
-  for (; b < blocks; b += 4) {
-    const int kb = it.key0 + 32 * b;
-    const int gone = fetched_gone;
-    if (gone) {
-      drop(kx, gone);
-      drop(vx, gone);
-    }
-    wave_lds_fence();
-    f32_store(kt[wave], lane, kx, it.key1 - kb);
-    f32_store(vt[wave], lane, vx, it.key1 - kb);
-    wave_lds_fence();
-    if (b + 4 < blocks) fetch(b + 4);
-    f32x16 s = zero16();
+  auto run = [&](auto how) {
+    constexpr bool careful = decltype(how)::value;
+    acc[0] = acc[1] = zero16();
+    m = kNegInf;
+    l = 0.f;
+    int b = wave;
+    if (b < blocks) fetch(b);
+    if (!careful) __syncthreads();  // the query's rows
+    for (; b < blocks; b += 4) {
+      const int kb = it.key0 + 32 * b;
+      const int gone = fetched_gone;
+      if (gone) {
+        drop(kx, gone);
+        drop(vx, gone);
+      }
+      wave_lds_fence();
+      f32_store(kt[wave], lane, kx, it.key1 - kb);
+      f32_store(vt[wave], lane, vx, it.key1 - kb);
+      const bool masked = kb + 32 > least || gone;
+      wave_lds_fence();
+      if (b + 4 < blocks) fetch(b + 4);
+      f32x16 s = zero16();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const f32x4 kr = kt[wave].row4(lane, j), qr = qt.row4(lane, j);
+      for (int j = 0; j < 8; ++j) {
+        const f32x4 kr = kt[wave].row4(lane, j), qr = qt.row4(lane, j);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = mfma32x32x2(kr[e], qr[e], s);
-    }
-    if (kb + 32 > least || gone) mask_scores(s, kb, lim, gone, lane);
-    const float mx = halves_max(column_max(s));
-    if (__any(mx > m)) {
-      const float mnew = fmaxf(m, mx);
-      const float alpha = mnew == kNegInf ? 1.f : fast_exp2((m - mnew) * c);
-      m = mnew;
-      l *= alpha;
+        for (int e = 0; e < 4; ++e) s = mfma32x32x2(kr[e], qr[e], s);
+      }
+      if (masked) mask_scores(s, kb, lim, gone, lane);
+      const float mx = halves_max(column_max(s));
+      if (__any(mx > m)) {
+        const float mnew = fmaxf(m, mx);
+        const float alpha = mnew == kNegInf ? 1.f : fast_exp2((m - mnew) * c);
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          acc[0][r] *= alpha;
+          acc[1][r] *= alpha;
+        }
+      }
+      const float mc = m == kNegInf ? 0.f : m * c;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        acc[0][r] *= alpha;
-        acc[1][r] *= alpha;
+        s[r] = fast_exp2(fmaf(s[r], c, -mc));
+        l += s[r];
+      }
+      if (careful && masked) {
+        // (as in the bf16 kernel)
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key)
+#pragma unroll
+          for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float x = vt[wave].x[key * kF32Pitch + 32 * db + acc_row(r, lane)];
+              const uint32_t mine = kb + key < lim ? wild_mask(x) : 0u;
+              acc[db][r] = add_any(acc[db][r], __uint_as_float(__float_as_uint(x) & mine));
+            }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float v0 = vt[wave].col(lane, 0, r), v1 = vt[wave].col(lane, 1, r);
+        if (careful && masked) {
+          v0 = __uint_as_float(__float_as_uint(v0) & ~wild_mask(v0));
+          v1 = __uint_as_float(__float_as_uint(v1) & ~wild_mask(v1));
+        }
+        acc[0] = mfma32x32x2(v0, s[r], acc[0]);
+        acc[1] = mfma32x32x2(v1, s[r], acc[1]);
       }
     }
-    const float mc = m == kNegInf ? 0.f : m * c;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(fmaf(s[r], c, -mc));
-      l += s[r];
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      acc[0] = mfma32x32x2(vt[wave].col(lane, 0, r), s[r], acc[0]);
-      acc[1] = mfma32x32x2(vt[wave].col(lane, 1, r), s[r], acc[1]);
-    }
-  }
+  };
+  run(Plain{});
+  if (it.key1 > least && __any((wild_bits(acc[0]) | wild_bits(acc[1])) != 0)) run(Careful{});
   l = halves_sum(l);
   if (lane < 32) {
     lm[wave][lane] = m == kNegInf ? kNegInf : m * c;
@@ -904,7 +1073,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     f32x4 x[4], y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // (past the last item its results again, with no weight)
+      // (past the last item its results again, which then count as none)
       const size_t at = base + (size_t)min(s0 + i * sp, splits - 1) * step;
       ml[i] = a.ml[at];
       x[i] = *reinterpret_cast<const f32x4*>(a.acc + at * kD + d0);
@@ -913,7 +1082,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     float top = m;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (s0 + i * sp >= splits) ml[i] = make_float2(kNegInf, 0.f);
+      if (s0 + i * sp >= splits) {
+        ml[i] = make_float2(kNegInf, 0.f);
+        x[i] = y[i] = f32x4{0.f, 0.f, 0.f, 0.f};  // (0 times an infinity is NaN)
+      }
       top = fmaxf(top, ml[i].x);
     }
     const float wa = m == kNegInf ? 0.f : fast_exp2(m - top);

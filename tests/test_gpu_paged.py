@@ -186,6 +186,34 @@ def test_what_no_query_sees_does_not_count(junk, dtype, device):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("where", ["value", "key"])
+def test_a_later_token_does_not_reach_an_earlier_one(where, junk, dtype, device):
+    """New tokens with an infinity or NaN: earlier ones of their chunk are as without it."""
+    spans = [(6, 40), (100, 300), (3, 3), (260, 400)]
+    b = Batch(spans, 4, 2, 16, dtype, device, spread=1.0)
+    clean = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    pages = b.value_pages if where == "value" else b.key_pages
+    hit = []  # (sequence's first token, its new tokens, the new token that is hit)
+    for r, i in ((0, 4), (1, 37), (1, 90), (2, 2), (3, 130)):
+        n, context = spans[r]
+        page, slot = b.slots(r, [context - n + i])
+        pages[page, slot, 1, 5] = junk  # one dim of the second key head
+        hit.append((int(b.starts[r]), n, i))
+    out = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    sees = torch.zeros(b.tokens, dtype=torch.bool, device=device)
+    for start, n, i in hit:
+        sees[start + i:start + n] = True
+    assert torch.equal(out[~sees], clean[~sees])
+    assert torch.equal(out[:, :2], clean[:, :2])  # the other key head's queries
+    if where == "value":
+        dims = torch.arange(64, device=device) != 5
+        assert torch.equal(out[sees][:, 2:][..., dims], clean[sees][:, 2:][..., dims])
+        wild = out[sees][:, 2:, 5]
+        assert bool(torch.isnan(wild).all() if junk != junk else (wild == junk).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_pages_outside_the_pool_hold_no_keys(dtype, device):
     spans = [(1, 200), (2, 180), (90, 400), (1, 16), (50, 50)]
     b = Batch(spans, 4, 2, 16, dtype, device)
