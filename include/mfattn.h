@@ -285,7 +285,8 @@ int mf_rotate(const void* q, long long q_stride, const void* k,
  * have negative positions: not written, and attending to nothing.
  * The plan serves every layer of the step, on any stream ordered after it; it
  * depends on the batch's shapes, and on the table's entries while it is used:
- * the table must not change between the plan and the calls that take both. */
+ * the table must not change between the plan and the calls that take both.
+ * The functions of sizes return 0 for sizes that the calls refuse. */
 size_t mf_paged_plan_bytes(int sequences, int tokens, int q_heads,
                            int kv_heads, int dtype);
 int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
@@ -304,8 +305,9 @@ int mf_paged_plan(const int32_t* query_starts, const int32_t* context_lengths,
  * queries.  k, v [tokens, kv_heads, 64]; token strides in elements.
  * k_pages, v_pages: [pages][page_size][kv_heads][64] with strides
  * {page, slot, head} in elements (HOST arrays of 3; at most 2^26 between slots
- * and 2^29 between heads), the last dimension dense.
- * Where two tokens have the same page and slot, either remains. */
+ * and 2^29 between heads), the last dimension dense; slots that overlap are
+ * refused.  Where two tokens have the same page and slot, either remains
+ * (and of a vector's pieces some of each may). */
 int mf_paged_append(const void* q, long long q_stride, const void* k,
                     long long k_stride, const void* v, long long v_stride,
                     const void* q_gain, const void* k_gain, float eps,

@@ -2,6 +2,7 @@
 // launches.  Every check here runs on the host before anything is enqueued,
 // so a malformed call returns an MF_ERR_* code (and leaves a message for
 // mf_last_error) without touching the GPU.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -557,6 +558,13 @@ int check_token_stride(const char* what, long long stride, int heads, int dim) {
   return MF_OK;
 }
 
+// The sizes that check_paged lets through, for functions that return a size.
+bool paged_sizes(int sequences, int tokens, int q_heads, int kv_heads) {
+  return sequences >= 1 && sequences <= mf::kMaxSequences && tokens >= 1 && q_heads >= 1 &&
+         kv_heads >= 1 && kv_heads <= 1024 && q_heads % kv_heads == 0 &&
+         (long long)tokens * q_heads <= (1ll << 26);
+}
+
 int check_paged(int dtype, int sequences, int tokens, int q_heads, int kv_heads) {
   if (dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16)
     return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
@@ -607,6 +615,26 @@ int check_page_strides(const char* what, const long long* s, int page_size, int 
   if (s[2] > (1ll << 29))
     return fail(MF_ERR_SHAPE, "%s: %lld elements between heads (at most 2^29)", what, s[2]);
   *out = {s[0], s[1], s[2]};
+  return MF_OK;
+}
+
+// Pages that are written: no two slots share memory.
+int check_apart(const char* what, const mf::PagedStrides& s, int pages, int page_size, int kv_heads) {
+  struct Dim {
+    long long stride;
+    int count;
+  } d[3] = {{s.page, pages}, {s.slot, page_size}, {s.head, kv_heads}};
+  std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  long long row = mf::kD;
+  for (const Dim& x : d) {
+    if (x.count <= 1) continue;
+    if (x.stride < row)
+      return fail(MF_ERR_SHAPE, "%s: strides {%lld, %lld, %lld} of page, slot and head overlap", what,
+                  s.page, s.slot, s.head);
+    if (x.stride > (1ll << 60) / x.count)
+      return fail(MF_ERR_SHAPE, "%s: %lld elements between %d rows", what, x.stride, x.count);
+    row += x.stride * (x.count - 1);
+  }
   return MF_OK;
 }
 
@@ -661,7 +689,7 @@ int mf_rotate(const void* q, long long q_stride, const void* k, long long k_stri
 }
 
 size_t mf_paged_plan_bytes(int sequences, int tokens, int q_heads, int kv_heads, int dtype) {
-  if (sequences < 1 || tokens < 1 || q_heads < 1 || kv_heads < 1) return 0;
+  if (!paged_sizes(sequences, tokens, q_heads, kv_heads)) return 0;
   return mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32).total;
 }
 
@@ -718,6 +746,8 @@ int mf_paged_append(const void* q, long long q_stride, const void* k, long long 
   mf::PagedStrides ks, vs;
   if (int rc = check_page_strides("k_pages", k_strides, page_size, kv_heads, &ks)) return rc;
   if (int rc = check_page_strides("v_pages", v_strides, page_size, kv_heads, &vs)) return rc;
+  if (int rc = check_apart("k_pages", ks, pages, page_size, kv_heads)) return rc;
+  if (int rc = check_apart("v_pages", vs, pages, page_size, kv_heads)) return rc;
   const mf::PagedLayout lay =
       mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32);
   const mf::PagedToken* records = reinterpret_cast<const mf::PagedToken*>(
@@ -733,7 +763,7 @@ int mf_paged_append(const void* q, long long q_stride, const void* k, long long 
 
 size_t mf_paged_attn_workspace_bytes(int sequences, int tokens, int q_heads, int kv_heads,
                                      int dtype) {
-  if (sequences < 1 || tokens < 1 || q_heads < 1 || kv_heads < 1) return 0;
+  if (!paged_sizes(sequences, tokens, q_heads, kv_heads)) return 0;
   return mf::paged_workspace_bytes(
       mf::paged_layout(sequences, tokens, q_heads / kv_heads, kv_heads, dtype == MF_DTYPE_F32),
       kv_heads);

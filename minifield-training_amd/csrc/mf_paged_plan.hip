@@ -159,7 +159,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       const Span s = span_of(a, r);
       const long long rows = (long long)s.count * a.G;
       const int tr = is_few(a, rows) ? kFewRows : kManyRows;
-      tiles = (int)((rows + tr - 1) / tr);
+      // (never more than the bound, unless sequences overlap)
+      tiles = (int)min((rows + tr - 1) / tr, (long long)a.lay.cap_tiles);
       l.start[r] = s.start;
       l.count[r] = s.count;
       l.context[r] = s.context;
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     Two total;
     const Two ahead = block_prefix({tiles, 0}, l.sums, total);
     if (r < a.R) l.tiles[r] = ntiles + ahead.a;
-    ntiles += total.a;
+    ntiles = min(ntiles + total.a, 1 << 30);
   }
   ntiles = min(ntiles, a.lay.cap_tiles);
   __syncthreads();

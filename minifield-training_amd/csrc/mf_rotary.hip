@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void turn_rows_kernel(TurnArgs a) {
       Vec y0 = x0[j], y1 = x1[j];
       if constexpr (PAGED) {
         const void* gain = kind[j] == 0 ? a.gain[0] : a.gain[1];
-        if (gain) {  // (the same for every unit: both kinds have one or none)
+        if (gain) {  // (the same for a head's lanes)
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < V; ++i) ss = fmaf(u[i], u[i], fmaf(w[i], w[i], ss));
@@ -239,11 +239,12 @@ static hipError_t launch_turn_v(TurnArgs& a, hipStream_t stream) {
   a.div_units = make_fastdiv(a.units);
   a.div_uph = make_fastdiv(a.uph);
   a.div_half = make_fastdiv(a.half < 1 ? 1 : a.half);
-  const unsigned grid = (unsigned)((a.tokens + a.tpb - 1) / a.tpb);
+  const long long grid = ((long long)a.tokens + a.tpb - 1) / a.tpb;
+  if (grid >= (1 << 24)) return hipErrorInvalidConfiguration;  // 2^32 threads
   if (per > 256)
-    hipLaunchKernelGGL((turn_rows_kernel<T, V, 2, PAGED>), dim3(grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((turn_rows_kernel<T, V, 2, PAGED>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((turn_rows_kernel<T, V, 1, PAGED>), dim3(grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((turn_rows_kernel<T, V, 1, PAGED>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -34,9 +34,10 @@ class Plan:
     """One step's new tokens and work items on the device, for every layer of the step."""
 
     __slots__ = ("buf", "page_table", "sequences", "tokens", "query_heads", "kv_heads", "pages",
-                 "page_size", "pool", "code", "nbytes", "q_shape", "k_shape", "table_stride", "width")
+                 "page_size", "pool", "code", "nbytes", "q_shape", "k_shape", "table_stride", "width",
+                 "stream")
 
-    def __init__(self, buf, page_table, sequences, tokens, query_heads, pool, code):
+    def __init__(self, buf, page_table, sequences, tokens, query_heads, pool, code, stream=0):
         self.buf, self.page_table = buf, page_table
         self.sequences, self.tokens, self.query_heads = sequences, tokens, query_heads
         self.pages, self.page_size, self.kv_heads, d = pool
@@ -44,6 +45,14 @@ class Plan:
         self.q_shape, self.k_shape = (tokens, query_heads, d), (tokens, self.kv_heads, d)
         self.width = page_table.shape[1]
         self.table_stride = page_table.stride(0) if sequences > 1 else self.width
+        self.stream = stream
+
+    def used_on(self, stream: int, device: torch.device) -> None:
+        """A launch on ``stream`` reads the plan: its memory is not given out anew before."""
+        if stream != self.stream:
+            current = torch.cuda.current_stream(device)
+            self.buf.record_stream(current)
+            self.page_table.record_stream(current)
 
     def token_records(self) -> torch.Tensor:
         """``[tokens, 4]`` int32: position, page (negative: none), slot and sequence of each."""
@@ -107,7 +116,9 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
     included.  Token position ``p`` of sequence ``r`` is slot ``p % page_size``
     of page ``page_table[r, p // page_size]``; entries outside the pool (-1, say,
     behind a context or for a page that was given up) hold no keys.  Nothing is
-    read back to the host.  The table must stay as it is while the plan is used.
+    read back to the host.  The table must stay as it is while the plan is used;
+    on another stream, once that waits for the plan's; a captured graph that reads
+    a plan made outside of it needs the plan kept.
     """
     if key_pages.dim() != 4:
         raise ValueError("pages must be [pages, page_size, heads, head_dim]")
@@ -128,10 +139,11 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
     device = require_device(key_pages, starts, contexts, table)
     nbytes, _ = _sizes(r, tokens, query_heads, kv_heads, code)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    stream = _raw_stream(device.index)
     launch(device, _lib.LIB.mf_paged_plan, starts.data_ptr(), contexts.data_ptr(), table.data_ptr(),
            table.stride(0) if r > 1 else width, r, tokens, width, page_size, pages, query_heads,
-           kv_heads, code, buf.data_ptr(), nbytes, _raw_stream(device.index))
-    return Plan(buf, table, r, tokens, query_heads, pool, code)
+           kv_heads, code, buf.data_ptr(), nbytes, stream)
+    return Plan(buf, table, r, tokens, query_heads, pool, code, stream)
 
 
 def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
@@ -184,12 +196,14 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     if query is not None:
         query, q_step = token_rows(query)
         out = torch.empty(plan.q_shape, dtype=dtype, device=device)
+    stream = _raw_stream(device.index)
+    plan.used_on(stream, device)
     launch(device, _lib.LIB.mf_paged_append, _ptr(query), q_step, key.data_ptr(), k_step,
            value.data_ptr(), v_step, _ptr(qg), _ptr(kg), eps, *turn, code, n, plan.sequences,
            plan.query_heads, plan.kv_heads, d, plan.page_size, plan.pages, plan.buf.data_ptr(),
            plan.nbytes, key_pages.data_ptr(), value_pages.data_ptr(),
            _pool_strides(key_pages.stride(), plan.pool),
-           _pool_strides(value_pages.stride(), plan.pool), _ptr(out), _raw_stream(device.index))
+           _pool_strides(value_pages.stride(), plan.pool), _ptr(out), stream)
     return out
 
 
@@ -218,6 +232,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
         raise ValueError("paged.attention has no backward; call it under torch.no_grad()")
     device = require_device(query, key_pages, value_pages, plan.buf)
     query, q_step = token_rows(query)
+    if query.data_ptr() % 16:
+        query = query.clone()
     zero_rest = out is None
     if zero_rest:
         out = torch.empty(shape, dtype=dtype, device=device)
@@ -227,12 +243,14 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     n, hq, d = shape
     _, ws_bytes = _sizes(plan.sequences, n, hq, plan.kv_heads, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    stream = _raw_stream(device.index)
+    plan.used_on(stream, device)
     launch(device, _lib.LIB.mf_paged_attn, query.data_ptr(), q_step, key_pages.data_ptr(),
            value_pages.data_ptr(), _pool_strides(key_pages.stride(), plan.pool),
            _pool_strides(value_pages.stride(), plan.pool), plan.page_table.data_ptr(),
            plan.table_stride, code, n, plan.sequences, plan.width, plan.page_size, plan.pages, hq,
            plan.kv_heads, d, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes,
-           zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes, _raw_stream(device.index))
+           zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes, stream)
     return out
 
 

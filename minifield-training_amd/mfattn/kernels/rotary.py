@@ -88,9 +88,19 @@ class Rotary:
         # the C ABI's arguments: host array, rotary_dim, interleaved, magnitude
         self._args = (ctypes.addressof(self._turns), r, int(self.interleaved), self.magnitude)
 
+    def __reduce__(self):
+        # (copies and pickles make turns of their own: the arguments hold an address)
+        return _rotary_of, (self.head_dim, self.rotary_dim, self.interleaved, self.frequencies,
+                            self.magnitude)
+
     def __repr__(self) -> str:
         return (f"Rotary(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, "
                 f"interleaved={self.interleaved}, magnitude={self.magnitude:g})")
+
+
+def _rotary_of(head_dim, rotary_dim, interleaved, frequencies, magnitude) -> Rotary:
+    return Rotary(head_dim, rotary_dim=rotary_dim, interleaved=interleaved,
+                  frequencies=frequencies, magnitude=magnitude)
 
 
 def _scaled(r, theta, scaling, factor, length, fast, slow) -> list[float]:
@@ -149,6 +159,8 @@ class Rotate(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
         if dq is None and dk is None:
             return None, None, None, None
         dq, dk = _launch(dq, dk, ctx.saved_tensors[0], ctx.rotary, True)
@@ -160,9 +172,12 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
     """Rotate ``query [B, T, Hq, D]`` and ``key [B, T, Hkv, D]`` (or ``[N, H, D]`` both).
 
     ``positions`` are integers: a scalar, ``[T]`` or ``[B, T]`` (``[N]`` for
-    three dimensions); ``None`` means ``0 .. T-1`` on every row.  ``key`` may be
-    ``None``.  Slices of one projection are read where they are as long as each
-    head is dense and tokens are evenly spaced.  Differentiable in both, once.
+    three dimensions) in int32's range; ``None`` means ``0 .. T-1`` on every row.
+    ``key`` may be ``None``.  Slices of one projection are read where they are as
+    long as each head is dense and tokens are evenly spaced.  Differentiable in
+    both, once.  A backward is captured into a graph together with its forward
+    and while no eager graph of the same leaves is alive, as for any operation:
+    autograd accumulates a leaf's gradient on the stream of its oldest graph.
     """
     if not isinstance(rotary, Rotary):
         raise ValueError("rotary must be a Rotary")
@@ -175,6 +190,11 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
                             or key.dtype != query.dtype):
         raise ValueError("query and key must share batch, length, head_dim and dtype")
     dtype_code(query)
+    if positions is not None:
+        positions = torch.as_tensor(positions)
+        if (positions.is_floating_point() or positions.is_complex()
+                or positions.dtype is torch.bool):
+            raise ValueError(f"positions must be integers, got {positions.dtype}")
     device = require_device(query) if key is None else require_device(query, key)
     if query.dim() == 4:
         pos = _positions(positions, query.shape[0], query.shape[1], device)

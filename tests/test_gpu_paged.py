@@ -338,6 +338,55 @@ def test_two_streams_share_a_plan(device):
     assert all(torch.equal(o, want) for group in outs for o in group)
 
 
+def test_a_plan_outlives_its_last_use_on_another_stream(device):
+    """A plan that is let go while another stream still reads it is not overwritten."""
+    b = Batch([(1, 3000), (50, 900), (1, 10)], 8, 4, 16, BF, device)
+    want = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    starts, contexts, table = b.on_device()
+    table = table.long()  # the plan makes an int32 copy that only it holds
+    big = torch.randn(2048, 2048, device=device)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    plan = paged.plan(starts, contexts, table, b.key_pages, tokens=b.tokens, query_heads=8)
+    size = plan.buf.numel()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            big = big @ big * 1e-3  # work before the attention on its stream
+        out = paged.attention(b.q, b.key_pages, b.value_pages, plan)
+    shape = plan.page_table.shape
+    del plan
+    junk = [torch.full((size,), 255, dtype=torch.uint8, device=device) for _ in range(4)]
+    tables = [torch.full(shape, -1, dtype=torch.int32, device=device) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and junk and tables
+
+
+def test_a_misaligned_query_is_read(device):
+    b = Batch([(1, 300), (40, 90)], 4, 2, 16, BF, device)
+    base = torch.zeros(b.q.numel() + 1, dtype=BF, device=device)
+    q = base[1:].view(b.q.shape)
+    q.copy_(b.q)
+    want = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    assert q.data_ptr() % 16 and torch.equal(
+        paged.attention(q, b.key_pages, b.value_pages, b.plan()), want)
+
+
+def test_starts_in_disorder_stay_in_bounds(device):
+    """What comes out is not defined; that the calls end and write only their rows is."""
+    b = Batch([(20, 90)] * 6, 4, 2, 16, BF, device)
+    _, contexts, table = b.on_device()
+    n = b.tokens
+    for starts in ([0, n, 0, n, 0, n, 0], [n, 90, 60, 50, 20, 10, 0], [-5, 1 << 30, -(1 << 30), 7, n, 3, n],
+                   [0, 0, 0, 0, 0, 0, 0], [n] * 7):
+        plan = paged.plan(torch.tensor(starts, dtype=torch.int32, device=device), contexts, table,
+                          b.key_pages, tokens=n, query_heads=4)
+        guard = torch.full((n + 64, 4, 64), 3.0, device=device).to(BF)
+        paged.attention(b.q, b.key_pages, b.value_pages, plan, out=guard[:n])
+        torch.cuda.synchronize()
+        assert bool((guard[n:] == 3).all())
+
+
 def test_replayed_steps(device):
     """A captured step (plan, append, attention) replayed as its sequences grow."""
     b = Batch([(1, 60), (1, 300), (3, 20)], 8, 4, 16, BF, device, width=30, spare=70)

@@ -172,3 +172,47 @@ def test_replayed_graph_and_other_stream(device):
         torch.cuda.synchronize()
         eq, ek = rotary.rotate(q, k, rot, pos)
         assert torch.equal(qo, eq) and torch.equal(ko, ek), i
+
+
+def test_replayed_backward(device):
+    """Forward and backward captured together, replayed, against eager passes."""
+    rot = rotary.Rotary(64, rotary_dim=32, interleaved=True)
+    q, k = _qk(torch.bfloat16, (2, 40), 4, 2, 64, device)
+    q, k = (x.contiguous().requires_grad_() for x in (q, k))
+    wq, wk = torch.randn_like(q), torch.randn_like(k)
+
+    def grads():
+        qo, ko = rotary.rotate(q, k, rot)
+        return torch.autograd.grad((qo, ko), (q, k), (wq, wk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dq, dk = grads()
+    for i in range(3):
+        wq.normal_()
+        wk.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        eq, ek = grads()
+        assert torch.equal(dq, eq) and torch.equal(dk, ek), i
+
+
+def test_only_what_needs_a_gradient_gets_one(device):
+    rot = rotary.Rotary(64)
+    q, k = _qk(torch.float32, (2, 5), 4, 2, 64, device)
+    q, k = q.contiguous().requires_grad_(), k.contiguous()
+    qo, ko = rotary.rotate(q, k, rot)
+    (qo.sum() + ko.sum()).backward()
+    assert k.grad is None
+    close(q.grad, *turned(torch.ones(2, 5, 4, 64), torch.arange(5).expand(2, 5), rot, back=True), "dq")
+    # an expanded key: one head's gradient is the sum over its copies
+    one = torch.randn(2, 5, 1, 64, device=device, requires_grad=True)
+    _, ko = rotary.rotate(q.detach(), one.expand(2, 5, 3, 64), rot)
+    ko.sum().backward()
+    want, bound = turned(torch.ones(2, 5, 1, 64), torch.arange(5).expand(2, 5), rot, back=True)
+    close(one.grad, 3 * want, 3 * bound + 2 * 2.0 ** -24 * 3 * abs(want), "shared")

@@ -5,8 +5,10 @@ Python functions with host tensors, and through the C ABI with pointers that
 are never followed.
 """
 
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -174,6 +176,25 @@ def test_cache_pages_refuses():
     assert pages.shape == (8, 16, 4, 64) and table.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7]]
 
 
+def test_rotate_refuses_positions_that_are_no_integers():
+    q = torch.zeros(1, 3, 2, 64)
+    for positions in (torch.zeros(3), 1.5, torch.ones(1, 3, dtype=torch.bool), [0.0, 1.0, 2.0]):
+        with pytest.raises(ValueError, match="positions must be integers"):
+            rotary.rotate(q, None, rotary.Rotary(64), positions)
+
+
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy,
+                                   lambda r: pickle.loads(pickle.dumps(r))])
+def test_copies_have_turns_of_their_own(again):
+    rot = rotary.Rotary(128, theta=5e5, rotary_dim=64, interleaved=True, scaling="ramp", factor=8.0,
+                        original_length=4096)
+    turns = list(rot._turns)
+    new = again(rot)
+    assert new._args[0] == ctypes.addressof(new._turns) != rot._args[0]
+    assert list(new._turns) == turns and new._args[1:] == rot._args[1:] == (64, 1, rot.magnitude)
+    assert (new.head_dim, new.frequencies) == (128, rot.frequencies)
+
+
 # ---------------------------------------------------------------- C ABI
 
 
@@ -287,6 +308,13 @@ def _append(**kw):
     (dict(vst=_strides(-2048, 128, 64)), _lib.ERR_SHAPE, "overlap"),
     (dict(vst=_strides(2048, 1 << 27, 64)), _lib.ERR_SHAPE, "2^26"),
     (dict(kst=_strides(2048, 128, 1 << 30)), _lib.ERR_SHAPE, "2^29"),
+    # pages that are written have slots of their own
+    (dict(kst=_strides(0, 128, 64)), _lib.ERR_SHAPE, "overlap"),
+    (dict(vst=_strides(1024, 128, 64)), _lib.ERR_SHAPE, "overlap"),
+    (dict(vst=_strides(2048, 64, 64)), _lib.ERR_SHAPE, "overlap"),
+    (dict(vst=_strides(2048, 64, 1000)), _lib.ERR_SHAPE, "overlap"),
+    (dict(kst=_strides(64, 128, 64)), _lib.ERR_SHAPE, "overlap"),
+    (dict(kst=_strides(1 << 62, 128, 64)), _lib.ERR_SHAPE, "between"),
 ])
 def test_append_abi_refuses(kw, code, text):
     assert _append(**kw) == code
@@ -326,5 +354,8 @@ def test_sizes_of_plan_and_workspace():
         w = L.mf_paged_attn_workspace_bytes(64, n, 16, 8, 1)
         assert p > 0 and w > 0 and p + w > last
         last = p + w
+    for sizes in ((0, 1, 16, 8), (5000, 1, 16, 8), (1, 1, 16, 3), (1, 1, 2, 4), (1, 1 << 23, 16, 8),
+                  (1, 1, 2048, 2048), (2, 0, 16, 8), (-1, 4, 16, 8)):
+        assert L.mf_paged_plan_bytes(*sizes, 1) == L.mf_paged_attn_workspace_bytes(*sizes, 0) == 0
     assert L.mf_paged_plan_bytes(0, 1, 16, 8, 1) == 0
     assert L.mf_paged_attn_workspace_bytes(1, 1, 0, 8, 1) == 0
