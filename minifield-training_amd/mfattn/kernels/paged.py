@@ -35,7 +35,7 @@ class Plan:
 
     __slots__ = ("buf", "page_table", "sequences", "tokens", "query_heads", "kv_heads", "pages",
                  "page_size", "pool", "code", "nbytes", "q_shape", "k_shape", "table_stride", "width",
-                 "stream")
+                 "stream", "workspace")
 
     def __init__(self, buf, page_table, sequences, tokens, query_heads, pool, code, stream=0):
         self.buf, self.page_table = buf, page_table
@@ -46,6 +46,7 @@ class Plan:
         self.width = page_table.shape[1]
         self.table_stride = page_table.stride(0) if sequences > 1 else self.width
         self.stream = stream
+        self.workspace = _sizes(sequences, tokens, query_heads, self.kv_heads, code)[1]
 
     def used_on(self, stream: int, device: torch.device) -> None:
         """A launch on ``stream`` reads the plan: its memory is not given out anew before."""
@@ -60,11 +61,18 @@ class Plan:
 
 
 @functools.lru_cache(maxsize=256)
-def _pool_strides(strides: tuple[int, ...], shape: tuple[int, ...]):
+def _strides_of(strides: tuple[int, ...], shape: tuple[int, ...]):
     """The C ABI's (page, slot, head) strides; a dimension of one is never stepped over."""
     if strides[3] != 1 and shape[3] > 1:
         raise ValueError("the pages' last dimension must be dense")
     return (ctypes.c_longlong * 3)(*(s if n > 1 else 0 for s, n in zip(strides[:3], shape)))
+
+
+def _pool_strides(key_pages: torch.Tensor, value_pages: torch.Tensor, pool: tuple[int, ...]):
+    """Both pools' strides, which mostly are the same."""
+    k, v = key_pages.stride(), value_pages.stride()
+    strides = _strides_of(k, pool)
+    return strides, strides if k == v else _strides_of(v, pool)
 
 
 @functools.lru_cache(maxsize=256)
@@ -202,8 +210,7 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
            value.data_ptr(), v_step, _ptr(qg), _ptr(kg), eps, *turn, code, n, plan.sequences,
            plan.query_heads, plan.kv_heads, d, plan.page_size, plan.pages, plan.buf.data_ptr(),
            plan.nbytes, key_pages.data_ptr(), value_pages.data_ptr(),
-           _pool_strides(key_pages.stride(), plan.pool),
-           _pool_strides(value_pages.stride(), plan.pool), _ptr(out), stream)
+           *_pool_strides(key_pages, value_pages, plan.pool), _ptr(out), stream)
     return out
 
 
@@ -228,7 +235,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     if code != plan.code:
         raise ValueError("the plan is for pages of another dtype")
     _check_pool(key_pages, value_pages, plan)
-    if torch.is_grad_enabled() and _records_grad(query, key_pages, value_pages):
+    if (query.requires_grad or key_pages.requires_grad or value_pages.requires_grad) \
+            and torch.is_grad_enabled():
         raise ValueError("paged.attention has no backward; call it under torch.no_grad()")
     device = require_device(query, key_pages, value_pages, plan.buf)
     query, q_step = token_rows(query)
@@ -241,13 +249,13 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
           or out.device != device):
         raise ValueError(f"out must be a contiguous {dtype} {list(shape)} on {device}")
     n, hq, d = shape
-    _, ws_bytes = _sizes(plan.sequences, n, hq, plan.kv_heads, code)
+    ws_bytes = plan.workspace
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     stream = _raw_stream(device.index)
     plan.used_on(stream, device)
     launch(device, _lib.LIB.mf_paged_attn, query.data_ptr(), q_step, key_pages.data_ptr(),
-           value_pages.data_ptr(), _pool_strides(key_pages.stride(), plan.pool),
-           _pool_strides(value_pages.stride(), plan.pool), plan.page_table.data_ptr(),
+           value_pages.data_ptr(), *_pool_strides(key_pages, value_pages, plan.pool),
+           plan.page_table.data_ptr(),
            plan.table_stride, code, n, plan.sequences, plan.width, plan.page_size, plan.pages, hq,
            plan.kv_heads, d, d ** -0.5 if scale is None else scale, plan.buf.data_ptr(), plan.nbytes,
            zero_rest, out.data_ptr(), ws.data_ptr(), ws_bytes, stream)

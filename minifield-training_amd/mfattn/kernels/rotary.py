@@ -147,24 +147,25 @@ def _launch(q, k, positions, rotary, backward):
 
 
 class Rotate(torch.autograd.Function):
-    """Rotation of queries and keys in one launch; the backward turns the gradients back."""
+    """Rotation of queries and keys in one launch; the backward turns the gradients back,
+    which is a rotation again (and differentiable as one)."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, rotary):
+    def forward(ctx, q, k, positions, rotary, back):
         ctx.save_for_backward(positions)
-        ctx.rotary = rotary
+        ctx.rotary, ctx.back = rotary, back
         ctx.set_materialize_grads(False)
-        return _launch(q, k, positions, rotary, False)
+        return _launch(q, k, positions, rotary, back)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is None and dk is None:
-            return None, None, None, None
-        dq, dk = _launch(dq, dk, ctx.saved_tensors[0], ctx.rotary, True)
-        return dq, dk, None, None
+            return None, None, None, None, None
+        turn = Rotate.apply if torch.is_grad_enabled() else _launch
+        dq, dk = turn(dq, dk, ctx.saved_tensors[0], ctx.rotary, not ctx.back)
+        return dq, dk, None, None, None
 
 
 def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positions=None
@@ -175,7 +176,7 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
     three dimensions) in int32's range; ``None`` means ``0 .. T-1`` on every row.
     ``key`` may be ``None``.  Slices of one projection are read where they are as
     long as each head is dense and tokens are evenly spaced.  Differentiable in
-    both, once.  A backward is captured into a graph together with its forward
+    both.  A backward is captured into a graph together with its forward
     and while no eager graph of the same leaves is alive, as for any operation:
     autograd accumulates a leaf's gradient on the stream of its oldest graph.
     """
@@ -203,4 +204,4 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
     if not torch.is_grad_enabled() or not (query.requires_grad
                                            or (key is not None and key.requires_grad)):
         return _launch(query, key, pos, rotary, False)
-    return Rotate.apply(query, key, pos, rotary)
+    return Rotate.apply(query, key, pos, rotary, False)

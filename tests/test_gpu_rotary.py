@@ -216,3 +216,20 @@ def test_only_what_needs_a_gradient_gets_one(device):
     ko.sum().backward()
     want, bound = turned(torch.ones(2, 5, 1, 64), torch.arange(5).expand(2, 5), rot, back=True)
     close(one.grad, 3 * want, 3 * bound + 2 * 2.0 ** -24 * 3 * abs(want), "shared")
+
+
+def test_gradient_of_a_gradient(device):
+    """The backward is linear in the incoming gradient: its own backward turns forward again."""
+    rot = rotary.Rotary(64, rotary_dim=48)
+    q, k = _qk(torch.float32, (1, 7), 3, 3, 64, device)
+    q, k = (x.contiguous().requires_grad_() for x in (q, k))
+    g = torch.Generator(device=device).manual_seed(5)
+    wq, wk, uq, uk = (torch.randn(q.shape, generator=g, device=device) for _ in range(4))
+    wq.requires_grad_()
+    qo, ko = rotary.rotate(q, k, rot)
+    dq, dk = torch.autograd.grad((qo, ko), (q, k), (wq, wk), create_graph=True)
+    (ddq,) = torch.autograd.grad((dq * uq).sum() + (dk * uk).sum(), (wq,))
+    close(ddq, *turned(uq, torch.arange(7)[None], rot), "second")
+    # and the gradients are not functions of what was rotated
+    dq, _ = torch.autograd.grad(rotary.rotate(q, k, rot), (q, k), (wq, wk), create_graph=True)
+    assert torch.autograd.grad(dq.sum(), (q,), allow_unused=True) == (None,)
