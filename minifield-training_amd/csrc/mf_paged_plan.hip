@@ -216,7 +216,6 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     const bool split = x.items > 1;
     before = block_prefix({split ? (x.nrows + kJoinRows - 1) / kJoinRows : 0,
                            split ? x.items * x.nrows : 0}, l.sums, sum);
-    const int round_joins = sum.a;
     l.join_at[tid] = before.a;
     // (overlapping sequences, which no caller should make, could need more rows
     // than there are: they share the first ones)
@@ -247,13 +246,17 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       if (k > 0 || at == 0 || (y.units > 0 && y.unit0 > 0 && (y.unit0 - 1) / per != s))
         if (s < a.lay.target[y.kind]) shares[y.kind][s] = at;
     }
-    for (int i = tid; i < round_joins; i += kPlanThreads) {
-      const int j = last_not_above(l.join_at, round, i);
+    // (eight threads a tile: a search for each record's tile cost 4 us at 160 tiles of
+    // many rows)
+    for (int j = tid >> 3; j < round; j += kPlanThreads / 8) {
       const Tile y = l.tile[j];
-      const int r0 = (i - l.join_at[j]) * kJoinRows;
-      if (nrest.a + i < a.lay.cap_joins)
-        joins[nrest.a + i] = PagedJoin{y.start, y.row0 + r0, min(y.nrows - r0, kJoinRows),
-                                       y.row + r0, y.items, y.nrows, {0, 0}};
+      if (y.items <= 1) continue;
+      const int first = nrest.a + l.join_at[j];
+      for (int g = tid & 7; g * kJoinRows < y.nrows; g += 8)
+        if (first + g < a.lay.cap_joins)
+          joins[first + g] = PagedJoin{y.start, y.row0 + g * kJoinRows,
+                                       min(y.nrows - g * kJoinRows, kJoinRows),
+                                       y.row + g * kJoinRows, y.items, y.nrows, {0, 0}};
     }
     __syncthreads();
     nrest.a += sum.a;
