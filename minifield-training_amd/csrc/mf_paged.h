@@ -31,7 +31,16 @@ constexpr int kManyGroups = 512;
 // A tile of many rows writes up to 66 KB of partial results per item and KV head:
 // its shares have at least this many units.
 constexpr int kManyUnits = 4;
-constexpr int kJoinRows = 8;  // rows of a split tile that one workgroup joins
+// Rows of a split tile that one workgroup joins: 8, whose items it shares out to four
+// groups of threads, or 32 of a tile of many rows with up to 8 items, which leaves a
+// quarter of the records to the plan (of a mixed step 6.4 us against 6.9, of 20912
+// prompt tokens 7.3 against 8.7; the join takes the same).  32 rows of fp32 tiles
+// made their join 1 us longer.
+constexpr int kJoinRows = 8;
+constexpr int kJoinManyRows = 32, kJoinFewItems = 8;
+__host__ __device__ inline int join_rows(int kind, int items) {
+  return kind != 0 && items <= kJoinFewItems ? kJoinManyRows : kJoinRows;
+}
 
 // One new token: where it is and where its key and value go (page < 0: nowhere).
 struct PagedToken {
@@ -48,7 +57,7 @@ struct PagedItem {
   int sequence;
 };
 
-// Up to kJoinRows rows of a tile that was split, whose items' partial results are
+// Up to join_rows() rows of a tile that was split, whose items' partial results are
 // joined: item i's are rows partial + i * step.
 struct PagedJoin {
   int start, row0, nrows, partial, splits, step, pad[2];

@@ -214,7 +214,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     nitems.a += sum.a;
     nitems.b += sum.b;
     const bool split = x.items > 1;
-    before = block_prefix({split ? (x.nrows + kJoinRows - 1) / kJoinRows : 0,
+    const int jr = join_rows(x.kind, x.items);
+    before = block_prefix({split ? (x.nrows + jr - 1) / jr : 0,
                            split ? x.items * x.nrows : 0}, l.sums, sum);
     l.join_at[tid] = before.a;
     // (overlapping sequences, which no caller should make, could need more rows
@@ -252,11 +253,11 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       const Tile y = l.tile[j];
       if (y.items <= 1) continue;
       const int first = nrest.a + l.join_at[j];
-      for (int g = tid & 7; g * kJoinRows < y.nrows; g += 8)
+      const int rows = join_rows(y.kind, y.items);
+      for (int g = tid & 7; g * rows < y.nrows; g += 8)
         if (first + g < a.lay.cap_joins)
-          joins[first + g] = PagedJoin{y.start, y.row0 + g * kJoinRows,
-                                       min(y.nrows - g * kJoinRows, kJoinRows),
-                                       y.row + g * kJoinRows, y.items, y.nrows, {0, 0}};
+          joins[first + g] = PagedJoin{y.start, y.row0 + g * rows, min(y.nrows - g * rows, rows),
+                                       y.row + g * rows, y.items, y.nrows, {0, 0}};
     }
     __syncthreads();
     nrest.a += sum.a;
