@@ -25,12 +25,17 @@ constexpr int kMaxSequences = 4096;
 constexpr int kKeyWaves = 4;                // waves of a workgroup, which share a few-rows item's keys
 constexpr int kFewKeys = 32 * kKeyWaves;    // keys come in units of this many there
 constexpr int kManyKeys = 64;               // and of this many here
-// Shares times workgroups of a share: what is resident at once, two per CU.
+// Shares times workgroups of a share: what is resident at once, two per CU.  Many
+// rows with 256, 384, 640, 768 and 1024: three chunks 97, 93, 96, 96 and 94 us, with
+// 512 83; a chunk over 28 K keys 355, 324 and 320 with 640 and more, with 512 309.
+// Few rows with 1024: drafts 80 us, with 512 76.
 constexpr int kFewGroups = 512;
 constexpr int kManyGroups = 512;
 // A tile of many rows writes up to 66 KB of partial results per item and KV head:
-// its shares have at least this many units.
-constexpr int kManyUnits = 4;
+// its shares have at least this many units.  With 1, 2, 3, 4 and 8, us: 300 tokens
+// behind 500 15.7, 15.9, 19.4, 21.1 and 26.4; 128 behind 2000 17.7, 15.5, 16.2, 16.4
+// and 23.1; 8 x 200 behind 300 27.8, 27.6, 27.5, 26.5 and 32.0.
+constexpr int kManyUnits = 2;
 // Rows of a split tile that one workgroup joins: 8, whose items it shares out to four
 // groups of threads, or 32 of a tile of many rows with up to 8 items, which leaves a
 // quarter of the records to the plan (of a mixed step 6.4 us against 6.9, of 20912

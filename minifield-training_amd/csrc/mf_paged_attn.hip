@@ -9,9 +9,19 @@
 //     heads and takes 32-key blocks of its own, through a K and a V buffer of its
 //     own in LDS: no barrier until the states of waves that share an item are
 //     merged.  Bound: HBM, each cached key and value is read once for all rows of
-//     its head.
+//     its head.  One token for each of 64 sequences of 129 to 8192 keys, 16/8 heads
+//     (494 MB): 84 us, 5.9 TB/s, and the join 5; 24 sequences of 3 to 8 drafts, 24/8
+//     heads (391 MB): 69 and 5.  Half the workgroups a CU take 3 % longer.
 //   up to 256 rows (chunks), one KV head: every wave holds 64 rows, all share
-//     64-key stages in a ring of four.  Bound: MFMA and the softmax between.
+//     64-key stages in a ring of four, so an operand read from LDS feeds two MFMAs.
+//     2048 tokens behind 28672, 16/8 heads: 285 to 310 us with the join, 800 to 870
+//     TFLOP/s; 16384 behind none 620 to 650 (a large bf16 matrix product on the card:
+//     1190 TFLOP/s).  MFMA
+//     busy 41 % of the cycles, VALU 58 %, and the clock: the same launch over zeros
+//     takes 14 % less.  (8 maxima less a block changed nothing.)
+//
+// The same sequences with 24 rows on the second path: 101 us instead of 76, so few
+// rows end at 32, what one MFMA holds.
 //
 // Both use S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: an accumulator
 // column is a row of the batch, so its maximum and sum are in-lane reductions and
@@ -86,7 +96,8 @@ __device__ __forceinline__ long long row_offset(const PagedArgs& a, const PagedS
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // LDS DMAs of 16 bytes a lane (mf_lds.h) that are not kept in cache: a few-rows
-// item's keys and values are read once.
+// item's keys and values are read once.  Kept, 64 single tokens take 101 us instead
+// of 91, two over 128 K keys 101 instead of 89, drafts 86 instead of 76.
 __device__ __forceinline__ void dma16_once(const void* sbase, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
                :: "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
@@ -265,7 +276,8 @@ __device__ __forceinline__ int row_limit(const PagedArgs& a, const ItemView& it,
 //
 // A wave's K (and V) block in LDS is 32 tokens of HW 128-byte rows; a DMA moves
 // 8 / HW tokens, HW * 128 consecutive bytes of each where heads lie next to each
-// other.  (Two heads: 256-byte pieces of a token's row instead of 128.)  The
+// other.  (Two heads: 256-byte pieces of a token's row instead of 128; 64 single
+// tokens 91 us instead of 96, drafts 76 instead of 82.)  The
 // 16-byte pieces of a token are permuted by XOR with few_swz(token), so that the
 // 16 tokens that an operand read covers fall on all banks, and the transposing
 // reads of eight tokens too.
@@ -806,7 +818,8 @@ __device__ __forceinline__ bool many_rows(const PagedArgs& a, const ItemView& it
 // Workgroups: the few-rows shares' (head pairs fastest) and the many-rows shares'
 // (KV heads fastest, so that with 8 of them each XCD's L2 holds one head's keys), in
 // turn 256 of each while there are both: one for every CU, so that a CU's two
-// workgroups are one that waits for memory and one that computes.
+// workgroups are one that waits for memory and one that computes, the longer of the
+// many rows first (40 single tokens and three chunks 129 us; the other way round 152).
 // ALIKE: the pools of keys and values have the same strides.
 template <int HW, bool ALIKE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))

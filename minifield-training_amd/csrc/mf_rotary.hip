@@ -26,7 +26,9 @@
 // pairs, so no exchange between lanes is needed but the norm's sum, which runs
 // over the 32 / V lanes of a head.  A workgroup takes whole tokens, and its
 // threads make the tokens' cos and sin in LDS once, for all heads, while the
-// first rows are in flight.
+// first rows are in flight.  8 x 4096 tokens of 16/8 heads of 64 in bf16 (201 MB a
+// direction) 35 to 38 us, 5.3 to 5.7 TB/s; the append of 20912 tokens (171 MB) 29 us,
+// 5.9; of 64 tokens 4 us, a launch.
 #include "mf_paged.h"
 
 namespace mf {
