@@ -214,6 +214,27 @@ def test_a_later_token_does_not_reach_an_earlier_one(where, junk, dtype, device)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads, layout", [((3, 3), "apart"), ((5, 1), "slots"), ((6, 2), "heads")])
+def test_a_later_value_through_other_layouts_and_splits(heads, layout, dtype, device):
+    """The same with odd numbers of key heads, and strides and a context that split its keys."""
+    hq, hkv = heads
+    n, context, i = 150, 6000, 61
+    b = Batch([(n, context), (4, 900)], hq, hkv, 24, dtype, device, spread=1.0, layout=layout)
+    clean = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    for r, at in ((0, context - n + i), (1, 898)):
+        page, slot = b.slots(r, [at])
+        b.value_pages[page, slot, hkv - 1, 63] = float("inf")
+    out = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    sees = torch.zeros(b.tokens, dtype=torch.bool, device=device)
+    sees[i:n] = sees[n + 2:] = True
+    group = hq // hkv
+    assert torch.equal(out[~sees], clean[~sees])
+    assert torch.equal(out[:, :hq - group], clean[:, :hq - group])
+    assert torch.equal(out[sees][..., :63], clean[sees][..., :63])
+    assert bool((out[sees][:, hq - group:, 63] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_pages_outside_the_pool_hold_no_keys(dtype, device):
     spans = [(1, 200), (2, 180), (90, 400), (1, 16), (50, 50)]
     b = Batch(spans, 4, 2, 16, dtype, device)
