@@ -280,9 +280,10 @@ int mf_rotate(const void* q, long long q_stride, const void* k,
  * sequence r, the new ones included; token position p is slot p % page_size of
  * page page_table[r * table_stride + p / page_size], max_pages entries a row.
  * Page sizes are multiples of 8.  An entry outside [0, pages) holds no keys:
- * tokens there are not written, and not attended to.  A context beyond the
- * table's reach is read as that reach; new tokens that exceed their context
- * have negative positions: not written, and attending to nothing.
+ * tokens there are not written, and not attended to.  New tokens beyond the
+ * table's reach are not written either, and see the keys within it; those that
+ * exceed their context have negative positions: not written, and attending to
+ * nothing.
  * The plan serves every layer of the step, on any stream ordered after it; it
  * depends on the batch's shapes, and on the table's entries while it is used:
  * the table must not change between the plan and the calls that take both.

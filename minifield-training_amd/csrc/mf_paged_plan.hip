@@ -6,8 +6,8 @@
 // few thousand tiles): one token of one sequence 4.8 us, 64 sequences 6.2, 20912
 // prompt tokens 6.7.  A step's layers share the plan.
 //
-// Lengths are taken as they come: starts are held to [0, tokens] and a context to
-// the table's reach, so no length can make a later kernel leave its buffers.
+// Lengths are taken as they come: starts are held to [0, tokens], and keys end at the
+// table's reach, so no length can make a later kernel leave its buffers.
 #include "mf_paged.h"
 
 namespace mf {
@@ -71,7 +71,7 @@ __device__ __forceinline__ Span span_of(const PlanArgs& a, int r) {
   const int start = a.starts[r], next = a.starts[r + 1], context = a.contexts[r];
   s.start = min(max(start, 0), a.N);
   s.count = max(min(max(next, 0), a.N) - s.start, 0);
-  s.context = min(max(context, 0), a.width * a.page_size);  // (at most 2^30)
+  s.context = max(context, 0);
   return s;
 }
 
@@ -119,7 +119,7 @@ __device__ __forceinline__ Tile tile_of(const PlanArgs& a, const PlanLds& l, int
   x.nrows = (int)max(min((long long)tr, rows - x.row0), 0ll);
   const int last = fast_div(x.row0 + max(x.nrows, 1) - 1, a.div_g);  // token of the last row
   x.base = context - count;
-  x.keys = max(min(x.base + last + 1, context), 0);
+  x.keys = max(min(x.base + last + 1, a.width * a.page_size), 0);  // (a reach of at most 2^30)
   const int unit = x.kind == kFew ? kFewKeys : kManyKeys;
   x.units = (x.keys + unit - 1) / unit;
   return x;
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     if (t >= s.start && t < s.start + s.count) {
       rec.position = s.context - s.count + (t - s.start);
       rec.sequence = r;
-      if (rec.position >= 0) {
+      if (rec.position >= 0 && rec.position < a.width * a.page_size) {
         const int p = fast_div(rec.position, a.div_page);
         rec.slot = rec.position - p * a.page_size;
         const int page = a.table[(long long)r * a.table_stride + p];

@@ -110,6 +110,8 @@ def _int32(x: torch.Tensor, shape: tuple[int, ...], what: str) -> torch.Tensor:
     if x.dtype is not torch.int32:
         if x.is_floating_point() or x.is_complex() or x.dtype is torch.bool:
             raise ValueError(f"{what} must hold integers, got {x.dtype}")
+        if x.dtype is torch.int64:  # (a number that int32 does not hold names no other one)
+            x = x.clamp(-2 ** 31, 2 ** 31 - 1)
         x = x.to(torch.int32)
     return x.contiguous()
 
@@ -123,8 +125,8 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
     ``context_lengths [R]`` counts each sequence's tokens, the new ones
     included.  Token position ``p`` of sequence ``r`` is slot ``p % page_size``
     of page ``page_table[r, p // page_size]``; entries outside the pool (-1, say,
-    behind a context or for a page that was given up) hold no keys.  Nothing is
-    read back to the host.  The table must stay as it is while the plan is used;
+    behind a context or for a page that was given up) hold no keys, nor do
+    positions beyond the table.  Nothing is read back to the host.  The table must stay as it is while the plan is used;
     on another stream, once that waits for the plan's; a captured graph that reads
     a plan made outside of it needs the plan kept.
     """

@@ -103,7 +103,7 @@ def attend(batch: Batch, q, key_pages, value_pages, scale=0.125):
         k = pool_k[np.maximum(page, 0), slot].double()
         v = pool_v[np.maximum(page, 0), slot].double()
         at = torch.arange(int(batch.starts[r]), int(batch.starts[r]) + n)
-        sees = torch.from_numpy(pos)[None] <= (torch.arange(n) + reach - n)[:, None]
+        sees = torch.from_numpy(pos)[None] <= (torch.arange(n) + context - n)[:, None]
         sees = sees & there[None]
         for h in range(batch.hq):
             kh, vh = k[:, h // group], v[:, h // group]

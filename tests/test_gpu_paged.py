@@ -249,12 +249,26 @@ def test_pages_outside_the_pool_hold_no_keys(dtype, device):
     assert not out[b.starts[3]].any()
 
 
-def test_context_beyond_the_table_is_its_reach(device):
-    b = Batch([(2, 64)], 4, 2, 16, BF, device)
-    starts, contexts, table = b.on_device()
-    plan = paged.plan(starts, contexts + 1000, table, b.key_pages, tokens=b.tokens, query_heads=4)
-    out = paged.attention(b.q, b.key_pages, b.value_pages, plan)
-    assert torch.equal(out, paged.attention(b.q, b.key_pages, b.value_pages, b.plan()))
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_positions_beyond_the_table(dtype, device):
+    """New tokens that the table has no place for are not written and see all that is there."""
+    b = Batch([(2, 64), (70, 100), (3, 7)], 4, 2, 16, dtype, device)
+    b.table = np.ascontiguousarray(b.table[:, :5])  # 80 slots
+    b.width, b.spans = 5, [(2, 64), (70, 100), (3, 2 ** 31 - 1)]
+    b.contexts = np.array([c for _, c in b.spans], np.int32)
+    plan = b.plan()
+    want, bound = attend(b, b.q, b.key_pages, b.value_pages)
+    close(paged.attention(b.q, b.key_pages, b.value_pages, plan), want, bound, "beyond")
+    rec = plan.token_records().cpu()
+    assert rec[:, 0].tolist() == [62, 63, *range(30, 100), *range(2 ** 31 - 4, 2 ** 31 - 1)]
+    assert (rec[2:52, 1] >= 0).all() and (rec[52:, 1] == -1).all()
+    before = b.key_pages.clone()
+    paged.append(b.k, b.v, b.key_pages, b.value_pages, plan)
+    for r, n in ((0, 62), (1, 30), (2, 7)):  # what was cached before, and the third's page
+        page, slot = b.slots(r, np.arange(n))
+        assert torch.equal(b.key_pages[page, slot], before[page, slot])
+    page, slot = b.slots(1, np.arange(30, 80))
+    assert torch.equal(b.key_pages[page, slot], b.k[2:52])
 
 
 def test_rows_behind_the_last_sequence(device):

@@ -167,6 +167,11 @@ def test_append_refuses():
             paged.append(*args, plan, **kw)
 
 
+def test_wide_integers_keep_their_order():
+    x = torch.tensor([2 ** 40, -2 ** 40, 2 ** 32, 5, -1])
+    assert paged._int32(x, (5,), "x").tolist() == [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, -1]
+
+
 def test_cache_pages_refuses():
     with pytest.raises(ValueError, match="whole pages"):
         paged.cache_pages(torch.zeros(2, 100, 2, 64), 16)
