@@ -34,8 +34,16 @@ constexpr int kManyGroups = 512;
 // A tile of many rows writes up to 66 KB of partial results per item and KV head:
 // its shares have at least this many units.  With 1, 2, 3, 4 and 8, us: 300 tokens
 // behind 500 15.7, 15.9, 19.4, 21.1 and 26.4; 128 behind 2000 17.7, 15.5, 16.2, 16.4
-// and 23.1; 8 x 200 behind 300 27.8, 27.6, 27.5, 26.5 and 32.0.
+// and 23.1.
 constexpr int kManyUnits = 2;
+// What the first item of a tile costs beside its keys, in units, where there is a unit for
+// every share: a share of many short tiles is then as long as one of a long tile's
+// middle.  Many rows with 0, 1, 2, 3 and 4, us: prompts of 491, 3814 and 699 tokens
+// 112, 103, 97, 98 and 96; 14 chunks of up to 624 behind 1000 to 2300 129, 129, 121,
+// 118 and 121.  Few rows with 0 and 1: drafts 76.5 and 75, 200 single tokens over up to
+// 500 keys 31.2 and 29.1.  (Where there are fewer units than shares, none has several
+// tiles: 300 tokens behind 500 16 without and 18 with.)
+constexpr int kFewStart = 1, kManyStart = 2;
 // Rows of a split tile that one workgroup joins: 8, whose items it shares out to four
 // groups of threads, or 32 of a tile of many rows with up to 8 items, which leaves a
 // quarter of the records to the plan (of a mixed step 6.4 us against 6.9, of 20912

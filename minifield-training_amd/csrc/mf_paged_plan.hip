@@ -42,24 +42,35 @@ __device__ __forceinline__ int wave_prefix_sum(int x) {
   return x;
 }
 
-// Exclusive prefix sums over the workgroup; `sum` gets the totals.
-__device__ __forceinline__ Two block_prefix(Two x, Two* lds, Two& sum) {
+// Exclusive prefix sums over the workgroup, in place; `sum` gets the totals.
+template <int N>
+__device__ __forceinline__ void block_prefix(int (&x)[N], int (*lds)[4], int (&sum)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Two y = {wave_prefix_sum(x.a), wave_prefix_sum(x.b)};
-  __syncthreads();  // the previous call's readers are done
-  if (lane == 63) lds[wave] = y;
-  __syncthreads();
-  y.a -= x.a;
-  y.b -= x.b;
-  sum = {0, 0};
+  int y[N];
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    const Two t = lds[w];
-    if (w < wave) y.a += t.a, y.b += t.b;
-    sum.a += t.a;
-    sum.b += t.b;
+  for (int i = 0; i < N; ++i) y[i] = wave_prefix_sum(x[i]);
+  __syncthreads();  // the previous call's readers are done
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds[wave][i] = y[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = y[i] - x[i];
+    sum[i] = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      const int t = lds[w][i];
+      x[i] += w < wave ? t : 0;
+      sum[i] += t;
+    }
   }
-  return y;
+}
+__device__ __forceinline__ Two block_prefix(Two x, int (*lds)[4], Two& sum) {
+  int y[2] = {x.a, x.b}, s[2];
+  block_prefix(y, lds, s);
+  sum = {s[0], s[1]};
+  return {y[0], y[1]};
 }
 
 struct Span {
@@ -75,19 +86,20 @@ __device__ __forceinline__ Span span_of(const PlanArgs& a, int r) {
   return s;
 }
 
-// A tile: its rows, the keys that its last row sees and those in units; where its
-// kind's units stand before it; its items (the first one's place, their number) and
-// its first partial row.
+// A tile: its rows, the keys that its last row sees and those in units; what it costs in
+// all (its units and the start of an item); the cost of its kind's tiles before it; its
+// items (the first one's place, their number) and its first partial row.
 struct Tile {
   int sequence, start, row0, nrows, base, keys, units, kind;
-  int unit0, item0, items, row;
+  int cost, cost0, item0, items, row;
 };
+
 
 // Workgroup 0's sequences, so that each is read once, and a round's tiles.
 struct PlanLds {
   int tiles[kMaxSequences];  // tiles before each sequence
   int start[kMaxSequences], count[kMaxSequences], context[kMaxSequences];
-  Two sums[kPlanThreads / 64];
+  int sums[kPlanThreads / 64][4];
   int item_at[kPlanThreads], join_at[kPlanThreads];  // before each tile of the round
   Tile tile[kPlanThreads];
 };
@@ -173,41 +185,57 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   }
   ntiles = min(ntiles, a.lay.cap_tiles);
   __syncthreads();
-  // units of keys over the tiles of each kind (below 2^31: the entry point checks
-  // tiles times the table's reach); the first round's are summed again in its turn
+  // the cost of each kind's tiles (below 2^31: the entry point checks tiles times the
+  // table's reach); the first round's is summed again in its turn
   Tile x = tid < ntiles ? tile_of(a, l, tid) : Tile{};
-  Two work = {0, 0}, sum, before;
+  int units[2] = {0, 0}, tiles[2] = {0, 0}, ahead[4] = {}, sum4[4];
   for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
     const Tile y = t0 == 0 ? x : t0 + tid < ntiles ? tile_of(a, l, t0 + tid) : Tile{};
-    before = block_prefix({y.kind == kFew ? y.units : 0, y.kind == kFew ? 0 : y.units}, l.sums, sum);
-    if (t0 == 0) x.unit0 = y.kind == kFew ? before.a : before.b;
-    work.a += sum.a;
-    work.b += sum.b;
+    const bool few = y.kind == kFew, some = y.units > 0;
+    int z[4] = {few ? y.units : 0, few ? 0 : y.units, few && some, !few && some};
+    block_prefix(z, l.sums, sum4);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      units[k] += sum4[k];
+      tiles[k] += sum4[2 + k];
+      if (t0 == 0) ahead[k] = z[k], ahead[2 + k] = z[2 + k];
+    }
   }
-  // units of a share
+  // What a start costs, where there is a unit for every share, and the cost of a share:
+  // more than a start's, so that every share has keys.
   const int target[2] = {a.lay.target[0], max(a.lay.target[1], 1)};
-  const int share[2] = {max((work.a + target[0] - 1) / target[0], 1),
-                        max((work.b + target[1] - 1) / target[1], kManyUnits)};
+  int begin[2], share[2], work[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    begin[k] = units[k] < target[k] ? 0 : k == kFew ? kFewStart : kManyStart;
+    work[k] = units[k] + begin[k] * tiles[k];
+    share[k] = max((work[k] + target[k] - 1) / target[k], max(begin[k] + 1, k == kFew ? 1 : kManyUnits));
+  }
+  Two sum, before;
+  x.cost0 = x.kind == kFew ? ahead[0] + begin[0] * ahead[2] : ahead[1] + begin[1] * ahead[3];
   int* shares[2] = {reinterpret_cast<int*>(a.plan + a.lay.shares[0]),
                     reinterpret_cast<int*>(a.plan + a.lay.shares[1])};
   PagedItem* items[2] = {reinterpret_cast<PagedItem*>(a.plan + a.lay.items[0]),
                          reinterpret_cast<PagedItem*>(a.plan + a.lay.items[1])};
   PagedJoin* joins = reinterpret_cast<PagedJoin*>(a.plan + a.lay.joins);
-  Two units = {0, 0}, nitems = {0, 0}, nrest = {0, 0};  // by kind; by kind; joins and partial rows
+  Two cost = {0, 0}, nitems = {0, 0}, nrest = {0, 0};  // by kind; by kind; joins and partial rows
   for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
     const bool live = t0 + tid < ntiles;
+    if (t0 > 0) x = live ? tile_of(a, l, t0 + tid) : Tile{};
+    x.cost = x.units > 0 ? x.units + (x.kind == kFew ? begin[0] : begin[1]) : 0;
     if (ntiles > kPlanThreads) {
-      if (t0 > 0) x = live ? tile_of(a, l, t0 + tid) : Tile{};
-      before = block_prefix({x.kind == kFew ? x.units : 0, x.kind == kFew ? 0 : x.units}, l.sums, sum);
-      x.unit0 = x.kind == kFew ? units.a + before.a : units.b + before.b;
-      units.a += sum.a;
-      units.b += sum.b;
+      before = block_prefix({x.kind == kFew ? x.cost : 0, x.kind == kFew ? 0 : x.cost}, l.sums, sum);
+      x.cost0 = x.kind == kFew ? cost.a + before.a : cost.b + before.b;
+      cost.a += sum.a;
+      cost.b += sum.b;
     } else {
-      units = work;
+      cost = {work[0], work[1]};
     }
     const bool few = x.kind == kFew;
     const int c = few ? share[0] : share[1];
-    x.items = !live ? 0 : x.units == 0 ? 1 : (x.unit0 + x.units - 1) / c - x.unit0 / c + 1;
+    // (from the share of its first unit on: its start goes with that)
+    x.items = !live ? 0 : x.units == 0 ? 1
+              : (x.cost0 + x.cost - 1) / c - (x.cost0 + (few ? begin[0] : begin[1])) / c + 1;
     before = block_prefix({few ? x.items : 0, few ? 0 : x.items}, l.sums, sum);
     const int round_items = sum.a + sum.b;
     l.item_at[tid] = before.a + before.b;
@@ -232,20 +260,21 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       const int k = i - l.item_at[j], per = y.kind == kFew ? share[0] : share[1];
       const int unit = y.kind == kFew ? kFewKeys : kManyKeys;
       // (a tile without keys goes with the unit before it)
-      const int s = y.units > 0 ? y.unit0 / per + k : max(y.unit0 - 1, 0) / per;
+      const int unit0 = y.cost0 + (y.kind == kFew ? begin[0] : begin[1]);
+      const int s = y.units > 0 ? unit0 / per + k : max(y.cost0 - 1, 0) / per;
       PagedItem it;
       it.start = y.start;
       it.row0 = y.row0;
       it.nrows = y.nrows;
       it.base = y.base;
-      it.key0 = k == 0 ? 0 : (s * per - y.unit0) * unit;
-      it.key1 = k == y.items - 1 ? y.keys : ((s + 1) * per - y.unit0) * unit;
+      it.key0 = k == 0 ? 0 : (s * per - unit0) * unit;
+      it.key1 = k == y.items - 1 ? y.keys : ((s + 1) * per - unit0) * unit;
       it.partial = y.items > 1 ? y.row + k * y.nrows : -1;
       it.sequence = y.sequence;
       const int at = y.item0 + k;
       if (at < a.lay.cap_items[y.kind]) items[y.kind][at] = it;
       // is it the first item of its share?
-      if (k > 0 || at == 0 || (y.units > 0 && y.unit0 > 0 && (y.unit0 - 1) / per != s))
+      if (k > 0 || at == 0 || (y.units > 0 && y.cost0 > 0 && (y.cost0 - 1) / per != s))
         if (s < a.lay.target[y.kind]) shares[y.kind][s] = at;
     }
     // (eight threads a tile: a search for each record's tile cost 4 us at 160 tiles of
@@ -266,10 +295,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   }
   if (tid == 0) {
     int* head = reinterpret_cast<int*>(a.plan);
-    const int all_units[2] = {units.a, units.b}, all_items[2] = {nitems.a, nitems.b};
+    const int all_cost[2] = {cost.a, cost.b}, all_items[2] = {nitems.a, nitems.b};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int used = min(all_units[k] > 0 ? (all_units[k] - 1) / share[k] + 1 : all_items[k] > 0,
+      const int used = min(all_cost[k] > 0 ? (all_cost[k] - 1) / share[k] + 1 : all_items[k] > 0,
                            a.lay.target[k]);
       head[kHeadShares + k] = used;
       shares[k][used] = min(all_items[k], a.lay.cap_items[k]);
