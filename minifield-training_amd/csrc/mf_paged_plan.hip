@@ -191,8 +191,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   int units[2] = {0, 0}, tiles[2] = {0, 0}, ahead[4] = {}, sum4[4];
   for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
     const Tile y = t0 == 0 ? x : t0 + tid < ntiles ? tile_of(a, l, t0 + tid) : Tile{};
+    // (a tile without keys, which writes zeros, counts as one unit)
     const bool few = y.kind == kFew, some = y.units > 0;
-    int z[4] = {few ? y.units : 0, few ? 0 : y.units, few && some, !few && some};
+    const int n = y.nrows > 0 ? max(y.units, 1) : 0;
+    int z[4] = {few ? n : 0, few ? 0 : n, few && some, !few && some};
     block_prefix(z, l.sums, sum4);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   for (int t0 = 0; t0 < ntiles; t0 += kPlanThreads) {
     const bool live = t0 + tid < ntiles;
     if (t0 > 0) x = live ? tile_of(a, l, t0 + tid) : Tile{};
-    x.cost = x.units > 0 ? x.units + (x.kind == kFew ? begin[0] : begin[1]) : 0;
+    x.cost = x.units > 0 ? x.units + (x.kind == kFew ? begin[0] : begin[1]) : x.nrows > 0 ? 1 : 0;
     if (ntiles > kPlanThreads) {
       before = block_prefix({x.kind == kFew ? x.cost : 0, x.kind == kFew ? 0 : x.cost}, l.sums, sum);
       x.cost0 = x.kind == kFew ? cost.a + before.a : cost.b + before.b;
@@ -259,9 +261,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       const Tile y = l.tile[j];
       const int k = i - l.item_at[j], per = y.kind == kFew ? share[0] : share[1];
       const int unit = y.kind == kFew ? kFewKeys : kManyKeys;
-      // (a tile without keys goes with the unit before it)
-      const int unit0 = y.cost0 + (y.kind == kFew ? begin[0] : begin[1]);
-      const int s = y.units > 0 ? unit0 / per + k : max(y.cost0 - 1, 0) / per;
+      const int unit0 = y.cost0 + (y.units == 0 ? 0 : y.kind == kFew ? begin[0] : begin[1]);
+      const int s = unit0 / per + k;
       PagedItem it;
       it.start = y.start;
       it.row0 = y.row0;
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       const int at = y.item0 + k;
       if (at < a.lay.cap_items[y.kind]) items[y.kind][at] = it;
       // is it the first item of its share?
-      if (k > 0 || at == 0 || (y.units > 0 && y.cost0 > 0 && (y.cost0 - 1) / per != s))
+      if (k > 0 || at == 0 || (y.cost0 > 0 && (y.cost0 - 1) / per != s))
         if (s < a.lay.target[y.kind]) shares[y.kind][s] = at;
     }
     // (eight threads a tile: a search for each record's tile cost 4 us at 160 tiles of

@@ -280,6 +280,20 @@ def test_rows_behind_the_last_sequence(device):
     assert not fresh[43:].any() and torch.equal(fresh[:43], out[:43])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_sequences_without_keys(first, dtype, device):
+    """A batch filled up with sequences that have a token and no context: zeros, and the others
+    as by themselves (their keys are shared out among other workgroups, so not to the bit)."""
+    real, pad = [(1, 700), (40, 90), (3, 5000)], [(1, 0)] * 500 + [(200, 0)]
+    b = Batch(pad + real if first else real + pad, 8, 4, 16, dtype, device)
+    out = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
+    want, bound = attend(b, b.q, b.key_pages, b.value_pages)
+    close(out, want, bound, "padded")
+    none = slice(0, 700) if first else slice(44, 744)
+    assert not out[none].any()
+
+
 def test_shared_pages_and_strided_operands(device):
     # two sequences with a common prefix: the same pages in both rows
     b = Batch([(1, 100), (1, 110)], 16, 8, 16, BF, device)
