@@ -10,12 +10,12 @@
 //     own in LDS: no barrier until the states of waves that share an item are
 //     merged.  Bound: HBM, each cached key and value is read once for all rows of
 //     its head.  One token for each of 64 sequences of 129 to 8192 keys, 16/8 heads
-//     (494 MB): 84 us, 5.9 TB/s, and the join 5; 24 sequences of 3 to 8 drafts, 24/8
-//     heads (391 MB): 69 and 5.  Half the workgroups a CU take 3 % longer.
+//     (494 MB): 82 us, 6.0 TB/s, and the join 5; 24 sequences of 3 to 8 drafts, 24/8
+//     heads (391 MB): 68 and 5.  Half the workgroups a CU take 3 % longer.
 //   up to 256 rows (chunks), one KV head: every wave holds 64 rows, all share
 //     64-key stages in a ring of four, so an operand read from LDS feeds two MFMAs.
 //     2048 tokens behind 28672, 16/8 heads: 285 to 310 us with the join, 800 to 870
-//     TFLOP/s; 16384 behind none 620 to 650 (a large bf16 matrix product on the card:
+//     TFLOP/s; 16384 behind none 605 to 640 (a large bf16 matrix product on the card:
 //     1190 TFLOP/s).  MFMA
 //     busy 41 % of the cycles, VALU 58 %, and the clock: the same launch over zeros
 //     takes 14 % less.  (8 maxima less a block changed nothing.)
