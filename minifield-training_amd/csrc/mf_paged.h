@@ -44,6 +44,12 @@ constexpr int kManyUnits = 2;
 // 500 keys 31.2 and 29.1.  (Where there are fewer units than shares, none has several
 // tiles: 300 tokens behind 500 16 without and 18 with.)
 constexpr int kFewStart = 1, kManyStart = 2;
+// Quarters of a later share of many rows that those of the first workgroup of each CU
+// get: its waves, the older ones, are served first (with equal shares it ends a chunk
+// after 229 us, the second after 290).  With 4, 5, 6 and 7, us: a chunk over 28 K keys
+// 302, 297, 292 and 298, 16 K causal 621, 605, 616 and 634, a mixed step 126, 125, 128
+// and 131, 8 x 200 tokens behind 300 26.0, 25.2, 25.4 and 26.4.
+constexpr int kEarlyShare = 5;
 // Rows of a split tile that one workgroup joins: 8, whose items it shares out to four
 // groups of threads, or 32 of a tile of many rows with up to 8 items, which leaves a
 // quarter of the records to the plan (of a mixed step 6.4 us against 6.9, of 20912

@@ -137,6 +137,19 @@ __device__ __forceinline__ Tile tile_of(const PlanArgs& a, const PlanLds& l, int
   return x;
 }
 
+// The shares of a kind: what the first `early` cost, and the others.
+struct Shares {
+  int early, first, then;
+  __device__ int of(int cost) const {
+    const int x = cost - early * first;
+    const bool is_early = x < 0;  // (one division)
+    return (is_early ? cost : x) / (is_early ? first : then) + (is_early ? 0 : early);
+  }
+  __device__ int begin(int share) const {
+    return share < early ? share * first : early * first + (share - early) * then;
+  }
+};
+
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   __shared__ PlanLds l;
   const int tid = threadIdx.x;
@@ -206,12 +219,23 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   // What a start costs, where there is a unit for every share, and the cost of a share:
   // more than a start's, so that every share has keys.
   const int target[2] = {a.lay.target[0], max(a.lay.target[1], 1)};
-  int begin[2], share[2], work[2];
+  int begin[2], work[2];
+  Shares share[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     begin[k] = units[k] < target[k] ? 0 : k == kFew ? kFewStart : kManyStart;
     work[k] = units[k] + begin[k] * tiles[k];
-    share[k] = max((work[k] + target[k] - 1) / target[k], max(begin[k] + 1, k == kFew ? 1 : kManyUnits));
+    const int least = max(begin[k] + 1, k == kFew ? 1 : kManyUnits);
+    share[k].early = 0;
+    share[k].then = max((work[k] + target[k] - 1) / target[k], least);
+    share[k].first = share[k].then;
+    if (k == kMany && begin[k] > 0) {
+      const int early = 256 / a.Hkv, late = target[k] - early;
+      const int parts = early * kEarlyShare + late * 4;  // quarters of a later share
+      share[k].early = early;
+      share[k].then = max((int)((4ll * work[k] + parts - 1) / parts), least);
+      share[k].first = (share[k].then * kEarlyShare + 3) / 4;
+    }
   }
   Two sum, before;
   x.cost0 = x.kind == kFew ? ahead[0] + begin[0] * ahead[2] : ahead[1] + begin[1] * ahead[3];
@@ -234,10 +258,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       cost = {work[0], work[1]};
     }
     const bool few = x.kind == kFew;
-    const int c = few ? share[0] : share[1];
+    const Shares& c = few ? share[0] : share[1];
     // (from the share of its first unit on: its start goes with that)
     x.items = !live ? 0 : x.units == 0 ? 1
-              : (x.cost0 + x.cost - 1) / c - (x.cost0 + (few ? begin[0] : begin[1])) / c + 1;
+              : c.of(x.cost0 + x.cost - 1) - c.of(x.cost0 + (few ? begin[0] : begin[1])) + 1;
     before = block_prefix({few ? x.items : 0, few ? 0 : x.items}, l.sums, sum);
     const int round_items = sum.a + sum.b;
     l.item_at[tid] = before.a + before.b;
@@ -259,23 +283,24 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     for (int i = tid; i < round_items; i += kPlanThreads) {
       const int j = last_not_above(l.item_at, round, i);
       const Tile y = l.tile[j];
-      const int k = i - l.item_at[j], per = y.kind == kFew ? share[0] : share[1];
+      const int k = i - l.item_at[j];
+      const Shares& per = y.kind == kFew ? share[0] : share[1];
       const int unit = y.kind == kFew ? kFewKeys : kManyKeys;
       const int unit0 = y.cost0 + (y.units == 0 ? 0 : y.kind == kFew ? begin[0] : begin[1]);
-      const int s = unit0 / per + k;
+      const int s = per.of(unit0) + k;
       PagedItem it;
       it.start = y.start;
       it.row0 = y.row0;
       it.nrows = y.nrows;
       it.base = y.base;
-      it.key0 = k == 0 ? 0 : (s * per - unit0) * unit;
-      it.key1 = k == y.items - 1 ? y.keys : ((s + 1) * per - unit0) * unit;
+      it.key0 = k == 0 ? 0 : (per.begin(s) - unit0) * unit;
+      it.key1 = k == y.items - 1 ? y.keys : (per.begin(s + 1) - unit0) * unit;
       it.partial = y.items > 1 ? y.row + k * y.nrows : -1;
       it.sequence = y.sequence;
       const int at = y.item0 + k;
       if (at < a.lay.cap_items[y.kind]) items[y.kind][at] = it;
       // is it the first item of its share?
-      if (k > 0 || at == 0 || (y.cost0 > 0 && (y.cost0 - 1) / per != s))
+      if (k > 0 || at == 0 || (y.cost0 > 0 && per.of(y.cost0 - 1) != s))
         if (s < a.lay.target[y.kind]) shares[y.kind][s] = at;
     }
     // (eight threads a tile: a search for each record's tile cost 4 us at 160 tiles of
@@ -299,7 +324,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     const int all_cost[2] = {cost.a, cost.b}, all_items[2] = {nitems.a, nitems.b};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int used = min(all_cost[k] > 0 ? (all_cost[k] - 1) / share[k] + 1 : all_items[k] > 0,
+      const int used = min(all_cost[k] > 0 ? share[k].of(all_cost[k] - 1) + 1 : all_items[k] > 0,
                            a.lay.target[k]);
       head[kHeadShares + k] = used;
       shares[k][used] = min(all_items[k], a.lay.cap_items[k]);
