@@ -14,9 +14,9 @@
 //     heads (391 MB): 68 and 5.  Half the workgroups a CU take 3 % longer.
 //   up to 256 rows (chunks), one KV head: every wave holds 64 rows, all share
 //     64-key stages in a ring of four, so an operand read from LDS feeds two MFMAs.
-//     2048 tokens behind 28672, 16/8 heads: 285 to 310 us with the join, 800 to 870
-//     TFLOP/s; 16384 behind none 605 to 640 (a large bf16 matrix product on the card:
-//     1190 TFLOP/s).  MFMA
+//     2048 tokens behind 28672, 16/8 heads: 275 to 300 us with the join, 830 to 900
+//     TFLOP/s; 16384 behind none 605 (a large bf16 matrix product on the card: 1190
+//     TFLOP/s).  MFMA
 //     busy 41 % of the cycles, VALU 58 %, and the clock: the same launch over zeros
 //     takes 14 % less.  (8 maxima less a block changed nothing.)
 //
