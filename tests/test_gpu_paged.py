@@ -411,6 +411,27 @@ def test_a_plan_outlives_its_last_use_on_another_stream(device):
     assert torch.equal(out, want) and junk and tables
 
 
+def test_layers_captured_over_an_eager_plan(device):
+    """A graph of several layers that read one plan made outside, replayed with new queries."""
+    b = Batch([(1, 500), (30, 200), (4, 40)], 8, 4, 16, BF, device)
+    plan = b.plan()
+    paged.attention(b.q, b.key_pages, b.value_pages, plan)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = b.q
+        for _ in range(3):
+            x = paged.attention(x, b.key_pages, b.value_pages, plan)
+    for i in range(3):
+        b.q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        y = b.q
+        for _ in range(3):
+            y = paged.attention(y, b.key_pages, b.value_pages, plan)
+        assert torch.equal(x, y), i
+
+
 def test_a_misaligned_query_is_read(device):
     b = Batch([(1, 300), (40, 90)], 4, 2, 16, BF, device)
     base = torch.zeros(b.q.numel() + 1, dtype=BF, device=device)
