@@ -322,7 +322,8 @@ int mf_paged_append(const void* q, long long q_stride, const void* k,
 /* Causal attention of a step's new tokens over their pages: a query at
  * position p sees slots 0 .. p of its sequence (what mf_decode computes for
  * one new token a row, kernels/attention.py:264-282, over pages and for any
- * number of new tokens; a query that sees no key yields zeros).  q
+ * number of new tokens; a query that sees no key yields zeros, and one of whose
+ * visible scores any is NaN or +infinity, or all are -infinity, NaN).  q
  * [tokens, q_heads, 64] with q_stride elements between tokens, out dense.
  * k_pages, v_pages and their strides as mf_paged_append, with 16-byte aligned
  * rows.  Rows of out past the last sequence are zeroed when

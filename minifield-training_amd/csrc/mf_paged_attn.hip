@@ -33,6 +33,15 @@
 // Items of a split tile write (max, sum, unnormalised output); a second launch
 // joins them in item order.  No atomics: the same inputs give the same bits.
 //
+// Rows.  A row that sees no key is zeros.  One that sees a key is what the definition
+// gives, whatever its scores are: NaN where one is NaN or +infinity, or all are
+// -infinity.  So "no key" is a state of its own: maximum -infinity and a sum whose bits
+// are zero.  A NaN marks the sum (a maximum passes over it), +infinity does so with the
+// subtraction of the shift, and a row that has only scores of -infinity gets a sum of
+// one at its end (mark_low): beside a finite maximum its weight is 2^-inf, and without
+// one the row is NaN (row_factor).  What tells sums apart looks at their bits: the file
+// is compiled as if no comparison saw a NaN.
+//
 // Pages.  Page sizes are multiples of 8 and blocks start at multiples of 32, so
 // eight keys of a block lie in one page: their page number is a scalar load, and
 // their rows are moved by LDS DMAs from a scalar base.  Keys that are not there
@@ -121,6 +130,45 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 struct RowState {
   float shift, lag, l0, l1;
 };
+
+// Whether a sum of weights is that of a row without keys.
+__device__ __forceinline__ bool no_weight(float l) { return __float_as_uint(l) == 0u; }
+
+// The weight of a state (m, l) where states are joined under the maximum `top`.
+__device__ __forceinline__ float state_weight(float m, float l, float top) {
+  return no_weight(l) ? 0.f : top == kNegInf ? 1.f : fast_exp2(m - top);
+}
+
+// What a row's outputs are multiplied by: zero without keys, NaN without a maximum.
+__device__ __forceinline__ float row_factor(float top, float sum) {
+  float nan;
+  asm("v_mov_b32 %0, 0x7fc00000" : "=v"(nan));  // (a constant NaN may be optimised away)
+  return no_weight(sum) ? 0.f : top == kNegInf ? nan : 1.f / sum;
+}
+
+// The first position from `from` (a page's or block's first key) up to `end` whose page
+// is in the pool, 2^31 - 1 if there is none; all lanes of the wave take part.
+__device__ __forceinline__ int first_key(const PagedArgs& a, const int* row, int from, int end) {
+  const int lane = fresh_lane_id();
+  const int last = fast_div(end - 1, a.div_page);
+  for (int p0 = fast_div(from, a.div_page); p0 <= last; p0 += 64) {
+    const bool there = p0 + lane <= last && (unsigned)row[min(p0 + lane, last)] < (unsigned)a.pages;
+    const uint64_t any = __ballot(there);
+    if (any) return max(from, (p0 + __ffsll((unsigned long long)any) - 1) * a.page_size);
+  }
+  return 0x7fffffff;
+}
+
+// The sum of a row that has no maximum: one instead of zero where it sees a key from
+// `from` on, which then has a score of -infinity (`lim`: keys that it sees, up to `end`).
+// Rows mostly have a maximum, and no table is read.
+__device__ __forceinline__ float mark_low(const PagedArgs& a, const int* row, int from, int end,
+                                          int lim, float l) {
+  const bool open = no_weight(l) && lim > from;
+  if (!__any(open)) return l;
+  const int first = first_key(a, row, from, end);
+  return open && first < lim ? 1.f : l;
+}
 
 __device__ __forceinline__ void grow(RowState& st, float mx, f32x16 (&acc)[2]) {
   const bool up = mx > st.lag;
@@ -490,7 +538,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
   // pieces permuted by the row
 #pragma unroll
   for (int h = 0; h < HW; ++h) {
-    const float l = halves_sum(st[h].l0 + st[h].l1);
+    const float l = mark_low(a, trow, it.key0 + (ALONE ? 0 : 32 * key_wave), it.key1, lim,
+                             halves_sum(st[h].l0 + st[h].l1));
     if (lane < 32) {
       lm[32 * h + lane] = st[h].lag > 0.f ? st[h].shift : kNegInf;
       ll[32 * h + lane] = l;
@@ -527,9 +576,9 @@ __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const float m = lm[first + w][at];
-      const float wt = m == kNegInf ? 0.f : fast_exp2(m - top);
-      sum = fmaf(wt, ll[first + w][at], sum);
+      const float m = lm[first + w][at], l = ll[first + w][at];
+      const float wt = state_weight(m, l, top);
+      sum = fmaf(wt, l, sum);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(
@@ -540,10 +589,11 @@ __device__ __forceinline__ void few_merge(const PagedArgs& a, const ItemView& it
     }
     if (it.partial < 0) {
       const RowOf ro = row_of(a, it, r, kvh);
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const bool none = no_weight(sum);
+      const float inv = row_factor(top, sum);
       bf16x8 y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (bf16)(sum > 0.f ? o[i] * inv : 0.f);
+      for (int i = 0; i < 8; ++i) y[i] = (bf16)(none ? 0.f : o[i] * inv);
       *reinterpret_cast<bf16x8*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2) + 16 * d8) = y;
     } else {
       const size_t to = (size_t)(kvh * a.cap_rows) + it.partial + r;
@@ -774,12 +824,12 @@ __device__ __forceinline__ bool many_rows(const PagedArgs& a, const ItemView& it
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       const int row = 64 * wave + 32 * rb + (elane & 31);
-      const float l = halves_sum(st[rb].l0 + st[rb].l1);
+      const float l = mark_low(a, trow, it.key0, it.key1, lim[rb], halves_sum(st[rb].l0 + st[rb].l1));
       if (row >= it.nrows) continue;
       const RowOf ro = row_of(a, it, row, kvh);
-      const bool has = l > 0.f;
+      const float inv = row_factor(st[rb].lag > 0.f ? st[rb].shift : kNegInf, l);
       store_bf16_rows(reinterpret_cast<bf16*>(a.out + ((long long)ro.token * a.Hq + ro.head) * (kD * 2)),
-                      acc[rb], has ? 1.f / l : 0.f, has, half);
+                      acc[rb], inv, !no_weight(l), half);
     }
     return true;
   }
@@ -791,7 +841,7 @@ __device__ __forceinline__ bool many_rows(const PagedArgs& a, const ItemView& it
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
     const int r = 32 * rb + (elane & 31);
-    const float l = halves_sum(st[rb].l0 + st[rb].l1);
+    const float l = mark_low(a, trow, it.key0, it.key1, lim[rb], halves_sum(st[rb].l0 + st[rb].l1));
     if (half == 0 && 64 * wave + r < it.nrows)
       a.ml[first + r] = make_float2(st[rb].lag > 0.f ? st[rb].shift : kNegInf, l);
 #pragma unroll
@@ -991,7 +1041,7 @@ __device__ __forceinline__ void f32_item(const PagedArgs& a, const ItemView& it,
   };
   run(Plain{});
   if (it.key1 > least && __any((wild_bits(acc[0]) | wild_bits(acc[1])) != 0)) run(Careful{});
-  l = halves_sum(l);
+  l = mark_low(a, trow, it.key0 + 32 * wave, it.key1, lim, halves_sum(l));
   if (lane < 32) {
     lm[wave][lane] = m == kNegInf ? kNegInf : m * c;
     ll[wave][lane] = l;
@@ -1007,12 +1057,13 @@ __device__ __forceinline__ void f32_item(const PagedArgs& a, const ItemView& it,
   float wt[4], sum = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    wt[w] = lm[w][r] == kNegInf ? 0.f : fast_exp2(lm[w][r] - top);
+    wt[w] = state_weight(lm[w][r], ll[w][r], top);
     sum = fmaf(wt[w], ll[w][r], sum);
   }
   const size_t at = (size_t)(kvh * a.cap_rows) + max(it.partial, 0) + r;
   const RowOf ro = row_of(a, it, r, kvh);
-  const float inv = it.partial >= 0 ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+  const bool none = no_weight(sum);
+  const float inv = it.partial >= 0 ? 1.f : row_factor(top, sum);
   float* dst = it.partial >= 0 ? a.acc + at * kD + d0
                                : reinterpret_cast<float*>(a.out) +
                                      ((long long)ro.token * a.Hq + ro.head) * kD + d0;
@@ -1022,7 +1073,7 @@ __device__ __forceinline__ void f32_item(const PagedArgs& a, const ItemView& it,
 #pragma unroll
     for (int w = 0; w < 4; ++w) o += f32_at(kt[w], r, d0 + 4 * h) * wt[w];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = sum > 0.f ? o[e] * inv : 0.f;
+    for (int e = 0; e < 4; ++e) o[e] = none ? 0.f : o[e] * inv;
     *reinterpret_cast<f32x4*>(dst + 4 * h) = o;
   }
   if (it.partial >= 0 && d0 == 0) a.ml[at] = make_float2(top, sum);
@@ -1103,13 +1154,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
       }
       top = fmaxf(top, ml[i].x);
     }
-    const float wa = m == kNegInf ? 0.f : fast_exp2(m - top);
+    const float wa = state_weight(m, l, top);
     l *= wa;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] *= wa;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float w = ml[i].x == kNegInf ? 0.f : fast_exp2(ml[i].x - top);
+      const float w = state_weight(ml[i].x, ml[i].y, top);
       l = fmaf(w, ml[i].y, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -1131,15 +1182,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     float sum = 0.f, z0 = 0.f, z1 = 0.f;
     for (int x = 0; x < sp; ++x) {
       const float2 ml = pml[(x << log_rp) + er];
-      const float w = ml.x == kNegInf ? 0.f : fast_exp2(ml.x - top);
+      const float w = state_weight(ml.x, ml.y, top);
       sum = fmaf(w, ml.y, sum);
       z0 = fmaf(w, part[(x << log_rp) + er][e0], z0);
       z1 = fmaf(w, part[(x << log_rp) + er][e0 + 1], z1);
     }
     const RowOf ro = row_of(a, it, er, kvh);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    z0 = sum > 0.f ? z0 * inv : 0.f;
-    z1 = sum > 0.f ? z1 * inv : 0.f;
+    const bool none = no_weight(sum);
+    const float inv = row_factor(top, sum);
+    z0 = none ? 0.f : z0 * inv;
+    z1 = none ? 0.f : z1 * inv;
     const long long at = ((long long)ro.token * a.Hq + ro.head) * kD + e0;
     if constexpr (F32) {
       *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(z0, z1);

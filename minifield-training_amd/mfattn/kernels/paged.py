@@ -222,7 +222,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
 
     ``query [tokens, Hq, 64]``: the query at position ``p`` of its sequence sees
     the keys at positions ``0 .. p`` (the step's own keys must be in their pages:
-    :func:`append`).  A query that sees no key yields zeros.  ``scale`` defaults
+    :func:`append`).  A query that sees no key yields zeros; a NaN or +infinity
+    among its scores, or none above -infinity, yields NaN.  ``scale`` defaults
     to ``64 ** -0.5``.  Rows behind the last sequence are zeros, or left as they
     are in an ``out`` that is given.  Slots behind a context may hold anything.
     Forward only; the same inputs give the same bits.
