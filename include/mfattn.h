@@ -275,8 +275,8 @@ int mf_rotate(const void* q, long long q_stride, const void* k,
 
 /* The plan of a paged serving step.  `sequences` (up to 4096) ragged sequences
  * bring new tokens query_starts[r] .. query_starts[r + 1] - 1 (int32
- * [sequences + 1], ascending) of a [tokens, heads, 64] batch; tokens past the
- * last sequence belong to nobody.  context_lengths[r] counts the tokens of
+ * [sequences + 1], ascending) of a [tokens, heads, 64] batch; tokens before the
+ * first sequence and past the last belong to nobody.  context_lengths[r] counts the tokens of
  * sequence r, the new ones included; token position p is slot p % page_size of
  * page page_table[r * table_stride + p / page_size], max_pages entries a row.
  * Page sizes are multiples of 8.  An entry outside [0, pages) holds no keys:
@@ -326,7 +326,7 @@ int mf_paged_append(const void* q, long long q_stride, const void* k,
  * visible scores any is NaN or +infinity, or all are -infinity, NaN).  q
  * [tokens, q_heads, 64] with q_stride elements between tokens, out dense.
  * k_pages, v_pages and their strides as mf_paged_append, with 16-byte aligned
- * rows.  Rows of out past the last sequence are zeroed when
+ * rows.  Rows of out before the first sequence and past the last are zeroed when
  * zero_rest != 0 and left as they are otherwise.  Deterministic.  `workspace`
  * holds the partial results of keys split over workgroups
  * (mf_paged_attn_workspace_bytes); it is this call's alone while it runs. */

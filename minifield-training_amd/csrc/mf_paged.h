@@ -93,8 +93,9 @@ struct PagedLayout {
   size_t cap_rows;     // rows of partial results
 };
 
-// header (ints)
-constexpr int kHeadShares = 0, kHeadJoins = 2, kHeadEnd = 3;  // shares of each kind: 0 and 1
+// header (ints): shares of each kind (0 and 1), join records, the first sequence's first
+// token and the one behind the last sequence
+constexpr int kHeadShares = 0, kHeadJoins = 2, kHeadEnd = 3, kHeadBegin = 4;
 
 // Bounds: a sequence of M rows has one tile (M <= 32) or ceil(M / 256), so at
 // most sequences + tokens G / 256 in all.  Every boundary between shares adds an

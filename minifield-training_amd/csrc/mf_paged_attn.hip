@@ -1110,10 +1110,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ float2 pml[32];
   if ((int)blockIdx.x >= a.join_blocks) {
     const long long row = (long long)a.Hq * kD * (F32 ? 4 : 2);
+    const long long begin = ld_const(a.head, kHeadBegin) * row;
     const long long end = ld_const(a.head, kHeadEnd) * row;
     const long long at = (long long)(blockIdx.x - a.join_blocks) * 16384;
     for (long long x = at + 16 * threadIdx.x; x < min(at + 16384, a.out_bytes); x += 16 * 256)
-      if (x >= end) st_u32x4(a.out + x, u32x4{0, 0, 0, 0});
+      if (x < begin || x >= end) st_u32x4(a.out + x, u32x4{0, 0, 0, 0});
     return;
   }
   const int t = uniform(fast_div(blockIdx.x, a.div_hkv));

@@ -121,7 +121,7 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
     """Plan one step of ``R`` sequences over the pool ``key_pages`` (values have its shape).
 
     ``query_starts [R + 1]`` (ascending) delimits the sequences' new tokens in a
-    batch of ``tokens``; those past the last belong to nobody.
+    batch of ``tokens``; those before the first and past the last belong to nobody.
     ``context_lengths [R]`` counts each sequence's tokens, the new ones
     included.  Token position ``p`` of sequence ``r`` is slot ``p % page_size``
     of page ``page_table[r, p // page_size]``; entries outside the pool (-1, say,
@@ -224,8 +224,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     the keys at positions ``0 .. p`` (the step's own keys must be in their pages:
     :func:`append`).  A query that sees no key yields zeros; a NaN or +infinity
     among its scores, or none above -infinity, yields NaN.  ``scale`` defaults
-    to ``64 ** -0.5``.  Rows behind the last sequence are zeros, or left as they
-    are in an ``out`` that is given.  Slots behind a context may hold anything.
+    to ``64 ** -0.5``.  Rows before the first sequence and behind the last are
+    zeros, or left as they are in an ``out`` that is given.  Slots behind a context may hold anything.
     Forward only; the same inputs give the same bits.
     """
     shape, dtype = plan.q_shape, query.dtype
