@@ -26,7 +26,8 @@ import functools
 import torch
 
 from .. import _lib
-from ..ops import _ptr, _raw_stream, dtype_code, launch, require_device, token_rows
+from ..ops import (_ptr, _raw_stream, carries_tangent, dtype_code, launch, require_device,
+                   token_rows)
 from .rotary import Rotary
 
 
@@ -179,6 +180,8 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     if torch.is_grad_enabled() and _records_grad(key, value, key_pages, value_pages, query,
                                                  query_gain, key_gain):
         raise ValueError("paged.append has no backward; call it under torch.no_grad()")
+    if carries_tangent(key, value, key_pages, value_pages, query, query_gain, key_gain):
+        raise ValueError("paged.append has no derivative; an operand carries a tangent")
     _check_pool(key_pages, value_pages, plan)
     if key.shape != plan.k_shape or value.shape != plan.k_shape:
         raise ValueError(f"keys and values must be {list(plan.k_shape)}, got "
@@ -241,6 +244,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     if (query.requires_grad or key_pages.requires_grad or value_pages.requires_grad) \
             and torch.is_grad_enabled():
         raise ValueError("paged.attention has no backward; call it under torch.no_grad()")
+    if carries_tangent(query, key_pages, value_pages):
+        raise ValueError("paged.attention has no derivative; an operand carries a tangent")
     device = require_device(query, key_pages, value_pages, plan.buf)
     query, q_step = token_rows(query)
     if query.data_ptr() % 16:

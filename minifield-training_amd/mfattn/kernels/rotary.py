@@ -16,7 +16,7 @@ import math
 import torch
 
 from .. import _lib
-from ..ops import _ptr, _raw_stream, dtype_code, launch, require_device, token_rows
+from ..ops import _ptr, _raw_stream, carries_tangent, dtype_code, launch, require_device, token_rows
 from .prologue import _positions
 
 _SCALINGS = ("none", "linear", "base", "bands", "ramp")
@@ -148,12 +148,15 @@ def _launch(q, k, positions, rotary, backward):
 
 class Rotate(torch.autograd.Function):
     """Rotation of queries and keys in one launch; the backward turns the gradients back,
-    which is a rotation again (and differentiable as one)."""
+    which is a rotation again (and differentiable as one), and tangents turn as their
+    tensors do."""
 
     @staticmethod
     def forward(ctx, q, k, positions, rotary, back):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.back = rotary, back
+        ctx.shapes = tuple(None if x is None else x.shape for x in (q, k))
         ctx.set_materialize_grads(False)
         return _launch(q, k, positions, rotary, back)
 
@@ -163,9 +166,18 @@ class Rotate(torch.autograd.Function):
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is None and dk is None:
             return None, None, None, None, None
-        turn = Rotate.apply if torch.is_grad_enabled() else _launch
+        turn = Rotate.apply if torch.is_grad_enabled() or carries_tangent(dq, dk) else _launch
         dq, dk = turn(dq, dk, ctx.saved_tensors[0], ctx.rotary, not ctx.back)
         return dq, dk, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        turn = Rotate.apply if torch.is_grad_enabled() else _launch
+        out = turn(tq, tk, ctx.saved_tensors[0], ctx.rotary, ctx.back)
+        one = out[0] if out[1] is None else out[1]
+        # (an output that has a tangent beside it needs one too)
+        return tuple(one.new_zeros(s) if t is None and s is not None else t
+                     for t, s in zip(out, ctx.shapes))
 
 
 def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positions=None
@@ -176,8 +188,8 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
     three dimensions) in int32's range; ``None`` means ``0 .. T-1`` on every row.
     ``key`` may be ``None``.  Slices of one projection are read where they are as
     long as each head is dense and tokens are evenly spaced.  Differentiable in
-    both.  A backward is captured into a graph together with its forward
-    and while no eager graph of the same leaves is alive, as for any operation:
+    both, in reverse and in forward mode.  A backward is captured into a graph
+    together with its forward and while no eager graph of the same leaves is alive, as for any operation:
     autograd accumulates a leaf's gradient on the stream of its oldest graph.
     """
     if not isinstance(rotary, Rotary):
@@ -201,7 +213,8 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
         pos = _positions(positions, query.shape[0], query.shape[1], device)
     else:
         pos = _positions(positions, 1, query.shape[0], device)
-    if not torch.is_grad_enabled() or not (query.requires_grad
-                                           or (key is not None and key.requires_grad)):
+    if (not torch.is_grad_enabled() or not (query.requires_grad
+                                            or (key is not None and key.requires_grad))) \
+            and not carries_tangent(query, key):
         return _launch(query, key, pos, rotary, False)
     return Rotate.apply(query, key, pos, rotary, False)

@@ -14,6 +14,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -47,6 +48,14 @@ def require_device(*tensors: torch.Tensor) -> torch.device:
         if t.get_device() != index:
             raise ValueError("all operands must be on the same device")
     return device
+
+
+def carries_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether an operand is a dual tensor of forward-mode differentiation, whose
+    ``requires_grad`` does not show it.  (A level is entered before any tensor is one; a torch
+    without that number is asked for each tensor.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def dtype_code(t: torch.Tensor) -> int:
