@@ -257,8 +257,8 @@ int mf_rotary_turns(const double* frequencies, int pairs, uint64_t* turns);
  * whole heads in the half layout): pair i of the first rotary_dim dims of each
  * head -- dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved --
  * turns by position * turns[i] and is multiplied by magnitude; the other
- * dims are copied.  fp32 arithmetic (angles exact at any position), one
- * rounding.  backward != 0 turns the other way (the transpose): q and k are
+ * dims are copied.  fp32 arithmetic (turns are counted in whole numbers: no
+ * error grows with the position), one rounding.  backward != 0 turns the other way (the transpose): q and k are
  * then the gradients of q_out and k_out.
  * q [tokens] x [q_heads, head_dim] with q_stride elements between tokens (each
  * head dense), k likewise; q_out and k_out are dense and may be q and k where

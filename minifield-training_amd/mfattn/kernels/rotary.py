@@ -3,9 +3,10 @@
 The general form of ``apply_rotary`` (``kernels/rotary.py:7-39`` of the
 reference, which rotates whole heads in the half layout): pair ``i`` of the
 ``rotary_dim`` rotated dims turns by ``position * frequencies[i]`` and the
-other dims pass.  Arithmetic is float32 (angles exact at any position), rounded
-once to the tensors' dtype; :func:`prologue.qk_norm_rope` rounds every step, as
-the reference's declared types do, so its results differ in the last bit.
+other dims pass.  Arithmetic is float32 (turns are counted in whole
+numbers, so no error grows with the position), rounded once to the tensors'
+dtype; :func:`prologue.qk_norm_rope` rounds every step, as the reference's
+declared types do, so its results differ in the last bit.
 """
 
 from __future__ import annotations
