@@ -99,8 +99,15 @@ constexpr int kHeadShares = 0, kHeadJoins = 2, kHeadEnd = 3, kHeadBegin = 4;
 
 // Bounds: a sequence of M rows has one tile (M <= 32) or ceil(M / 256), so at
 // most sequences + tokens G / 256 in all.  Every boundary between shares adds an
-// item, so there are at most shares + tiles of each kind, and rows of a tile * shares
-// + sum n partial rows.
+// item, so there are at most shares + tiles of each kind.  Only a tile that a boundary
+// cuts has partial rows, an item's worth for each boundary and one more: fewer than
+// rows of a tile * shares for the boundaries, and for the tiles not more than that again
+// nor than there are rows.  And only such a tile has join records: four (32 rows by 8),
+// or, of many rows, 8 with up to 8 items and 32 with more, which takes 8 boundaries.
+// (Of 131072 tokens, 16/8 heads: 87 MB of partial results.  Bounded by the rows of all
+// tiles it was 600.)
+static_assert(kManyRows / kJoinRows <= kJoinFewItems * (kManyRows / kJoinManyRows),
+              "a tile's records against the boundaries that cut it");
 __host__ __device__ inline PagedLayout paged_layout(int sequences, int tokens, int G, int Hkv,
                                                     bool f32) {
   PagedLayout p;
@@ -113,9 +120,14 @@ __host__ __device__ inline PagedLayout paged_layout(int sequences, int tokens, i
   p.cap_tiles = (int)(sequences + rows / (f32 ? kFewRows : kManyRows));
   p.cap_items[kFew] = p.target[kFew] + (f32 ? p.cap_tiles : sequences);
   p.cap_items[kMany] = many ? p.target[kMany] + p.cap_tiles : 0;
-  p.cap_joins = (int)(p.cap_tiles + rows / kJoinRows);
+  const long long joins = p.cap_tiles + rows / kJoinRows;
+  const long long cut_joins = (long long)(kFewRows / kJoinRows) * p.target[kFew] +
+                              (long long)(kManyRows / kJoinManyRows) * p.target[kMany];
+  p.cap_joins = (int)(joins < cut_joins ? joins : cut_joins);
+  const long long cut_rows = (long long)kFewRows * p.target[kFew] + (long long)kManyRows * p.target[kMany];
   p.cap_rows = (size_t)((rows < kFewRows ? rows : kFewRows) * p.target[kFew] +
-                        (rows < kManyRows ? rows : kManyRows) * p.target[kMany] + rows);
+                        (rows < kManyRows ? rows : kManyRows) * p.target[kMany] +
+                        (rows < cut_rows ? rows : cut_rows));
   size_t off = 256;
   p.zeros = off;  off += 256;
   p.tokens = off; off = align256(off + sizeof(PagedToken) * (size_t)tokens);
