@@ -26,9 +26,14 @@
 // Both use S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: an accumulator
 // column is a row of the batch, so its maximum and sum are in-lane reductions and
 // one exchange between the halves, and the probabilities are already the operand
-// of the second product.  Probabilities are rounded to bf16 for it (half a step,
-// 2^-9 of each, of either sign); the sum adds the same rounded values, so that
-// the weights still add to one.
+// of the second product.  Of few rows they go into it as two bf16 parts, within 2^-16
+// of each, so that an output is off by its own rounding alone (1.65e-3 in the mean
+// square; with one part 2.3e-3).  The second part takes single tokens 2 to 3 % longer
+// (64 of them 89.5 us instead of 87, drafts 77 instead of 75.5).  It would take many rows
+// 35 % longer (a chunk over 28 K keys 414 us instead of 307, 16 K causal 853 instead of
+// 610): theirs are rounded to bf16 once, by 2^-8 of each at most, of either sign, as in
+// the packed forward that trains the model; the sum adds the same rounded values, so
+// that the weights still add to one.
 //
 // Items of a split tile write (max, sum, unnormalised output); a second launch
 // joins them in item order.  No atomics: the same inputs give the same bits.
@@ -211,6 +216,29 @@ __device__ __forceinline__ void block_probs(f32x16& s, RowState& st, float c, bf
     const uint32_t a0 = w0[j], a1 = w1[j];
     st.l0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a0), ones, st.l0, false);
     st.l1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a1), ones, st.l1, false);
+  }
+}
+
+// The same in two bf16 parts, p and what p leaves (r): together within 2^-16 of a
+// probability.  The sum adds the probabilities themselves.
+__device__ __forceinline__ void block_probs_split(f32x16& s, RowState& st, float c, bf16x8 (&p)[2],
+                                                  bf16x8 (&r)[2]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], c, -st.shift));
+  p[0] = pack8(s, 0);
+  p[1] = pack8(s, 8);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const u32x4 w = __builtin_bit_cast(u32x4, p[j]);
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = s[8 * j + 2 * i], b = s[8 * j + 2 * i + 1];
+      st.l0 += a;
+      st.l1 += b;
+      x[i] = round_bf16_pair(a - bf16_lo(w[i]), b - bf16_hi(w[i]));
+    }
+    r[j] = __builtin_bit_cast(bf16x8, x);
   }
 }
 
@@ -481,7 +509,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
       __builtin_amdgcn_sched_barrier(0);
       if (more) fetch_keys(next);
       const bool masked = kb + 32 > least || gone;
-      bf16x8 p[HW][2];
+      bf16x8 p[HW][2], rest[HW][2];
 #pragma unroll
       for (int h = 0; h < HW; ++h) {
         if (masked) mask_scores(s[h], opaque(kb), lim, gone, lane);
@@ -490,7 +518,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
           grow(st[h], fmaf(halves_max(mx), c, -st[h].shift), acc[h]);
           if (ALONE) top[h] = (st[h].shift + st[h].lag) * (1.f / c);
         }
-        block_probs(s[h], st[h], c, p[h][0], p[h][1]);
+        if constexpr (ALONE) block_probs(s[h], st[h], c, p[h][0], p[h][1]);
+        else block_probs_split(s[h], st[h], c, p[h], rest[h]);
       }
       if (more) wait_vm_lds<4 * HW>(); else wait_vm_lds<0>();
 #pragma unroll
@@ -522,7 +551,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[h][db] = mfma32x32x16(v[db][j], p[h][j], acc[h][db]);
+          for (int j = 0; j < 2; ++j) {
+            acc[h][db] = mfma32x32x16(v[db][j], p[h][j], acc[h][db]);
+            if constexpr (!ALONE) acc[h][db] = mfma32x32x16(v[db][j], rest[h][j], acc[h][db]);
+          }
       }
       wait_lds();
       __builtin_amdgcn_sched_barrier(0);

@@ -20,11 +20,12 @@ NAN, INF = float("nan"), float("inf")
 SPANS = [(1, 45), (6, 40), (100, 300), (1, 6000), (150, 3000), (1, 0), (5, 3), (33, 900)]
 
 
-def softmax_rows(b, q, key_pages, value_pages, rows, scale=0.125):
+def softmax_rows(b, q, key_pages, value_pages, rows, scale=0.125, weights=2 * HALF_STEP[BF]):
     """(out, bound) of rows (token, head) in float64, by the definition: NaN where a visible score
     is NaN or +inf or all are -inf; a score of -inf has no weight; zeros without a key.
 
-    The bound is that of ``_paged.attend``, over the keys that have a weight."""
+    The bound is that of ``_paged.attend``, over the keys that have a weight; ``weights`` is what
+    rounding them to bf16 may change."""
     out = torch.zeros(len(rows), 64, dtype=torch.float64)
     bound = torch.zeros_like(out)
     group = b.hq // b.hkv
@@ -51,7 +52,7 @@ def softmax_rows(b, q, key_pages, value_pages, rows, scale=0.125):
         out[x] = p @ v[w]
         rel = (2 * 65 * mag + 8 + int(w.sum())) * EPS24
         if b.dtype is BF:
-            rel += 2 * HALF_STEP[BF]
+            rel += weights
         bound[x] = rel * (p @ v[w].abs()) + HALF_STEP[b.dtype] * out[x].abs()
     return out, bound
 
