@@ -166,8 +166,10 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     Keys and the query (where given) are RMS-normalised over each head with
     their gain, if they have one, then rotated at their token's position, if
     ``rotary`` is given; values are copied.  Tokens without a page are left out
-    (their query is still returned).  float32 arithmetic, one rounding.  Pages
-    that several sequences share must not be appended to.  Forward only.
+    (their query is still returned).  Gains are taken in the pages' dtype, as the
+    training prologue (``prologue.qk_norm_rope``) takes them in its tensors': a
+    float32 gain of a bfloat16 model is rounded first.  float32 arithmetic from
+    there, one rounding.  Pages that several sequences share must not be appended to.  Forward only.
     """
     dtype = key_pages.dtype
     for t in (key, value, value_pages) if query is None else (query, key, value, value_pages):
