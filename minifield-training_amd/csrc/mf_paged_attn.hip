@@ -28,11 +28,12 @@
 // one exchange between the halves, and the probabilities are already the operand
 // of the second product.  Of few rows they go into it as two bf16 parts, within 2^-16
 // of each, so that an output is off by its own rounding alone (1.65e-3 in the mean
-// square; with one part 2.3e-3).  The second part takes single tokens 2 to 3 % longer
-// (64 of them 89.5 us instead of 87, drafts 77 instead of 75.5).  It would take many rows
-// 35 % longer (a chunk over 28 K keys 414 us instead of 307, 16 K causal 853 instead of
-// 610): theirs are rounded to bf16 once, by 2^-8 of each at most, of either sign, as in
-// the packed forward that trains the model; the sum adds the same rounded values, so
+// square; with one part 2.3e-3).  The second part takes single tokens and drafts 2 %
+// longer (64 tokens 92.7 us with the join instead of 90.6, drafts 76.1 instead of 75.0);
+// made before the first part's products instead of under them, 3 %.  It would take many
+// rows 35 % longer (a chunk over 28 K keys 414 us instead of 307, 16 K causal 853 instead
+// of 610): theirs are rounded to bf16 once, by 2^-8 of each at most, of either sign, as
+// in the packed forward that trains the model; the sum adds the same rounded values, so
 // that the weights still add to one.
 //
 // Items of a split tile write (max, sum, unnormalised output); a second launch
@@ -219,14 +220,16 @@ __device__ __forceinline__ void block_probs(f32x16& s, RowState& st, float c, bf
   }
 }
 
-// The same in two bf16 parts, p and what p leaves (r): together within 2^-16 of a
-// probability.  The sum adds the probabilities themselves.
-__device__ __forceinline__ void block_probs_split(f32x16& s, RowState& st, float c, bf16x8 (&p)[2],
-                                                  bf16x8 (&r)[2]) {
+// The same, the probabilities themselves kept for their second part.
+__device__ __forceinline__ void block_probs_first(f32x16& s, const RowState& st, float c, bf16x8 (&p)[2]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], c, -st.shift));
   p[0] = pack8(s, 0);
   p[1] = pack8(s, 8);
+}
+// What p leaves of the probabilities, in bf16 too: together within 2^-16 of each.  The
+// sum adds the probabilities.
+__device__ __forceinline__ void block_probs_rest(const f32x16& s, RowState& st, bf16x8 (&p)[2]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const u32x4 w = __builtin_bit_cast(u32x4, p[j]);
@@ -238,7 +241,7 @@ __device__ __forceinline__ void block_probs_split(f32x16& s, RowState& st, float
       st.l1 += b;
       x[i] = round_bf16_pair(a - bf16_lo(w[i]), b - bf16_hi(w[i]));
     }
-    r[j] = __builtin_bit_cast(bf16x8, x);
+    p[j] = __builtin_bit_cast(bf16x8, x);
   }
 }
 
@@ -509,7 +512,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
       __builtin_amdgcn_sched_barrier(0);
       if (more) fetch_keys(next);
       const bool masked = kb + 32 > least || gone;
-      bf16x8 p[HW][2], rest[HW][2];
+      bf16x8 p[HW][2];
 #pragma unroll
       for (int h = 0; h < HW; ++h) {
         if (masked) mask_scores(s[h], opaque(kb), lim, gone, lane);
@@ -519,7 +522,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
           if (ALONE) top[h] = (st[h].shift + st[h].lag) * (1.f / c);
         }
         if constexpr (ALONE) block_probs(s[h], st[h], c, p[h][0], p[h][1]);
-        else block_probs_split(s[h], st[h], c, p[h], rest[h]);
+        else block_probs_first(s[h], st[h], c, p[h]);
       }
       if (more) wait_vm_lds<4 * HW>(); else wait_vm_lds<0>();
 #pragma unroll
@@ -549,12 +552,14 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const ItemView& it,
           }
         }
 #pragma unroll
-        for (int db = 0; db < 2; ++db)
+        for (int part = 0; part < (ALONE ? 1 : 2); ++part) {
+          // (the second part is made under the first one's products)
+          if (part == 1) block_probs_rest(s[h], st[h], p[h]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            acc[h][db] = mfma32x32x16(v[db][j], p[h][j], acc[h][db]);
-            if constexpr (!ALONE) acc[h][db] = mfma32x32x16(v[db][j], rest[h][j], acc[h][db]);
-          }
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int db = 0; db < 2; ++db) acc[h][db] = mfma32x32x16(v[db][j], p[h][j], acc[h][db]);
+        }
       }
       wait_lds();
       __builtin_amdgcn_sched_barrier(0);
