@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     }
     head[kHeadJoins] = min(nrest.a, a.lay.cap_joins);
     head[kHeadEnd] = min(max(a.starts[a.R], 0), a.N);
-    head[kHeadBegin] = min(max(a.starts[0], 0), a.N);
+    head[kHeadBegin] = l.start[0];
   }
 }
 
