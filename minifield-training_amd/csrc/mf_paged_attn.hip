@@ -10,15 +10,14 @@
 //     own in LDS: no barrier until the states of waves that share an item are
 //     merged.  Bound: HBM, each cached key and value is read once for all rows of
 //     its head.  One token for each of 64 sequences of 129 to 8192 keys, 16/8 heads
-//     (494 MB): 82 us, 6.0 TB/s, and the join 5; 24 sequences of 3 to 8 drafts, 24/8
-//     heads (391 MB): 68 and 5.  Half the workgroups a CU take 3 % longer.
+//     (494 MB): 84 us, 5.9 TB/s, and the join 5; 24 sequences of 3 to 8 drafts, 24/8
+//     heads (391 MB): 70 and 5.  Half the workgroups a CU take 3 % longer.
 //   up to 256 rows (chunks), one KV head: every wave holds 64 rows, all share
 //     64-key stages in a ring of four, so an operand read from LDS feeds two MFMAs.
 //     2048 tokens behind 28672, 16/8 heads: 275 to 300 us with the join, 830 to 900
 //     TFLOP/s; 16384 behind none 605 (a large bf16 matrix product on the card: 1190
-//     TFLOP/s).  MFMA
-//     busy 41 % of the cycles, VALU 58 %, and the clock: the same launch over zeros
-//     takes 14 % less.  (8 maxima less a block changed nothing.)
+//     TFLOP/s).  MFMA busy 41 % of the cycles, VALU 58 %, and the clock: the same launch
+//     over zeros takes 14 % less.  (8 maxima less a block changed nothing.)
 //
 // The same sequences with 24 rows on the second path: 101 us instead of 76, so few
 // rows end at 32, what one MFMA holds.
