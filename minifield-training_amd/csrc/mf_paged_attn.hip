@@ -44,8 +44,8 @@
 // are zero.  A NaN marks the sum (a maximum passes over it), +infinity does so with the
 // subtraction of the shift, and a row that has only scores of -infinity gets the lowest
 // finite maximum and a sum of one at its end (mark_low): beside any other maximum its
-// weight is 0, and without one the row is NaN (row_factor).  What tells sums apart looks at their bits: the file
-// is compiled as if no comparison saw a NaN.
+// weight is 0, and without one the row is NaN (row_factor).  What tells sums apart looks
+// at their bits: the file is compiled as if no comparison saw a NaN.
 //
 // Pages.  Page sizes are multiples of 8 and blocks start at multiples of 32, so
 // eight keys of a block lie in one page: their page number is a scalar load, and

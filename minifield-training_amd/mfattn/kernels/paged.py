@@ -127,9 +127,10 @@ def plan(query_starts: torch.Tensor, context_lengths: torch.Tensor, page_table: 
     included.  Token position ``p`` of sequence ``r`` is slot ``p % page_size``
     of page ``page_table[r, p // page_size]``; entries outside the pool (-1, say,
     behind a context or for a page that was given up) hold no keys, nor do
-    positions beyond the table.  Nothing is read back to the host.  The table must stay as it is while the plan is used;
-    on another stream, once that waits for the plan's; a captured graph that reads
-    a plan made outside of it needs the plan kept.
+    positions beyond the table.  Nothing is read back to the host.  The table
+    must stay as it is while the plan is used.  Another stream may use the plan
+    once it waits for the plan's; a captured graph that reads a plan made outside
+    of it needs the plan kept.
     """
     if key_pages.dim() != 4:
         raise ValueError("pages must be [pages, page_size, heads, head_dim]")
@@ -169,7 +170,8 @@ def append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
     (their query is still returned).  Gains are taken in the pages' dtype, as the
     training prologue (``prologue.qk_norm_rope``) takes them in its tensors': a
     float32 gain of a bfloat16 model is rounded first.  float32 arithmetic from
-    there, one rounding.  Pages that several sequences share must not be appended to.  Forward only.
+    there, one rounding.  Pages that several sequences share must not be
+    appended to.  Forward only.
     """
     dtype = key_pages.dtype
     for t in (key, value, value_pages) if query is None else (query, key, value, value_pages):
@@ -230,7 +232,8 @@ def attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.T
     :func:`append`).  A query that sees no key yields zeros; a NaN or +infinity
     among its scores, or none above -infinity, yields NaN.  ``scale`` defaults
     to ``64 ** -0.5``.  Rows before the first sequence and behind the last are
-    zeros, or left as they are in an ``out`` that is given.  Slots behind a context may hold anything.
+    zeros, or left as they are in an ``out`` that is given.  Slots behind a
+    context may hold anything.
     Forward only; the same inputs give the same bits.
     """
     shape, dtype = plan.q_shape, query.dtype

@@ -190,8 +190,9 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, rotary: Rotary, positi
     ``key`` may be ``None``.  Slices of one projection are read where they are as
     long as each head is dense and tokens are evenly spaced.  Differentiable in
     both, in reverse and in forward mode.  A backward is captured into a graph
-    together with its forward and while no eager graph of the same leaves is alive, as for any operation:
-    autograd accumulates a leaf's gradient on the stream of its oldest graph.
+    together with its forward and while no eager graph of the same leaves is
+    alive, as for any operation: autograd accumulates a leaf's
+    gradient on the stream of its oldest graph.
     """
     if not isinstance(rotary, Rotary):
         raise ValueError("rotary must be a Rotary")

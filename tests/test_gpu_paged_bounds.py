@@ -37,7 +37,8 @@ def test_rows_of_tiles_that_are_cut(case, dtype, device):
     b = Batch(spans, hq, hkv, 16, dtype, device, seed=len(spans))
     out = paged.attention(b.q, b.key_pages, b.value_pages, b.plan())
     rng = np.random.default_rng(hq)
-    tokens = np.unique(np.concatenate((rng.integers(0, b.tokens, 60), b.starts[:-1][:20], b.starts[1:][:20] - 1)))
+    tokens = np.unique(np.concatenate((rng.integers(0, b.tokens, 60), b.starts[:20][:len(spans)],
+                                       b.starts[1:21] - 1)))
     rows = [(int(t), int(rng.integers(0, hq))) for t in tokens]
     want, bound = softmax_rows(b, b.q, b.key_pages, b.value_pages, rows)
     got = torch.stack([out[t, h] for t, h in rows]).double().cpu()
