@@ -1,0 +1,435 @@
+"""The two ends of a packed training step and the norm between them, as cases.
+
+A case is one pass through an operator: ``norm`` (layer norm or RMS norm over the
+hidden width, with its backward pass in training), ``embed`` (embedding lookup with
+scaling, with the table's gradient in training) or ``distill`` (the loss against a
+teacher's top logits: alone, with its backward pass, or loss and gradient in one
+call).  Sizes are those of the framework's own layouts (16 heads of 64, 8 x 4096
+packed tokens) with the smaller, longer and odd ones around them.
+
+``listed()`` names the cases, ``draw(rng)`` gives more of the same ranges,
+``prepare`` makes what a program holds before the call, ``run`` is the call: in
+elementary operations where ``own`` is false, through the framework where it is
+true.  ``exact`` is the operators' definition in 64 bits.
+"""
+
+from __future__ import annotations
+
+import math
+import pathlib
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+_BYTES = {"bfloat16": 2, "float32": 4}
+_EPS = 1e-5
+
+
+# --------------------------------------------------------------------------- cases
+
+
+def _norm(dtype, rows, dim, train, center=True, bias=True):
+    """``center``: layer norm, RMS norm otherwise."""
+    return {"kind": "norm", "dtype": dtype, "rows": rows, "dim": dim, "train": train,
+            "center": center, "bias": bias and center}
+
+
+def _embed(dtype, tokens, vocabulary, dim, train, scale=1.0, skew=1.0, pad=0.0):
+    """Token frequencies fall as ``rank ** -skew``; a share ``pad`` of the tokens is padding."""
+    return {"kind": "embed", "dtype": dtype, "tokens": tokens, "vocabulary": vocabulary, "dim": dim,
+            "train": train, "scale": scale, "skew": skew, "pad": pad}
+
+
+def _distill(dtype, rows, vocabulary, top, how, temperature=1.0, total=False, masked=0.0,
+             short=0.0):
+    """``how``: loss (alone), train (with its backward pass) or both (loss and gradient in one
+    call).  ``total``: the teacher's whole mass is known.  A share ``masked`` of the rows weighs
+    nothing, a share ``short`` has half of its teacher's entries."""
+    return {"kind": "distill", "dtype": dtype, "rows": rows, "vocabulary": vocabulary, "top": top,
+            "how": how, "temperature": temperature, "total": total, "masked": masked,
+            "short": short}
+
+
+def listed():
+    return [
+        # the norm in front of a decode step's mixer: launches
+        {"name": "norm_step", **_norm("bfloat16", 64, 1024, False, center=False)},
+        # layer norm of a packed training step at the framework's headline layout
+        {"name": "norm_train", **_norm("bfloat16", 8 * 4096, 1024, True)},
+        # RMS norm of a wide model's step
+        {"name": "norm_train_wide", **_norm("bfloat16", 4096, 8192, True, center=False)},
+        # a float32 check of a small model: odd width, ragged rows
+        {"name": "norm_train_fp32", **_norm("float32", 3 * 333, 771, True)},
+        # a serving batch's next tokens: launches
+        {"name": "embed_step", **_embed("bfloat16", 64, 65536, 1024, False)},
+        # the tokens of a packed training step, an eighth of them padding: rows in, whole
+        # table's gradient out
+        {"name": "embed_train", **_embed("bfloat16", 8 * 4096, 65536, 1024, True,
+                                         scale=32.0, pad=0.125)},
+        # a small vocabulary in float32: every row met many times, odd width
+        {"name": "embed_train_fp32", **_embed("float32", 5001, 1003, 129, True, skew=1.3)},
+        # the loss over a batch of the last tokens' logits, evaluation
+        {"name": "distill_loss", **_distill("bfloat16", 64, 65536, 32, "loss", 2.0)},
+        # a training step of one packed row through autograd, with padding
+        {"name": "distill_train", **_distill("bfloat16", 4096, 65536, 64, "train", 2.0,
+                                             masked=0.125)},
+        # the same with loss and gradient in one call and the teacher's whole mass
+        {"name": "distill_both", **_distill("bfloat16", 4096, 65536, 64, "both", 1.0, True,
+                                            masked=0.125)},
+        # a float32 check over an odd vocabulary, short teacher rows
+        {"name": "distill_fp32", **_distill("float32", 333, 32003, 100, "both", 1.5, True,
+                                            short=0.2)},
+        # few tokens of a vision-and-text vocabulary, latency of a small step
+        {"name": "distill_few", **_distill("bfloat16", 24, 131077, 16, "train", 1.0, short=0.1)},
+    ]
+
+
+def _log_int(rng, low, high):
+    return min(high, max(low, int(math.exp(rng.uniform(math.log(low), math.log(high + 1))))))
+
+
+_DIMS = (1024, 1024, 256, 768, 2048, 4096, 8192)
+_VOCABULARIES = (65536, 65536, 32000, 50000, 128000)
+_MOST = 1.05e9  # bytes of the largest listed case, about
+
+
+def draw(rng):
+    """One more case: the listed kinds at sizes spread over their ranges."""
+    kind = rng.choice(("norm", "embed", "distill"))
+    dtype = "float32" if rng.random() < 0.25 else "bfloat16"
+    size = _BYTES[dtype]
+    if kind == "norm":
+        dim = rng.choice(_DIMS) if rng.random() < 0.5 else _log_int(rng, 16, 8192)
+        rows = _log_int(rng, 1, min(65536, int(4e8) // (4 * dim * size)))
+        return _norm(dtype, rows, dim, rng.random() < 0.7, rng.random() < 0.6, rng.random() < 0.8)
+    if kind == "embed":
+        dim = rng.choice(_DIMS[:5]) if rng.random() < 0.6 else _log_int(rng, 16, 4096)
+        most = int(4e8) // (dim * size)
+        vocabulary = rng.choice(_VOCABULARIES) if rng.random() < 0.5 else _log_int(rng, 100, 131072)
+        vocabulary = min(vocabulary, most)
+        tokens = _log_int(rng, 1, min(65536, most // 2))
+        return _embed(dtype, tokens, vocabulary, dim, rng.random() < 0.7,
+                      rng.choice((1.0, 1.0, dim ** 0.5)), rng.choice((0.0, 0.8, 1.0, 1.3)),
+                      rng.choice((0.0, 0.0, 0.1, 0.4)))
+    how = rng.choice(("loss", "train", "both"))
+    vocabulary = rng.choice(_VOCABULARIES) if rng.random() < 0.5 else _log_int(rng, 300, 150000)
+    rows = _log_int(rng, 1, min(8192, int(_MOST) // (2 * vocabulary * size)))
+    return _distill(dtype, rows, vocabulary, _log_int(rng, 1, 256), how,
+                    rng.choice((1.0, 1.0, 2.0, 1.5, 0.7, 4.0)), rng.random() < 0.5,
+                    rng.choice((0.0, 0.0, 0.1, 0.5)), rng.choice((0.0, 0.0, 0.2)))
+
+
+# --------------------------------------------------------------------------- inputs
+
+
+def _shares(case):
+    """The frequency of every token id, in 64 bits."""
+    p = (2.0 + np.arange(case["vocabulary"])) ** -case["skew"]
+    return p / p.sum()
+
+
+def _later(n, device):
+    return torch.arange(n, device=device) > 0
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    dtype = _DTYPES[case["dtype"]]
+
+    def normal(*shape, kind=dtype):
+        return torch.randn(shape, generator=gen, device=dev, dtype=kind)
+
+    def uniform(*shape):
+        return torch.rand(shape, generator=gen, device=dev)
+
+    state = {"case": case}
+    if case["kind"] == "norm":
+        n, d = case["rows"], case["dim"]
+        # rows of a residual stream: a size and an offset of their own
+        x = normal(n, d) * (0.5 + 2 * uniform(n, 1)).to(dtype) + normal(n, 1)
+        state["x"] = x.to(dtype)
+        state["weight"] = (1 + 0.2 * normal(d, kind=torch.float32)).to(dtype)
+        state["bias"] = (0.2 * normal(d, kind=torch.float32)).to(dtype) if case["bias"] else None
+        if case["train"]:
+            state["dy"] = normal(n, d)
+            for name in ("x", "weight", "bias"):
+                if state[name] is not None:
+                    state[name].requires_grad_()
+        return state
+    if case["kind"] == "embed":
+        n, v, d = case["tokens"], case["vocabulary"], case["dim"]
+        p = torch.from_numpy(_shares(case)).to(dev)
+        u = torch.rand(n, generator=gen, device=dev, dtype=torch.float64)
+        ids = torch.searchsorted(p.cumsum(0), u).clamp(max=v - 1)
+        # padding as a packer leaves it; a batch has a token
+        state["ids"] = ids.masked_fill((uniform(n) < case["pad"]) & _later(n, dev), -1)
+        state["table"] = normal(v, d)
+        if case["train"]:
+            state["table"].requires_grad_()
+            state["dout"] = normal(n, d)
+        return state
+    n, v, k, t = case["rows"], case["vocabulary"], case["top"], case["temperature"]
+    # the teacher's entries: places of their own in the vocabulary, sizes that fall off
+    gap = torch.randint(1, max(1, v // k) + 1, (n, k), generator=gen, device=dev)
+    places = gap.cumsum(1) - 1
+    ids = places.gather(1, uniform(n, k).argsort(1))
+    teacher = 9 - (0.02 + uniform(n, k)).mul_(8 / k).cumsum(1) + 0.1 * uniform(n, k)
+    teacher = teacher.to(dtype)
+    # a student that has learned some of it
+    logits = normal(n, v).mul_(1.5)
+    logits.scatter_add_(1, ids, teacher * 0.7 + normal(n, k))
+    if case["total"]:
+        beyond = 0.02 + 0.2 * uniform(n)
+        state["total"] = torch.logsumexp(teacher.float() / t, 1) + torch.log1p(beyond)
+    half = (torch.arange(k, device=dev) >= (k + 1) // 2) & (uniform(n, 1) < case["short"])
+    state["teacher_ids"] = ids.masked_fill(half, -1).to(torch.int32)
+    state["teacher_logits"], state["logits"] = teacher, logits
+    gone = (uniform(n) < case["masked"]) & _later(n, dev)
+    state["weights"] = (0.5 + uniform(n)).masked_fill(gone, 0)
+    if case["how"] == "train":
+        logits.requires_grad_()
+        # the mean over the batch's rows
+        state["dloss"] = torch.full((n,), 1 / n, device=dev)
+    return state
+
+
+# --------------------------------------------------------------------------- the call
+
+
+def run(state):
+    case = state["case"]
+    if own:
+        return _call(case, state)
+    return {"norm": _plain_norm, "embed": _plain_embed, "distill": _plain_distill}[case["kind"]](
+        case, state)
+
+
+def _call(case, s):
+    """The same pass through the framework."""
+    package = str(pathlib.Path(__file__).resolve().parents[1] / "minifield-training_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from mfattn.kernels import distillation, embedding, normalization
+
+    if case["kind"] == "norm":
+        if case["center"]:
+            y = normalization.layer_norm(s["x"], s["weight"], s["bias"], eps=_EPS)
+        else:
+            y = normalization.rms_norm(s["x"], s["weight"], eps=_EPS)
+        if not case["train"]:
+            return {"y": y}
+        names = [n for n in ("x", "weight", "bias") if s[n] is not None]
+        grads = torch.autograd.grad(y, [s[n] for n in names], s["dy"])
+        return {"y": y.detach(), **{"d" + n: g for n, g in zip(names, grads)}}
+    if case["kind"] == "embed":
+        out = embedding.embed(s["ids"], s["table"], scale=case["scale"])
+        if not case["train"]:
+            return {"out": out}
+        (dtable,) = torch.autograd.grad(out, s["table"], s["dout"])
+        return {"out": out.detach(), "dtable": dtable}
+    args = (s["logits"], s["teacher_logits"], s["teacher_ids"])
+    more = {"temperature": case["temperature"], "teacher_total": s.get("total"),
+            "weights": s["weights"]}
+    if case["how"] == "both":
+        loss, dlogits = distillation.top_logits_loss_and_gradient(*args, **more)
+        return {"loss": loss, "dlogits": dlogits}
+    loss = distillation.top_logits_loss(*args, **more)
+    if case["how"] == "loss":
+        return {"loss": loss}
+    (dlogits,) = torch.autograd.grad(loss, s["logits"], s["dloss"])
+    return {"loss": loss.detach(), "dlogits": dlogits}
+
+
+# --------------------------------------------------------------------------- plain forms
+
+
+@torch.no_grad()
+def _plain_norm(case, s):
+    dtype = s["x"].dtype
+    x, w = s["x"].float(), s["weight"].float()
+    if case["center"]:
+        x = x - x.mean(-1, keepdim=True)
+    rstd = torch.rsqrt((x * x).mean(-1, keepdim=True) + _EPS)
+    xhat = x * rstd
+    y = xhat * w
+    if case["bias"]:
+        y = y + s["bias"].float()
+    res = {"y": y.to(dtype)}
+    if case["train"]:
+        dy = s["dy"].float()
+        g = dy * w
+        dx = g - xhat * (g * xhat).mean(-1, keepdim=True)
+        if case["center"]:
+            dx = dx - g.mean(-1, keepdim=True)
+        res["dx"] = (dx * rstd).to(dtype)
+        res["dweight"] = (dy * xhat).sum(0).to(dtype)
+        if case["bias"]:
+            res["dbias"] = dy.sum(0).to(dtype)
+    return res
+
+
+@torch.no_grad()
+def _plain_embed(case, s):
+    table, ids = s["table"], s["ids"]
+    met = ids >= 0
+    at = ids.clamp(min=0)
+    out = table[at].float() * case["scale"]
+    res = {"out": torch.where(met[:, None], out, 0).to(table.dtype)}
+    if case["train"]:
+        d = torch.where(met[:, None], s["dout"].float() * case["scale"], 0)
+        res["dtable"] = torch.zeros(table.shape, device=table.device).index_add_(0, at, d).to(table.dtype)
+    return res
+
+
+@torch.no_grad()
+def _plain_distill(case, s):
+    dtype, t = s["logits"].dtype, case["temperature"]
+    v = case["vocabulary"]
+    z = s["logits"].float() / t
+    top = z.amax(1, keepdim=True)
+    e = torch.exp(z - top)
+    total = e.sum(1, keepdim=True)
+    there = s["teacher_ids"] >= 0
+    at = s["teacher_ids"].long().clamp(min=0)
+    u = (s["teacher_logits"].float() / t).masked_fill(~there, -math.inf)
+    if case["total"]:
+        logp = u - s["total"][:, None]
+    else:
+        most = u.amax(1, keepdim=True)
+        logp = u - most - torch.log(torch.exp(u - most).sum(1, keepdim=True))
+    p = torch.exp(logp)
+    logq = z.gather(1, at) - top - torch.log(total)
+    loss = torch.where(there, p * (logp - logq), 0).sum(1)
+    if case["total"]:
+        # what is left of one: in 64 bits
+        rest = (1 - torch.exp(u.double() - s["total"].double()[:, None]).sum(1)).clamp(min=0).float()
+        named = torch.zeros((z.shape[0], v + 1), dtype=torch.bool, device=z.device)
+        named = named.scatter_(1, torch.where(there, at, v), True)[:, :v]
+        beyond = torch.where(named, 0, e).sum(1)
+        loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - torch.log(beyond / total[:, 0])), 0)
+    w = s["weights"] * (t * t)
+    res = {"loss": torch.where(w != 0, loss * w, 0)}
+    if case["how"] != "loss":
+        w = s["weights"] * t
+        if case["how"] == "train":
+            w = w * s["dloss"]
+        d = e / total
+        if case["total"]:
+            d = d - torch.where(named, 0, e * (rest / beyond)[:, None])
+        d.scatter_add_(1, at, -p)  # entries that are not there have no mass
+        res["dlogits"] = torch.where(w[:, None] != 0, d * w[:, None], 0).to(dtype)
+    return res
+
+
+# --------------------------------------------------------------------------- work
+
+
+def work(case):
+    size = _BYTES[case["dtype"]]
+    if case["kind"] == "norm":
+        values, d = case["rows"] * case["dim"], case["dim"]
+        params = d * size * (2 if case["bias"] else 1)
+        passes = 4 if case["train"] else 2
+        return {"bytes": passes * values * size + params * (2 if case["train"] else 1),
+                "flops": values * (22 if case["train"] else 8)}
+    if case["kind"] == "embed":
+        n, v, d = case["tokens"], case["vocabulary"], case["dim"]
+        real = n * (1 - case["pad"])
+        rows = float((1 - (1 - _shares(case)) ** real).sum())  # different ones, expected
+        nbytes, flops = 8 * n + (rows + n) * d * size, n * d
+        if case["train"]:
+            nbytes += (real + v) * d * size
+            flops += n * d
+        return {"bytes": nbytes, "flops": flops}
+    n, v, k = case["rows"], case["vocabulary"], case["top"]
+    live = n * (1 - case["masked"])
+    nbytes = live * (v * size + k * (size + 4)) + 8 * n + (4 * n if case["total"] else 0)
+    flops = live * v * 5
+    if case["how"] != "loss":
+        nbytes += n * v * size
+        flops += live * v * 4
+    return {"bytes": nbytes, "flops": flops}
+
+
+# --------------------------------------------------------------------------- 64 bits
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"norm": _exact_norm, "embed": _exact_embed, "distill": _exact_distill}[case["kind"]](
+        case, s)
+
+
+def _exact_norm(case, s):
+    """The definition, differentiated by torch."""
+    leaves = {n: s[n].detach().double().requires_grad_() for n in ("x", "weight", "bias")
+              if s[n] is not None}
+    x = leaves["x"]
+    mean = x.sum(1) / x.shape[1] if case["center"] else x.new_zeros(x.shape[0])
+    off = x - mean[:, None]
+    spread = torch.sqrt(off.pow(2).sum(1) / x.shape[1] + _EPS)
+    y = off / spread[:, None] * leaves["weight"]
+    if case["bias"]:
+        y = y + leaves["bias"]
+    if not case["train"]:
+        return {"y": y.detach()}
+    grads = torch.autograd.grad(y, list(leaves.values()), s["dy"].double())
+    return {"y": y.detach(), **{"d" + n: g for n, g in zip(leaves, grads)}}
+
+
+def _exact_embed(case, s):
+    table, ids = s["table"].detach().double(), s["ids"]
+    real = ids >= 0
+    out = torch.zeros((len(ids), case["dim"]), dtype=torch.float64, device=ids.device)
+    out[real] = table.index_select(0, ids[real]) * case["scale"]
+    if not case["train"]:
+        return {"out": out}
+    # tokens in the order of their ids: a row's gradient is the difference of two running sums
+    order = ids[real].argsort(stable=True)
+    met, count = torch.unique_consecutive(ids[real][order], return_counts=True)
+    last = count.cumsum(0)
+    running = torch.cat((out.new_zeros(1, case["dim"]), s["dout"][real][order].double().cumsum(0)))
+    dtable = torch.zeros_like(table)
+    dtable[met] = (running[last] - running[last - count]) * case["scale"]
+    return {"out": out, "dtable": dtable}
+
+
+def _exact_distill(case, s):
+    """The definition row by row, in blocks of rows, differentiated by torch."""
+    losses, grads = [], []
+    step = max(1, (1 << 25) // case["vocabulary"])
+    for first in range(0, case["rows"], step):
+        rows = slice(first, first + step)
+        z = s["logits"][rows].detach().double().requires_grad_(case["how"] != "loss")
+        w = s["weights"][rows].double()
+        if case["how"] == "train":
+            w = w * s["dloss"][rows].double()
+        logq = torch.log_softmax(z / case["temperature"], 1)
+        ids = s["teacher_ids"][rows].long()
+        here = ids >= 0
+        u = s["teacher_logits"][rows].double() / case["temperature"]
+        whole = s["total"][rows].double() if case["total"] else \
+            torch.logsumexp(torch.where(here, u, -math.inf), 1)
+        logp = u - whole[:, None]
+        p = torch.where(here, logp.exp(), 0)
+        kl = (p * (logp - logq.gather(1, ids.clamp(min=0)))).sum(1)
+        if case["total"]:
+            rest = (1 - p.sum(1)).clamp(min=0)
+            # the student's mass beyond the named entries: without them, not one less them
+            hidden = torch.zeros_like(z, requires_grad=False)
+            hidden.scatter_add_(1, ids.clamp(min=0), here.double())
+            beyond = torch.logsumexp(logq.masked_fill(hidden > 0, -math.inf), 1)
+            kl = kl + torch.where(rest > 0, rest * (rest.clamp(min=1e-300).log() - beyond), 0)
+        kl = kl * case["temperature"] ** 2
+        if case["how"] != "loss":
+            grads.append(torch.autograd.grad((kl * w).sum(), z)[0])
+        losses.append(kl.detach() * s["weights"][rows].double())
+    res = {"loss": torch.cat(losses)}
+    if grads:
+        res["dlogits"] = torch.cat(grads)
+    return res
