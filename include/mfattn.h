@@ -376,6 +376,88 @@ int mf_segmented_conv_bwd(const void* b_gate, const void* c_gate,
                           void* d_c_gate, void* d_values, float* d_taps,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* Layer norm (center != 0) or RMS norm of every row of x [rows, dim], x_stride
+ * elements between rows:  y = (x - mean) * rstd * weight + bias,  rstd =
+ * (mean of (x - mean)^2 + eps)^-1/2, the mean being zero for the RMS norm
+ * (kernels/bidirectional.py's layer norm and kernels/normalization.py:7-22 over
+ * the hidden width).  fp32 arithmetic, one rounding.  weight [dim] and bias
+ * [dim] (NULL: none; none with the RMS norm) in param_dtype, which is dtype or
+ * MF_DTYPE_F32.  y is dense, and may be x where that is.  stats, NULL or
+ * [rows][2] fp32, receives mean and rstd for mf_norm_bwd.  dim up to 16384, up
+ * to 2^22 rows. */
+int mf_norm(const void* x, long long x_stride, const void* weight,
+            const void* bias, int dtype, int param_dtype, int rows, int dim,
+            int center, float eps, void* y, float* stats, void* stream);
+
+/* Backward of mf_norm: dx [rows, dim] (dense; may be dy where that is), and
+ * dweight and dbias [dim] in param_dtype, summed over the rows in fp32 in a fixed
+ * order; each may be NULL where it is not wanted.  `workspace` holds the sums of the
+ * launch's workgroups (mf_norm_bwd_workspace_bytes, 0 for sizes that the call
+ * refuses). */
+size_t mf_norm_bwd_workspace_bytes(int rows, int dim, int dtype);
+int mf_norm_bwd(const void* x, long long x_stride, const void* weight,
+                const float* stats, const void* dy, long long dy_stride,
+                int dtype, int param_dtype, int rows, int dim, int center,
+                void* dx, void* dweight, void* dbias, void* workspace,
+                size_t workspace_bytes, void* stream);
+
+/* Embedding lookup: out[n] = scale * table[ids[n]] (fp32, one rounding) for
+ * tokens ids of id_bytes (4 or 8) each, table [vocabulary, dim] with table_stride
+ * elements between rows, out [tokens, dim] dense.  Ids outside the table, and
+ * padding_id (-1: none), give rows of zeros. */
+int mf_embed(const void* ids, int id_bytes, const void* table,
+             long long table_stride, int dtype, int tokens, int vocabulary,
+             int dim, long long padding_id, float scale, void* out,
+             void* stream);
+
+/* Gradient of mf_embed's table: dtable[v] (dense, 16-byte aligned, written whole)
+ * = scale * the sum of dout[n] over the tokens with ids[n] = v, in fp32 in
+ * an order that depends on the ids alone: the same inputs give the same bits.
+ * dout [tokens, dim] with dout_stride elements between rows.  `workspace`
+ * (16-byte aligned, mf_embed_bwd_workspace_bytes) holds the sorted tokens; it is this
+ * call's alone while it runs. */
+size_t mf_embed_bwd_workspace_bytes(int tokens, int vocabulary, int dim);
+int mf_embed_bwd(const void* ids, int id_bytes, const void* dout,
+                 long long dout_stride, int dtype, int tokens, int vocabulary,
+                 int dim, long long padding_id, float scale, void* dtable,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits.  For row n of logits [rows,
+ * vocabulary] (stride elements between rows), q = softmax(logits / temperature),
+ * and the teacher's entries (teacher_ids[n][k], teacher[n][k]), k < top:
+ *   p = softmax(teacher / temperature) over the row's entries, or, where total
+ *   [rows] fp32 holds the logarithm of the teacher's whole sum,
+ *   exp(teacher / temperature - total), with what is left of one, r = 1 - sum p
+ *   (at least 0), on the other ids together;
+ *   loss[n] = weights[n] * temperature^2 * (sum_k p_k (log p_k - log q_k)
+ *             + r (log r - log of q's sum over the ids that no entry names)).
+ * Entries whose id is outside the vocabulary are not there.  A row of weight zero
+ * (weights [rows] fp32, NULL: ones) has loss zero and no gradient, whatever it
+ * holds, and so has one without entries (and without total).  Masses and sums
+ * of a row in 64 bits, its exponentials in fp32.  teacher [rows, top] in
+ * teacher_dtype, teacher_ids [rows, top] of id_bytes (4 or 8) each.  up to 1024
+ * entries a row, vocabularies up to 393216, and 2^35 logits.
+ * With dlogits (grad_stride elements between rows; may be logits itself) also
+ * the gradient of the sum of the losses, in dtype, in the same pass.  stats, NULL or
+ * rows * (4 + top) fp32, receives what mf_distill_bwd needs. */
+size_t mf_distill_stats_bytes(int rows, int top);
+int mf_distill(const void* logits, long long stride, const void* teacher,
+               int teacher_dtype, const void* teacher_ids, int id_bytes,
+               const float* total, const float* weights, int dtype, int rows,
+               int vocabulary, int top, double temperature, float* loss,
+               float* stats, size_t stats_bytes, void* dlogits,
+               long long grad_stride, void* stream);
+
+/* Backward of mf_distill's loss: dlogits of the sum of dloss[n] * loss[n] (dloss
+ * [rows] fp32), from the same operands and the stats that the forward wrote.
+ * dlogits must not overlap the logits. */
+int mf_distill_bwd(const void* logits, long long stride,
+                   const void* teacher_ids, int id_bytes, const float* weights,
+                   const float* stats, size_t stats_bytes, const float* dloss,
+                   int dtype, int rows, int vocabulary, int top,
+                   double temperature, void* dlogits, long long grad_stride,
+                   void* stream);
+
 /* mf_decode without a workspace argument, for callers that cannot allocate
  * (code under HIP graph capture, tight serving loops, harnesses that forbid
  * hipMalloc); no counterpart in the reference.  The same kernels as mf_decode

@@ -11,6 +11,9 @@
 
 #include "../../include/mfattn.h"
 #include "mf_common.h"
+#include "mf_distill.h"
+#include "mf_embed.h"
+#include "mf_norm.h"
 #include "mf_paged.h"
 
 namespace mf {
@@ -84,6 +87,29 @@ hipError_t launch_paged_attn(const void* q, long long q_stride, const void* k_pa
                              int page_size, int pages, int Hq, int Hkv, float scale,
                              const void* plan, bool zero_rest, void* out, void* workspace,
                              hipStream_t stream);
+hipError_t launch_norm(const void* x, long long x_stride, const void* weight, const void* bias,
+                       bool f32, bool param_f32, int rows, int dim, bool center, float eps, void* y,
+                       float* stats, hipStream_t stream);
+size_t norm_bwd_workspace_bytes(int rows, int dim, bool f32);
+hipError_t launch_norm_bwd(const void* x, long long x_stride, const void* weight,
+                           const float* stats, const void* dy, long long dy_stride, bool f32,
+                           bool param_f32, int rows, int dim, bool center, void* dx, void* dweight,
+                           void* dbias, void* workspace, hipStream_t stream);
+hipError_t launch_embed(const void* ids, bool ids64, const void* table, long long stride, bool f32,
+                        int tokens, int vocabulary, int dim, long long padding, float scale,
+                        void* out, hipStream_t stream);
+hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long long stride,
+                            bool f32, int tokens, int vocabulary, int dim, long long padding,
+                            float scale, void* dtable, void* workspace, hipStream_t stream);
+hipError_t launch_distill(const void* logits, long long stride, const void* teacher,
+                          bool teacher_f32, const void* ids, bool ids64, const float* total,
+                          const float* weights, bool f32, int rows, int vocabulary, int top,
+                          double temperature, float* loss, float* stats, void* grad,
+                          long long grad_stride, hipStream_t stream);
+hipError_t launch_distill_bwd(const void* logits, long long stride, const void* ids, bool ids64,
+                              const float* weights, const float* stats, const float* upstream,
+                              bool f32, int rows, int vocabulary, int top, double temperature,
+                              void* grad, long long grad_stride, hipStream_t stream);
 }  // namespace mf
 
 namespace {
@@ -838,3 +864,216 @@ int abi_check_decode_shape(int dtype, int batch, int capacity, int q_heads, int 
 }
 
 }  // namespace mf
+
+namespace {
+
+// Rows of `width` elements that start `stride` apart.
+int check_rows(const char* what, long long stride, int width) {
+  if (stride < width)
+    return fail(MF_ERR_SHAPE, "%s: %lld elements between rows, rows have %d", what, stride, width);
+  return MF_OK;
+}
+
+bool known_dtype(int dtype) { return dtype == MF_DTYPE_F32 || dtype == MF_DTYPE_BF16; }
+
+bool norm_sizes(int rows, int dim) {
+  return rows >= 1 && rows <= mf::kNormMostRows && dim >= 1 && dim <= mf::kNormMostDim;
+}
+
+int check_norm(int dtype, int param_dtype, int rows, int dim) {
+  if (!known_dtype(dtype)) return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
+  if (param_dtype != dtype && param_dtype != MF_DTYPE_F32)
+    return fail(MF_ERR_DTYPE, "weight and bias must be in the rows' dtype or float32 (code %d)",
+                param_dtype);
+  if (rows < 1 || dim < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT, "Sizes must be positive (rows=%d dim=%d)", rows, dim);
+  if (!norm_sizes(rows, dim))
+    return fail(MF_ERR_SHAPE, "at most %d rows of at most %d (got %d of %d)", mf::kNormMostRows,
+                mf::kNormMostDim, rows, dim);
+  return MF_OK;
+}
+
+bool embed_sizes(int tokens, int vocabulary, int dim) {
+  return tokens >= 1 && tokens <= mf::kEmbedMostTokens && vocabulary >= 1 &&
+         vocabulary <= mf::kEmbedMostVocabulary && dim >= 1 && dim <= mf::kEmbedMostDim &&
+         (long long)tokens * dim <= mf::kEmbedMostValues;
+}
+
+int check_embed(int dtype, int id_bytes, int tokens, int vocabulary, int dim, float scale) {
+  if (!known_dtype(dtype)) return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
+  if (id_bytes != 4 && id_bytes != 8)
+    return fail(MF_ERR_DTYPE, "ids must have 4 or 8 bytes (got %d)", id_bytes);
+  if (tokens < 1 || vocabulary < 1 || dim < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT, "Sizes must be positive (tokens=%d vocabulary=%d dim=%d)",
+                tokens, vocabulary, dim);
+  if (!embed_sizes(tokens, vocabulary, dim))
+    return fail(MF_ERR_SHAPE,
+                "at most %d tokens, %d rows of %d and %lld values (got %d tokens, %d rows of %d)",
+                mf::kEmbedMostTokens, mf::kEmbedMostVocabulary, mf::kEmbedMostDim,
+                mf::kEmbedMostValues, tokens, vocabulary, dim);
+  if (!std::isfinite(scale))
+    return fail(MF_ERR_INVALID_ARGUMENT, "scale must be finite (got %g)", (double)scale);
+  return MF_OK;
+}
+
+bool distill_sizes(int rows, int top) {
+  return rows >= 1 && rows <= mf::kDistillMostRows && top >= 1 && top <= mf::kDistillMostTop;
+}
+
+int check_distill(int dtype, int id_bytes, int rows, int vocabulary, int top, double temperature) {
+  if (!known_dtype(dtype)) return fail(MF_ERR_DTYPE, "Unsupported dtype code %d", dtype);
+  if (id_bytes != 4 && id_bytes != 8)
+    return fail(MF_ERR_DTYPE, "teacher_ids must have 4 or 8 bytes (got %d)", id_bytes);
+  if (rows < 1 || vocabulary < 1 || top < 1)
+    return fail(MF_ERR_INVALID_ARGUMENT, "Sizes must be positive (rows=%d vocabulary=%d top=%d)",
+                rows, vocabulary, top);
+  if (!distill_sizes(rows, top) || vocabulary > mf::kDistillMostVocabulary ||
+      (long long)rows * vocabulary > mf::kDistillMostLogits)
+    return fail(MF_ERR_SHAPE,
+                "at most %d rows, %d logits a row, %lld in all and %d entries (got %d of %d, %d)",
+                mf::kDistillMostRows, mf::kDistillMostVocabulary, mf::kDistillMostLogits,
+                mf::kDistillMostTop, rows, vocabulary, top);
+  if (!(std::isfinite(temperature) && temperature > 0))
+    return fail(MF_ERR_INVALID_ARGUMENT, "temperature must be finite and positive (got %g)",
+                temperature);
+  return MF_OK;
+}
+
+int check_stats(const float* stats, size_t bytes, int rows, int top) {
+  const size_t need = mf::distill_stats_bytes(rows, top);
+  if (stats && bytes < need)
+    return fail(MF_ERR_WORKSPACE, "stats hold %zu bytes, %zu needed", bytes, need);
+  return MF_OK;
+}
+
+}  // namespace
+
+int mf_norm(const void* x, long long x_stride, const void* weight, const void* bias, int dtype,
+            int param_dtype, int rows, int dim, int center, float eps, void* y, float* stats,
+            void* stream) {
+  if (int rc = check_norm(dtype, param_dtype, rows, dim)) return rc;
+  if (!x || !weight || !y)
+    return fail(MF_ERR_INVALID_ARGUMENT, "x, weight and y must be non-null");
+  if (bias && !center) return fail(MF_ERR_INVALID_ARGUMENT, "the RMS norm has no bias");
+  if (!(std::isfinite(eps) && eps >= 0))
+    return fail(MF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative (got %g)", (double)eps);
+  if (int rc = check_rows("x", x_stride, dim)) return rc;
+  return check_hip(mf::launch_norm(x, x_stride, weight, bias, dtype == MF_DTYPE_F32,
+                                   param_dtype == MF_DTYPE_F32, rows, dim, center != 0, eps, y,
+                                   stats, static_cast<hipStream_t>(stream)),
+                   "mf_norm launch");
+}
+
+size_t mf_norm_bwd_workspace_bytes(int rows, int dim, int dtype) {
+  if (!norm_sizes(rows, dim) || !known_dtype(dtype)) return 0;
+  return mf::norm_bwd_workspace_bytes(rows, dim, dtype == MF_DTYPE_F32);
+}
+
+int mf_norm_bwd(const void* x, long long x_stride, const void* weight, const float* stats,
+                const void* dy, long long dy_stride, int dtype, int param_dtype, int rows, int dim,
+                int center, void* dx, void* dweight, void* dbias, void* workspace,
+                size_t workspace_bytes, void* stream) {
+  if (int rc = check_norm(dtype, param_dtype, rows, dim)) return rc;
+  if (!x || !weight || !stats || !dy)
+    return fail(MF_ERR_INVALID_ARGUMENT, "x, weight, stats and dy must be non-null");
+  if (!dx && !dweight && !dbias) return ok();
+  if (dbias && !center) return fail(MF_ERR_INVALID_ARGUMENT, "the RMS norm has no bias");
+  if (int rc = check_rows("x", x_stride, dim)) return rc;
+  if (int rc = check_rows("dy", dy_stride, dim)) return rc;
+  if (dweight || dbias) {
+    const size_t need = mf_norm_bwd_workspace_bytes(rows, dim, dtype);
+    if (!workspace || workspace_bytes < need)
+      return fail(MF_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed",
+                  workspace ? workspace_bytes : 0, need);
+  }
+  return check_hip(mf::launch_norm_bwd(x, x_stride, weight, stats, dy, dy_stride,
+                                       dtype == MF_DTYPE_F32, param_dtype == MF_DTYPE_F32, rows,
+                                       dim, center != 0, dx, dweight, dbias, workspace,
+                                       static_cast<hipStream_t>(stream)),
+                   "mf_norm_bwd launch");
+}
+
+int mf_embed(const void* ids, int id_bytes, const void* table, long long table_stride, int dtype,
+             int tokens, int vocabulary, int dim, long long padding_id, float scale, void* out,
+             void* stream) {
+  if (int rc = check_embed(dtype, id_bytes, tokens, vocabulary, dim, scale)) return rc;
+  if (!ids || !table || !out)
+    return fail(MF_ERR_INVALID_ARGUMENT, "ids, table and out must be non-null");
+  if (int rc = check_rows("table", table_stride, dim)) return rc;
+  return check_hip(mf::launch_embed(ids, id_bytes == 8, table, table_stride, dtype == MF_DTYPE_F32,
+                                    tokens, vocabulary, dim, padding_id, scale, out,
+                                    static_cast<hipStream_t>(stream)),
+                   "mf_embed launch");
+}
+
+size_t mf_embed_bwd_workspace_bytes(int tokens, int vocabulary, int dim) {
+  if (!embed_sizes(tokens, vocabulary, dim)) return 0;
+  return mf::embed_layout(tokens, vocabulary, dim).total;
+}
+
+int mf_embed_bwd(const void* ids, int id_bytes, const void* dout, long long dout_stride, int dtype,
+                 int tokens, int vocabulary, int dim, long long padding_id, float scale,
+                 void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_embed(dtype, id_bytes, tokens, vocabulary, dim, scale)) return rc;
+  if (!ids || !dout || !dtable)
+    return fail(MF_ERR_INVALID_ARGUMENT, "ids, dout and dtable must be non-null");
+  if (int rc = check_rows("dout", dout_stride, dim)) return rc;
+  if (reinterpret_cast<uintptr_t>(dtable) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(MF_ERR_INVALID_ARGUMENT, "dtable and workspace must be 16-byte aligned");
+  const size_t need = mf::embed_layout(tokens, vocabulary, dim).total;
+  if (!workspace || workspace_bytes < need)
+    return fail(MF_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed",
+                workspace ? workspace_bytes : 0, need);
+  return check_hip(mf::launch_embed_bwd(ids, id_bytes == 8, dout, dout_stride,
+                                        dtype == MF_DTYPE_F32, tokens, vocabulary, dim, padding_id,
+                                        scale, dtable, workspace, static_cast<hipStream_t>(stream)),
+                   "mf_embed_bwd launch");
+}
+
+size_t mf_distill_stats_bytes(int rows, int top) {
+  return distill_sizes(rows, top) ? mf::distill_stats_bytes(rows, top) : 0;
+}
+
+int mf_distill(const void* logits, long long stride, const void* teacher, int teacher_dtype,
+               const void* teacher_ids, int id_bytes, const float* total, const float* weights,
+               int dtype, int rows, int vocabulary, int top, double temperature, float* loss,
+               float* stats, size_t stats_bytes, void* dlogits, long long grad_stride,
+               void* stream) {
+  if (int rc = check_distill(dtype, id_bytes, rows, vocabulary, top, temperature)) return rc;
+  if (!known_dtype(teacher_dtype))
+    return fail(MF_ERR_DTYPE, "Unsupported teacher dtype code %d", teacher_dtype);
+  if (!logits || !teacher || !teacher_ids || !loss)
+    return fail(MF_ERR_INVALID_ARGUMENT, "logits, teacher, teacher_ids and loss must be non-null");
+  if (int rc = check_rows("logits", stride, vocabulary)) return rc;
+  if (dlogits)
+    if (int rc = check_rows("dlogits", grad_stride, vocabulary)) return rc;
+  if (dlogits == logits && dlogits && stride != grad_stride)
+    return fail(MF_ERR_SHAPE, "a gradient in the logits' place must have their stride");
+  if (int rc = check_stats(stats, stats_bytes, rows, top)) return rc;
+  return check_hip(mf::launch_distill(logits, stride, teacher, teacher_dtype == MF_DTYPE_F32,
+                                      teacher_ids, id_bytes == 8, total, weights,
+                                      dtype == MF_DTYPE_F32, rows, vocabulary, top, temperature,
+                                      loss, stats, dlogits, grad_stride,
+                                      static_cast<hipStream_t>(stream)),
+                   "mf_distill launch");
+}
+
+int mf_distill_bwd(const void* logits, long long stride, const void* teacher_ids, int id_bytes,
+                   const float* weights, const float* stats, size_t stats_bytes,
+                   const float* dloss, int dtype, int rows, int vocabulary, int top,
+                   double temperature, void* dlogits, long long grad_stride, void* stream) {
+  if (int rc = check_distill(dtype, id_bytes, rows, vocabulary, top, temperature)) return rc;
+  if (!logits || !teacher_ids || !stats || !dloss || !dlogits)
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "logits, teacher_ids, stats, dloss and dlogits must be non-null");
+  if (int rc = check_rows("logits", stride, vocabulary)) return rc;
+  if (int rc = check_rows("dlogits", grad_stride, vocabulary)) return rc;
+  if (logits == dlogits)
+    return fail(MF_ERR_INVALID_ARGUMENT, "dlogits must not be the logits");
+  if (int rc = check_stats(stats, stats_bytes, rows, top)) return rc;
+  return check_hip(mf::launch_distill_bwd(logits, stride, teacher_ids, id_bytes == 8, weights,
+                                          stats, dloss, dtype == MF_DTYPE_F32, rows, vocabulary,
+                                          top, temperature, dlogits, grad_stride,
+                                          static_cast<hipStream_t>(stream)),
+                   "mf_distill_bwd launch");
+}

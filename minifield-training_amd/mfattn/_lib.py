@@ -74,6 +74,15 @@ EXPORTS = (
     "mf_segmented_conv",
     "mf_segmented_conv_bwd_workspace_bytes",
     "mf_segmented_conv_bwd",
+    "mf_norm",
+    "mf_norm_bwd_workspace_bytes",
+    "mf_norm_bwd",
+    "mf_embed",
+    "mf_embed_bwd_workspace_bytes",
+    "mf_embed_bwd",
+    "mf_distill_stats_bytes",
+    "mf_distill",
+    "mf_distill_bwd",
     "mf_static_scratch_bytes",
     "mf_decode_static",
     "mf_last_error",
@@ -177,6 +186,28 @@ def _load() -> ctypes.CDLL:
     lib.mf_block_map_placements.restype = i32
     lib.mf_segmented_conv.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]
     lib.mf_segmented_conv.restype = i32
+    lib.mf_norm.argtypes = [vp, i64, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp, vp]
+    lib.mf_norm.restype = i32
+    lib.mf_norm_bwd_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.mf_norm_bwd_workspace_bytes.restype = sz
+    lib.mf_norm_bwd.argtypes = [vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp,
+                                sz, vp]
+    lib.mf_norm_bwd.restype = i32
+    lib.mf_embed.argtypes = [vp, i32, vp, i64, i32, i32, i32, i32, i64, f32, vp, vp]
+    lib.mf_embed.restype = i32
+    lib.mf_embed_bwd_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.mf_embed_bwd_workspace_bytes.restype = sz
+    lib.mf_embed_bwd.argtypes = [vp, i32, vp, i64, i32, i32, i32, i32, i64, f32, vp, vp, sz, vp]
+    lib.mf_embed_bwd.restype = i32
+    lib.mf_distill_stats_bytes.argtypes = [i32, i32]
+    lib.mf_distill_stats_bytes.restype = sz
+    f64 = ctypes.c_double
+    lib.mf_distill.argtypes = [vp, i64, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, f64, vp, vp,
+                               sz, vp, i64, vp]
+    lib.mf_distill.restype = i32
+    lib.mf_distill_bwd.argtypes = [vp, i64, vp, i32, vp, vp, sz, vp, i32, i32, i32, i32, f64, vp,
+                                   i64, vp]
+    lib.mf_distill_bwd.restype = i32
     lib.mf_static_scratch_bytes.argtypes = []
     lib.mf_static_scratch_bytes.restype = sz
     lib.mf_decode_static.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp]

@@ -141,6 +141,34 @@ def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x.contiguous(), h * d
 
 
+def even_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``x [..., D]`` and the elements between its rows, copied only where its last
+    dimension is not dense or its rows are not evenly spaced or overlap."""
+    d = x.shape[-1]
+    if x.is_contiguous():
+        return x, d
+    try:
+        rows = x.view(-1, d)
+    except RuntimeError:
+        return x.contiguous(), d
+    step, dense = rows.stride()
+    if rows.shape[0] <= 1:
+        step = d
+    return (x, step) if step >= d and (dense == 1 or d == 1) else (x.contiguous(), d)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    if carries_tangent(*tensors):
+        raise ValueError(f"{what} has no forward-mode derivative; an operand carries a tangent")
+
+
+def refuse_second_order(what: str) -> None:
+    """A backward pass that runs to be differentiated itself (create_graph=True)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once: its backward pass records no graph "
+                           "(create_graph=True)")
+
+
 def _require_lse(lse: torch.Tensor, b: int, hq: int, t: int) -> None:
     if lse.dtype != torch.float32:
         raise ValueError("lse must be float32")
