@@ -46,7 +46,7 @@ struct DistillArgs {
   bool teacher_f32, ids64;
 };
 
-constexpr int kDistillThreads = 1024;
+constexpr int kDistillThreads = 512;
 
 __device__ __forceinline__ int teacher_id(const DistillArgs& a, size_t at) {
   const long long id = a.ids64 ? reinterpret_cast<const long long*>(a.ids)[at]
@@ -59,6 +59,11 @@ __device__ __forceinline__ double sum64d(double x) {
   for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
   return x;
 }
+__device__ __forceinline__ double max64d(double x) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) x = fmax(x, __shfl_xor(x, m));
+  return x;
+}
 
 // exp((z - top) / T).  The difference first: a product of the type's lowest value
 // with `scale` would be infinite, and a row of nothing else not uniform.
@@ -66,226 +71,326 @@ __device__ __forceinline__ float weight_of(float z, float top, float scale) {
   return fast_exp2((z - top) * scale);
 }
 
-// The named elements of a row's gradient: one thread each, after the dense ones.
+// A named element of a row's gradient: after the dense ones.
 template <typename T>
 __device__ __forceinline__ void store_named(T* grad, int id, float z, float mass, float top,
                                             float scale, float factor, float w) {
   grad[id] = (T)fmaf(weight_of(z, top, scale), factor, -w * mass);
 }
 
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  return (Vec<T>)__builtin_nontemporal_load(reinterpret_cast<const typename RowVec<T>::U*>(p));
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[kVec<T>]) {
+  typename RowVec<T>::U u;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) u[i] = (T)x[i];
+  __builtin_nontemporal_store(u, reinterpret_cast<typename RowVec<T>::U*>(p));
+}
+
+// A row's entries in LDS, and what wave 0 makes of them in 64 bits.
+struct Teacher {
+  int id[kDistillMostTop];  // -1: not there
+  float z[kDistillMostTop], mass[kDistillMostTop];
+  float whole, rest;        // P + r and r
+  int none, bad;            // no entry at all; one that is NaN or +infinity
+};
+
+// Wave 0, before the row's own loads are waited for: masses, P, and the loss but for
+// the logarithm of the student's sum, sum p_k (log p_k - (z_k - z_ref) / T).
+__device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, int lane,
+                                              Teacher& t, double& P, double& kl, float& z_ref) {
+  const int K = a.top;
+  const double per = 1.0 / a.temperature, inf = __builtin_huge_val();
+  const bool tail = a.total != nullptr;
+  bool there = false, bad = false;
+  auto entry = [&](int k) {
+    if (t.id[k] < 0) return -inf;
+    const float u = element(a.teacher, a.teacher_f32, row * K + k);
+    bad |= !(u < kPosInf);
+    there |= u != kNegInf;
+    return (double)u * per;
+  };
+  double most = -inf;
+  float ref = kNegInf;
+  for (int k = lane; k < K; k += 64) {
+    most = fmax(most, entry(k));
+    if (t.id[k] >= 0) ref = fmaxf(ref, t.z[k]);
+  }
+  ref = max64(ref);
+  z_ref = ref > kNegInf && ref < kPosInf ? ref : 0.f;
+  double total;
+  if (tail) {
+    total = a.total[row];
+    bad |= !(total < inf);
+  } else {
+    most = max64d(most);
+    double s = 0;
+    for (int k = lane; k < K; k += 64) s += exp(entry(k) - most);
+    // (entries that are all -infinity have no mass, like none at all)
+    total = most == -inf ? 0.0 : most + log(sum64d(s));
+  }
+  P = kl = 0;
+  for (int k = lane; k < K; k += 64) {
+    double mass = 0;
+    if (t.id[k] >= 0) {
+      const double logp = entry(k) - total;
+      mass = exp(logp);
+      if (mass > 0) kl += mass * (logp - ((double)t.z[k] - z_ref) * per);
+    }
+    t.mass[k] = (float)mass;
+    P += mass;
+  }
+  P = sum64d(P);
+  kl = sum64d(kl);
+  // without an entry there is no loss and no gradient, whatever the row holds; otherwise
+  // an entry or a total that is NaN or +infinity makes the row NaN
+  const bool none = !tail && !__any(there);
+  bad = !none && __any(bad);
+  if (lane == 0) {
+    const double r = tail ? fmax(0.0, 1.0 - P) : 0.0;
+    t.whole = (float)(P + r);
+    t.rest = (float)r;
+    t.none = none;
+    t.bad = bad;
+  }
+}
+
 // LOSS: the loss (and with `stats` what the backward needs); GRAD: the gradient of
 // the weighted loss.  U: vectors a thread has in flight; RESIDENT: they are the row.
-template <typename T, bool GRAD, int U, bool RESIDENT, bool TAIL>
-__global__ __launch_bounds__(kDistillThreads) void distill_kernel(DistillArgs a) {
+template <typename T, bool GRAD, int U, bool RESIDENT>
+__global__ __launch_bounds__(kDistillThreads) __attribute__((amdgpu_waves_per_eu(U > 16 ? 2 : 4)))
+void distill_kernel(DistillArgs a) {
   constexpr int N = kVec<T>, W = kDistillThreads / 64;
   extern __shared__ uint32_t named[];  // a bit per logit, where the total is known
-  __shared__ int id_of[kDistillMostTop];
-  __shared__ float z_of[kDistillMostTop], mass_of[kDistillMostTop];
+  __shared__ Teacher t;
   __shared__ float part[3][W];
-  __shared__ float row_factors[3];  // w T (P + r) / S, the dense factor, w T
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const size_t row = blockIdx.x;
   const int V = a.vocabulary, K = a.top;
-  const float w = a.weights ? a.weights[row] : 1.f;
+  // (by a scalar load: the row's own wait for nothing else)
+  typedef const __attribute__((address_space(4))) float* Scalars;
+  const float w = a.weights ? ((Scalars)a.weights)[row] : 1.f;
   const T* z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   T* grad = GRAD ? reinterpret_cast<T*>(a.grad) + row * a.grad_stride : nullptr;
-  const int vectors = (V + N - 1) / N;
+  // whole vectors; what is left of the row is one more value of each of the first threads
+  const int vectors = V / N, odd = vectors * N + tid;
+  auto no_gradient = [&] {
+    const float zero[N] = {};
+    for (int v = tid; v < vectors; v += kDistillThreads) store_vec<T>(grad + (size_t)v * N, zero);
+    if (odd < V) grad[odd] = (T)0.f;
+  };
   if (w == 0.f) {  // whatever the row holds
     if (tid == 0) a.loss[row] = 0.f;
-    if constexpr (GRAD) {
-      const float zero[N] = {};
-      for (int v = tid; v < vectors; v += kDistillThreads)
-        store_row<T, TAIL, true>(grad, v * N, V, zero);
-    }
+    if constexpr (GRAD) no_gradient();
     return;
   }
   const bool tail = a.total != nullptr;
-  // the first vectors are on their way while the teacher's entries are looked at
+  // wave 0 asks for the entries and their logits in front of the row: loads return in order
+  if (wave == 0)
+    for (int k = lane; k < K; k += 64) {
+      const int id = teacher_id(a, row * K + k);
+      t.id[k] = id;
+      t.z[k] = id >= 0 ? (float)z[id] : 0.f;
+    }
+  constexpr int STEP = U * kDistillThreads;
   Vec<T> raw[U];
-  auto fetch = [&](int first) {
+  // (loads have no condition: vectors beyond the row are its last)
+  auto fetch = [&](Vec<T> (&to)[U], int first) {
+    if (vectors == 0) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      to[u] = load_vec<T>(z + (size_t)min(first + u * kDistillThreads + tid, vectors - 1) * N);
+  };
+  auto blank = [&](int first) {
+    if (first + STEP <= vectors) return;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int v = first + u * kDistillThreads + tid;
-      raw[u] = load_row<T, TAIL, true>(z, v * N, V, kNegInf);
+      const u32x4 x = __builtin_bit_cast(u32x4, raw[u]);
+      constexpr uint32_t low = N == 8 ? 0xff80ff80u : 0xff800000u;  // -infinity
+      const bool in = first + u * kDistillThreads + tid < vectors;
+      raw[u] = __builtin_bit_cast(Vec<T>, u32x4{in ? x[0] : low, in ? x[1] : low, in ? x[2] : low,
+                                                in ? x[3] : low});
     }
   };
-  fetch(0);
+  const float extra = odd < V ? (float)z[odd] : kNegInf;
+  fetch(raw, 0);
   if (tail)
     for (int i = tid; i < (V + 31) / 32; i += kDistillThreads) named[i] = 0;
-  if (tid < K) {
-    const int id = teacher_id(a, row * K + tid);
-    id_of[tid] = id;
-    z_of[tid] = id >= 0 ? (float)z[id] : 0.f;
-  }
-  __syncthreads();
+  // A vector of the row as it was loaded.  Each pass widens its values anew, one vector at
+  // a time (left to itself the compiler keeps the first pass's, twice the registers in
+  // bf16, and all exponentials of a pass: scratch).
+  auto as_loaded = [&](int u) {
+    u32x4 x = __builtin_bit_cast(u32x4, raw[u]);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(x));
+    return __builtin_bit_cast(Vec<T>, x);
+  };
+  double P = 0, kl = 0;
+  float z_ref = 0.f;
   if (tail) {
-    if (tid < K && id_of[tid] >= 0) atomicOr(&named[id_of[tid] >> 5], 1u << (id_of[tid] & 31));
+    __syncthreads();
+    for (int k = tid; k < K; k += kDistillThreads)
+      if (t.id[k] >= 0) atomicOr(&named[t.id[k] >> 5], 1u << (t.id[k] & 31));
     __syncthreads();
   }
-  // maximum and sums
-  float top = kNegInf, rest = 0.f, held = 0.f;  // sums beside `top`, not named and named
-  for (int first = 0; first < vectors; first += U * kDistillThreads) {
-    if (!RESIDENT && first) fetch(first);
+  // (the other waves go on with the row; they meet wave 0 at its largest logit)
+  if (wave == 0) weigh_teacher(a, row, lane, t, P, kl, z_ref);
+  // sums beside `top`, of what is not named and what is
+  float top = kNegInf, rest = 0.f, held = 0.f;
+  auto largest = [&] {
     float m = top;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < N; ++i) m = fmaxf(m, (float)raw[u][i]);
-    // (a thread whose logits are all -infinity has a sum of zero, not NaN)
-    const float base = m == kNegInf ? 0.f : m;
-    const float old = weight_of(top, base, a.scale);
-    rest *= old;
-    held *= old;
-    top = m;
+    return m;
+  };
+  auto add = [&](int first, float base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = first + u * kDistillThreads + tid;
-      uint32_t bits = 0;
-      if (tail && v < vectors)
-        bits = (named[v * N >> 5] >> (v * N & 31)) & ((1u << N) - 1);
+      const Vec<T> x = as_loaded(u);
       float e[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = weight_of((float)raw[u][i], base, a.scale);
+      for (int i = 0; i < N; ++i) e[i] = weight_of((float)x[i], base, a.scale);
+      uint32_t bits = 0;
+      if (tail && v < vectors) bits = (named[v * N >> 5] >> (v * N & 31)) & ((1u << N) - 1);
       if (bits) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           held += bits >> i & 1 ? e[i] : 0.f;
-          rest += bits >> i & 1 ? 0.f : e[i];
+          e[i] = bits >> i & 1 ? 0.f : e[i];
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) rest += e[i];
       }
+#pragma unroll
+      for (int i = 0; i < N; ++i) rest += e[i];
+      asm volatile("" : "+v"(rest));  // (added here, not all behind the last vector)
+    }
+  };
+  auto add_extra = [&](float base) {
+    const float e = weight_of(extra, base, a.scale);
+    const bool is_named = tail && odd < V && named[odd >> 5] >> (odd & 31) & 1;
+    held += is_named ? e : 0.f;
+    rest += is_named ? 0.f : e;
+  };
+  if constexpr (RESIDENT) {
+    blank(0);
+    top = fmaxf(largest(), extra);
+  } else {
+    top = extra;
+    add_extra(extra == kNegInf ? 0.f : extra);
+    for (int first = 0; first < vectors; first += STEP) {
+      Vec<T> next[U];
+      fetch(next, first + STEP);
+      blank(first);
+      const float m = largest();
+      // (a thread whose logits are all -infinity has a sum of zero, not NaN)
+      const float base = m == kNegInf ? 0.f : m, old = weight_of(top, base, a.scale);
+      rest *= old;
+      held *= old;
+      top = m;
+      add(first, base);
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
     }
   }
   const float wave_top = max64(top);
   if (lane == 0) part[0][wave] = wave_top;
   __syncthreads();
-  float all = part[0][0];
+  float base = part[0][0];
 #pragma unroll
-  for (int i = 1; i < W; ++i) all = fmaxf(all, part[0][i]);
-  const float base = all == kNegInf ? 0.f : all;
-  const float mine = weight_of(top, base, a.scale);
-  rest = sum64(rest * mine);
-  held = sum64(held * mine);
+  for (int i = 1; i < W; ++i) base = fmaxf(base, part[0][i]);
+  base = base == kNegInf ? 0.f : base;
+  if constexpr (RESIDENT) {
+    add(0, base);
+    add_extra(base);
+  } else {
+    const float mine = weight_of(top, base, a.scale);
+    rest *= mine;
+    held *= mine;
+  }
+  rest = sum64(rest);
+  if (tail) held = sum64(held);
   if (lane == 0) {
     part[1][wave] = rest;
     part[2][wave] = held;
   }
   __syncthreads();
-  // the row's few numbers in 64 bits, by one wave
-  if (wave == 0) {
-    float srest = 0.f, sheld = 0.f;
+  rest = held = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      srest += part[1][i];
-      sheld += part[2][i];
-    }
-    const double sum = (double)srest + (double)sheld;
-    const double per = 1.0 / a.temperature;
-    const double log_sum = log(sum);  // beside the largest logit
-    double whole, P = 0, kl = 0;
-    bool there = false, bad = !(sum > 0 && sum < __builtin_huge_val());
-    auto entry = [&](int k) {
-      if (id_of[k] < 0) return -__builtin_huge_val();
-      const float t = element(a.teacher, a.teacher_f32, row * K + k);
-      bad |= !(t < kPosInf);
-      there |= t != kNegInf;
-      return (double)t * per;
-    };
-    if (tail) {
-      bad |= !(a.total[row] < kPosInf);
-      whole = a.total[row];
+  for (int i = 0; i < W; ++i) {
+    rest += part[1][i];
+    held += part[2][i];
+  }
+  const float sum = rest + held;
+  // so does a logit that is NaN or +infinity, and a row of -infinity alone
+  const bool none = t.none, bad = !none && (t.bad || !(sum > 0.f && sum < kPosInf));
+  const float wt = (float)(w * a.temperature);
+  const float one = none ? 0.f : bad ? __builtin_nanf("") : wt * (t.whole / sum);
+  const float dense = one - (rest > 0.f ? wt * (t.rest / rest) : 0.f);
+  if constexpr (GRAD) {
+    if (none) {
+      no_gradient();
     } else {
-      double most = -__builtin_huge_val(), s = 0;
-      for (int k = lane; k < K; k += 64) most = fmax(most, entry(k));
+      for (int first = 0; first < vectors; first += STEP) {
+        if (!RESIDENT) fetch(raw, first);
 #pragma unroll
-      for (int m = 1; m < 64; m <<= 1) most = fmax(most, __shfl_xor(most, m));
-      for (int k = lane; k < K; k += 64)
-        s += exp(entry(k) - most);
-      // (entries that are all -infinity have no mass, like none at all)
-      whole = most == -__builtin_huge_val() ? 0.0 : most + log(sum64d(s));
-    }
-    for (int k = lane; k < K; k += 64) {
-      double mass = 0;
-      if (id_of[k] >= 0) {
-        const double logp = entry(k) - whole;
-        mass = exp(logp);
-        if (mass > 0) kl += mass * (logp + log_sum - ((double)z_of[k] - base) * per);
-      }
-      mass_of[k] = (float)mass;
-      P += mass;
-    }
-    P = sum64d(P);
-    kl = sum64d(kl);
-    const double r = tail ? fmax(0.0, 1.0 - P) : 0.0;
-    if (r > 0) kl += r * (log(r) - log((double)srest / sum));
-    // without a teacher's entry no loss and no gradient, whatever the row holds; otherwise a
-    // logit, an entry or a total that is NaN or +infinity makes the row NaN, and so does a
-    // row of -infinity alone
-    const bool none = !tail && !__any(there);
-    bad = !none && __any(bad);
-    if (lane == 0) {
-      const double keep = bad ? __builtin_nan("") : 1.0;
-      a.loss[row] = none ? 0.f : (float)(w * a.temperature * a.temperature * kl * keep);
-      const double one = none ? 0.0 : (P + r) / sum;
-      const double dense = one - (srest > 0.f ? r / srest : 0.0);
-      const double wt = w * a.temperature;
-      row_factors[0] = (float)(wt * one * keep);
-      row_factors[1] = (float)(wt * dense * keep);
-      row_factors[2] = (float)wt;
-      if (a.stats) {
-        float* st = a.stats + row * (kDistillStats + K);
-        st[0] = base;
+        for (int u = 0; u < U; ++u) {
+          const int v = first + u * kDistillThreads + tid;
+          const Vec<T> x = as_loaded(u);
+          float g[N];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) st[1 + i] = row_factors[i];
+          for (int i = 0; i < N; ++i) g[i] = weight_of((float)x[i], base, a.scale) * dense;
+          if (v < vectors) store_vec<T>(grad + (size_t)v * N, g);
+        }
       }
+      if (odd < V) grad[odd] = (T)(weight_of(extra, base, a.scale) * dense);
     }
   }
-  if (!GRAD && !a.stats) return;
-  __syncthreads();
   // an element that several entries name has the mass of all of them
-  float mass = 0.f;
-  const int id = tid < K ? id_of[tid] : -1;
-  if (id >= 0)
-    for (int k = 0; k < K; ++k) mass += id_of[k] == id ? mass_of[k] : 0.f;
-  if constexpr (!GRAD) {
-    if (tid < K) a.stats[row * (kDistillStats + K) + kDistillStats + tid] = mass;
-    return;
+  auto mass_of = [&](int k) {
+    float m = 0.f;
+    for (int j = 0; j < K; ++j) m += t.id[j] == t.id[k] ? t.mass[j] : 0.f;
+    return m;
+  };
+  if (GRAD && !none) {
+    // the dense stores have arrived before a named element is written anew
+    drain_memory();
+    __syncthreads();
+    for (int k = tid; k < K; k += kDistillThreads)
+      if (t.id[k] >= 0) store_named(grad, t.id[k], t.z[k], mass_of(k), base, a.scale, one, wt);
   }
-  const float dense = row_factors[1];
-  if (row_factors[0] == 0.f) {  // no teacher: no gradient, whatever the row holds
-    const float zero[N] = {};
-    for (int v = tid; v < vectors; v += kDistillThreads)
-      store_row<T, TAIL, true>(grad, v * N, V, zero);
-    return;
-  }
-  for (int first = 0; first < vectors; first += U * kDistillThreads) {
-    if (!RESIDENT) fetch(first);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = first + u * kDistillThreads + tid;
-      float g[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) g[i] = weight_of((float)raw[u][i], base, a.scale) * dense;
-      store_row<T, TAIL, true>(grad, v * N, V, g);
+  if (!GRAD && a.stats) {
+    float* st = a.stats + row * (kDistillStats + K);
+    for (int k = tid; k < K; k += kDistillThreads) st[kDistillStats + k] = mass_of(k);
+    if (tid == 0) {
+      st[0] = base;
+      st[1] = one;
+      st[2] = dense;
+      st[3] = wt;
     }
   }
-  // the dense stores have arrived before a named element is written anew
-  drain_memory();
-  __syncthreads();
-  if (id >= 0)
-    store_named(grad, id, z_of[tid], mass, base, a.scale, row_factors[0], row_factors[2]);
+  if (tid == 0) {
+    const double T_ = a.temperature, r = tail ? fmax(0.0, 1.0 - P) : 0.0, all = (double)rest + held;
+    kl += P * (log(all) + ((double)base - z_ref) / T_);
+    if (r > 0) kl += r * (log(r) - log((double)rest / all));
+    a.loss[row] = none ? 0.f : bad ? __builtin_nanf("") : (float)(w * T_ * T_ * kl);
+  }
 }
 
 // The gradient from what the forward pass saved: a workgroup takes a part of a row.
-template <typename T, int U, bool TAIL>
+template <typename T, int U>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int parts) {
-  constexpr int N = kVec<T>, span = U * 256 * N;
+  constexpr int N = kVec<T>, SPAN = U * 256;
   const int tid = threadIdx.x;
   const size_t row = blockIdx.x / parts;
-  const int first = (int)(blockIdx.x % parts) * span;
+  const int part = (int)(blockIdx.x % parts), first = part * SPAN;
   const int V = a.vocabulary, K = a.top;
+  // the last part has the odd values behind the row's whole vectors
+  const int vectors = V / N, odd = part == parts - 1 ? vectors * N + tid : V;
   const float up = a.upstream[row];
   const float* st = a.stats + row * (kDistillStats + K);
   // (the stats of a row without weight are not there; one without a teacher has no factors)
@@ -293,30 +398,38 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int par
   if (live) live = st[1] != 0.f;
   const T* z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   T* grad = reinterpret_cast<T*>(a.grad) + row * a.grad_stride;
+  auto store = [&](int u, const float (&g)[N]) {
+    const int v = first + u * 256 + tid;
+    if (v < vectors) store_vec<T>(grad + (size_t)v * N, g);
+  };
   if (!live) {
     const float zero[N] = {};
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      store_row<T, TAIL, true>(grad, first + (u * 256 + tid) * N, V, zero);
+    for (int u = 0; u < U; ++u) store(u, zero);
+    if (odd < V) grad[odd] = (T)0.f;
     return;
   }
   Vec<T> raw[U];
+  if (vectors > 0) {
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    raw[u] = load_row<T, TAIL, true>(z, first + (u * 256 + tid) * N, V, kNegInf);
+    for (int u = 0; u < U; ++u)
+      raw[u] = load_vec<T>(z + (size_t)min(first + u * 256 + tid, vectors - 1) * N);
+  }
   const float base = st[0], one = st[1] * up, dense = st[2] * up, wt = st[3] * up;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float g[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = weight_of((float)raw[u][i], base, a.scale) * dense;
-    store_row<T, TAIL, true>(grad, first + (u * 256 + tid) * N, V, g);
+    store(u, g);
   }
+  if (odd < V) grad[odd] = (T)(weight_of((float)z[odd], base, a.scale) * dense);
   drain_memory();
   __syncthreads();
+  const int last = part == parts - 1 ? V : (first + SPAN) * N;
   for (int k = tid; k < K; k += 256) {
     const int id = teacher_id(a, row * K + k);
-    if (id >= first && id < first + span)
+    if (id >= first * N && id < last)
       store_named(grad, id, (float)z[id], st[kDistillStats + k], base, a.scale, one, wt);
   }
 }
@@ -324,43 +437,34 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int par
 template <typename T, bool GRAD, int U, bool RESIDENT>
 static void launch_row(const DistillArgs& a, int rows, hipStream_t stream) {
   const size_t lds = a.total ? ((size_t)a.vocabulary + 31) / 32 * 4 : 0;
-  if (a.vocabulary % kVec<T>)
-    hipLaunchKernelGGL((distill_kernel<T, GRAD, U, RESIDENT, true>), dim3(rows),
-                       dim3(kDistillThreads), lds, stream, a);
-  else
-    hipLaunchKernelGGL((distill_kernel<T, GRAD, U, RESIDENT, false>), dim3(rows),
-                       dim3(kDistillThreads), lds, stream, a);
+  hipLaunchKernelGGL((distill_kernel<T, GRAD, U, RESIDENT>), dim3(rows), dim3(kDistillThreads), lds,
+                     stream, a);
 }
 
 template <typename T>
 static hipError_t launch_distill_t(const DistillArgs& a, int rows, hipStream_t stream) {
-  const int per = (a.vocabulary + kVec<T> * kDistillThreads - 1) / (kVec<T> * kDistillThreads);
-  if (!a.grad) {
+  const int vectors = a.vocabulary / kVec<T>;
+  if (!a.grad)
     launch_row<T, false, 4, false>(a, rows, stream);
-  } else if (per <= 2) {
-    launch_row<T, true, 2, true>(a, rows, stream);
-  } else if (per <= 4) {
+  else if (vectors <= 4 * kDistillThreads)
     launch_row<T, true, 4, true>(a, rows, stream);
-  } else if (per <= 8) {
+  else if (vectors <= 8 * kDistillThreads)
     launch_row<T, true, 8, true>(a, rows, stream);
-  } else if (per <= 16) {
+  else if (vectors <= 16 * kDistillThreads)
     launch_row<T, true, 16, true>(a, rows, stream);
-  } else {
+  else if (vectors <= 32 * kDistillThreads)
+    launch_row<T, true, 32, true>(a, rows, stream);
+  else
     launch_row<T, true, 4, false>(a, rows, stream);
-  }
   return hipGetLastError();
 }
 
 template <typename T>
 static hipError_t launch_distill_bwd_t(const DistillArgs& a, int rows, hipStream_t stream) {
-  constexpr int U = 4, span = U * 256 * kVec<T>;
-  const int parts = (a.vocabulary + span - 1) / span;
-  if (a.vocabulary % kVec<T>)
-    hipLaunchKernelGGL((distill_bwd_kernel<T, U, true>), dim3((unsigned)rows * parts), dim3(256), 0,
-                       stream, a, parts);
-  else
-    hipLaunchKernelGGL((distill_bwd_kernel<T, U, false>), dim3((unsigned)rows * parts), dim3(256),
-                       0, stream, a, parts);
+  constexpr int U = 4, SPAN = U * 256;
+  const int parts = std::max(1, (a.vocabulary / kVec<T> + SPAN - 1) / SPAN);
+  hipLaunchKernelGGL((distill_bwd_kernel<T, U>), dim3((unsigned)rows * parts), dim3(256), 0, stream,
+                     a, parts);
   return hipGetLastError();
 }
 

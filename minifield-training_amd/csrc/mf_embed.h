@@ -13,9 +13,13 @@ constexpr int kEmbedMostDim = 1 << 16;
 constexpr long long kEmbedMostValues = 1ll << 34;  // of the output: launches stay below 2^32 threads
 
 constexpr int kSortDigit = 9;               // bits of a key in one pass
+constexpr int kSortFewest = 5;              // (kernels are made for 5 to 9)
 constexpr int kSortBins = 1 << kSortDigit;
-constexpr int kSortTiles = 128;             // waves that share the tokens, at most
-constexpr int kEmbedChunk = 32;             // sorted tokens that a wave adds
+constexpr int kSortTiles = 64;              // waves that share the tokens, at most
+constexpr int kSortOne = 8192;              // tokens that one workgroup sorts
+constexpr int kEmbedMinChunk = 8;           // sorted tokens that a wave adds, at least
+constexpr int kEmbedMaxChunk = 64;          // (one for each lane)
+constexpr int kEmbedWaves = 2048;           // waves that the chunks are made for
 
 // A token and the row of the table that it adds to (the vocabulary: none).
 struct SortedToken {
@@ -24,8 +28,9 @@ struct SortedToken {
 
 struct EmbedLayout {
   int passes, bits;    // of the sort: digits and their bits
-  int tiles, rounds;   // waves, and the 64 tokens each that they take in turn
-  int chunks;
+  int tiles, rounds;   // waves, and the 64 tokens each that they take in turn; 0: one workgroup
+  int chunk, chunks;   // sorted tokens that a wave adds, and how many such
+  int width;           // of a piece of a row: a multiple of 4
   size_t histogram, tokens[2], partials, total;  // offsets in bytes
 };
 
@@ -35,11 +40,17 @@ inline EmbedLayout embed_layout(int tokens, int vocabulary, int dim) {
   while (bits < 31 && vocabulary >> bits) ++bits;  // of the key `vocabulary`
   l.passes = (bits + kSortDigit - 1) / kSortDigit;
   l.bits = (bits + l.passes - 1) / l.passes;
+  if (l.bits < kSortFewest) l.bits = kSortFewest;
   const int waves = (tokens + 63) / 64;
   l.rounds = (waves + kSortTiles - 1) / kSortTiles;
   if (l.rounds < 4) l.rounds = 4;
   l.tiles = (waves + l.rounds - 1) / l.rounds;
-  l.chunks = (tokens + kEmbedChunk - 1) / kEmbedChunk;
+  if (tokens <= kSortOne) l.tiles = l.rounds = 0;
+  // (512 columns a wave: chunks that leave the card idle are not worth their fewer pieces)
+  l.chunk = kEmbedMinChunk;
+  const long long slabs = (dim + 511) / 512;
+  while (l.chunk < kEmbedMaxChunk && tokens * slabs > (long long)l.chunk * kEmbedWaves) l.chunk *= 2;
+  l.chunks = (tokens + l.chunk - 1) / l.chunk;
   auto align = [](size_t x) { return (x + 255) & ~(size_t)255; };
   size_t at = 0;
   l.histogram = at;
@@ -49,7 +60,8 @@ inline EmbedLayout embed_layout(int tokens, int vocabulary, int dim) {
     at += align(sizeof(SortedToken) * (size_t)tokens);
   }
   l.partials = at;
-  at += align(sizeof(float) * 2 * (size_t)l.chunks * dim);
+  l.width = (dim + 3) / 4 * 4;
+  at += align(sizeof(float) * 2 * (size_t)l.chunks * l.width);
   l.total = at;
   return l;
 }

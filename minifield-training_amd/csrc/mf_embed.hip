@@ -37,33 +37,39 @@ struct EmbedArgs {
   bool ids64;
 };
 
-// The table's row of token n, `vocabulary` for none.
-__device__ __forceinline__ uint32_t row_of(const EmbedArgs& a, int n) {
-  const long long id = a.ids64 ? reinterpret_cast<const long long*>(a.ids)[n]
-                               : (long long)reinterpret_cast<const int32_t*>(a.ids)[n];
+// Token n's id, and the table's row of an id: `vocabulary` for none.
+__device__ __forceinline__ long long id_of(const EmbedArgs& a, int n) {
+  return a.ids64 ? reinterpret_cast<const long long*>(a.ids)[n]
+                 : (long long)reinterpret_cast<const int32_t*>(a.ids)[n];
+}
+__device__ __forceinline__ uint32_t row_of(const EmbedArgs& a, long long id) {
   return id >= 0 && id < a.vocabulary && id != a.padding ? (uint32_t)id : (uint32_t)a.vocabulary;
 }
 
 // L lanes a token.
-template <typename T, int L, bool TAIL>
+template <typename T, int L, Edge E>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs a) {
-  constexpr int N = kVec<T>, C = 4;
+  constexpr int N = kVec<T>, C = 2;
   const int n = blockIdx.x * (256 / L) + threadIdx.x / L, lane = threadIdx.x % L;
   if (n >= a.tokens) return;
-  const uint32_t id = row_of(a, n);
+  const uint32_t id = row_of(a, id_of(a, n));
   const bool met = id < (uint32_t)a.vocabulary;
   const T* from = reinterpret_cast<const T*>(a.rows) + (size_t)(met ? id : 0) * a.stride;
   T* to = reinterpret_cast<T*>(a.out) + (size_t)n * a.dim;
-  for (int first = 0; first < a.dim; first += L * N * C) {
+  for (int first = 0; first * N < a.dim; first += L * C) {
+    RowPlace<T, E> at[C];
     Vec<T> v[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = load_row<T, TAIL>(from, first + (c * L + lane) * N, a.dim);
+    for (int c = 0; c < C; ++c) {
+      at[c] = RowPlace<T, E>(first + c * L + lane, a.dim);
+      v[c] = at[c].load(from);
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float x[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = met ? (float)v[c][i] * a.scale : 0.f;
-      store_row<T, TAIL>(to, first + (c * L + lane) * N, a.dim, x);
+      at[c].store(to, x);
     }
   }
 }
@@ -75,22 +81,34 @@ struct SortArgs {
   const SortedToken* from;  // null: the ids as they come
   SortedToken* to;
   int* histogram;           // [tiles][kSortBins]
-  int tiles, rounds, shift, bits, blocks;
-  // a share of the table's gradient to zero, in bytes
-  size_t zero_first, zero_last;
+  int tiles, rounds, shift, bits, passes, blocks;
+  // a share of the table's gradient to zero, in bytes, and what a workgroup takes of it
+  size_t zero_first, zero_last, zero_block;
 };
 
-__device__ __forceinline__ SortedToken sort_entry(const SortArgs& a, int n) {
-  return a.from ? a.from[n] : SortedToken{row_of(a.e, n), (uint32_t)n};
+// COUNT entries in runs of 64 from `first` on, loaded without a condition: those beyond the
+// last are the last again.
+template <int COUNT>
+__device__ __forceinline__ void sort_entries(const SortArgs& a, int first, int lane,
+                                             SortedToken (&t)[COUNT]) {
+  if (a.from) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) t[j] = a.from[min(first + 64 * j + lane, a.e.tokens - 1)];
+  } else {
+    long long id[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) id[j] = id_of(a.e, min(first + 64 * j + lane, a.e.tokens - 1));
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      t[j] = SortedToken{row_of(a.e, id[j]), (uint32_t)(first + 64 * j + lane)};
+  }
 }
 
-constexpr int kZeroBlock = 64 << 10;  // bytes that a workgroup zeroes
-
 __device__ __forceinline__ void zero_share(const SortArgs& a) {
-  const size_t first = a.zero_first + (size_t)(blockIdx.x - a.blocks) * kZeroBlock;
-  const size_t last = min(a.zero_last, first + kZeroBlock);
+  const size_t first = a.zero_first + (size_t)(blockIdx.x - a.blocks) * a.zero_block;
+  const size_t last = min(a.zero_last, first + a.zero_block);
   char* out = reinterpret_cast<char*>(a.e.out);
-  for (size_t at = first + threadIdx.x * 16; at < last; at += 256 * 16) {
+  for (size_t at = first + threadIdx.x * 16; at < last; at += blockDim.x * 16) {
     if (at + 16 <= last) {
       *reinterpret_cast<u32x4*>(out + at) = u32x4{0, 0, 0, 0};
     } else {
@@ -99,15 +117,39 @@ __device__ __forceinline__ void zero_share(const SortArgs& a) {
   }
 }
 
-// Lanes of the wave that have this lane's digit, among those that take part.
-__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool live) {
-  uint64_t same = __ballot(live);
-  for (int b = 0; b < bits; ++b) {
-    const uint64_t set = __ballot(digit >> b & 1);
-    same &= digit >> b & 1 ? set : ~set;
+// Lanes of the wave that have this lane's digit, among those that take part: for every
+// bit, the lanes whose bit is the lane's own (four instructions).
+template <int BITS>
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool live) {
+  const uint64_t all = __ballot(live);
+  uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const uint32_t own = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);
+    const uint64_t set = __ballot(own != 0);
+    lo &= ~((uint32_t)set ^ own);
+    hi &= ~((uint32_t)(set >> 32) ^ own);
   }
-  return same;
+  return (uint64_t)hi << 32 | lo;
 }
+
+// The lane's place among the tokens of its digit: behind those that `count` (a wave's own
+// counters) holds and the lanes before it; the counters then hold these too.  A wave's LDS
+// operations keep their order.
+template <int BITS>
+__device__ __forceinline__ int place_of(volatile int* count, uint32_t digits, bool live, int lane) {
+  const uint32_t digit = digits & ((1u << BITS) - 1);
+  const uint64_t same = same_digit<BITS>(digit, live);
+  const int before = __popcll(same & ((1ull << lane) - 1));
+  int to = 0;
+  if (live) {
+    to = count[digit] + before;
+    if (before == 0) count[digit] = to + __popcll(same);
+  }
+  return to;
+}
+
+constexpr int kSortAhead = 8;  // runs of 64 tokens that a wave has in flight
 
 // How many of its tokens each wave has of every digit.
 __global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
@@ -118,10 +160,14 @@ __global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
   for (int d = lane; d < kSortBins; d += 64) counts[wave][d] = 0;
   __syncthreads();
   if (tile < a.tiles)
-    for (int r = 0; r < a.rounds; ++r) {
-      const int n = (tile * a.rounds + r) * 64 + lane;
-      if (n < a.e.tokens)
-        atomicAdd(&counts[wave][sort_entry(a, n).key >> a.shift & ((1 << a.bits) - 1)], 1);
+    for (int r0 = 0; r0 < a.rounds; r0 += kSortAhead) {
+      const int first = (tile * a.rounds + r0) * 64;
+      SortedToken t[kSortAhead];
+      sort_entries(a, first, lane, t);
+#pragma unroll
+      for (int j = 0; j < kSortAhead; ++j)
+        if (r0 + j < a.rounds && first + 64 * j + lane < a.e.tokens)
+          atomicAdd(&counts[wave][t[j].key >> a.shift & ((1 << a.bits) - 1)], 1);
     }
   __syncthreads();
   if (tile < a.tiles)
@@ -129,18 +175,27 @@ __global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
       a.histogram[(size_t)tile * kSortBins + d] = counts[wave][d];
 }
 
+template <int BITS>
 __global__ __launch_bounds__(256) void sort_place_kernel(SortArgs a) {
   __shared__ int place[4][kSortBins];
   __shared__ int wave_sums[4];
   if ((int)blockIdx.x >= a.blocks) return zero_share(a);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  // digits 2 tid and 2 tid + 1: all of them, and those of the workgroup's waves' forerunners
-  int whole[2] = {0, 0};
-  for (int t = 0; t < a.tiles; ++t) {
-    if ((t & 3) == 0 && t == (int)blockIdx.x * 4) place[0][2 * tid] = whole[0], place[0][2 * tid + 1] = whole[1];
-    const int2 h = *reinterpret_cast<const int2*>(a.histogram + (size_t)t * kSortBins + 2 * tid);
-    whole[0] += h.x;
-    whole[1] += h.y;
+  // digits 2 tid and 2 tid + 1: those of the tiles before the workgroup's, and of all
+  const int2* counts = reinterpret_cast<const int2*>(a.histogram) + tid;
+  int before0 = 0, before1 = 0, whole[2] = {0, 0};
+  for (int t0 = 0; t0 < a.tiles; t0 += 64) {
+    int2 h[64];
+#pragma unroll
+    for (int j = 0; j < 64; ++j) h[j] = counts[(size_t)min(t0 + j, a.tiles - 1) * (kSortBins / 2)];
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+      const bool in = t0 + j < a.tiles, before = t0 + j < (int)blockIdx.x * 4;
+      whole[0] += in ? h[j].x : 0;
+      whole[1] += in ? h[j].y : 0;
+      before0 += before ? h[j].x : 0;
+      before1 += before ? h[j].y : 0;
+    }
   }
   // first place of the thread's two digits: an exclusive sum over the threads
   const int pair = whole[0] + whole[1];
@@ -154,13 +209,14 @@ __global__ __launch_bounds__(256) void sort_place_kernel(SortArgs a) {
   __syncthreads();
   int start = sum - pair;
   for (int i = 0; i < wave; ++i) start += wave_sums[i];
-  int at[2] = {start + place[0][2 * tid], start + whole[0] + place[0][2 * tid + 1]};
+  int at[2] = {start + before0, start + whole[0] + before1};
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
     place[i][2 * tid] = at[0];
     place[i][2 * tid + 1] = at[1];
     const int t = blockIdx.x * 4 + i;
     if (t < a.tiles) {
-      const int2 h = *reinterpret_cast<const int2*>(a.histogram + (size_t)t * kSortBins + 2 * tid);
+      const int2 h = counts[(size_t)t * (kSortBins / 2)];
       at[0] += h.x;
       at[1] += h.y;
     }
@@ -168,22 +224,77 @@ __global__ __launch_bounds__(256) void sort_place_kernel(SortArgs a) {
   __syncthreads();
   const int tile = blockIdx.x * 4 + wave;
   if (tile >= a.tiles) return;
-  for (int r = 0; r < a.rounds; ++r) {
-    const int n = (tile * a.rounds + r) * 64 + lane;
-    const bool live = n < a.e.tokens;
-    const SortedToken t = live ? sort_entry(a, n) : SortedToken{0, 0};
-    const uint32_t digit = t.key >> a.shift & ((1 << a.bits) - 1);
-    const uint64_t same = same_digit(digit, a.bits, live);
-    const int before = __popcll(same & ((1ull << lane) - 1));
-    // (the wave's own counters; its LDS operations keep their order)
-    volatile int* counter = &place[wave][digit];
-    int to = 0;
-    if (live) {
-      to = *counter + before;
-      if (before == 0) *counter = to + __popcll(same);
-      a.to[to] = t;
+  for (int r0 = 0; r0 < a.rounds; r0 += kSortAhead) {
+    const int first = (tile * a.rounds + r0) * 64;
+    SortedToken t[kSortAhead];
+    sort_entries(a, first, lane, t);
+#pragma unroll
+    for (int j = 0; j < kSortAhead; ++j) {
+      const bool live = r0 + j < a.rounds && first + 64 * j + lane < a.e.tokens;
+      const int to = place_of<BITS>(place[wave], t[j].key >> a.shift, live, lane);
+      if (live) a.to[to] = t[j];
     }
   }
+}
+
+// Up to kSortOne tokens, all digits in one launch: 16 waves with eight runs of 64 each, kept in
+// registers and exchanged through LDS from digit to digit.
+template <int BITS>
+__global__ __launch_bounds__(1024) void sort_one_kernel(SortArgs a) {
+  constexpr int WAVES = 16, ITEMS = kSortOne / 1024;
+  __shared__ int place[WAVES][kSortBins];
+  __shared__ SortedToken list[kSortOne];
+  __shared__ int wave_sums[kSortBins / 64];
+  if ((int)blockIdx.x >= a.blocks) return zero_share(a);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int n0 = wave * 64 * ITEMS + lane;
+  SortedToken t[ITEMS];
+  sort_entries(a, n0 - lane, lane, t);
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = pass * BITS;
+    for (int d = lane; d < kSortBins; d += 64) place[wave][d] = 0;
+    int to[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)  // among the wave's own of the digit
+      to[j] = place_of<BITS>(place[wave], t[j].key >> shift, n0 + 64 * j < a.e.tokens, lane);
+    __syncthreads();
+    // first places: over the digits, then over a digit's waves
+    int whole = 0, sum = 0;
+    if (tid < kSortBins) {
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const int c = place[i][tid];
+        place[i][tid] = whole;
+        whole += c;
+      }
+      sum = whole;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(sum, m);
+        if (lane >= m) sum += o;
+      }
+      if (lane == 63) wave_sums[wave] = sum;
+    }
+    __syncthreads();
+    if (tid < kSortBins) {
+      int start = sum - whole;
+      for (int i = 0; i < wave; ++i) start += wave_sums[i];
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) place[i][tid] += start;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (n0 + 64 * j < a.e.tokens)
+        list[place[wave][t[j].key >> shift & ((1 << BITS) - 1)] + to[j]] = t[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (n0 + 64 * j < a.e.tokens) t[j] = list[n0 + 64 * j];
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    if (n0 + 64 * j < a.e.tokens) a.to[n0 + 64 * j] = t[j];
 }
 
 // ---------------------------------------------------------------------------
@@ -192,41 +303,47 @@ struct SumArgs {
   const SortedToken* sorted;
   const void* dout;
   void* dtable;
-  float* partials;  // [chunks][2][dim]: what a chunk has of the run it begins in, and ends in
+  float* partials;  // [chunks][2][width]: what a chunk has of the run it begins in, and ends in
   long long stride;
-  int tokens, vocabulary, dim, chunks, slabs;
+  int tokens, vocabulary, dim, width, chunk, chunks, slabs;
   float scale;
 };
 
 // A wave adds the tokens of a chunk over 64 vectors of columns.
-template <typename T, bool TAIL>
+template <typename T, Edge E>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
   constexpr int N = kVec<T>, AHEAD = 8;
   const int lane = threadIdx.x & 63;
   const int item = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int chunk = item / a.slabs, col = ((item % a.slabs) * 64 + lane) * N;
+  const int chunk = item / a.slabs;
+  const RowPlace<T, E> at((item % a.slabs) * 64 + lane, a.dim);
   if (chunk >= a.chunks) return;
-  const int first = chunk * kEmbedChunk, count = min(kEmbedChunk, a.tokens - first);
-  // lane i < 32 holds entry i; the keys on either side of the chunk beside them
+  const int first = chunk * a.chunk, count = min(a.chunk, a.tokens - first);
+  // lane i holds entry i; the keys on either side of the chunk beside them
   const SortedToken mine = a.sorted[first + min(lane, count - 1)];
   const uint32_t none = a.vocabulary;
   const uint32_t before = first > 0 ? a.sorted[first - 1].key : none;
   const uint32_t behind = first + count < a.tokens ? a.sorted[first + count].key : none;
   // tokens without a row come last
   const int live = __popcll(__ballot(lane < count && mine.key < none));
-  const T* dout = reinterpret_cast<const T*>(a.dout);
+  if (live == 0) return;
   auto key_at = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane(mine.key, i); };
+  const T* dout = reinterpret_cast<const T*>(a.dout);
   auto fetch = [&](int i) {
-    const uint32_t token = __builtin_amdgcn_readlane(mine.token, min(i, count - 1));
-    return load_row<T, TAIL, true>(dout + (size_t)token * a.stride, col, a.dim);
+    const uint32_t token = __builtin_amdgcn_readlane(mine.token, min(i, live - 1));
+    return at.template load<true>(dout + (size_t)token * a.stride);
   };
   float sum[N] = {};
-  bool head = live > 0 && key_at(0) == before;
+  bool head = key_at(0) == before;
+  Vec<T> ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) ahead[j] = fetch(j);
   for (int i0 = 0; i0 < live; i0 += AHEAD) {
     Vec<T> v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (i0 + j < live) v[j] = fetch(i0 + j);
+    for (int j = 0; j < AHEAD; ++j) v[j] = ahead[j];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) ahead[j] = fetch(i0 + AHEAD + j);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int i = i0 + j;
@@ -238,15 +355,15 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
       // the run ends here, or with the chunk
       const bool open = next == key;
       if (head || open) {
-        float* to = a.partials + ((size_t)chunk * 2 + (head ? 0 : 1)) * a.dim;
+        float* to = a.partials + ((size_t)chunk * 2 + (head ? 0 : 1)) * a.width;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (col + e < a.dim) to[col + e] = sum[e];
+          if (at.any() && at.mine(e)) to[at.at + e] = sum[e];
       } else {
         float x[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) x[e] = sum[e] * a.scale;
-        store_row<T, TAIL>(reinterpret_cast<T*>(a.dtable) + (size_t)key * a.dim, col, a.dim, x);
+        at.store(reinterpret_cast<T*>(a.dtable) + (size_t)key * a.dim, x);
       }
       head = false;
 #pragma unroll
@@ -256,54 +373,54 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
 }
 
 // The runs that pass a chunk's end: the workgroup of the chunk that one begins in adds
-// its pieces, each wave a quarter of the chunks, in order.
+// its pieces over 256 columns, each wave a quarter of the chunks, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
-  __shared__ float sums[4][64];
-  const int chunk = blockIdx.x, first = chunk * kEmbedChunk;
-  const int next = first + kEmbedChunk;
-  if (next >= a.tokens) return;
-  const uint32_t key = a.sorted[next - 1].key;
-  if (key >= (uint32_t)a.vocabulary || a.sorted[next].key != key) return;
-  // the run fills the chunk from an earlier one on: it is that one's
-  if (first > 0 && a.sorted[first - 1].key == key) return;
-  // the run's end, by bisection
-  int lo = next, hi = a.tokens;  // sorted[lo] has the key; the first beyond it is in (lo, hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.sorted[mid].key == key)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const int last = lo / kEmbedChunk;  // the last chunk with a piece
+  __shared__ f32x4 sums[4][64];
+  const int chunk = blockIdx.x, first = chunk * a.chunk, next = first + a.chunk;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = blockIdx.y * 64 + lane;
-  const int per = (last - chunk + 4) / 4;
-  const int from = chunk + wave * per, to = min(last + 1, from + per);
-  float s = 0.f;
-  if (col < a.dim) {
+  // the keys on both sides of the chunk's end and in front of its start
+  const uint32_t none = a.vocabulary;
+  const uint32_t key = a.sorted[next - 1].key, behind = a.sorted[next].key;
+  const uint32_t before = first > 0 ? a.sorted[first - 1].key : none;
+  // (a run that fills the chunk from an earlier one on is that one's)
+  if (key >= none || behind != key || before == key) return;
+  // the chunks that begin within the run, 64 at a time
+  int count = 0;
+  for (int more = 64; more == 64; count += more) {
+    const long long at = (long long)(chunk + 1 + count + lane) * a.chunk;
+    const uint64_t in = __ballot(at < a.tokens && a.sorted[min(at, a.tokens - 1ll)].key == key);
+    more = in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
+  }
+  const int col = (blockIdx.y * 64 + lane) * 4;
+  const int per = (count + 4) / 4, from = wave * per, to = min(count + 1, from + per);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  // (rows of `width`, a multiple of 4; lanes beyond it read its start)
+  const float* piece = a.partials + ((size_t)chunk * 2 + 1) * a.width + (col < a.width ? col : 0);
 #pragma unroll 8
-    for (int c = from; c < to; ++c)
-      s += a.partials[((size_t)c * 2 + (c == chunk ? 1 : 0)) * a.dim + col];
+  for (int c = from; c < to; ++c) {
+    // the run's first piece is its chunk's second, the others their chunks' first
+    s += *reinterpret_cast<const f32x4*>(piece + (c == 0 ? 0ll : (2ll * c - 1) * a.width));
   }
   sums[wave][lane] = s;
   __syncthreads();
-  if (wave || col >= a.dim) return;
-  s += sums[1][lane];
-  s += sums[2][lane];
-  s += sums[3][lane];
-  reinterpret_cast<T*>(a.dtable)[(size_t)key * a.dim + col] = (T)(s * a.scale);
+  if (wave) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s += sums[i][lane];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < a.dim)
+      reinterpret_cast<T*>(a.dtable)[(size_t)key * a.dim + col + i] = (T)(s[i] * a.scale);
 }
 
 // ---------------------------------------------------------------------------
 
-template <typename T, bool TAIL>
-static void launch_embed_t(const EmbedArgs& a, hipStream_t stream) {
+template <typename T, Edge E>
+static void launch_embed_e(const EmbedArgs& a, hipStream_t stream) {
   const int vectors = (a.dim + kVec<T> - 1) / kVec<T>;
   auto go = [&](auto l) {
     constexpr int L = decltype(l)::value;
-    hipLaunchKernelGGL((embed_kernel<T, L, TAIL>), dim3((a.tokens + 256 / L - 1) / (256 / L)),
+    hipLaunchKernelGGL((embed_kernel<T, L, E>), dim3((a.tokens + 256 / L - 1) / (256 / L)),
                        dim3(256), 0, stream, a);
   };
   if (vectors <= 16)
@@ -312,30 +429,53 @@ static void launch_embed_t(const EmbedArgs& a, hipStream_t stream) {
     go(std::integral_constant<int, 64>{});
 }
 
+template <typename T>
+static hipError_t launch_embed_t(const EmbedArgs& a, hipStream_t stream) {
+  switch (edge_of<T>(a.dim)) {
+    case EDGE_WHOLE: launch_embed_e<T, EDGE_WHOLE>(a, stream); break;
+    case EDGE_CUT: launch_embed_e<T, EDGE_CUT>(a, stream); break;
+    default: launch_embed_e<T, EDGE_SHORT>(a, stream);
+  }
+  return hipGetLastError();
+}
+
 hipError_t launch_embed(const void* ids, bool ids64, const void* table, long long stride, bool f32,
                         int tokens, int vocabulary, int dim, long long padding, float scale,
                         void* out, hipStream_t stream) {
   const EmbedArgs a{ids, table, out, stride, padding, tokens, vocabulary, dim, scale, ids64};
-  const bool tail = dim % (f32 ? 4 : 8);
-  if (f32)
-    tail ? launch_embed_t<float, true>(a, stream) : launch_embed_t<float, false>(a, stream);
-  else
-    tail ? launch_embed_t<bf16, true>(a, stream) : launch_embed_t<bf16, false>(a, stream);
-  return hipGetLastError();
+  return f32 ? launch_embed_t<float>(a, stream) : launch_embed_t<bf16>(a, stream);
 }
 
 template <typename T>
 static hipError_t launch_sums(SumArgs a, hipStream_t stream) {
   a.slabs = (a.dim + 64 * kVec<T> - 1) / (64 * kVec<T>);
   const dim3 grid((unsigned)(((long long)a.chunks * a.slabs + 3) / 4));
-  if (a.dim % kVec<T>)
-    hipLaunchKernelGGL((embed_sum_kernel<T, true>), grid, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((embed_sum_kernel<T, false>), grid, dim3(256), 0, stream, a);
+  switch (edge_of<T>(a.dim)) {
+    case EDGE_WHOLE:
+      hipLaunchKernelGGL((embed_sum_kernel<T, EDGE_WHOLE>), grid, dim3(256), 0, stream, a);
+      break;
+    case EDGE_CUT:
+      hipLaunchKernelGGL((embed_sum_kernel<T, EDGE_CUT>), grid, dim3(256), 0, stream, a);
+      break;
+    default:
+      hipLaunchKernelGGL((embed_sum_kernel<T, EDGE_SHORT>), grid, dim3(256), 0, stream, a);
+  }
   if (a.chunks > 1)
-    hipLaunchKernelGGL((embed_join_kernel<T>), dim3(a.chunks - 1, (a.dim + 63) / 64), dim3(256), 0,
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3(a.chunks - 1, (a.dim + 255) / 256), dim3(256), 0,
                        stream, a);
   return hipGetLastError();
+}
+
+template <typename F>
+static void with_bits(int bits, F&& f) {
+  using std::integral_constant;
+  switch (bits) {
+    case 5: return f(integral_constant<int, 5>{});
+    case 6: return f(integral_constant<int, 6>{});
+    case 7: return f(integral_constant<int, 7>{});
+    case 8: return f(integral_constant<int, 8>{});
+    default: return f(integral_constant<int, 9>{});
+  }
 }
 
 hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long long stride,
@@ -350,29 +490,44 @@ hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long 
   s.histogram = reinterpret_cast<int*>(ws + l.histogram);
   s.tiles = l.tiles;
   s.rounds = l.rounds;
-  s.blocks = (l.tiles + 3) / 4;
+  s.bits = l.bits;
+  s.passes = l.passes;
   const size_t bytes = (size_t)vocabulary * dim * (f32 ? 4 : 2);
-  const int launches = 2 * l.passes;
-  const size_t share = (bytes / launches / kZeroBlock + 1) * kZeroBlock;
-  for (int pass = 0; pass < l.passes; ++pass) {
-    s.shift = pass * l.bits;
-    s.bits = l.bits;
-    s.from = pass ? lists[(pass + 1) & 1] : nullptr;
-    s.to = lists[pass & 1];
-    for (int step = 0; step < 2; ++step) {
-      const size_t k = 2 * pass + step;
-      s.zero_first = std::min(bytes, k * share);
-      s.zero_last = std::min(bytes, (k + 1) * share);
-      const unsigned zero = (unsigned)((s.zero_last - s.zero_first + kZeroBlock - 1) / kZeroBlock);
+  SortedToken* sorted = lists[0];
+  if (l.tiles == 0) {
+    s.blocks = 1;
+    s.to = sorted;
+    s.zero_last = bytes;
+    s.zero_block = 256 << 10;  // (few workgroups: the sort's LDS leaves a CU room for one)
+    const unsigned zero = (unsigned)((bytes + s.zero_block - 1) / s.zero_block);
+    with_bits(l.bits, [&](auto b) {
+      hipLaunchKernelGGL((sort_one_kernel<decltype(b)::value>), dim3(1 + zero), dim3(1024), 0,
+                         stream, s);
+    });
+  } else {
+    s.blocks = (l.tiles + 3) / 4;
+    s.zero_block = 64 << 10;
+    const size_t share = (bytes / (2 * l.passes) / s.zero_block + 1) * s.zero_block;
+    for (int step = 0; step < 2 * l.passes; ++step) {
+      const int pass = step / 2;
+      s.shift = pass * l.bits;
+      s.from = pass ? lists[(pass + 1) & 1] : nullptr;
+      s.to = sorted = lists[pass & 1];
+      s.zero_first = std::min(bytes, step * share);
+      s.zero_last = std::min(bytes, (step + 1) * share);
+      const unsigned zero =
+          (unsigned)((s.zero_last - s.zero_first + s.zero_block - 1) / s.zero_block);
       const dim3 grid((unsigned)s.blocks + zero);
-      if (step == 0)
+      if (step % 2 == 0)
         hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, stream, s);
       else
-        hipLaunchKernelGGL(sort_place_kernel, grid, dim3(256), 0, stream, s);
+        with_bits(l.bits, [&](auto b) {
+          hipLaunchKernelGGL((sort_place_kernel<decltype(b)::value>), grid, dim3(256), 0, stream, s);
+        });
     }
   }
-  SumArgs a{lists[(l.passes + 1) & 1], dout, dtable, reinterpret_cast<float*>(ws + l.partials), stride,
-            tokens, vocabulary, dim, l.chunks, 0, scale};
+  const SumArgs a{sorted, dout, dtable, reinterpret_cast<float*>(ws + l.partials), stride, tokens,
+                  vocabulary, dim, l.width, l.chunk, l.chunks, 0, scale};
   return f32 ? launch_sums<float>(a, stream) : launch_sums<bf16>(a, stream);
 }
 

@@ -51,58 +51,61 @@ __device__ __forceinline__ float row_sum(float x, float* part) {
 }
 
 // The lane's share of a parameter, in its own dtype (uniform branch).
-template <typename T, int C, int L, bool TAIL>
-__device__ __forceinline__ void load_params(const void* p, bool f32, int lane, int dim,
+template <typename T, Edge E, int C>
+__device__ __forceinline__ void load_params(const void* p, bool f32, const RowPlace<T, E> (&at)[C],
                                             float (&w)[C][kVec<T>]) {
   constexpr int N = kVec<T>;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int col = (c * L + lane) * N;
     if (f32 == (N == 4)) {
-      const Vec<T> v = load_row<T, TAIL>(reinterpret_cast<const T*>(p), col, dim);
+      const Vec<T> v = at[c].load(reinterpret_cast<const T*>(p));
 #pragma unroll
       for (int i = 0; i < N; ++i) w[c][i] = (float)v[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[c][i] = col + i < dim ? element(p, f32, col + i) : 0.f;
+      for (int i = 0; i < N; ++i)
+        w[c][i] = reinterpret_cast<const float*>(p)[E == EDGE_SHORT ? min(i, at[c].dim - 1)
+                                                                    : at[c].at + i];
     }
   }
 }
 
-template <typename T, int L, int C, bool TAIL>
+template <typename T, int L, int C, Edge E>
 __global__ __launch_bounds__(L > 64 ? L : 256) void norm_kernel(NormArgs a) {
   constexpr int N = kVec<T>, R = L > 64 ? 1 : 256 / L;
   __shared__ float part[2][L > 64 ? L / 64 : 1];
   const int lane = threadIdx.x % L;
   const int row = blockIdx.x * R + threadIdx.x / L;
-  if (L <= 64 && row >= a.rows) return;
+  if (R > 1 && row >= a.rows) return;
   const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.x_stride;
+  RowPlace<T, E> at[C];
   Vec<T> raw[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) raw[c] = load_row<T, TAIL>(x, (c * L + lane) * N, a.dim);
+  for (int c = 0; c < C; ++c) {
+    at[c] = RowPlace<T, E>(c * L + lane, a.dim);
+    raw[c] = at[c].load(x);
+  }
   float w[C][N], b[C][N];
-  load_params<T, C, L, TAIL>(a.weight, a.param_f32, lane, a.dim, w);
-  if (a.bias) load_params<T, C, L, TAIL>(a.bias, a.param_f32, lane, a.dim, b);
-  float mean = 0.f;
-  if (a.center) {
+  load_params<T, E, C>(a.weight, a.param_f32, at, w);
+  if (a.bias) load_params<T, E, C>(a.bias, a.param_f32, at, b);
+  // sum over the row of f(value)
+  auto sum = [&](auto f, float* lds) {
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += (float)raw[c][i];
-    mean = row_sum<L>(s, part[0]) * a.inv_dim;
-  }
-  float s = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = (float)raw[c][i] - mean;
-      if (!TAIL && (c * L + lane) * N >= a.dim) continue;
-      if (TAIL && (c * L + lane) * N + i >= a.dim) continue;
-      s = fmaf(d, d, s);
+      for (int i = 0; i < N; ++i) {
+        const float y = f((float)raw[c][i]);
+        v += at[c].mine(i) ? y : 0.f;
+      }
+      s += at[c].any() ? v : 0.f;
     }
-  const float rstd = rsqrtf(fmaf(row_sum<L>(s, part[1]), a.inv_dim, a.eps));
+    return row_sum<L>(s, lds);
+  };
+  const float mean = a.center ? sum([](float v) { return v; }, part[0]) * a.inv_dim : 0.f;
+  const float square = sum([mean](float v) { return (v - mean) * (v - mean); }, part[1]);
+  const float rstd = rsqrtf(fmaf(square, a.inv_dim, a.eps));
   T* y = reinterpret_cast<T*>(a.y) + (size_t)row * a.dim;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(L > 64 ? L : 256) void norm_kernel(NormArgs a) {
       o[i] = ((float)raw[c][i] - mean) * rstd * w[c][i];
       if (a.bias) o[i] += b[c][i];
     }
-    store_row<T, TAIL>(y, (c * L + lane) * N, a.dim, o);
+    at[c].store(y, o);
   }
   if (a.stats && lane == 0) a.stats[row] = float2{mean, rstd};
 }
@@ -132,54 +135,84 @@ struct NormBwdArgs {
   bool center, param_f32;
 };
 
-template <typename T, int L, int C, bool TAIL>
-__global__ __launch_bounds__(512) void norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int N = kVec<T>, R = 512 / L;
+// Waves a SIMD that the registers are held to: two workgroups a CU, one for the rows of most
+// registers a lane.
+template <typename T, int L, int C>
+constexpr int kNormBwdWaves = C * kVec<T> > (L < 512 ? 16 : 8) ? 2 : 4;
+
+template <typename T, int L, int C, Edge E>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(kNormBwdWaves<T, L, C>)))
+void norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int N = kVec<T>, R = 512 / L, W = L > 64 ? L / 64 : 1;
+  // a row is in flight beside the one that is computed, where the registers have room
+  constexpr bool AHEAD = C * N <= 16 || L == 64;
   extern __shared__ float lds[];  // the workgroup's sums [2][dim]
   __shared__ float part[2][2][8];
-  const int lane = threadIdx.x % L;
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  RowPlace<T, E> at[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) at[c] = RowPlace<T, E>(c * L + lane, a.dim);
   float w[C][N], dw[C][N], db[C][N];
-  load_params<T, C, L, TAIL>(a.weight, a.param_f32, lane, a.dim, w);
+  load_params<T, E, C>(a.weight, a.param_f32, at, w);
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < N; ++i) dw[c][i] = db[c][i] = 0.f;
-  // rows of the workgroup: the next one is fetched while one is computed
   const int step = gridDim.x * R;
-  int row = blockIdx.x * R + threadIdx.x / L;
   Vec<T> xr[C], gr[C];
   float2 st = {0.f, 0.f};
-  auto fetch = [&](int r) {
+  auto fetch = [&](int first) {  // (a row beyond the last is read again, not used)
+    const int r = min(first + group, a.rows - 1);
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)r * a.x_stride;
     const T* g = reinterpret_cast<const T*>(a.dy) + (size_t)r * a.dy_stride;
-#pragma unroll
-    for (int c = 0; c < C; ++c) xr[c] = load_row<T, TAIL>(x, (c * L + lane) * N, a.dim);
-#pragma unroll
-    for (int c = 0; c < C; ++c) gr[c] = load_row<T, TAIL>(g, (c * L + lane) * N, a.dim);
     st = a.stats[r];
+#pragma unroll
+    for (int c = 0; c < C; ++c) xr[c] = at[c].load(x);
+#pragma unroll
+    for (int c = 0; c < C; ++c) gr[c] = at[c].load(g);
   };
-  if (row < a.rows) fetch(row);
-  for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
-    float h[C][N], g[C][N], sg = 0.f, sgh = 0.f;
-    const float rstd = st.y;
+  int first = blockIdx.x * R;
+  if (AHEAD) fetch(first);
+  for (int turn = 0; first < a.rows; first += step, turn ^= 1) {
+    if (!AHEAD) fetch(first);
+    const int row = first + group;
+    const bool live = R == 1 || row < a.rows;
+    const float mean = st.x, rstd = st.y;
+    Vec<T> x[C], dy[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      x[c] = xr[c];
+      dy[c] = gr[c];
+    }
+    if (AHEAD) fetch(first + step);
+    float sg = 0.f, sgh = 0.f;
+    if (live) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float dy = (float)gr[c][i];
-        h[c][i] = ((float)xr[c][i] - st.x) * rstd;
-        dw[c][i] = fmaf(dy, h[c][i], dw[c][i]);
-        db[c][i] += dy;
-        g[c][i] = dy * w[c][i];  // zero past the row's end
-        sg += g[c][i];
-        sgh = fmaf(g[c][i], h[c][i], sgh);
+      for (int c = 0; c < C; ++c) {
+        float vg = 0.f, vgh = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float d = (float)dy[c][i], h = ((float)x[c][i] - mean) * rstd;
+          dw[c][i] = fmaf(d, h, dw[c][i]);
+          db[c][i] += d;
+          const float g = at[c].mine(i) ? d * w[c][i] : 0.f;
+          vg += g;
+          vgh = fmaf(g, h, vgh);
+        }
+        sg += at[c].any() ? vg : 0.f;
+        sgh += at[c].any() ? vgh : 0.f;
       }
-    const int next = row + step;
-    if (next < a.rows) fetch(next);
+    }
     if (!a.dx) continue;
-    if constexpr (L > 64) {
+    if constexpr (L == 16) {
+      sg = sum16(sg);
+      sgh = sum16(sgh);
+    } else {
       sg = sum64(sg);
       sgh = sum64(sgh);
+    }
+    if constexpr (W > 1) {
+      // (two sets of sums in turn: one barrier a row)
       if ((threadIdx.x & 63) == 0) {
         part[turn][0][threadIdx.x >> 6] = sg;
         part[turn][1][threadIdx.x >> 6] = sgh;
@@ -187,23 +220,28 @@ __global__ __launch_bounds__(512) void norm_bwd_kernel(NormBwdArgs a) {
       __syncthreads();
       sg = sgh = 0.f;
 #pragma unroll
-      for (int i = 0; i < L / 64; ++i) {
-        sg += part[turn][0][i];
-        sgh += part[turn][1][i];
+      for (int i = 0; i < W; ++i) {
+        sg += part[turn][0][group * W + i];
+        sgh += part[turn][1][group * W + i];
       }
-    } else {
-      sg = row_sum<L>(sg, nullptr);
-      sgh = row_sum<L>(sgh, nullptr);
     }
+    if (!live) continue;
     sg = a.center ? sg * a.inv_dim : 0.f;
     sgh *= a.inv_dim;
     T* dx = reinterpret_cast<T*>(a.dx) + (size_t)row * a.dim;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      // (the row as it was loaded: what the first pass made of it would take twice its registers)
+      u32x4 xs = __builtin_bit_cast(u32x4, x[c]), ds = __builtin_bit_cast(u32x4, dy[c]);
+      asm volatile("" : "+v"(xs), "+v"(ds));
+      const Vec<T> xv = __builtin_bit_cast(Vec<T>, xs), dv = __builtin_bit_cast(Vec<T>, ds);
       float o[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = rstd * (g[c][i] - fmaf(h[c][i], sgh, sg));
-      store_row<T, TAIL>(dx, (c * L + lane) * N, a.dim, o);
+      for (int i = 0; i < N; ++i) {
+        const float h = ((float)xv[i] - mean) * rstd;
+        o[i] = rstd * fmaf((float)dv[i], w[c][i], -fmaf(h, sgh, sg));
+      }
+      at[c].store(dx, o);
     }
   }
   if (!a.partials) return;
@@ -218,23 +256,23 @@ __global__ __launch_bounds__(512) void norm_bwd_kernel(NormBwdArgs a) {
       }
   }
   float* out = a.partials + (size_t)blockIdx.x * 2 * a.dim;
-  constexpr int W = L > 64 ? 1 : 8;
-  for (int wave = 0; wave < W; ++wave) {
-    if (W == 1 || (int)(threadIdx.x >> 6) == wave) {
+  constexpr int G = R > 8 ? 8 : R;  // groups of lanes with sums of their own
+  float* to = G > 1 ? lds : out;
+  for (int g = 0; g < G; ++g) {
+    if ((int)(L == 16 ? threadIdx.x >> 6 : group) == g && (L > 16 || (threadIdx.x & 63) < 16)) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int col = (c * L + lane) * N + i;
-          if (col >= a.dim || (L == 16 && (threadIdx.x & 63) >= 16)) continue;
-          float* to = W == 1 ? out : lds;
-          to[col] = (wave ? lds[col] : 0.f) + dw[c][i];
-          to[a.dim + col] = (wave ? lds[a.dim + col] : 0.f) + db[c][i];
+          if (!at[c].any() || !at[c].mine(i)) continue;
+          const int col = at[c].at + i;
+          to[col] = (g ? lds[col] : 0.f) + dw[c][i];
+          to[a.dim + col] = (g ? lds[a.dim + col] : 0.f) + db[c][i];
         }
     }
-    if (W > 1) __syncthreads();
+    if (G > 1) __syncthreads();
   }
-  if (W > 1)
+  if (G > 1)
     for (int i = threadIdx.x; i < 2 * a.dim; i += 512) out[i] = lds[i];
 }
 
@@ -272,8 +310,9 @@ struct NormShape {
 };
 static NormShape norm_shape(int vectors) {
   if (vectors <= 16) return {16, 1};
-  for (int c = 1; c <= 4; c *= 2)
-    if (vectors <= 64 * c) return {64, c};
+  if (vectors <= 64) return {64, 1};
+  if (vectors <= 128) return {64, 2};
+  if (vectors <= 256) return {256, 1};
   for (int c = 1; c < kNormMostVectors; c *= 2)
     if (vectors <= 512 * c) return {512, c};
   return {512, kNormMostVectors};
@@ -296,33 +335,41 @@ template <typename T, typename F>
 static void with_shape(int dim, F&& f) {
   constexpr int N = kVec<T>;
   const NormShape s = norm_shape((dim + N - 1) / N);
-  const bool tail = dim % N != 0;
-  auto go = [&](auto l, auto c) {
-    if (tail)
-      f(l, c, std::true_type{});
-    else
-      f(l, c, std::false_type{});
-  };
   using std::integral_constant;
-  if (s.lanes == 16) return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  if (s.lanes == 64) {
-    if (s.vectors == 1) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    if (s.vectors == 2) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  }
-  if (s.vectors == 1) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-  if (s.vectors == 2) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-  if (s.vectors == 4) return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-  // (a bf16 row of kNormMostDim has four)
-  if constexpr (N == 4) go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+  auto go = [&](auto l, auto c) {
+    if (edge_of<T>(dim) == EDGE_WHOLE)
+      f(l, c, integral_constant<Edge, EDGE_WHOLE>{});
+    else
+      f(l, c, integral_constant<Edge, EDGE_CUT>{});
+  };
+  auto wide = [&](auto c) { go(integral_constant<int, 512>{}, c); };
+  if (edge_of<T>(dim) == EDGE_SHORT)
+    f(integral_constant<int, 16>{}, integral_constant<int, 1>{},
+      integral_constant<Edge, EDGE_SHORT>{});
+  else if (s.lanes == 16)
+    go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (s.lanes == 64 && s.vectors == 1)
+    go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (s.lanes == 64)
+    go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (s.lanes == 256)
+    go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (s.vectors == 1)
+    wide(integral_constant<int, 1>{});
+  else if (s.vectors == 2)
+    wide(integral_constant<int, 2>{});
+  else if (s.vectors == 4)
+    wide(integral_constant<int, 4>{});
+  else if constexpr (N == 4)  // (a bf16 row of kNormMostDim has four)
+    wide(integral_constant<int, 8>{});
 }
 
 template <typename T>
 static hipError_t launch_norm_t(const NormArgs& a, hipStream_t stream) {
-  with_shape<T>(a.dim, [&](auto l, auto c, auto tail) {
+  with_shape<T>(a.dim, [&](auto l, auto c, auto edge) {
     constexpr int L = decltype(l)::value;
     constexpr int R = L > 64 ? 1 : 256 / L;
-    hipLaunchKernelGGL((norm_kernel<T, L, decltype(c)::value, decltype(tail)::value>),
+    hipLaunchKernelGGL((norm_kernel<T, L, decltype(c)::value, decltype(edge)::value>),
                        dim3((a.rows + R - 1) / R), dim3(L > 64 ? L : 256), 0, stream, a);
   });
   return hipGetLastError();
@@ -338,10 +385,10 @@ hipError_t launch_norm(const void* x, long long x_stride, const void* weight, co
 
 template <typename T>
 static hipError_t launch_norm_bwd_t(const NormBwdArgs& a, int blocks, hipStream_t stream) {
-  with_shape<T>(a.dim, [&](auto l, auto c, auto tail) {
+  with_shape<T>(a.dim, [&](auto l, auto c, auto edge) {
     constexpr int L = decltype(l)::value;
-    const size_t lds = L > 64 || !a.partials ? 0 : sizeof(float) * 2 * a.dim;
-    hipLaunchKernelGGL((norm_bwd_kernel<T, L, decltype(c)::value, decltype(tail)::value>),
+    const size_t lds = L > 256 || !a.partials ? 0 : sizeof(float) * 2 * a.dim;
+    hipLaunchKernelGGL((norm_bwd_kernel<T, L, decltype(c)::value, decltype(edge)::value>),
                        dim3(blocks), dim3(512), lds, stream, a);
   });
   return hipGetLastError();

@@ -1,10 +1,13 @@
 // Rows of any width and alignment: vectors of 16 bytes, and sums over lanes.
 //
-// A row of `dim` elements is read in vectors of 16 bytes (8 bf16, 4 fp32) from its
-// first element on.  Global loads and stores of 16 bytes need no more than their
-// element's alignment on gfx950 (unaligned access mode), so rows of an odd width
-// or at an odd offset take the same instructions as aligned ones; only the vector
-// that the row ends in goes element by element.
+// A row of `dim` elements is taken in vectors of 16 bytes (8 bf16, 4 fp32).  Global loads
+// and stores of 16 bytes need no more than their element's alignment on gfx950
+// (unaligned access mode), so rows of an odd width or at an odd offset take the same
+// instructions as aligned ones.  Loads have no condition: a wait counts the loads
+// behind it, and behind a branch it can only wait for all.  A lane whose vector is
+// beyond the row loads one inside, and one that the row ends in (EDGE_CUT) takes the
+// row's last N elements, those in front of its own twice with another lane.  Rows
+// shorter than a vector (EDGE_SHORT) go element by element.
 #pragma once
 
 #include "mf_common.h"
@@ -25,48 +28,72 @@ template <> struct RowVec<float> {
 template <typename T> using Vec = typename RowVec<T>::V;
 template <typename T> constexpr int kVec = RowVec<T>::N;
 
-// Elements col .. col + N - 1 of a row of `dim`, `fill` past its end (TAIL: a
-// vector may be cut; otherwise it is whole or beyond the row).
-template <typename T, bool TAIL, bool STREAM = false>
-__device__ __forceinline__ Vec<T> load_row(const T* row, int col, int dim, float fill = 0.f) {
-  typedef typename RowVec<T>::U U;
-  constexpr int N = kVec<T>;
-  Vec<T> v;
-  if (col + N <= dim) {
-    const U* p = reinterpret_cast<const U*>(row + col);
-    const U u = STREAM ? __builtin_nontemporal_load(p) : *p;
-    v = u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (T)fill;
-    if constexpr (TAIL) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (col + i < dim) v[i] = row[col + i];
-    }
-  }
-  return v;
+enum Edge { EDGE_WHOLE, EDGE_CUT, EDGE_SHORT };
+
+template <typename T>
+inline Edge edge_of(int dim) {
+  return dim < kVec<T> ? EDGE_SHORT : dim % kVec<T> ? EDGE_CUT : EDGE_WHOLE;
 }
 
-template <typename T, bool TAIL, bool STREAM = false>
-__device__ __forceinline__ void store_row(T* row, int col, int dim, const float (&x)[kVec<T>]) {
-  typedef typename RowVec<T>::U U;
-  constexpr int N = kVec<T>;
-  if (col + N <= dim) {
-    U u;
-#pragma unroll
-    for (int i = 0; i < N; ++i) u[i] = (T)x[i];
-    U* p = reinterpret_cast<U*>(row + col);
-    if constexpr (STREAM)
-      __builtin_nontemporal_store(u, p);
-    else
-      *p = u;
-  } else if constexpr (TAIL) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (col + i < dim) row[col + i] = (T)x[i];
+// Where the lane that owns vector `v` of a row loads and stores.
+template <typename T, Edge E>
+struct RowPlace {
+  static constexpr int N = kVec<T>;
+  int at;    // first element
+  int own;   // elements in front of this index in the vector are another lane's; N: all are
+  int dim;
+
+  __device__ __forceinline__ RowPlace() {}
+  __device__ __forceinline__ RowPlace(int v, int dim_) : dim(dim_) {
+    const int col = v * N;
+    if constexpr (E == EDGE_SHORT) {
+      at = 0;
+      own = v == 0 ? 0 : N;
+    } else {
+      at = min(col, dim - N);
+      own = col < dim ? col - at : N;
+    }
   }
-}
+  __device__ __forceinline__ bool any() const { return own < N; }
+  // whether element i counts in sums
+  __device__ __forceinline__ bool mine(int i) const {
+    if constexpr (E == EDGE_WHOLE) return true;  // (with any())
+    if constexpr (E == EDGE_CUT) return i >= own;
+    return i < dim;
+  }
+  template <bool STREAM = false>
+  __device__ __forceinline__ Vec<T> load(const T* row) const {
+    typedef typename RowVec<T>::U U;
+    Vec<T> x;
+    if constexpr (E == EDGE_SHORT) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = i < dim ? row[i] : (T)0.f;
+    } else {
+      const U* p = reinterpret_cast<const U*>(row + at);
+      x = STREAM ? __builtin_nontemporal_load(p) : *p;
+    }
+    return x;
+  }
+  template <bool STREAM = false>
+  __device__ __forceinline__ void store(T* row, const float (&x)[N]) const {
+    typedef typename RowVec<T>::U U;
+    if (!any()) return;
+    if constexpr (E == EDGE_SHORT) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < dim) row[i] = (T)x[i];
+    } else {
+      U u;
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = (T)x[i];
+      U* p = reinterpret_cast<U*>(row + at);
+      if constexpr (STREAM)
+        __builtin_nontemporal_store(u, p);
+      else
+        *p = u;
+    }
+  }
+};
 
 // Element `i` of an array that holds fp32 or bf16.
 __device__ __forceinline__ float element(const void* p, bool f32, size_t i) {
