@@ -51,23 +51,25 @@ __device__ __forceinline__ float row_sum(float x, float* part) {
 }
 
 // The lane's share of a parameter, in its own dtype (uniform branch).
+template <typename T, Edge E>
+__device__ __forceinline__ void load_param(const void* p, bool f32, const RowPlace<T, E>& at,
+                                           float (&w)[kVec<T>]) {
+  constexpr int N = kVec<T>;
+  if (f32 == (N == 4)) {
+    const Vec<T> v = at.load(reinterpret_cast<const T*>(p));
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = (float)v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      w[i] = reinterpret_cast<const float*>(p)[E == EDGE_SHORT ? min(i, at.dim - 1) : at.at + i];
+  }
+}
 template <typename T, Edge E, int C>
 __device__ __forceinline__ void load_params(const void* p, bool f32, const RowPlace<T, E> (&at)[C],
                                             float (&w)[C][kVec<T>]) {
-  constexpr int N = kVec<T>;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    if (f32 == (N == 4)) {
-      const Vec<T> v = at[c].load(reinterpret_cast<const T*>(p));
-#pragma unroll
-      for (int i = 0; i < N; ++i) w[c][i] = (float)v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        w[c][i] = reinterpret_cast<const float*>(p)[E == EDGE_SHORT ? min(i, at[c].dim - 1)
-                                                                    : at[c].at + i];
-    }
-  }
+  for (int c = 0; c < C; ++c) load_param<T, E>(p, f32, at[c], w[c]);
 }
 
 template <typename T, int L, int C, Edge E>
@@ -152,8 +154,18 @@ void norm_bwd_kernel(NormBwdArgs a) {
   RowPlace<T, E> at[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) at[c] = RowPlace<T, E>(c * L + lane, a.dim);
-  float w[C][N], dw[C][N], db[C][N];
-  load_params<T, E, C>(a.weight, a.param_f32, at, w);
+  // the weights stay in registers, but for the rows of most registers a lane: from the cache
+  constexpr bool HOLD = C * N <= 16;
+  float held[HOLD ? C : 1][N], dw[C][N], db[C][N];
+  if constexpr (HOLD) load_params<T, E, C>(a.weight, a.param_f32, at, held);
+  auto weights = [&](int c, float (&w)[N]) {
+    if constexpr (HOLD) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = held[c][i];
+    } else {
+      load_param<T, E>(a.weight, a.param_f32, at[c], w);
+    }
+  };
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -189,13 +201,14 @@ void norm_bwd_kernel(NormBwdArgs a) {
     if (live) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        float vg = 0.f, vgh = 0.f;
+        float vg = 0.f, vgh = 0.f, w[N];
+        weights(c, w);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float d = (float)dy[c][i], h = ((float)x[c][i] - mean) * rstd;
           dw[c][i] = fmaf(d, h, dw[c][i]);
           db[c][i] += d;
-          const float g = at[c].mine(i) ? d * w[c][i] : 0.f;
+          const float g = at[c].mine(i) ? d * w[i] : 0.f;
           vg += g;
           vgh = fmaf(g, h, vgh);
         }
@@ -235,11 +248,12 @@ void norm_bwd_kernel(NormBwdArgs a) {
       u32x4 xs = __builtin_bit_cast(u32x4, x[c]), ds = __builtin_bit_cast(u32x4, dy[c]);
       asm volatile("" : "+v"(xs), "+v"(ds));
       const Vec<T> xv = __builtin_bit_cast(Vec<T>, xs), dv = __builtin_bit_cast(Vec<T>, ds);
-      float o[N];
+      float o[N], w[N];
+      weights(c, w);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float h = ((float)xv[i] - mean) * rstd;
-        o[i] = rstd * fmaf((float)dv[i], w[c][i], -fmaf(h, sgh, sg));
+        o[i] = rstd * fmaf((float)dv[i], w[i], -fmaf(h, sgh, sg));
       }
       at[c].store(dx, o);
     }

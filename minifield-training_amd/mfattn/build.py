@@ -4,7 +4,8 @@
 package needs the library it builds) or
 ``mfattn.build.build()``.  Every ``.hip`` file under ``csrc/`` is compiled
 with ``hipcc --offload-arch=gfx950`` into an object in ``csrc/_build`` and
-linked into ``mfattn/libmfattn.so``.  Packed-FP32 instructions are disabled
+linked into ``mfattn/libmfattn.so``; the autograd nodes of ``csrc/nodes`` become
+``mfattn/_mfnodes.so``.  Packed-FP32 instructions are disabled
 (``-packed-fp32-ops``); the host pass warns that it does not know that
 feature, which is harmless.
 """
@@ -17,11 +18,13 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 OUT = PKG / "libmfattn.so"
+NODES = PKG / "_mfnodes.so"
 ARCH = "gfx950"
 
 FLAGS = [
@@ -74,13 +77,35 @@ def _compile(src: pathlib.Path, obj: pathlib.Path) -> None:
         print(err, file=sys.stderr)
 
 
+def _build_nodes() -> None:
+    """The autograd nodes (``csrc/nodes``): host code over torch's C++ API, no GPU code."""
+    import torch
+
+    root = pathlib.Path(torch.__file__).resolve().parent
+    include, tmp = root / "include", NODES.with_suffix(".so.tmp")
+    cmd = [_hipcc(), "-x", "c++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(include), "-isystem", str(include / "torch/csrc/api/include"),
+           "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", str(pathlib.Path(_hipcc()).resolve().parents[1] / "include"),
+           str(CSRC / "nodes" / "nodes.cpp"), "-o", str(tmp), "-L", str(root / "lib"),
+           "-ltorch", "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"hipcc failed for the autograd nodes:\n{proc.stderr}")
+    os.replace(tmp, NODES)
+
+
 def build(verbose: bool = True) -> pathlib.Path:
     sources = sorted(CSRC.glob("*.hip"))
     objdir = CSRC / "_build"
     objdir.mkdir(exist_ok=True)
     objs = [objdir / (s.stem + ".o") for s in sources]
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources))) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as pool:
+        nodes = pool.submit(_build_nodes)  # (the longest of them)
         list(pool.map(_compile, sources, objs))
+        nodes.result()
     tmp = OUT.with_suffix(".so.tmp")
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

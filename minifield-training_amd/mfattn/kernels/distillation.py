@@ -19,53 +19,8 @@ import math
 
 import torch
 
-from .. import _lib
-from ..ops import (_ptr, _raw_stream, dtype_code, even_rows, launch, refuse_second_order,
-                   refuse_tangents, require_device)
-
-
-def _launch(logits, teacher, ids, total, weights, temperature, with_stats, grad):
-    """Loss of every row, the backward's stats and, into ``grad``, the gradient."""
-    v, k, device = logits.shape[-1], ids.shape[-1], logits.device
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-    rows = loss.numel()
-    stats, nbytes = None, 0
-    if with_stats:
-        stats = torch.empty(_lib.LIB.mf_distill_stats_bytes(rows, k) // 4, dtype=torch.float32,
-                            device=device)
-        nbytes = 4 * stats.numel()
-    if rows:
-        launch(device, _lib.LIB.mf_distill, logits.data_ptr(), even_rows(logits)[1],
-               teacher.data_ptr(), dtype_code(teacher), ids.data_ptr(), ids.element_size(),
-               _ptr(total), _ptr(weights), dtype_code(logits), rows, v, k, temperature,
-               loss.data_ptr(), _ptr(stats), nbytes, _ptr(grad),
-               0 if grad is None else even_rows(grad)[1], _raw_stream(device.index))
-    return loss, stats
-
-
-class TopLogitsLoss(torch.autograd.Function):
-    """The loss with a HIP forward and a HIP backward; the gradient reaches the logits."""
-
-    @staticmethod
-    def forward(ctx, logits, teacher, ids, total, weights, temperature):
-        loss, stats = _launch(logits, teacher, ids, total, weights, temperature, True, None)
-        ctx.save_for_backward(logits, ids, weights, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss):
-        refuse_second_order("the loss")
-        logits, ids, weights, stats = ctx.saved_tensors
-        v, device = logits.shape[-1], logits.device
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-        dloss = dloss.contiguous()
-        if dloss.numel():
-            launch(device, _lib.LIB.mf_distill_bwd, logits.data_ptr(), even_rows(logits)[1],
-                   ids.data_ptr(), ids.element_size(), _ptr(weights), stats.data_ptr(),
-                   4 * stats.numel(), dloss.data_ptr(), dtype_code(logits), dloss.numel(), v,
-                   ids.shape[-1], ctx.temperature, grad.data_ptr(), v, _raw_stream(device.index))
-        return grad, None, None, None, None, None
+from .. import _nodes
+from ..ops import dtype_code, even_rows, refuse_tangents, require_device
 
 
 def _checked(what, logits, teacher, ids, total, weights, temperature):
@@ -123,10 +78,8 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     """
     teacher, ids, total, weights = _checked("top_logits_loss", logits, teacher_logits, teacher_ids,
                                             teacher_total, weights, temperature)
-    logits = even_rows(logits)[0]
-    if logits.requires_grad and torch.is_grad_enabled():
-        return TopLogitsLoss.apply(logits, teacher, ids, total, weights, temperature)
-    return _launch(logits, teacher, ids, total, weights, temperature, False, None)[0]
+    record = logits.requires_grad and torch.is_grad_enabled()
+    return _nodes.distill(even_rows(logits), teacher, ids, total, weights, temperature, record, None)
 
 
 def top_logits_loss_and_gradient(logits: torch.Tensor, teacher_logits: torch.Tensor,
@@ -149,18 +102,18 @@ def top_logits_loss_and_gradient(logits: torch.Tensor, teacher_logits: torch.Ten
     teacher, ids, total, weights = _checked("top_logits_loss_and_gradient", logits, teacher_logits,
                                             teacher_ids, teacher_total, weights, temperature)
     if out is None:
-        logits = even_rows(logits)[0]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return _launch(logits, teacher, ids, total, weights, temperature, False, grad)[0], grad
+        return _nodes.distill(even_rows(logits), teacher, ids, total, weights, temperature, False,
+                              grad), grad
     if out.shape != logits.shape or out.dtype is not logits.dtype or out.device != logits.device:
         raise ValueError(f"out must be a {logits.dtype} {list(logits.shape)} on {logits.device}")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError("out must not require a gradient")
-    if even_rows(out)[0] is not out:
+    if even_rows(out) is not out:
         raise ValueError("out must have evenly spaced rows and a dense last dimension")
     same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
     if not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
         raise ValueError("out must be the logits or share no memory with them")
-    loss = _launch(even_rows(logits)[0], teacher, ids, total, weights, temperature, False, out)[0]
+    loss = _nodes.distill(even_rows(logits), teacher, ids, total, weights, temperature, False, out)
     torch.autograd.graph.increment_version(out)
     return loss, out

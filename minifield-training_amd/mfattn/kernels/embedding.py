@@ -10,61 +10,8 @@ import math
 
 import torch
 
-from .. import _lib
-from ..ops import _raw_stream, dtype_code, even_rows, launch, refuse_tangents, require_device
-
-
-def _launch(ids, table, scale, padding):
-    v, d = table.shape
-    out = torch.empty((*ids.shape, d), dtype=table.dtype, device=table.device)
-    if ids.numel():
-        launch(table.device, _lib.LIB.mf_embed, ids.data_ptr(), ids.element_size(),
-               table.data_ptr(), even_rows(table)[1], dtype_code(table), ids.numel(), v, d,
-               padding, scale, out.data_ptr(), _raw_stream(table.device.index))
-    return out
-
-
-def _launch_gradient(dout, ids, v, scale, padding):
-    n, d, device = ids.numel(), dout.shape[-1], dout.device
-    if not n:
-        return dout.new_zeros((v, d))
-    dout, step = even_rows(dout)
-    dtable = torch.empty((v, d), dtype=dout.dtype, device=device)
-    ws_bytes = _lib.LIB.mf_embed_bwd_workspace_bytes(n, v, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    launch(device, _lib.LIB.mf_embed_bwd, ids.data_ptr(), ids.element_size(), dout.data_ptr(),
-           step, dtype_code(dout), n, v, d, padding, scale, dtable.data_ptr(), ws.data_ptr(),
-           ws_bytes, _raw_stream(device.index))
-    return dtable
-
-
-class Embed(torch.autograd.Function):
-    """The lookup with a HIP forward and a HIP backward; the gradient reaches the table.  It is
-    linear in what comes in, and the lookup is its transpose: differentiable as often as asked."""
-
-    @staticmethod
-    def forward(ctx, ids, table, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.args = (table.shape[0], scale, padding)
-        return _launch(ids, table, scale, padding)
-
-    @staticmethod
-    def backward(ctx, dout):
-        gradient = EmbedGradient.apply if torch.is_grad_enabled() else _launch_gradient
-        return None, gradient(dout, ctx.saved_tensors[0], *ctx.args), None, None
-
-
-class EmbedGradient(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, dout, ids, v, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.args = (scale, padding)
-        return _launch_gradient(dout, ids, v, scale, padding)
-
-    @staticmethod
-    def backward(ctx, g):
-        lookup = Embed.apply if torch.is_grad_enabled() else _launch
-        return lookup(ctx.saved_tensors[0], even_rows(g)[0], *ctx.args), None, None, None, None
+from .. import _nodes
+from ..ops import dtype_code, even_rows, refuse_tangents, require_device
 
 
 def embed(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
@@ -92,7 +39,5 @@ def embed(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
     require_device(table, ids)
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         ids = ids.to(torch.int64)
-    ids, table = ids.contiguous(), even_rows(table)[0]
-    if table.requires_grad and torch.is_grad_enabled():
-        return Embed.apply(ids, table, scale, padding_id)
-    return _launch(ids, table, scale, padding_id)
+    return _nodes.embed(ids.contiguous(), even_rows(table), scale, padding_id,
+                        table.requires_grad and torch.is_grad_enabled())

@@ -13,58 +13,8 @@ import math
 
 import torch
 
-from .. import _lib
-from ..ops import (_ptr, _raw_stream, dtype_code, even_rows, launch, refuse_second_order,
-                   refuse_tangents, require_device)
-
-
-def _launch(x, weight, bias, eps, center, with_stats):
-    d = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rows = x.numel() // d
-    stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device) if with_stats else None
-    if rows:
-        launch(x.device, _lib.LIB.mf_norm, x.data_ptr(), even_rows(x)[1], weight.data_ptr(),
-               _ptr(bias), dtype_code(x), dtype_code(weight), rows, d, center, eps, y.data_ptr(),
-               _ptr(stats), _raw_stream(x.device.index))
-    return y, stats
-
-
-class Norm(torch.autograd.Function):
-    """A norm with a HIP forward and a HIP backward; gradients reach x, weight and bias."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, center):
-        y, stats = _launch(x, weight, bias, eps, center, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.center = center
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        refuse_second_order("the norm")
-        x, weight, stats = ctx.saved_tensors
-        d, device = x.shape[-1], x.device
-        rows = x.numel() // d
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if not rows:
-            zeros = torch.zeros_like
-            return (zeros(x) if need_x else None, zeros(weight) if need_w else None,
-                    zeros(weight) if need_b else None, None, None)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
-        dw = torch.empty(d, dtype=weight.dtype, device=device) if need_w else None
-        db = torch.empty(d, dtype=weight.dtype, device=device) if need_b else None
-        code = dtype_code(x)
-        ws, ws_bytes = None, 0
-        if need_w or need_b:
-            ws_bytes = _lib.LIB.mf_norm_bwd_workspace_bytes(rows, d, code)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        dy, dy_step = even_rows(dy)
-        launch(device, _lib.LIB.mf_norm_bwd, x.data_ptr(), even_rows(x)[1], weight.data_ptr(),
-               stats.data_ptr(), dy.data_ptr(), dy_step, code, dtype_code(weight), rows, d,
-               ctx.center, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes,
-               _raw_stream(device.index))
-        return dx, dw, db, None, None
+from .. import _nodes
+from ..ops import dtype_code, even_rows, refuse_tangents, require_device
 
 
 def _norm(what, x, weight, bias, eps, center):
@@ -89,12 +39,9 @@ def _norm(what, x, weight, bias, eps, center):
     else:
         require_device(x, weight, bias)
         bias = bias.contiguous()
-    weight = weight.contiguous()
-    x = even_rows(x)[0]
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
-        return Norm.apply(x, weight, bias, eps, center)
-    return _launch(x, weight, bias, eps, center, False)[0]
+    record = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                          or (bias is not None and bias.requires_grad))
+    return _nodes.norm(even_rows(x), weight.contiguous(), bias, eps, center, record)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,

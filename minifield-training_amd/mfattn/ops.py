@@ -16,7 +16,7 @@ import weakref
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
+from . import _lib, _nodes
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -141,32 +141,15 @@ def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x.contiguous(), h * d
 
 
-def even_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``x [..., D]`` and the elements between its rows, copied only where its last
-    dimension is not dense or its rows are not evenly spaced or overlap."""
-    d = x.shape[-1]
-    if x.is_contiguous():
-        return x, d
-    try:
-        rows = x.view(-1, d)
-    except RuntimeError:
-        return x.contiguous(), d
-    step, dense = rows.stride()
-    if rows.shape[0] <= 1:
-        step = d
-    return (x, step) if step >= d and (dense == 1 or d == 1) else (x.contiguous(), d)
+def even_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x [..., D]``, copied only where its last dimension is not dense or its rows are not
+    evenly spaced or overlap."""
+    return x if x.is_contiguous() or _nodes.rows_even(x) else x.contiguous()
 
 
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     if carries_tangent(*tensors):
         raise ValueError(f"{what} has no forward-mode derivative; an operand carries a tangent")
-
-
-def refuse_second_order(what: str) -> None:
-    """A backward pass that runs to be differentiated itself (create_graph=True)."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what} is differentiable once: its backward pass records no graph "
-                           "(create_graph=True)")
 
 
 def _require_lse(lse: torch.Tensor, b: int, hq: int, t: int) -> None:
