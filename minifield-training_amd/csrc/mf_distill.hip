@@ -42,7 +42,7 @@ struct DistillArgs {
   long long stride, grad_stride;
   int vocabulary, top;
   float scale;  // log2(e) / T
-  double temperature;
+  double temperature, per;  // T and 1 / T
   bool teacher_f32, ids64;
 };
 
@@ -52,17 +52,6 @@ __device__ __forceinline__ int teacher_id(const DistillArgs& a, size_t at) {
   const long long id = a.ids64 ? reinterpret_cast<const long long*>(a.ids)[at]
                                : (long long)reinterpret_cast<const int32_t*>(a.ids)[at];
   return id >= 0 && id < a.vocabulary ? (int)id : -1;
-}
-
-__device__ __forceinline__ double sum64d(double x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-  return x;
-}
-__device__ __forceinline__ double max64d(double x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x = fmax(x, __shfl_xor(x, m));
-  return x;
 }
 
 // exp((z - top) / T).  The difference first: a product of the type's lowest value
@@ -78,9 +67,10 @@ __device__ __forceinline__ void store_named(T* grad, int id, float z, float mass
   grad[id] = (T)fmaf(weight_of(z, top, scale), factor, -w * mass);
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ Vec<T> load_vec(const T* p) {
-  return (Vec<T>)__builtin_nontemporal_load(reinterpret_cast<const typename RowVec<T>::U*>(p));
+  const auto* u = reinterpret_cast<const typename RowVec<T>::U*>(p);
+  return (Vec<T>)(STREAM ? __builtin_nontemporal_load(u) : *u);
 }
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[kVec<T>]) {
@@ -92,59 +82,53 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[kVec<T>]) {
 
 // A row's entries in LDS, and what wave 0 makes of them in 64 bits.
 struct Teacher {
-  int id[kDistillMostTop];  // -1: not there
-  float z[kDistillMostTop], mass[kDistillMostTop];
-  float whole, rest;        // P + r and r
-  int none, bad;            // no entry at all; one that is NaN or +infinity
+  int id[kDistillMostTop];  // -1: not there, nor behind the last up to a multiple of 8
+  float z[kDistillMostTop];
+  double mass[kDistillMostTop];
+  float whole, rest;  // P + r and r
+  int none, bad;      // no entry at all; one that is NaN or +infinity
 };
 
-// Wave 0, before the row's own loads are waited for: masses, P, and the loss but for
-// the logarithm of the student's sum, sum p_k (log p_k - (z_k - z_ref) / T).
+// Wave 0, while the row is on its way: masses, P, and the part of the loss that knows the
+// teacher alone, sum p_k log p_k.
 __device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, int lane,
-                                              Teacher& t, double& P, double& kl, float& z_ref) {
+                                              Teacher& t, double& P, double& kl) {
   const int K = a.top;
-  const double per = 1.0 / a.temperature, inf = __builtin_huge_val();
   const bool tail = a.total != nullptr;
   bool there = false, bad = false;
   auto entry = [&](int k) {
-    if (t.id[k] < 0) return -inf;
+    if (k >= K || t.id[k] < 0) return kNegInf;
     const float u = element(a.teacher, a.teacher_f32, row * K + k);
     bad |= !(u < kPosInf);
     there |= u != kNegInf;
-    return (double)u * per;
+    return u;
   };
-  double most = -inf;
-  float ref = kNegInf;
-  for (int k = lane; k < K; k += 64) {
-    most = fmax(most, entry(k));
-    if (t.id[k] >= 0) ref = fmaxf(ref, t.z[k]);
-  }
-  ref = max64(ref);
-  z_ref = ref > kNegInf && ref < kPosInf ? ref : 0.f;
-  double total;
+  const float first = entry(lane);
+  double shift, total;  // what the entries are taken beside, and the logarithm of their sum there
   if (tail) {
+    shift = 0;
     total = a.total[row];
-    bad |= !(total < inf);
+    bad |= !(a.total[row] < kPosInf);
   } else {
-    most = max64d(most);
-    double s = 0;
-    for (int k = lane; k < K; k += 64) s += exp(entry(k) - most);
+    float most = first;
+    for (int k = lane + 64; k < K; k += 64) most = fmaxf(most, entry(k));
+    most = max64(most);
     // (entries that are all -infinity have no mass, like none at all)
-    total = most == -inf ? 0.0 : most + log(sum64d(s));
+    shift = most == kNegInf ? 0.0 : (double)most;
+    double s = exp((first - shift) * a.per);
+    for (int k = lane + 64; k < K; k += 64) s += exp((entry(k) - shift) * a.per);
+    s = sum64(s);
+    total = s > 0 ? log(s) : 0.0;
   }
   P = kl = 0;
   for (int k = lane; k < K; k += 64) {
-    double mass = 0;
-    if (t.id[k] >= 0) {
-      const double logp = entry(k) - total;
-      mass = exp(logp);
-      if (mass > 0) kl += mass * (logp - ((double)t.z[k] - z_ref) * per);
-    }
-    t.mass[k] = (float)mass;
+    const double logp = ((k == lane ? first : entry(k)) - shift) * a.per - total;
+    const double mass = exp(logp);
+    if (mass > 0) kl += mass * logp;
+    t.mass[k] = mass;
     P += mass;
   }
-  P = sum64d(P);
-  kl = sum64d(kl);
+  P = sum64(P);
   // without an entry there is no loss and no gradient, whatever the row holds; otherwise
   // an entry or a total that is NaN or +infinity makes the row NaN
   const bool none = !tail && !__any(there);
@@ -188,21 +172,16 @@ void distill_kernel(DistillArgs a) {
     return;
   }
   const bool tail = a.total != nullptr;
-  // wave 0 asks for the entries and their logits in front of the row: loads return in order
-  if (wave == 0)
-    for (int k = lane; k < K; k += 64) {
-      const int id = teacher_id(a, row * K + k);
-      t.id[k] = id;
-      t.z[k] = id >= 0 ? (float)z[id] : 0.f;
-    }
   constexpr int STEP = U * kDistillThreads;
   Vec<T> raw[U];
-  // (loads have no condition: vectors beyond the row are its last)
+  // (loads have no condition: vectors beyond the row are its last.  The loss alone leaves
+  // the logits in the last-level cache for the backward pass: read as a stream, its 4096 x
+  // 65536 bf16 take 184 us, so 172)
   auto fetch = [&](Vec<T> (&to)[U], int first) {
     if (vectors == 0) return;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      to[u] = load_vec<T>(z + (size_t)min(first + u * kDistillThreads + tid, vectors - 1) * N);
+      to[u] = load_vec<T, GRAD>(z + (size_t)min(first + u * kDistillThreads + tid, vectors - 1) * N);
   };
   auto blank = [&](int first) {
     if (first + STEP <= vectors) return;
@@ -215,8 +194,23 @@ void distill_kernel(DistillArgs a) {
                                                 in ? x[3] : low});
     }
   };
+  // wave 0 asks for the entries in front of the row, and for their logits behind it: loads
+  // return in order, and what is needed first comes first
+  const int K8 = (K + 7) & ~7;
+  int id0 = -1;
+  if (wave == 0 && lane < K) id0 = teacher_id(a, row * K + lane);
   const float extra = odd < V ? (float)z[odd] : kNegInf;
   fetch(raw, 0);
+  float z0 = 0.f;
+  if (wave == 0) {
+    if (id0 >= 0) z0 = (float)z[id0];
+    if (lane < K8) t.id[lane] = id0;
+    for (int k = lane + 64; k < K8; k += 64) {
+      const int id = k < K ? teacher_id(a, row * K + k) : -1;
+      t.id[k] = id;
+      t.z[k] = id >= 0 ? (float)z[id] : 0.f;
+    }
+  }
   if (tail)
     for (int i = tid; i < (V + 31) / 32; i += kDistillThreads) named[i] = 0;
   // A vector of the row as it was loaded.  Each pass widens its values anew, one vector at
@@ -229,7 +223,6 @@ void distill_kernel(DistillArgs a) {
     return __builtin_bit_cast(Vec<T>, x);
   };
   double P = 0, kl = 0;
-  float z_ref = 0.f;
   if (tail) {
     __syncthreads();
     for (int k = tid; k < K; k += kDistillThreads)
@@ -237,7 +230,10 @@ void distill_kernel(DistillArgs a) {
     __syncthreads();
   }
   // (the other waves go on with the row; they meet wave 0 at its largest logit)
-  if (wave == 0) weigh_teacher(a, row, lane, t, P, kl, z_ref);
+  if (wave == 0) {
+    weigh_teacher(a, row, lane, t, P, kl);
+    if (lane < K) t.z[lane] = z0;
+  }
   // sums beside `top`, of what is not named and what is
   float top = kNegInf, rest = 0.f, held = 0.f;
   auto largest = [&] {
@@ -352,20 +348,29 @@ void distill_kernel(DistillArgs a) {
   }
   // an element that several entries name has the mass of all of them
   auto mass_of = [&](int k) {
-    float m = 0.f;
-    for (int j = 0; j < K; ++j) m += t.id[j] == t.id[k] ? t.mass[j] : 0.f;
-    return m;
+    const int id = t.id[k];
+    double m = 0;
+    for (int j = 0; j < K8; j += 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t.id[j + i] == id) m += t.mass[j + i];
+    }
+    return (float)m;
   };
   if (GRAD && !none) {
+    // (the first entries' masses while the stores are on their way)
+    const float mass0 = tid < K && t.id[tid] >= 0 ? mass_of(tid) : 0.f;
     // the dense stores have arrived before a named element is written anew
     drain_memory();
     __syncthreads();
     for (int k = tid; k < K; k += kDistillThreads)
-      if (t.id[k] >= 0) store_named(grad, t.id[k], t.z[k], mass_of(k), base, a.scale, one, wt);
+      if (t.id[k] >= 0)
+        store_named(grad, t.id[k], t.z[k], k == tid ? mass0 : mass_of(k), base, a.scale, one, wt);
   }
   if (!GRAD && a.stats) {
     float* st = a.stats + row * (kDistillStats + K);
-    for (int k = tid; k < K; k += kDistillThreads) st[kDistillStats + k] = mass_of(k);
+    for (int k = tid; k < K; k += kDistillThreads)
+      st[kDistillStats + k] = t.id[k] >= 0 ? mass_of(k) : 0.f;
     if (tid == 0) {
       st[0] = base;
       st[1] = one;
@@ -373,11 +378,19 @@ void distill_kernel(DistillArgs a) {
       st[3] = wt;
     }
   }
-  if (tid == 0) {
-    const double T_ = a.temperature, r = tail ? fmax(0.0, 1.0 - P) : 0.0, all = (double)rest + held;
-    kl += P * (log(all) + ((double)base - z_ref) / T_);
-    if (r > 0) kl += r * (log(r) - log((double)rest / all));
-    a.loss[row] = none ? 0.f : bad ? __builtin_nanf("") : (float)(w * T_ * T_ * kl);
+  if (wave == 0) {
+    // the student's part of the loss: sum p_k (z_k - base) / T, and its sums' logarithms
+    for (int k = lane; k < K; k += 64)
+      if (t.mass[k] > 0) kl -= t.mass[k] * (((double)t.z[k] - base) * a.per);
+    kl = sum64(kl);
+    if (lane == 0) {
+      const double r = tail ? fmax(0.0, 1.0 - P) : 0.0, all = (double)rest + held;
+      kl += P * log(all);
+      if (r > 0) kl += r * (log(r) - log((double)rest / all));
+      a.loss[row] = none ? 0.f
+                    : bad ? __builtin_nanf("")
+                          : (float)(w * a.temperature * a.temperature * kl);
+    }
   }
 }
 
@@ -386,7 +399,8 @@ template <typename T, int U>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int parts) {
   constexpr int N = kVec<T>, SPAN = U * 256;
   const int tid = threadIdx.x;
-  const size_t row = blockIdx.x / parts;
+  // (the last rows first: the forward pass has just read them)
+  const size_t row = (gridDim.x - 1 - blockIdx.x) / parts;
   const int part = (int)(blockIdx.x % parts), first = part * SPAN;
   const int V = a.vocabulary, K = a.top;
   // the last part has the odd values behind the row's whole vectors
@@ -413,7 +427,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int par
   if (vectors > 0) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      raw[u] = load_vec<T>(z + (size_t)min(first + u * 256 + tid, vectors - 1) * N);
+      raw[u] = load_vec<T, true>(z + (size_t)min(first + u * 256 + tid, vectors - 1) * N);
   }
   const float base = st[0], one = st[1] * up, dense = st[2] * up, wt = st[3] * up;
 #pragma unroll
@@ -475,7 +489,7 @@ hipError_t launch_distill(const void* logits, long long stride, const void* teac
                           long long grad_stride, hipStream_t stream) {
   const DistillArgs a{logits, teacher, ids, total, weights, nullptr, grad, loss, stats, stride,
                       grad_stride, vocabulary, top, (float)(1.4426950408889634 / temperature),
-                      temperature, teacher_f32, ids64};
+                      temperature, 1.0 / temperature, teacher_f32, ids64};
   return f32 ? launch_distill_t<float>(a, rows, stream) : launch_distill_t<bf16>(a, rows, stream);
 }
 
@@ -485,7 +499,8 @@ hipError_t launch_distill_bwd(const void* logits, long long stride, const void* 
                               void* grad, long long grad_stride, hipStream_t stream) {
   const DistillArgs a{logits, nullptr, ids, nullptr, weights, upstream, grad, nullptr,
                       const_cast<float*>(stats), stride, grad_stride, vocabulary, top,
-                      (float)(1.4426950408889634 / temperature), temperature, false, ids64};
+                      (float)(1.4426950408889634 / temperature), temperature,
+                      1.0 / temperature, false, ids64};
   return f32 ? launch_distill_bwd_t<float>(a, rows, stream)
              : launch_distill_bwd_t<bf16>(a, rows, stream);
 }

@@ -46,7 +46,8 @@ __device__ __forceinline__ uint32_t row_of(const EmbedArgs& a, long long id) {
   return id >= 0 && id < a.vocabulary && id != a.padding ? (uint32_t)id : (uint32_t)a.vocabulary;
 }
 
-// L lanes a token.
+// L lanes a token.  (Four tokens a group of lanes, for more loads in flight, measured 21 us
+// against 21 at 32768 x 1024 bf16 and 3.3 against 2.7 at 64.)
 template <typename T, int L, Edge E>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs a) {
   constexpr int N = kVec<T>, C = 2;

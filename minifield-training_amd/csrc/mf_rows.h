@@ -126,6 +126,34 @@ __device__ __forceinline__ float sum16(float x) {
 }
 __device__ __forceinline__ float sum64(float x) { return halves_sum(rows16_sum(sum16(x))); }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Sum over the wave in 64 bits, in all lanes.
+__device__ __forceinline__ double sum64(double x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  x += dpp<0x140>(x);
+#pragma unroll
+  for (int rows = 1; rows <= 2; ++rows) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+    const auto l = rows == 1 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false)
+                             : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = rows == 1 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false)
+                             : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    x = __builtin_bit_cast(double, (uint64_t)h[0] << 32 | l[0]) +
+        __builtin_bit_cast(double, (uint64_t)h[1] << 32 | l[1]);
+  }
+  return x;
+}
+
 __device__ __forceinline__ float max64(float x) {
   x = fmaxf(x, dpp<0xB1>(x));
   x = fmaxf(x, dpp<0x4E>(x));

@@ -53,8 +53,8 @@ def _check(z, t, ids, more, upstream=None):
     return loss, grad, g
 
 
-# less than a vector, one workgroup's, two and more vectors a thread, beyond the registers
-VOCABULARIES = [1, 5, 8, 100, 1023, 8192, 8193, 20000, 65536, 65541, 131072, 131080, 140001]
+# less than a vector, one workgroup's, two and more vectors a thread, beyond the registers, the most
+VOCABULARIES = [1, 5, 8, 100, 1023, 8192, 8193, 20000, 65536, 65541, 131072, 131080, 140001, 393216]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
