@@ -933,9 +933,9 @@ int check_distill(int dtype, int id_bytes, int rows, int vocabulary, int top, do
                 "at most %d rows, %d logits a row, %lld in all and %d entries (got %d of %d, %d)",
                 mf::kDistillMostRows, mf::kDistillMostVocabulary, mf::kDistillMostLogits,
                 mf::kDistillMostTop, rows, vocabulary, top);
-  if (!(std::isfinite(temperature) && temperature > 0))
-    return fail(MF_ERR_INVALID_ARGUMENT, "temperature must be finite and positive (got %g)",
-                temperature);
+  if (!(temperature >= mf::kDistillLeastTemperature && temperature <= mf::kDistillMostTemperature))
+    return fail(MF_ERR_INVALID_ARGUMENT, "temperature must be in [%g, %g] (got %g)",
+                mf::kDistillLeastTemperature, mf::kDistillMostTemperature, temperature);
   return MF_OK;
 }
 

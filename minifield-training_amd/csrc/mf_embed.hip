@@ -508,14 +508,15 @@ hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long 
   } else {
     s.blocks = (l.tiles + 3) / 4;
     s.zero_block = 64 << 10;
-    const size_t share = (bytes / (2 * l.passes) / s.zero_block + 1) * s.zero_block;
+    // placing takes about three times what counting does: so are their shares
+    const size_t share = (bytes / (4 * l.passes) / s.zero_block + 1) * s.zero_block;
     for (int step = 0; step < 2 * l.passes; ++step) {
       const int pass = step / 2;
       s.shift = pass * l.bits;
       s.from = pass ? lists[(pass + 1) & 1] : nullptr;
       s.to = sorted = lists[pass & 1];
-      s.zero_first = std::min(bytes, step * share);
-      s.zero_last = std::min(bytes, (step + 1) * share);
+      s.zero_first = s.zero_last;
+      s.zero_last = std::min(bytes, (pass * 4 + (step % 2 ? 4 : 1)) * share);
       const unsigned zero =
           (unsigned)((s.zero_last - s.zero_first + s.zero_block - 1) / s.zero_block);
       const dim3 grid((unsigned)s.blocks + zero);

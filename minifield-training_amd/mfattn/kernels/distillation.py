@@ -15,8 +15,6 @@ they leave of one, and ``s`` what the student has on the ids without an entry.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .. import _nodes
@@ -44,8 +42,8 @@ def _checked(what, logits, teacher, ids, total, weights, temperature):
         if not t.is_floating_point():
             raise ValueError(f"{name} must be floating, got {t.dtype}")
         tensors.append(t)
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be finite and positive (got {temperature})")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6] (got {temperature})")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (teacher, total, weights)):
         raise ValueError(f"{what} has a gradient for the logits alone; detach the teacher and "
@@ -72,8 +70,8 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     say) is not there; entries with the same id add up.  ``teacher_total [...]``
     counts the teacher's other tokens in (see the module).  ``weights [...]`` multiplies
     the losses; a row of weight zero has loss and gradient zero whatever its logits
-    hold, and so has a row without entries (where no total is given).  V up to 393216, K up to 1024.  Differentiable in
-    the logits, once; :func:`top_logits_loss_and_gradient` needs half the memory
+    hold, and so has a row without entries (where no total is given).  V up to
+    393216, K up to 1024, temperatures in [1e-6, 1e6].  Differentiable in the logits, once; :func:`top_logits_loss_and_gradient` needs half the memory
     and two passes over the logits instead of three.
     """
     teacher, ids, total, weights = _checked("top_logits_loss", logits, teacher_logits, teacher_ids,
