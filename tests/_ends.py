@@ -122,6 +122,9 @@ def distill(z, teacher, ids, temperature=1.0, total=None, weights=None, upstream
         off = rest / s if s > 0 else 0.0
         grad[n] = w * (q * mass - named - torch.where(beyond, q * off, 0.0))
         own = (3 * arg + 8) * E
-        grad_e[n] = abs(w) * (q * mass * (own + sums) + named * 6 * E * max(1, len(at) ** 0.5)
+        # an exponential below 2^-126 is zero; beside a logit of the row the sum of all is 1 at
+        # least, so its factor in the gradient is w (mass + off) at most
+        grad_e[n] += abs(w) * 2.0 ** -126 * (mass + off)
+        grad_e[n] += abs(w) * (q * mass * (own + sums) + named * 6 * E * max(1, len(at) ** 0.5)
                               + torch.where(beyond, q * off * (own + rest_sums), 0.0))
     return loss, loss_e, grad, grad_e

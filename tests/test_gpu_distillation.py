@@ -310,3 +310,31 @@ def test_graphs_of_the_backward_pass_are_refused(device):
     loss = distillation.top_logits_loss(z.requires_grad_(), t, ids, **more)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(loss.sum(), z, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [700, 9000, 65536, 140001])
+@pytest.mark.parametrize("total", [False, True], ids=["softmax", "total"])
+def test_largest_logits_far_behind_the_first(v, dtype, total, device):
+    """Exponentials are taken beside a logit near the front: what lies hundreds of units above or
+    below it further on, in one place, in many or nowhere, counts as the definition says."""
+    z, t, ids, more = _operands(dtype, 10, v, 5, device, total=total)
+    low = torch.finfo(dtype).min
+    half = v // 2
+    z[0, half:] += 300            # exp overflows beside the first
+    z[1, :half] += 300            # and vanishes
+    z[2, -1] = 500
+    z[3, ::997] += 200
+    z[4, :half] = -math.inf
+    z[5, :half] = low
+    z[6] -= 1000
+    z[7] = torch.linspace(-400, 400, v, device=device).to(dtype)
+    z[8] = torch.linspace(400, -400, v, device=device).to(dtype)
+    z[9, :-1] = -math.inf
+    for r in range(10):           # entries that the student does not rule out
+        z[r, ids[r]] = z[r][z[r].float().argmax()].clone()
+    _check(z, t, ids, more)
+    more["temperature"] = 0.1
+    if total:
+        more["teacher_total"] = torch.logsumexp(t.float() / 0.1, 1) + 0.2
+    _check(z, t, ids, more)

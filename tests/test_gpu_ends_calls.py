@@ -1,0 +1,170 @@
+"""Ways to call the norms, the embedding and the distillation loss that their documentation allows:
+in place through the C ABI, from several threads, under checkpointing, past their limits."""
+
+import threading
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from mfattn import _lib
+from mfattn.kernels import distillation, embedding, normalization
+
+pytestmark = pytest.mark.gpu
+
+L = _lib.LIB
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+@pytest.mark.parametrize("center", [1, 0], ids=["layer", "rms"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [5, 64, 100, 771, 1024, 2047, 4096, 5001, 16384])
+def test_norms_in_place(d, dtype, center, device):
+    rows, code = 67, _lib.DTYPE_BF16 if dtype is torch.bfloat16 else _lib.DTYPE_F32
+    g = torch.Generator(device=device).manual_seed(d)
+    x, dy = (torch.randn(rows, d, generator=g, device=device).to(dtype) for _ in range(2))
+    w = torch.randn(d, generator=g, device=device).to(dtype)
+    y, dx, stats = torch.empty_like(x), torch.empty_like(x), torch.empty(rows, 2, device=device)
+    dw, ws = torch.empty_like(w), torch.empty(L.mf_norm_bwd_workspace_bytes(rows, d, code),
+                                              dtype=torch.uint8, device=device)
+
+    def forward(x, y):
+        _lib.check(L.mf_norm(x.data_ptr(), d, w.data_ptr(), None, code, code, rows, d, center, 1e-5,
+                             y.data_ptr(), stats.data_ptr(), _stream()))
+
+    def backward(dy, dx):
+        _lib.check(L.mf_norm_bwd(x.data_ptr(), d, w.data_ptr(), stats.data_ptr(), dy.data_ptr(), d,
+                                 code, code, rows, d, center, dx.data_ptr(), dw.data_ptr(), None,
+                                 ws.data_ptr(), ws.numel(), _stream()))
+
+    forward(x, y)
+    backward(dy, dx)
+    first = dw.clone()
+    backward(dy, dy)
+    assert torch.equal(dy, dx) and torch.equal(first, dw)
+    forward(x, x)
+    assert torch.equal(x, y)
+
+
+def test_limits_are_errors_with_the_librarys_message(device):
+    f = torch.zeros
+    for call, text in (
+            (lambda: normalization.layer_norm(f(2, 16385, device=device), f(16385, device=device)),
+             "at most"),
+            (lambda: embedding.embed(f(3, dtype=torch.int64, device=device),
+                                     f(2, 65537, device=device)), "at most"),
+            (lambda: embedding.embed(f(3, dtype=torch.int64, device=device),
+                                     f(2, 8, device=device), scale=1e39), "scale must be finite"),
+            (lambda: distillation.top_logits_loss(f(1, 2000, device=device), f(1, 1025, device=device),
+                                                  f(1, 1025, dtype=torch.int32, device=device)),
+             "at most"),
+            (lambda: distillation.top_logits_loss_and_gradient(
+                f(1, 393217, device=device), f(1, 5, device=device),
+                f(1, 5, dtype=torch.int32, device=device)), "at most")):
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(_lib.MfValueError, match=text) as e:
+                call()
+            assert e.value.code in (_lib.ERR_SHAPE, _lib.ERR_INVALID_ARGUMENT)
+    with pytest.raises(_lib.MfValueError, match="at most"):  # and where a graph is recorded
+        normalization.rms_norm(f(1, 16385, device=device, requires_grad=True), f(16385, device=device))
+    # the same thread goes on
+    assert normalization.rms_norm(torch.ones(1, 4, device=device), torch.ones(4, device=device)).sum() > 3.9
+
+
+def test_parameters_at_odd_offsets(device):
+    flat = torch.randn(4000, device=device).bfloat16()
+    x = torch.randn(9, 1001, device=device).bfloat16()
+    w, b = flat[1:1002], flat[1501:2502]
+    assert torch.equal(normalization.layer_norm(x, w, b), normalization.layer_norm(x, w.clone(), b.clone()))
+    wide = torch.randn(9, 1030, device=device).bfloat16()
+    for params in (flat, flat.float()):
+        got = normalization.rms_norm(wide[:, 7:1008], params[3:1004])
+        assert torch.equal(got, normalization.rms_norm(wide[:, 7:1008].clone(), params[3:1004].clone()))
+
+
+def _losses(device, seed):
+    g = torch.Generator(device=device).manual_seed(seed)
+    table = torch.randn(700, 256, generator=g, device=device).requires_grad_()
+    w = torch.randn(256, generator=g, device=device).requires_grad_()
+    ids = torch.randint(0, 700, (90,), generator=g, device=device)
+    tids = torch.rand(90, 700, generator=g, device=device).argsort(1)[:, :7].contiguous()
+    t = torch.randn(90, 7, generator=g, device=device)
+
+    def head(x, w, table):
+        return distillation.top_logits_loss(normalization.rms_norm(x, w) @ table.t(), t, tids,
+                                            temperature=3.0)
+
+    return table, w, ids, head
+
+
+def test_checkpointed_layers(device):
+    table, w, ids, head = _losses(device, 1)
+    x = embedding.embed(ids, table, scale=2.0)
+    want = torch.autograd.grad(head(x, w, table).sum(), (table, w))
+    x = embedding.embed(ids, table, scale=2.0)
+    loss = checkpoint(head, x, w, table, use_reentrant=False)
+    got = torch.autograd.grad(loss.sum(), (table, w))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_several_threads_at_once(device):
+    want, got = {}, {}
+
+    def work(k, to, rounds):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(rounds):
+                table, w, ids, head = _losses(device, k)
+                loss = head(embedding.embed(ids, table), w, table)
+                to[k] = (loss.detach(), *torch.autograd.grad(loss.sum(), (table, w)))
+            torch.cuda.current_stream().synchronize()
+
+    for k in range(4):
+        work(k, want, 1)
+    threads = [threading.Thread(target=work, args=(k, got, 12)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(4):
+        for a, b in zip(got[k], want[k]):
+            assert torch.equal(a, b)
+
+
+def test_the_operands_may_not_change_before_the_backward_pass(device):
+    x = torch.randn(4, 64, device=device)
+    w = torch.ones(64, device=device, requires_grad=True)
+    y = normalization.rms_norm(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z = torch.randn(4, 64, device=device, requires_grad=True)
+    held = z * 1
+    t, tids = torch.zeros(4, 2, device=device), torch.tensor([[1, 2]] * 4, device=device)
+    loss = distillation.top_logits_loss(held, t, tids)
+    with torch.no_grad():
+        distillation.top_logits_loss_and_gradient(held, t, tids, out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
+def test_a_graph_walked_twice(device):
+    table, w, ids, head = _losses(device, 2)
+    loss = head(embedding.embed(ids, table), w, table).sum()
+    first = torch.autograd.grad(loss, (table, w), retain_graph=True)
+    second = torch.autograd.grad(loss, (table, w))
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+def test_tensors_on_the_host_beside_device_tensors(device):
+    x = torch.ones(2, 8, device=device)
+    with pytest.raises(ValueError, match="GPU only"):
+        normalization.rms_norm(x, torch.ones(8))
+    with pytest.raises(ValueError, match="GPU only"):
+        embedding.embed(torch.zeros(3, dtype=torch.int64), x)
+    with pytest.raises(ValueError, match="GPU only"):
+        distillation.top_logits_loss(x, torch.ones(2, 3), torch.zeros(2, 3, dtype=torch.int64, device=device))
