@@ -982,7 +982,7 @@ int mf_norm_bwd(const void* x, long long x_stride, const void* weight, const flo
   if (int rc = check_rows("dy", dy_stride, dim)) return rc;
   if (dweight || dbias) {
     const size_t need = mf_norm_bwd_workspace_bytes(rows, dim, dtype);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
       return fail(MF_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed",
                   workspace ? workspace_bytes : 0, need);
   }

@@ -11,12 +11,17 @@
 // All in fp32, each output rounded once.  (The prologue's per-head norm rounds the
 // normalised value before the gain, as the reference's declared types do.)
 //
-// Bound: memory.  A row belongs to 16 lanes, a wave or a workgroup of 512, by its
-// width, each lane holding up to kMostVectors vectors of 16 bytes of it.  The
-// backward's workgroups take rows in a grid-wide stride and keep the sums of dw and
-// db for their own columns in registers; what each workgroup has at the end is
-// written once and added by a second launch in workgroup order: no atomics, the
-// same bits every time.
+// Bound: memory.  A row belongs to 16, 64, 256 or 512 lanes by its width, each lane holding
+// up to kNormMostVectors vectors of 16 bytes of it.  The backward's workgroups take rows in
+// a grid-wide stride and keep the sums of dw and db for their own columns in registers, with
+// the next two rows in flight; what each workgroup has at the end is written once and added
+// by a second launch in workgroup order.  Of few rows the sums are taken by workgroups of
+// the same launch, which read the rows again by columns.  No atomics: the same bits every
+// time.
+//
+// Measured, 32768 x 1024 bf16 (64 MiB a tensor, what the last pass left in the cache
+// included): forward 30 us (4.5 TB/s read and written), backward 36 (5.6), its second launch
+// 4.0; 8192 x 4096 bf16: 28, 36 and 4.1; 999 x 771 fp32: 3.8 and 10.5 (one launch).
 #include <algorithm>
 
 #include "mf_norm.h"
@@ -132,12 +137,82 @@ struct NormBwdArgs {
   const void* weight;
   const float2* stats;
   void* dx;         // or null
-  float* partials;  // [gridDim.x][2][dim], or null
+  float* partials;  // [row_blocks][2][dim], or null
+  void* dweight;    // of a launch that sums over the rows itself, or null
+  void* dbias;
   long long x_stride, dy_stride;
-  int rows, dim;
+  int rows, dim, row_blocks;
   float inv_dim;
   bool center, param_f32;
 };
+
+__device__ __forceinline__ void store_param(void* p, bool f32, int i, float x) {
+  if (f32)
+    reinterpret_cast<float*>(p)[i] = x;
+  else
+    reinterpret_cast<bf16*>(p)[i] = (bf16)x;
+}
+
+// dweight and dbias of 8 vectors of columns, by a workgroup that goes through all rows: 64
+// groups of 8 lanes with every 64th row each.  `lds`: [8][8 N][2].
+constexpr int kColumnLanes = 8;
+
+template <typename T, Edge E>
+__device__ __forceinline__ void sum_columns(const NormBwdArgs& a, int block, float* lds) {
+  constexpr int N = kVec<T>, L = kColumnLanes, G = 512 / L, AHEAD = 4;
+  const int lane = threadIdx.x % L, group = threadIdx.x / L, wave = threadIdx.x >> 6;
+  const bool first = (threadIdx.x & 63) < L;  // of the wave's groups
+  const RowPlace<T, E> at(block * L + lane, a.dim);
+  float dw[N] = {}, db[N] = {};
+  for (int r0 = group; r0 < a.rows; r0 += G * AHEAD) {
+    Vec<T> x[AHEAD], dy[AHEAD];
+    float2 st[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int r = min(r0 + G * j, a.rows - 1);
+      st[j] = a.stats[r];
+      x[j] = at.load(reinterpret_cast<const T*>(a.x) + (size_t)r * a.x_stride);
+      dy[j] = at.load(reinterpret_cast<const T*>(a.dy) + (size_t)r * a.dy_stride);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (r0 + G * j >= a.rows) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = (float)dy[j][i];
+        dw[i] = fmaf(d, ((float)x[j][i] - st[j].x) * st[j].y, dw[i]);
+        db[i] += d;
+      }
+    }
+  }
+  float* mine = lds + (wave * L + lane) * N * 2;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // the wave's groups: lanes 8, 16 and 32 apart
+    dw[i] += dpp<0x128>(dw[i]);
+    db[i] += dpp<0x128>(db[i]);
+    dw[i] = halves_sum(rows16_sum(dw[i]));
+    db[i] = halves_sum(rows16_sum(db[i]));
+    if (first) {
+      mine[2 * i] = dw[i];
+      mine[2 * i + 1] = db[i];
+    }
+  }
+  __syncthreads();
+  if (wave > 0 || !first || !at.any()) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float w = 0.f, b = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      w += lds[((k * L + lane) * N + i) * 2];
+      b += lds[((k * L + lane) * N + i) * 2 + 1];
+    }
+    if (!at.mine(i)) continue;
+    if (a.dweight) store_param(a.dweight, a.param_f32, at.at + i, w);
+    if (a.dbias) store_param(a.dbias, a.param_f32, at.at + i, b);
+  }
+}
 
 // Waves a SIMD that the registers are held to: two workgroups a CU, one for the rows of most
 // registers a lane.
@@ -150,8 +225,9 @@ void norm_bwd_kernel(NormBwdArgs a) {
   constexpr int N = kVec<T>, R = 512 / L, W = L > 64 ? L / 64 : 1;
   // rows in flight beside the one that is computed, as the registers have room
   constexpr int AHEAD = C * N <= 16 ? 2 : 0, SLOTS = AHEAD ? AHEAD : 1;
-  extern __shared__ float lds[];  // the workgroup's sums [2][dim]
+  extern __shared__ float lds[];  // the workgroup's sums, or sum_columns'
   __shared__ float part[2][2][8];
+  if ((int)blockIdx.x >= a.row_blocks) return sum_columns<T, E>(a, blockIdx.x - a.row_blocks, lds);
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
   RowPlace<T, E> at[C];
 #pragma unroll
@@ -172,7 +248,7 @@ void norm_bwd_kernel(NormBwdArgs a) {
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < N; ++i) dw[c][i] = db[c][i] = 0.f;
-  const int step = gridDim.x * R;
+  const int step = a.row_blocks * R;
   Vec<T> xr[SLOTS][C], gr[SLOTS][C];
   float2 st[SLOTS];
   auto fetch = [&](int n, int first) {  // (a row beyond the last is read again, not used)
@@ -279,24 +355,56 @@ void norm_bwd_kernel(NormBwdArgs a) {
       }
   }
   float* out = a.partials + (size_t)blockIdx.x * 2 * a.dim;
+  auto store_sums = [&](float* to, const RowPlace<T, E>& at, const float (&x)[N]) {
+    if (!at.any()) return;
+    if constexpr (E == EDGE_WHOLE) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        *reinterpret_cast<RowVec<float>::U*>(to + at.at + i) =
+            RowVec<float>::U{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at.mine(i)) to[at.at + i] = x[i];
+    }
+  };
   constexpr int G = R > 8 ? 8 : R;  // groups of lanes with sums of their own
-  float* to = G > 1 ? lds : out;
+  if constexpr (G == 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      store_sums(out, at[c], dw[c]);
+      store_sums(out + a.dim, at[c], db[c]);
+    }
+    return;
+  }
+  // (a value's lanes side by side: by columns, lanes would be N values apart and meet in a
+  // bank eight at a time)
+  auto slot = [&](int c, int i, int lane) { return (c * N + i) * L + lane; };
+  constexpr int HALF = C * N * L;
   for (int g = 0; g < G; ++g) {
     if ((int)(L == 16 ? threadIdx.x >> 6 : group) == g && (L > 16 || (threadIdx.x & 63) < 16)) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          if (!at[c].any() || !at[c].mine(i)) continue;
-          const int col = at[c].at + i;
-          to[col] = (g ? lds[col] : 0.f) + dw[c][i];
-          to[a.dim + col] = (g ? lds[a.dim + col] : 0.f) + db[c][i];
+          const int k = slot(c, i, lane);
+          lds[k] = (g ? lds[k] : 0.f) + dw[c][i];
+          lds[HALF + k] = (g ? lds[HALF + k] : 0.f) + db[c][i];
         }
     }
-    if (G > 1) __syncthreads();
+    __syncthreads();
   }
-  if (G > 1)
-    for (int i = threadIdx.x; i < 2 * a.dim; i += 512) out[i] = lds[i];
+  for (int v = threadIdx.x; v < C * L; v += 512) {
+    const RowPlace<T, E> place(v, a.dim);
+    float w[N], b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i] = lds[slot(v / L, i, v % L)];
+      b[i] = lds[HALF + slot(v / L, i, v % L)];
+    }
+    store_sums(out, place, w);
+    store_sums(out + a.dim, place, b);
+  }
 }
 
 // dweight and dbias from the workgroups' sums: 64 columns a workgroup, its 16
@@ -320,11 +428,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* partials
   for (int i = 1; i < 16; ++i) s += sums[i][lane];
   void* out = col < dim ? dweight : dbias;
   const int at = col < dim ? col : col - dim;
-  if (!out) return;
-  if (f32)
-    reinterpret_cast<float*>(out)[at] = s;
-  else
-    reinterpret_cast<bf16*>(out)[at] = (bf16)s;
+  if (out) store_param(out, f32, at, s);
 }
 
 // Lanes and vectors a row by its width (in vectors).
@@ -351,8 +455,19 @@ static int norm_bwd_blocks(int rows, int dim, bool f32) {
   return (int)std::min<long long>(most, std::max<long long>(1, (rows + per - 1) / per));
 }
 
+// Rows that are few enough for the workgroups of sum_columns to read again instead of a
+// second launch over the others' sums.  Forward and backward, us, second launch -> none:
+//   bf16  64 x 1024  19.3 ->  7.5   fp32  64 x 1024   8.5 ->  5.9
+//        512 x 1024  19.7 -> 10.4        512 x 1024   9.6 ->  7.6
+//       1024 x 1024  20.4 -> 13.7       1024 x 1024  11.3 -> 10.8
+//       1024 x 8192  35.6 -> 28.9        999 x 771   11.1 -> 12.7
+//       2048 x 1024  21.2 -> 19.9       2048 x 1024  15.5 -> 22.8
+//       2048 x  256  13.0 -> 19.0       2048 x  256  10.4 -> 15.3
+// A workgroup of theirs goes through all rows, so their time grows with the rows.
+static bool norm_small(int rows) { return rows <= kNormFewRows; }
+
 size_t norm_bwd_workspace_bytes(int rows, int dim, bool f32) {
-  return sizeof(float) * 2 * (size_t)norm_bwd_blocks(rows, dim, f32) * dim;
+  return norm_small(rows) ? 0 : sizeof(float) * 2 * (size_t)norm_bwd_blocks(rows, dim, f32) * dim;
 }
 
 template <typename T, typename F>
@@ -408,10 +523,15 @@ hipError_t launch_norm(const void* x, long long x_stride, const void* weight, co
 }
 
 template <typename T>
-static hipError_t launch_norm_bwd_t(const NormBwdArgs& a, int blocks, hipStream_t stream) {
+static hipError_t launch_norm_bwd_t(const NormBwdArgs& a, hipStream_t stream) {
+  constexpr int N = kVec<T>;
+  const bool columns = a.dweight || a.dbias;
+  constexpr int S = kColumnLanes * N;  // columns of a workgroup that sums them
+  const int blocks = a.row_blocks + (columns ? (a.dim + S - 1) / S : 0);
   with_shape<T>(a.dim, [&](auto l, auto c, auto edge) {
     constexpr int L = decltype(l)::value;
-    const size_t lds = L > 256 || !a.partials ? 0 : sizeof(float) * 2 * a.dim;
+    const size_t lds = columns ? sizeof(float) * 2 * 8 * S
+                       : L > 256 || !a.partials ? 0 : sizeof(float) * 2 * decltype(c)::value * N * L;
     hipLaunchKernelGGL((norm_bwd_kernel<T, L, decltype(c)::value, decltype(edge)::value>),
                        dim3(blocks), dim3(512), lds, stream, a);
   });
@@ -422,14 +542,25 @@ hipError_t launch_norm_bwd(const void* x, long long x_stride, const void* weight
                            const float* stats, const void* dy, long long dy_stride, bool f32,
                            bool param_f32, int rows, int dim, bool center, void* dx, void* dweight,
                            void* dbias, void* workspace, hipStream_t stream) {
-  const bool sums = dweight || dbias;
-  const int blocks = norm_bwd_blocks(rows, dim, f32);
-  const NormBwdArgs a{x, dy, weight, reinterpret_cast<const float2*>(stats), dx,
-                      sums ? reinterpret_cast<float*>(workspace) : nullptr, x_stride, dy_stride,
-                      rows, dim, (float)(1.0 / dim), center, param_f32};
-  hipError_t e = f32 ? launch_norm_bwd_t<float>(a, blocks, stream)
-                     : launch_norm_bwd_t<bf16>(a, blocks, stream);
-  if (e != hipSuccess || !sums) return e;
+  const bool sums = dweight || dbias, small = norm_small(rows);
+  const bool partials = sums && !small;
+  const int blocks = dx || partials ? norm_bwd_blocks(rows, dim, f32) : 0;
+  NormBwdArgs a{x, dy, weight, reinterpret_cast<const float2*>(stats), dx,
+                partials ? reinterpret_cast<float*>(workspace) : nullptr,
+                small ? dweight : nullptr, small ? dbias : nullptr, x_stride, dy_stride,
+                rows, dim, blocks, (float)(1.0 / dim), center, param_f32};
+  auto launch = [&] {
+    return f32 ? launch_norm_bwd_t<float>(a, stream) : launch_norm_bwd_t<bf16>(a, stream);
+  };
+  hipError_t e;
+  if (small && sums && dx == dy) {  // the columns are read before dx takes dy's place
+    a.row_blocks = 0;
+    if ((e = launch()) != hipSuccess) return e;
+    a.row_blocks = blocks;
+    a.dweight = a.dbias = nullptr;
+  }
+  e = launch();
+  if (e != hipSuccess || !partials) return e;
   hipLaunchKernelGGL(norm_reduce_kernel, dim3((2 * dim + 63) / 64), dim3(1024), 0, stream,
                      a.partials, blocks, dim, dweight, dbias, param_f32);
   return hipGetLastError();

@@ -177,7 +177,7 @@ struct Norm : public Function<Norm> {
     size_t need = 0;
     if (need_w || need_b) {
       need = lib.mf_norm_bwd_workspace_bytes((int)rows, (int)d, code_of(x));
-      ws = bytes(need, x);
+      if (need) ws = bytes(need, x);
     }
     in_backward([&] {
       check(lib.mf_norm_bwd(data(x), row_step(x), data(weight), data_as<float>(stats), data(dy),

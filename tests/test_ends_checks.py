@@ -73,8 +73,8 @@ ARG, SHAPE, DTYPE, WS = (_lib.ERR_INVALID_ARGUMENT, _lib.ERR_SHAPE, _lib.ERR_DTY
     (_norm, dict(center=0, b=P), ARG, "no bias"),
     (_norm_bwd, dict(st=None), ARG, "non-null"),
     (_norm_bwd, dict(dys=3), SHAPE, "dy: 3 elements"),
-    (_norm_bwd, dict(n=8), WS, "workspace holds 8"),
-    (_norm_bwd, dict(ws=None), WS, "workspace holds 0"),
+    (_norm_bwd, dict(rows=1 << 20, n=8), WS, "workspace holds 8"),
+    (_norm_bwd, dict(rows=1 << 20, ws=None), WS, "workspace holds 0"),
     (_norm_bwd, dict(center=0), ARG, "no bias"),
     (_norm_bwd, dict(rows=0), ARG, "positive"),
     (_embed, dict(table=None) and dict(t=None), ARG, "non-null"),

@@ -9,12 +9,13 @@ L = _lib.LIB
 
 @pytest.mark.parametrize("dtype", [_lib.DTYPE_F32, _lib.DTYPE_BF16])
 def test_norm_workspace_holds_every_workgroup(dtype):
-    for rows in (1, 2, 63, 64, 1000, 32768, 1 << 22):
+    for rows in (1, 2, 63, 64, 1000, 1024, 1025, 32768, 1 << 22):
         for dim in (1, 7, 64, 771, 1024, 2048, 2056, 8192, 16384):
             n = L.mf_norm_bwd_workspace_bytes(rows, dim, dtype)
-            # pairs of rows of dim floats: one a workgroup, at most 512
-            assert n % (8 * dim) == 0 and 1 <= n // (8 * dim) <= 512
+            # pairs of rows of dim floats: one a workgroup, at most 512; none for few rows
+            assert n % (8 * dim) == 0 and n // (8 * dim) <= 512
             assert n // (8 * dim) <= max(1, rows)
+            assert (n > 0) == (rows > 1024)
 
 
 def test_embedding_workspace():

@@ -22,8 +22,9 @@ def _stream():
 @pytest.mark.parametrize("center", [1, 0], ids=["layer", "rms"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("d", [5, 64, 100, 771, 1024, 2047, 4096, 5001, 16384])
-def test_norms_in_place(d, dtype, center, device):
-    rows, code = 67, _lib.DTYPE_BF16 if dtype is torch.bfloat16 else _lib.DTYPE_F32
+@pytest.mark.parametrize("rows", [67, 1024, 1500])
+def test_norms_in_place(rows, d, dtype, center, device):
+    code = _lib.DTYPE_BF16 if dtype is torch.bfloat16 else _lib.DTYPE_F32
     g = torch.Generator(device=device).manual_seed(d)
     x, dy = (torch.randn(rows, d, generator=g, device=device).to(dtype) for _ in range(2))
     w = torch.randn(d, generator=g, device=device).to(dtype)
