@@ -15,7 +15,11 @@ constexpr long long kEmbedMostValues = 1ll << 34;  // of the output: launches st
 constexpr int kSortDigit = 9;               // bits of a key in one pass
 constexpr int kSortFewest = 5;              // (kernels are made for 5 to 9)
 constexpr int kSortBins = 1 << kSortDigit;
-constexpr int kSortTiles = 64;              // waves that share the tokens, at most
+constexpr int kSortTiles = 64;              // workgroups that share the tokens, at most
+constexpr int kSortWaves = 8;               // of each
+constexpr int kSortRuns = 2;                // runs of 64 tokens that a wave takes in a step
+constexpr int kSortStep = kSortWaves * kSortRuns * 64;
+static_assert(kSortBins == kSortWaves * 64, "a thread for each digit");
 constexpr int kSortOne = 8192;              // tokens that one workgroup sorts
 constexpr int kEmbedMinChunk = 8;           // sorted tokens that a wave adds, at least
 constexpr int kEmbedMaxChunk = 64;          // (one for each lane)
@@ -28,7 +32,7 @@ struct SortedToken {
 
 struct EmbedLayout {
   int passes, bits;    // of the sort: digits and their bits
-  int tiles, rounds;   // waves, and the 64 tokens each that they take in turn; 0: one workgroup
+  int tiles, steps;    // workgroups, and how many kSortStep tokens each takes; 1, 0: all at once
   int chunk, chunks;   // sorted tokens that a wave adds, and how many such
   int width;           // of a piece of a row: a multiple of 4
   size_t histogram, tokens[2], partials, total;  // offsets in bytes
@@ -41,11 +45,13 @@ inline EmbedLayout embed_layout(int tokens, int vocabulary, int dim) {
   l.passes = (bits + kSortDigit - 1) / kSortDigit;
   l.bits = (bits + l.passes - 1) / l.passes;
   if (l.bits < kSortFewest) l.bits = kSortFewest;
-  const int waves = (tokens + 63) / 64;
-  l.rounds = (waves + kSortTiles - 1) / kSortTiles;
-  if (l.rounds < 4) l.rounds = 4;
-  l.tiles = (waves + l.rounds - 1) / l.rounds;
-  if (tokens <= kSortOne) l.tiles = l.rounds = 0;
+  const int steps = (tokens + kSortStep - 1) / kSortStep;
+  l.steps = (steps + kSortTiles - 1) / kSortTiles;
+  l.tiles = (steps + l.steps - 1) / l.steps;
+  if (tokens <= kSortOne) {
+    l.tiles = 1;
+    l.steps = 0;
+  }
   // (512 columns a wave: chunks that leave the card idle are not worth their fewer pieces)
   l.chunk = kEmbedMinChunk;
   const long long slabs = (dim + 511) / 512;

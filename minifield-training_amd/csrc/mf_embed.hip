@@ -16,10 +16,16 @@
 // launches that sort, which are a few waves' work each, zero the whole table beside
 // it, a share each.
 //
-// The sort goes by digits of up to 9 bits from the lowest.  A wave takes a run of
-// tokens, 64 at a time; lanes with one digit find each other by ballots over its
-// bits, so that a lane's place is its digit's first place, what the waves and rounds
-// before have of that digit, and the lanes before it.
+// The sort goes by digits of up to 9 bits from the lowest, each in two launches: tiles of
+// the tokens count their digits, and then place their tokens.  A wave takes runs of 64;
+// lanes with one digit find each other by ballots over its bits, so that a lane's place is
+// its digit's first place, what the tiles, steps and waves before have of that digit, and
+// the lanes before it.  Few tokens are sorted by one workgroup in one launch.
+//
+// Measured, 32768 tokens of 65536 x 1024 bf16, us: lookup 17 (64 MiB written, the table's
+// rows from the cache); zeroing 128 MiB beside sorting 28 (4.7 TB/s; the four launches
+// alone 18, the zeros alone 20), sums 18.6 (6 TB/s with the rows and pieces they write),
+// joining 4.5.  5001 tokens of 1003 x 129 fp32: sorting 11, sums 4.1, joining 4.7.
 #include <algorithm>
 
 #include "mf_embed.h"
@@ -84,7 +90,7 @@ struct SortArgs {
   const SortedToken* from;  // null: the ids as they come
   SortedToken* to;
   int* histogram;           // [tiles][kSortBins]
-  int tiles, rounds, shift, bits, passes, blocks;
+  int tiles, steps, shift, bits, passes;
   // a share of the table's gradient to zero, in bytes, and what a workgroup takes of it
   size_t zero_first, zero_last, zero_block;
 };
@@ -109,7 +115,7 @@ __device__ __forceinline__ void sort_entries(const SortArgs& a, int first, int l
 
 // (as streams: what reads the gradient next comes long after the launches that add to it)
 __device__ __forceinline__ void zero_share(const SortArgs& a) {
-  const size_t first = a.zero_first + (size_t)(blockIdx.x - a.blocks) * a.zero_block;
+  const size_t first = a.zero_first + (size_t)(blockIdx.x - a.tiles) * a.zero_block;
   const size_t last = min(a.zero_last, first + a.zero_block);
   char* out = reinterpret_cast<char*>(a.e.out);
   for (size_t at = first + threadIdx.x * 16; at < last; at += blockDim.x * 16) {
@@ -153,91 +159,87 @@ __device__ __forceinline__ int place_of(volatile int* count, uint32_t digits, bo
   return to;
 }
 
-constexpr int kSortAhead = 8;  // runs of 64 tokens that a wave has in flight
-
-// How many of its tokens each wave has of every digit.
-__global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
-  __shared__ int counts[4][kSortBins];
-  if ((int)blockIdx.x >= a.blocks) return zero_share(a);
+// How many of its tokens each tile has of every digit.
+__global__ __launch_bounds__(512) void sort_count_kernel(SortArgs a) {
+  constexpr int AHEAD = 4;  // runs of 64 tokens that a wave has in flight
+  __shared__ int counts[kSortBins];
+  if ((int)blockIdx.x >= a.tiles) return zero_share(a);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int tile = blockIdx.x * 4 + wave;
-  for (int d = lane; d < kSortBins; d += 64) counts[wave][d] = 0;
+  const int runs = a.steps * kSortRuns;
+  counts[threadIdx.x] = 0;
   __syncthreads();
-  if (tile < a.tiles)
-    for (int r0 = 0; r0 < a.rounds; r0 += kSortAhead) {
-      const int first = (tile * a.rounds + r0) * 64;
-      SortedToken t[kSortAhead];
-      sort_entries(a, first, lane, t);
+  for (int r0 = 0; r0 < runs; r0 += AHEAD) {
+    const int first = ((blockIdx.x * kSortWaves + wave) * runs + r0) * 64;
+    SortedToken t[AHEAD];
+    sort_entries(a, first, lane, t);
 #pragma unroll
-      for (int j = 0; j < kSortAhead; ++j)
-        if (r0 + j < a.rounds && first + 64 * j + lane < a.e.tokens)
-          atomicAdd(&counts[wave][t[j].key >> a.shift & ((1 << a.bits) - 1)], 1);
-    }
+    for (int j = 0; j < AHEAD; ++j)
+      if (r0 + j < runs && first + 64 * j + lane < a.e.tokens)
+        atomicAdd(&counts[t[j].key >> a.shift & ((1 << a.bits) - 1)], 1);
+  }
   __syncthreads();
-  if (tile < a.tiles)
-    for (int d = lane; d < kSortBins; d += 64)
-      a.histogram[(size_t)tile * kSortBins + d] = counts[wave][d];
+  a.histogram[(size_t)blockIdx.x * kSortBins + threadIdx.x] = counts[threadIdx.x];
 }
 
+// Each tile's tokens to their places by one digit, kSortStep at a time.  Thread d keeps where
+// the tile's next token of digit d goes.
 template <int BITS>
-__global__ __launch_bounds__(256) void sort_place_kernel(SortArgs a) {
-  __shared__ int place[4][kSortBins];
-  __shared__ int wave_sums[4];
-  if ((int)blockIdx.x >= a.blocks) return zero_share(a);
+__global__ __launch_bounds__(512) void sort_place_kernel(SortArgs a) {
+  constexpr int ROWS = 32;  // of the histogram in flight
+  __shared__ int place[kSortWaves][kSortBins];
+  __shared__ int wave_sums[kSortWaves];
+  if ((int)blockIdx.x >= a.tiles) return zero_share(a);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  // digits 2 tid and 2 tid + 1: those of the tiles before the workgroup's, and of all
-  const int2* counts = reinterpret_cast<const int2*>(a.histogram) + tid;
-  int before0 = 0, before1 = 0, whole[2] = {0, 0};
-  for (int t0 = 0; t0 < a.tiles; t0 += 64) {
-    int2 h[64];
+  int first = blockIdx.x * a.steps * kSortStep + wave * kSortRuns * 64;
+  SortedToken t[kSortRuns];
+  sort_entries(a, first, lane, t);
+  // digit tid: what the tiles before have of it, and all of them
+  int before = 0, whole = 0;
+  for (int t0 = 0; t0 < a.tiles; t0 += ROWS) {
+    int h[ROWS];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) h[j] = counts[(size_t)min(t0 + j, a.tiles - 1) * (kSortBins / 2)];
+    for (int j = 0; j < ROWS; ++j)
+      h[j] = a.histogram[(size_t)min(t0 + j, a.tiles - 1) * kSortBins + tid];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-      const bool in = t0 + j < a.tiles, before = t0 + j < (int)blockIdx.x * 4;
-      whole[0] += in ? h[j].x : 0;
-      whole[1] += in ? h[j].y : 0;
-      before0 += before ? h[j].x : 0;
-      before1 += before ? h[j].y : 0;
+    for (int j = 0; j < ROWS; ++j) {
+      whole += t0 + j < a.tiles ? h[j] : 0;
+      before += t0 + j < (int)blockIdx.x ? h[j] : 0;
     }
   }
-  // first place of the thread's two digits: an exclusive sum over the threads
-  const int pair = whole[0] + whole[1];
-  int sum = pair;
+  int sum = whole;  // of the digits up to this in the wave
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const int o = __shfl_up(sum, m);
     if (lane >= m) sum += o;
   }
   if (lane == 63) wave_sums[wave] = sum;
-  __syncthreads();
-  int start = sum - pair;
-  for (int i = 0; i < wave; ++i) start += wave_sums[i];
-  int at[2] = {start + before0, start + whole[0] + before1};
+  int next = sum - whole + before;
+  for (int step = 0; step < a.steps; ++step, first += kSortStep) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    place[i][2 * tid] = at[0];
-    place[i][2 * tid + 1] = at[1];
-    const int t = blockIdx.x * 4 + i;
-    if (t < a.tiles) {
-      const int2 h = counts[(size_t)t * (kSortBins / 2)];
-      at[0] += h.x;
-      at[1] += h.y;
-    }
-  }
-  __syncthreads();
-  const int tile = blockIdx.x * 4 + wave;
-  if (tile >= a.tiles) return;
-  for (int r0 = 0; r0 < a.rounds; r0 += kSortAhead) {
-    const int first = (tile * a.rounds + r0) * 64;
-    SortedToken t[kSortAhead];
-    sort_entries(a, first, lane, t);
+    for (int d = 0; d < kSortBins; d += 64) place[wave][d + lane] = 0;
+    int to[kSortRuns];
+    bool live[kSortRuns];
+    SortedToken now[kSortRuns];
 #pragma unroll
-    for (int j = 0; j < kSortAhead; ++j) {
-      const bool live = r0 + j < a.rounds && first + 64 * j + lane < a.e.tokens;
-      const int to = place_of<BITS>(place[wave], t[j].key >> a.shift, live, lane);
-      if (live) a.to[to] = t[j];
+    for (int j = 0; j < kSortRuns; ++j) {  // among the wave's own of the digit
+      now[j] = t[j];
+      live[j] = first + 64 * j + lane < a.e.tokens;
+      to[j] = place_of<BITS>(place[wave], now[j].key >> a.shift, live[j], lane);
     }
+    if (step + 1 < a.steps) sort_entries(a, first + kSortStep, lane, t);
+    __syncthreads();
+    if (step == 0)
+      for (int i = 0; i < wave; ++i) next += wave_sums[i];
+#pragma unroll
+    for (int i = 0; i < kSortWaves; ++i) {
+      const int c = place[i][tid];
+      place[i][tid] = next;
+      next += c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kSortRuns; ++j)
+      if (live[j]) a.to[place[wave][now[j].key >> a.shift & ((1 << BITS) - 1)] + to[j]] = now[j];
   }
 }
 
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(1024) void sort_one_kernel(SortArgs a) {
   __shared__ int place[WAVES][kSortBins];
   __shared__ SortedToken list[kSortOne];
   __shared__ int wave_sums[kSortBins / 64];
-  if ((int)blockIdx.x >= a.blocks) return zero_share(a);
+  if (blockIdx.x >= 1) return zero_share(a);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n0 = wave * 64 * ITEMS + lane;
   SortedToken t[ITEMS];
@@ -493,13 +495,12 @@ hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long 
   s.e = EmbedArgs{ids, nullptr, dtable, stride, padding, tokens, vocabulary, dim, scale, ids64};
   s.histogram = reinterpret_cast<int*>(ws + l.histogram);
   s.tiles = l.tiles;
-  s.rounds = l.rounds;
+  s.steps = l.steps;
   s.bits = l.bits;
   s.passes = l.passes;
   const size_t bytes = (size_t)vocabulary * dim * (f32 ? 4 : 2);
   SortedToken* sorted = lists[0];
-  if (l.tiles == 0) {
-    s.blocks = 1;
+  if (l.steps == 0) {
     s.to = sorted;
     s.zero_last = bytes;
     s.zero_block = 256 << 10;  // (few workgroups: the sort's LDS leaves a CU room for one)
@@ -509,25 +510,25 @@ hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long 
                          stream, s);
     });
   } else {
-    s.blocks = (l.tiles + 3) / 4;
     s.zero_block = 64 << 10;
-    // placing takes about three times what counting does: so are their shares
-    const size_t share = (bytes / (4 * l.passes) / s.zero_block + 1) * s.zero_block;
+    // placing takes about twice what counting does (5.8 us and 3.3 at 32768 tokens, by
+    // themselves): so are their shares
+    const size_t share = (bytes / (3 * l.passes) / s.zero_block + 1) * s.zero_block;
     for (int step = 0; step < 2 * l.passes; ++step) {
       const int pass = step / 2;
       s.shift = pass * l.bits;
       s.from = pass ? lists[(pass + 1) & 1] : nullptr;
       s.to = sorted = lists[pass & 1];
       s.zero_first = s.zero_last;
-      s.zero_last = std::min(bytes, (pass * 4 + (step % 2 ? 4 : 1)) * share);
+      s.zero_last = std::min(bytes, (pass * 3 + (step % 2 ? 3 : 1)) * share);
       const unsigned zero =
           (unsigned)((s.zero_last - s.zero_first + s.zero_block - 1) / s.zero_block);
-      const dim3 grid((unsigned)s.blocks + zero);
+      const dim3 grid((unsigned)s.tiles + zero);
       if (step % 2 == 0)
-        hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, stream, s);
+        hipLaunchKernelGGL(sort_count_kernel, grid, dim3(512), 0, stream, s);
       else
         with_bits(l.bits, [&](auto b) {
-          hipLaunchKernelGGL((sort_place_kernel<decltype(b)::value>), grid, dim3(256), 0, stream, s);
+          hipLaunchKernelGGL((sort_place_kernel<decltype(b)::value>), grid, dim3(512), 0, stream, s);
         });
     }
   }

@@ -44,8 +44,9 @@ def test_widths(d, dtype, device):
     _check(_ids(700, 300, device), table, scale=d ** 0.5)
 
 
-# chunks of 32, waves of 64, tiles of 256 tokens, more than one workgroup's and many rounds
-@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 255, 256, 257, 1025, 9000, 40000])
+# chunks of 32, waves of 64, one workgroup's most, tiles of 1024 tokens and of several steps
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 255, 256, 257, 1025, 8192, 8193, 9000,
+                               40000, 65536, 65537, 200001])
 @pytest.mark.parametrize("skew", [True, False], ids=["skewed", "even"])
 def test_lengths(n, skew, device):
     say("embed length", n, skew)
@@ -63,7 +64,16 @@ def test_vocabularies(v, device):
     _check(ids, table, scale=2.0)
 
 
-@pytest.mark.parametrize("n", [1, 32, 64, 96, 1000, 5000])
+@pytest.mark.parametrize("v", [30, 511, 1003, 65536, 262144])
+def test_vocabularies_of_many_tokens(v, device):
+    say("embed vocabulary, tiles of two steps", v)
+    table = torch.randn(v, 8, device=device)
+    ids = _ids(70001, v, device, skew=False)
+    ids[-5:] = v - 1
+    _check(ids, table, scale=0.5)
+
+
+@pytest.mark.parametrize("n", [1, 32, 64, 96, 1000, 5000, 70000])
 def test_one_token_over_and_over(n, device):
     table = torch.randn(1000, 136, device=device)
     _check(torch.full((n,), 7, device=device), table)
