@@ -433,12 +433,12 @@ int mf_embed_bwd(const void* ids, int id_bytes, const void* dout,
  *             + r (log r - log of q's sum over the ids that no entry names)).
  * Entries whose id is outside the vocabulary are not there.  A row of weight zero
  * (weights [rows] fp32, NULL: ones) has loss zero and no gradient, whatever it
- * holds, and so has one without entries (and without total).  Masses and sums
- * of a row in 64 bits, its exponentials in fp32.  teacher [rows, top] in
+ * holds, and so has one without entries (and without total).  The masses and the
+ * logarithms in 64 bits, exponentials of logits and their sums in fp32.  teacher [rows, top] in
  * teacher_dtype, teacher_ids [rows, top] of id_bytes (4 or 8) each.  Up to 1024
  * entries a row, vocabularies up to 393216, 2^35 logits, and temperatures in
  * [1e-6, 1e6].
- * With dlogits (grad_stride elements between rows; may be logits itself) also
+ * With dlogits (grad_stride elements between rows; may be the logits themselves) also
  * the gradient of the sum of the losses, in dtype, in the same pass.  stats, NULL or
  * rows * (4 + top) fp32, receives what mf_distill_bwd needs. */
 size_t mf_distill_stats_bytes(int rows, int top);

@@ -71,8 +71,12 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     counts the teacher's other tokens in (see the module).  ``weights [...]`` multiplies
     the losses; a row of weight zero has loss and gradient zero whatever its logits
     hold, and so has a row without entries (where no total is given).  V up to
-    393216, K up to 1024, temperatures in [1e-6, 1e6].  Differentiable in the logits, once; :func:`top_logits_loss_and_gradient` needs half the memory
-    and two passes over the logits instead of three.
+    393216, K up to 1024, temperatures in [1e-6, 1e6].  The teacher's masses and the
+    logarithms are 64-bit, exponentials of logits and their sums float32: a loss is
+    off by some 1e-7 times ``weight * temperature ** 2``.  Differentiable in the logits, once;
+    :func:`top_logits_loss_and_gradient` needs half the memory and two passes over the
+    logits instead of three.  (A backward captured into a graph: see
+    :func:`normalization.layer_norm`.)
     """
     teacher, ids, total, weights = _checked("top_logits_loss", logits, teacher_logits, teacher_ids,
                                             teacher_total, weights, temperature)
@@ -110,8 +114,13 @@ def top_logits_loss_and_gradient(logits: torch.Tensor, teacher_logits: torch.Ten
     if even_rows(out) is not out:
         raise ValueError("out must have evenly spaced rows and a dense last dimension")
     same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
-    if not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
+    memory = out.untyped_storage().data_ptr() or None  # (none of an empty tensor)
+    if not same and memory == logits.untyped_storage().data_ptr():
         raise ValueError("out must be the logits or share no memory with them")
+    # (rows are written while others' entries are yet to be read)
+    if any(t is not None and memory == t.untyped_storage().data_ptr()
+           for t in (teacher, ids, total, weights)):
+        raise ValueError("out must share no memory with the teacher or the weights")
     loss = _nodes.distill(even_rows(logits), teacher, ids, total, weights, temperature, False, out)
     torch.autograd.graph.increment_version(out)
     return loss, out

@@ -21,8 +21,9 @@ def embed(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
     Ids outside ``0 .. V-1`` and ``padding_id`` have rows of zeros and no part in the
     gradient (nothing is read back to the host to refuse them).  The table's gradient
     is dense, in the table's dtype; a row's tokens are added in float32 in an order that
-    depends on the ids alone, so the same inputs give the same bits.  Differentiable
-    in the table.
+    depends on the ids alone, so the same inputs give the same bits.  V up to 2**27, D up
+    to 65536, up to 2**24 ids and 2**34 values.  Differentiable in the table.  (A
+    backward captured into a graph: see :func:`normalization.layer_norm`.)
     """
     if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
         raise ValueError("table must be [V, D] with V and D positive")

@@ -52,6 +52,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     gradients have their dtype.  Mean and spread are those of the row itself, in
     float32.  D up to 16384, up to 2**22 rows, evenly spaced or copied.
     Differentiable in x, weight and bias, once; the same inputs give the same bits.
+    A backward is captured into a graph together with its forward and while no eager
+    graph of the same leaves is alive, as for any operation: autograd accumulates a
+    leaf's gradient on the stream of its oldest graph.
     """
     return _norm("layer_norm", x, weight, bias, eps, True)
 

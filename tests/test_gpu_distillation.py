@@ -252,6 +252,14 @@ def test_outputs_that_are_refused(device):
             call(z, t, ids, out=out, **more)
     with pytest.raises(ValueError, match="share no memory"):
         call(wide[:, :90], t, ids, out=wide[:, 5:95], **more)
+    # the teacher or the weights beside the gradient
+    wide[:, 90:99] = t
+    with pytest.raises(ValueError, match="teacher or the weights"):
+        call(z, wide.view(-1)[455:500].view(5, 9), ids, out=wide.view(-1)[:450].view(5, 90), **more)
+    with pytest.raises(ValueError, match="teacher or the weights"):
+        call(z, t, ids, weights=wide.view(-1)[495:], out=wide.view(-1)[:450].view(5, 90))
+    empty = torch.empty(0, 90, device=device)
+    assert call(empty, t[:0], ids[:0], out=empty)[1] is empty
 
 
 def test_zero_rows(device):
