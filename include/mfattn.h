@@ -393,7 +393,7 @@ int mf_norm(const void* x, long long x_stride, const void* weight,
  * dweight and dbias [dim] in param_dtype, summed over the rows in fp32 in a fixed
  * order; each may be NULL where it is not wanted.  `workspace` holds the sums of the
  * launch's workgroups (mf_norm_bwd_workspace_bytes; NULL where that is 0: for few
- * rows, and for sizes that the call refuses). */
+ * rows, and for sizes that the call refuses).  Nothing else may overlap. */
 size_t mf_norm_bwd_workspace_bytes(int rows, int dim, int dtype);
 int mf_norm_bwd(const void* x, long long x_stride, const void* weight,
                 const float* stats, const void* dy, long long dy_stride,

@@ -958,6 +958,8 @@ int mf_norm(const void* x, long long x_stride, const void* weight, const void* b
   if (!(std::isfinite(eps) && eps >= 0))
     return fail(MF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative (got %g)", (double)eps);
   if (int rc = check_rows("x", x_stride, dim)) return rc;
+  if (y == x && x_stride != dim)
+    return fail(MF_ERR_SHAPE, "y in the place of x, whose rows are not dense");
   return check_hip(mf::launch_norm(x, x_stride, weight, bias, dtype == MF_DTYPE_F32,
                                    param_dtype == MF_DTYPE_F32, rows, dim, center != 0, eps, y,
                                    stats, static_cast<hipStream_t>(stream)),
@@ -980,6 +982,9 @@ int mf_norm_bwd(const void* x, long long x_stride, const void* weight, const flo
   if (dbias && !center) return fail(MF_ERR_INVALID_ARGUMENT, "the RMS norm has no bias");
   if (int rc = check_rows("x", x_stride, dim)) return rc;
   if (int rc = check_rows("dy", dy_stride, dim)) return rc;
+  if (dx == x) return fail(MF_ERR_INVALID_ARGUMENT, "dx must not be x");
+  if (dx == dy && dy_stride != dim)
+    return fail(MF_ERR_SHAPE, "dx in the place of dy, whose rows are not dense");
   if (dweight || dbias) {
     const size_t need = mf_norm_bwd_workspace_bytes(rows, dim, dtype);
     if (need && (!workspace || workspace_bytes < need))

@@ -16,14 +16,15 @@ def _msg():
 
 
 def _norm(**kw):
-    a = dict(x=P, xs=64, w=P, b=None, dt=1, pdt=1, rows=4, dim=64, center=1, eps=1e-5, y=P, st=None)
+    a = dict(x=P, xs=64, w=P, b=None, dt=1, pdt=1, rows=4, dim=64, center=1, eps=1e-5, y=2 * P,
+             st=None)
     a.update(kw)
     return L.mf_norm(*a.values(), None)
 
 
 def _norm_bwd(**kw):
-    a = dict(x=P, xs=64, w=P, st=P, dy=P, dys=64, dt=1, pdt=1, rows=4, dim=64, center=1, dx=P, dw=P,
-             db=P, ws=P, n=1 << 30)
+    a = dict(x=P, xs=64, w=P, st=P, dy=P, dys=64, dt=1, pdt=1, rows=4, dim=64, center=1, dx=2 * P,
+             dw=P, db=P, ws=P, n=1 << 30)
     a.update(kw)
     return L.mf_norm_bwd(*a.values(), None)
 
@@ -71,8 +72,11 @@ ARG, SHAPE, DTYPE, WS = (_lib.ERR_INVALID_ARGUMENT, _lib.ERR_SHAPE, _lib.ERR_DTY
     (_norm, dict(eps=-1.0), ARG, "eps"),
     (_norm, dict(eps=float("nan")), ARG, "eps"),
     (_norm, dict(center=0, b=P), ARG, "no bias"),
+    (_norm, dict(xs=65, y=P), SHAPE, "not dense"),
     (_norm_bwd, dict(st=None), ARG, "non-null"),
     (_norm_bwd, dict(dys=3), SHAPE, "dy: 3 elements"),
+    (_norm_bwd, dict(dx=P), ARG, "must not be x"),
+    (_norm_bwd, dict(dy=2 * P, dys=65), SHAPE, "not dense"),
     (_norm_bwd, dict(rows=1 << 20, n=8), WS, "workspace holds 8"),
     (_norm_bwd, dict(rows=1 << 20, ws=None), WS, "workspace holds 0"),
     (_norm_bwd, dict(center=0), ARG, "no bias"),
