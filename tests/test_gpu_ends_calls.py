@@ -169,3 +169,39 @@ def test_tensors_on_the_host_beside_device_tensors(device):
         embedding.embed(torch.zeros(3, dtype=torch.int64), x)
     with pytest.raises(ValueError, match="GPU only"):
         distillation.top_logits_loss(x, torch.ones(2, 3), torch.zeros(2, 3, dtype=torch.int64, device=device))
+
+
+def test_function_transforms_are_refused(device):
+    x = torch.randn(3, 4, 32, device=device)
+    w = torch.randn(32, device=device)
+    ids = torch.randint(0, 32, (3, 4, 5), device=device)
+    t = torch.randn(3, 4, 5, device=device)
+    for call in (lambda x: normalization.layer_norm(x, w).sum(),
+                 lambda x: embedding.embed(ids[0], x[0]).sum(),
+                 lambda x: distillation.top_logits_loss(x[0], t[0], ids[0]).sum()):
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.grad(call)(x)
+    for call in (lambda x: normalization.layer_norm(x, w),
+                 lambda x: embedding.embed(ids[0], x),
+                 lambda x: distillation.top_logits_loss(x, t[0], ids[0])):
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.vmap(call)(x)
+    # nothing was launched on the way, and eager calls go on
+    torch.cuda.synchronize()
+    assert normalization.layer_norm(x, w).shape == x.shape
+
+
+def test_inference_mode(device):
+    x, w = torch.randn(5, 64, device=device), torch.randn(64, device=device)
+    ids, t = torch.randint(0, 64, (5, 3), device=device), torch.randn(5, 3, device=device)
+    y = normalization.layer_norm(x, w)
+    e = embedding.embed(ids, torch.stack([w] * 64))
+    alone = distillation.top_logits_loss(x, t, ids)
+    loss, grad = distillation.top_logits_loss_and_gradient(x, t, ids)
+    with torch.inference_mode():
+        assert torch.equal(normalization.layer_norm(x, w), y)
+        assert torch.equal(embedding.embed(ids, torch.stack([w] * 64)), e)
+        assert torch.equal(distillation.top_logits_loss(x, t, ids), alone)
+        mine = x.clone()
+        assert torch.equal(distillation.top_logits_loss_and_gradient(mine, t, ids, out=mine)[0], loss)
+        assert torch.equal(mine, grad)
