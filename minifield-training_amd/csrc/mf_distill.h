@@ -7,7 +7,7 @@ namespace mf {
 
 constexpr int kDistillMostTop = 1024;             // teacher entries a row
 constexpr int kDistillMostVocabulary = 3 << 17;   // one bit each in 48 KB of LDS
-constexpr int kDistillMostRows = 1 << 21;         // 512 threads a row stay below 2^32
+constexpr int kDistillMostRows = 1 << 21;         // 1024 threads a row stay below 2^32
 constexpr long long kDistillMostLogits = 1ll << 35;  // (and 256 threads a part of 4096)
 // (log2(e) / T and differences of logits times it stay numbers in fp32)
 constexpr double kDistillLeastTemperature = 1e-6, kDistillMostTemperature = 1e6;

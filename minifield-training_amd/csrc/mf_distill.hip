@@ -20,8 +20,8 @@
 // they cancel: at log q = -20 and a loss of 1 the fp32 terms alone would cost 1e-6.
 //
 // Bound: memory, one read of the logits and one write of the gradient.  A workgroup
-// of 512 takes a row.  Rows of up to 32 vectors of 16 bytes a thread stay in registers
-// between the maximum, the sum and the gradient; longer ones are read again.
+// of 256, 512 or 1024 takes a row.  Rows of up to 16 vectors of 16 bytes a thread stay in
+// registers between the maximum, the sum and the gradient; longer ones are read again.
 //
 // Measured, 4096 x 65536 bf16 (512 MiB), 64 entries a row: loss 101-110 us (4.9-5.3
 // TB/s), gradient from what it saved 172 (6.2 TB/s, a part of the logits still in the
@@ -51,8 +51,6 @@ struct DistillArgs {
   double temperature, per;  // T and 1 / T
   bool teacher_f32, ids64;
 };
-
-constexpr int kDistillThreads = 512;
 
 __device__ __forceinline__ int teacher_id(const DistillArgs& a, size_t at) {
   const long long id = a.ids64 ? reinterpret_cast<const long long*>(a.ids)[at]
@@ -150,10 +148,10 @@ __device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, 
 
 // LOSS: the loss (and with `stats` what the backward needs); GRAD: the gradient of
 // the weighted loss.  U: vectors a thread has in flight; RESIDENT: they are the row.
-template <typename T, bool GRAD, int U, bool RESIDENT>
-__global__ __launch_bounds__(kDistillThreads) __attribute__((amdgpu_waves_per_eu(U > 16 ? 2 : 4)))
+template <typename T, bool GRAD, int THREADS, int U, bool RESIDENT>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4)))
 void distill_kernel(DistillArgs a) {
-  constexpr int N = kVec<T>, W = kDistillThreads / 64;
+  constexpr int N = kVec<T>, W = THREADS / 64;
   extern __shared__ uint32_t named[];  // a bit per logit, where the total is known
   __shared__ Teacher t;
   __shared__ float part[3][W];
@@ -169,7 +167,7 @@ void distill_kernel(DistillArgs a) {
   const int vectors = V / N, odd = vectors * N + tid;
   auto no_gradient = [&] {
     const float zero[N] = {};
-    for (int v = tid; v < vectors; v += kDistillThreads) store_vec<T>(grad + (size_t)v * N, zero);
+    for (int v = tid; v < vectors; v += THREADS) store_vec<T>(grad + (size_t)v * N, zero);
     if (odd < V) grad[odd] = (T)0.f;
   };
   if (w == 0.f) {  // whatever the row holds
@@ -178,7 +176,7 @@ void distill_kernel(DistillArgs a) {
     return;
   }
   const bool tail = a.total != nullptr;
-  constexpr int STEP = U * kDistillThreads;
+  constexpr int STEP = U * THREADS;
   Vec<T> raw[U];
   // (loads have no condition: vectors beyond the row are its last.  The loss alone leaves
   // the logits in the last-level cache for the backward pass: read as a stream, its 4096 x
@@ -187,7 +185,7 @@ void distill_kernel(DistillArgs a) {
     if (vectors == 0) return;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      to[u] = load_vec<T, GRAD>(z + (size_t)min(first + u * kDistillThreads + tid, vectors - 1) * N);
+      to[u] = load_vec<T, GRAD>(z + (size_t)min(first + u * THREADS + tid, vectors - 1) * N);
   };
   auto blank = [&](int first) {
     if (first + STEP <= vectors) return;
@@ -195,7 +193,7 @@ void distill_kernel(DistillArgs a) {
     for (int u = 0; u < U; ++u) {
       const u32x4 x = __builtin_bit_cast(u32x4, raw[u]);
       constexpr uint32_t low = N == 8 ? 0xff80ff80u : 0xff800000u;  // -infinity
-      const bool in = first + u * kDistillThreads + tid < vectors;
+      const bool in = first + u * THREADS + tid < vectors;
       raw[u] = __builtin_bit_cast(Vec<T>, u32x4{in ? x[0] : low, in ? x[1] : low, in ? x[2] : low,
                                                 in ? x[3] : low});
     }
@@ -218,7 +216,7 @@ void distill_kernel(DistillArgs a) {
     }
   }
   if (tail)
-    for (int i = tid; i < (V + 31) / 32; i += kDistillThreads) named[i] = 0;
+    for (int i = tid; i < (V + 31) / 32; i += THREADS) named[i] = 0;
   // A vector of the row as it was loaded.  Each pass widens its values anew, one vector at
   // a time (left to itself the compiler keeps the first pass's, twice the registers in
   // bf16, and all exponentials of a pass: scratch).
@@ -231,7 +229,7 @@ void distill_kernel(DistillArgs a) {
   double P = 0, kl = 0;
   if (tail) {
     __syncthreads();
-    for (int k = tid; k < K; k += kDistillThreads)
+    for (int k = tid; k < K; k += THREADS)
       if (t.id[k] >= 0) atomicOr(&named[t.id[k] >> 5], 1u << (t.id[k] & 31));
     __syncthreads();
   }
@@ -253,7 +251,7 @@ void distill_kernel(DistillArgs a) {
   auto add = [&](int first, float base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int v = first + u * kDistillThreads + tid;
+      const int v = first + u * THREADS + tid;
       const Vec<T> x = as_loaded(u);
       float e[N];
 #pragma unroll
@@ -341,7 +339,7 @@ void distill_kernel(DistillArgs a) {
         if (!RESIDENT) fetch(raw, first);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int v = first + u * kDistillThreads + tid;
+          const int v = first + u * THREADS + tid;
           const Vec<T> x = as_loaded(u);
           float g[N];
 #pragma unroll
@@ -369,13 +367,13 @@ void distill_kernel(DistillArgs a) {
     // the dense stores have arrived before a named element is written anew
     drain_memory();
     __syncthreads();
-    for (int k = tid; k < K; k += kDistillThreads)
+    for (int k = tid; k < K; k += THREADS)
       if (t.id[k] >= 0)
         store_named(grad, t.id[k], t.z[k], k == tid ? mass0 : mass_of(k), base, a.scale, one, wt);
   }
   if (!GRAD && a.stats) {
     float* st = a.stats + row * (kDistillStats + K);
-    for (int k = tid; k < K; k += kDistillThreads)
+    for (int k = tid; k < K; k += THREADS)
       st[kDistillStats + k] = t.id[k] >= 0 ? mass_of(k) : 0.f;
     if (tid == 0) {
       st[0] = base;
@@ -454,31 +452,53 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int par
   }
 }
 
-template <typename T, bool GRAD, int U, bool RESIDENT>
+template <typename T, bool GRAD, int THREADS, int U, bool RESIDENT>
 static void launch_row(const DistillArgs& a, int rows, hipStream_t stream) {
   const size_t lds = a.total ? ((size_t)a.vocabulary + 31) / 32 * 4 : 0;
-  hipLaunchKernelGGL((distill_kernel<T, GRAD, U, RESIDENT>), dim3(rows), dim3(kDistillThreads), lds,
+  hipLaunchKernelGGL((distill_kernel<T, GRAD, THREADS, U, RESIDENT>), dim3(rows), dim3(THREADS), lds,
                      stream, a);
 }
 
-// The loss alone streams its rows: it needs each logit once, and rows kept in registers took
-// 17.3 us instead of 14.2 at 64 x 131077 bf16, 175 instead of 122 at 2000 x 131077, 5.6
-// instead of 5.4 at 64 x 8192.  With the gradient, rows that fit are read once.
+// With the gradient, rows that fit are kept in registers.  The loss alone streams its rows: it
+// needs each logit once, and rows kept in registers took 17.3 us instead of 14.2 at 64 x
+// 131077 bf16, 175 instead of 122 at 2000 x 131077, 5.6 instead of 5.4 at 64 x 8192.
+//
+// Threads: a row's start and end (its first loads, the teacher, the sums over its waves) take
+// what a row of any length takes, so short rows are taken by fewer threads and more of them
+// at once; but not where all rows are in flight by then (512: two of 512 threads a CU).
+// us, 512 threads -> 256, loss and gradient:
+//   bf16 4096 x  8192  59.7 ->  39.4   1024 x  8192  20.9 -> 15.1    256 x 8192  10.1 -> 10.0
+//        4096 x 32003 143.1 -> 123.9   1024 x 32003  39.7 -> 35.0    512 x 32003 21.7 -> 23.4
+//        4096 x 65536 201.5 -> 221.4
+//   fp32 4096 x 16384 112.7 -> 106.5   4096 x 32003 209.9 -> 221.7
+// and the loss alone: bf16 4096 x 8192 37.6 -> 25.0, 4096 x 32003 81.9 -> 72.0, 4096 x 65536
+// 100.6 -> 103.0.  The longest rows that fit, and longer ones, take 1024 threads: 512 -> 1024,
+// bf16 4096 x 131077 591 -> 562, 64 x 131077 31.8 -> 28.8, 64 x 200000 50.9 -> 41.0, 512 x 200000
+// 115 -> 119, fp32 2048 x 131077 682 -> 643; the loss alone 237 -> 301 at bf16 4096 x 131077.
 template <typename T>
 static hipError_t launch_distill_t(const DistillArgs& a, int rows, hipStream_t stream) {
   const int vectors = a.vocabulary / kVec<T>;
-  if (!a.grad)
-    launch_row<T, false, 4, false>(a, rows, stream);
-  else if (vectors <= 4 * kDistillThreads)
-    launch_row<T, true, 4, true>(a, rows, stream);
-  else if (vectors <= 8 * kDistillThreads)
-    launch_row<T, true, 8, true>(a, rows, stream);
-  else if (vectors <= 16 * kDistillThreads)
-    launch_row<T, true, 16, true>(a, rows, stream);
-  else if (vectors <= 32 * kDistillThreads)
-    launch_row<T, true, 32, true>(a, rows, stream);
+  const bool narrow = vectors <= 16 * 256 && rows > 512;
+  if (!a.grad && narrow)
+    launch_row<T, false, 256, 4, false>(a, rows, stream);
+  else if (!a.grad)
+    launch_row<T, false, 512, 4, false>(a, rows, stream);
+  else if (narrow && vectors <= 4 * 256)
+    launch_row<T, true, 256, 4, true>(a, rows, stream);
+  else if (narrow && vectors <= 8 * 256)
+    launch_row<T, true, 256, 8, true>(a, rows, stream);
+  else if (narrow)
+    launch_row<T, true, 256, 16, true>(a, rows, stream);
+  else if (vectors <= 4 * 512)
+    launch_row<T, true, 512, 4, true>(a, rows, stream);
+  else if (vectors <= 8 * 512)
+    launch_row<T, true, 512, 8, true>(a, rows, stream);
+  else if (vectors <= 16 * 512)
+    launch_row<T, true, 512, 16, true>(a, rows, stream);
+  else if (vectors <= 16 * 1024)
+    launch_row<T, true, 1024, 16, true>(a, rows, stream);
   else
-    launch_row<T, true, 4, false>(a, rows, stream);
+    launch_row<T, true, 1024, 4, false>(a, rows, stream);
   return hipGetLastError();
 }
 

@@ -106,14 +106,15 @@ def distill(z, teacher, ids, temperature=1.0, total=None, weights=None, upstream
             kl += rest * (math.log(rest) - (math.log(s) if s > 0 else -math.inf))
         loss[n] = w * temperature ** 2 * kl
         # an exponential's argument z' = (z - max) / T has three roundings and the exponential
-        # two steps; under q, |z'| is log V at most on average; a thread adds its share of the
-        # row, then 6 + 16 sums
+        # two steps; under q, |z'| is log V at most on average; a thread (one of 256 at least, of
+        # 512 where the row is longer than 2^15) adds its share of the row, then 6 + 16 sums
         arg = (z[n] - z[n].max()).abs() / temperature
         arg = torch.where(q > 0, arg, 0.0)
         mean_arg = float((q * arg).sum())
-        sums = (v // 1024 + 8 + 22 + 4 + 3 * mean_arg) * E
+        share = v // (256 if v <= 1 << 15 else 512)
+        sums = (share + 8 + 22 + 4 + 3 * mean_arg) * E
         rest_arg = float((q * arg)[beyond].sum()) / s if s > 0 else 0.0
-        rest_sums = (v // 1024 + 8 + 22 + 4 + 3 * rest_arg) * E
+        rest_sums = (share + 8 + 22 + 4 + 3 * rest_arg) * E
         mass = float(p.sum()) + rest
         loss_e[n] = abs(w) * temperature ** 2 * (mass * sums + rest * (sums + rest_sums)) \
             + 2 * E * abs(float(loss[n]))

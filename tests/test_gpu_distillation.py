@@ -73,6 +73,16 @@ def test_entries(k, dtype, total, device):
     _check(*_operands(dtype, 5, 1500, k, device, temperature=0.7, total=total))
 
 
+# rows of 256 threads: two, one and half of their ranges, and the first row too long for them
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [3, 4096, 8193, 16389, 32771, 32776])
+@pytest.mark.parametrize("total", [False, True], ids=["softmax", "total"])
+def test_more_rows_than_are_taken_at_once(v, dtype, total, device):
+    say("distill rows", v, dtype, total)
+    z, t, ids, more = _operands(dtype, 515, v, min(v, 70), device, temperature=1.5, total=total)
+    _check(z, t, ids, more)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 300, 5000])
 def test_rows(rows, device):
     z, t, ids, more = _operands(torch.bfloat16, rows, 333, 8, device, total=True)
