@@ -2,7 +2,11 @@
 //
 // The Python layer checks a call and hands it over here: outputs and workspaces are
 // allocated, the C ABI is called on the current stream, and what a backward pass needs
-// is saved, all without the interpreter.  A backward pass runs in the engine's own
+// is saved, all without the interpreter.  A call whose operands are all of the ordinary
+// kind takes one step less: the usual_* functions make the same checks here and run it,
+// and answer None to any other, which then goes through the Python layer's checks, for
+// its conversions and its errors (norm of 64 x 1024: 5.2 us -> 4.1; a loss of 4 x 1000
+// with weights: 8.3 -> 4.2).  A backward pass runs in the engine's own
 // thread; one written in Python has to be handed the interpreter's lock there first
 // and finds its caches cold.  Host time of a layer norm of 64 x 1024, forward and
 // backward, with the nodes in Python: 130 us; here: 42.
@@ -11,6 +15,8 @@
 // module links to none of it.
 #include <Python.h>
 #include <limits.h>
+
+#include <cmath>
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -436,6 +442,116 @@ PyObject* py_distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// Ordinary calls
+// ---------------------------------------------------------------------------
+
+// A device tensor of a dtype that the kernels have and without a tangent; one of `like`'s
+// device.
+bool usual(const Tensor& t, const Tensor& like) {
+  const auto dtype = t.scalar_type();
+  return t.is_cuda() && (dtype == at::kFloat || dtype == at::kBFloat16) &&
+         t.device() == like.device() && !t._fw_grad(0).defined();
+}
+
+bool usual_ids(const Tensor& t, const Tensor& like) {
+  return t.is_cuda() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) &&
+         t.device() == like.device() && t.is_contiguous();
+}
+
+// None or a tensor; false: neither.
+bool take(PyObject* o, Tensor& t) {
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  t = THPVariable_Unpack(o);
+  return true;
+}
+
+bool take_tensor(PyObject* o, Tensor& t) { return take(o, t) && t.defined(); }
+
+bool records(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// usual_norm(x, weight, bias, eps, center)
+PyObject* py_usual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 5);
+  Tensor x, w, b;
+  if (!take_tensor(a[0], x) || !take_tensor(a[1], w) || !take(a[2], b) || !PyFloat_Check(a[3]))
+    Py_RETURN_NONE;
+  const double eps = PyFloat_AS_DOUBLE(a[3]);
+  const bool center = a[4] == Py_True;
+  auto parameter = [&](const Tensor& p) {
+    return usual(p, x) && p.dim() == 1 && p.size(0) == x.size(-1) && p.is_contiguous() &&
+           p.scalar_type() == w.scalar_type();
+  };
+  if (!usual(x, x) || x.dim() == 0 || x.size(-1) == 0 || !rows_even(x) || !parameter(w) ||
+      (w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat) ||
+      (b.defined() && !parameter(b)) || !(eps >= 0 && std::isfinite(eps)))
+    Py_RETURN_NONE;
+  const bool record = records({&x, &w, &b});
+  return tensor_of([&] {
+    return record ? Norm::apply(x, w, maybe(b), eps, center) : norm(x, w, b, eps, center, nullptr);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// usual_embed(ids, table, scale, padding)
+PyObject* py_usual_embed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 4);
+  Tensor ids, table;
+  if (!take_tensor(a[0], ids) || !take_tensor(a[1], table) || !PyFloat_Check(a[2]))
+    Py_RETURN_NONE;
+  const double scale = PyFloat_AS_DOUBLE(a[2]);
+  int64_t padding = -1;
+  if (a[3] != Py_None) {
+    if (!PyLong_CheckExact(a[3])) Py_RETURN_NONE;
+    int overflow = 0;
+    padding = PyLong_AsLongLongAndOverflow(a[3], &overflow);
+    if (overflow) Py_RETURN_NONE;
+  }
+  if (!usual(table, table) || table.dim() != 2 || table.numel() == 0 || !rows_even(table) ||
+      !usual_ids(ids, table) || !std::isfinite(scale))
+    Py_RETURN_NONE;
+  const bool record = records({&table});
+  return tensor_of([&] {
+    return record ? Embed::apply(ids, table, scale, padding) : embed(ids, table, scale, padding);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// usual_distill(logits, teacher, ids, total, weights, temperature)
+PyObject* py_usual_distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 6);
+  Tensor z, t, ids, total, weights;
+  if (!take_tensor(a[0], z) || !take_tensor(a[1], t) || !take_tensor(a[2], ids) ||
+      !take(a[3], total) || !take(a[4], weights) || !PyFloat_Check(a[5]))
+    Py_RETURN_NONE;
+  const double temperature = PyFloat_AS_DOUBLE(a[5]);
+  auto lead = [&] { return z.sizes().slice(0, z.dim() - 1); };
+  auto per_row = [&](const Tensor& r) {
+    return usual(r, z) && r.scalar_type() == at::kFloat && r.is_contiguous() && r.sizes() == lead();
+  };
+  if (!usual(z, z) || z.dim() == 0 || z.size(-1) == 0 || !rows_even(z) || !usual_ids(ids, z) ||
+      ids.dim() != z.dim() || ids.size(-1) == 0 || ids.sizes().slice(0, z.dim() - 1) != lead() ||
+      !usual(t, z) || t.sizes() != ids.sizes() || !t.is_contiguous() ||
+      (total.defined() && !per_row(total)) || (weights.defined() && !per_row(weights)) ||
+      !(temperature >= 1e-6 && temperature <= 1e6) || records({&t, &total, &weights}))
+    Py_RETURN_NONE;
+  const bool record = records({&z});
+  return tensor_of([&] {
+    return record ? TopLogitsLoss::apply(z, t, ids, maybe(total), maybe(weights), temperature)
+                  : distill(z, t, ids, total, weights, temperature, nullptr, Tensor());
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 // rows_even(x)
 PyObject* py_rows_even(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -447,8 +563,11 @@ PyObject* py_rows_even(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define MF_METHOD(name)                                                                   \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, \
    nullptr}
-PyMethodDef methods[] = {MF_METHOD(init),    MF_METHOD(norm),      MF_METHOD(embed),
-                         MF_METHOD(distill), MF_METHOD(rows_even), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {MF_METHOD(init),          MF_METHOD(norm),
+                         MF_METHOD(embed),         MF_METHOD(distill),
+                         MF_METHOD(usual_norm),    MF_METHOD(usual_embed),
+                         MF_METHOD(usual_distill), MF_METHOD(rows_even),
+                         {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mfnodes", "Autograd nodes over the C ABI.", -1,
                       methods, nullptr, nullptr, nullptr, nullptr};

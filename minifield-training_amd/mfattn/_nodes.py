@@ -36,3 +36,6 @@ def _load():
 
 _module = _load()
 norm, embed, distill, rows_even = _module.norm, _module.embed, _module.distill, _module.rows_even
+# the same with the checks of ordinary operands: None to a call that has others
+usual_norm, usual_embed, usual_distill = (_module.usual_norm, _module.usual_embed,
+                                          _module.usual_distill)

@@ -78,6 +78,9 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     logits instead of three.  (A backward captured into a graph: see
     :func:`normalization.layer_norm`.)
     """
+    loss = _nodes.usual_distill(logits, teacher_logits, teacher_ids, teacher_total, weights, temperature)
+    if loss is not None:
+        return loss
     teacher, ids, total, weights = _checked("top_logits_loss", logits, teacher_logits, teacher_ids,
                                             teacher_total, weights, temperature)
     record = logits.requires_grad and torch.is_grad_enabled()

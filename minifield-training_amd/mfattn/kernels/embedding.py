@@ -25,6 +25,12 @@ def embed(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,
     to 65536, up to 2**24 ids and 2**34 values.  Differentiable in the table.  (A
     backward captured into a graph: see :func:`normalization.layer_norm`.)
     """
+    out = _nodes.usual_embed(ids, table, scale, padding_id)
+    return _other(ids, table, scale, padding_id) if out is None else out
+
+
+def _other(ids, table, scale, padding_id):
+    """A call whose operands are not all of the ordinary kind, or wrong."""
     if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
         raise ValueError("table must be [V, D] with V and D positive")
     if ids.is_floating_point() or ids.is_complex() or ids.dtype is torch.bool:

@@ -18,6 +18,12 @@ from ..ops import dtype_code, even_rows, refuse_tangents, require_device
 
 
 def _norm(what, x, weight, bias, eps, center):
+    y = _nodes.usual_norm(x, weight, bias, eps, center)
+    return _other(what, x, weight, bias, eps, center) if y is None else y
+
+
+def _other(what, x, weight, bias, eps, center):
+    """A call whose operands are not all of the ordinary kind, or wrong."""
     d = x.shape[-1] if x.dim() else 0
     if not d:
         raise ValueError("x must be [..., D] with D positive")

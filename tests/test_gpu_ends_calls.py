@@ -5,6 +5,7 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from mfattn import _lib
@@ -205,3 +206,89 @@ def test_inference_mode(device):
         mine = x.clone()
         assert torch.equal(distillation.top_logits_loss_and_gradient(mine, t, ids, out=mine)[0], loss)
         assert torch.equal(mine, grad)
+
+
+def _wrong_calls(device):
+    f = lambda *shape, **kw: torch.zeros(*shape, device=device, **kw)  # noqa: E731
+    half, brain = torch.float16, torch.bfloat16
+    norm, rms = normalization.layer_norm, normalization.rms_norm
+    x, w, g = f(3, 8), f(8), f(8, requires_grad=True)
+    yield "weight", lambda: norm(x, f(9))
+    yield "D", lambda: norm(f(()), w)
+    yield "D", lambda: rms(f(3, 0), f(0))
+    yield "weight", lambda: norm(x, f(8, 1))
+    yield "weight", lambda: norm(x, f(8, dtype=brain))
+    yield "bias", lambda: norm(x, w, f(7))
+    yield "bias", lambda: norm(x.bfloat16(), w, f(8, dtype=brain))
+    yield "dtype", lambda: norm(x.to(half), w.to(half))
+    yield "dtype", lambda: norm(x.double(), w)
+    yield "eps", lambda: norm(x, w, eps=float("nan"))
+    yield "eps", lambda: rms(x, w, eps=-1e-9)
+    yield "eps", lambda: rms(x, w, eps=float("inf"))
+    ids, table = f(4, dtype=torch.int64), f(5, 8)
+    yield "table", lambda: embedding.embed(ids, w)
+    yield "table", lambda: embedding.embed(ids, f(0, 8))
+    yield "integers", lambda: embedding.embed(f(4), table)
+    yield "integers", lambda: embedding.embed(f(4, dtype=torch.bool), table)
+    yield "scale", lambda: embedding.embed(ids, table, scale=float("inf"))
+    yield "padding", lambda: embedding.embed(ids, table, padding_id=1 << 63)
+    yield "dtype", lambda: embedding.embed(ids, table.to(half))
+    z, t, k, n = f(3, 8), f(3, 2), f(3, 2, dtype=torch.int32), f(3)
+    loss = distillation.top_logits_loss
+    yield "teacher", lambda: loss(z, f(3, 3), k)
+    yield "teacher", lambda: loss(z, f(2, 2), f(2, 2, dtype=torch.int32))
+    yield "teacher", lambda: loss(z, f(3, 0), f(3, 0, dtype=torch.int32))
+    yield "teacher", lambda: loss(z, t[0], k[0])
+    yield "integers", lambda: loss(z, t, t)
+    yield "logits", lambda: loss(f(3, 0), t, k)
+    yield "dtype", lambda: loss(z.to(half), t, k)
+    yield "dtype", lambda: loss(z, t.to(half), k)
+    yield "teacher_total", lambda: loss(z, t, k, teacher_total=f(3, 1))
+    yield "weights", lambda: loss(z, t, k, weights=f(1))
+    yield "weights", lambda: loss(z, t, k, weights=f(3, dtype=torch.int32))
+    yield "temperature", lambda: loss(z, t, k, temperature=0.0)
+    yield "temperature", lambda: loss(z, t, k, temperature=2e6)
+    yield "detach", lambda: loss(z, t.clone().requires_grad_(), k)
+    yield "detach", lambda: loss(z, t, k, weights=n.clone().requires_grad_())
+
+    def dual(call, x):
+        with forward_ad.dual_level():
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+    yield "tangent", lambda: dual(lambda x: norm(x, g), x)
+    yield "tangent", lambda: dual(lambda w: norm(x, w), w)
+    yield "tangent", lambda: dual(lambda b: norm(x, w, b), w)
+    yield "tangent", lambda: dual(lambda table: embedding.embed(ids, table), table)
+    yield "tangent", lambda: dual(lambda z: loss(z, t, k), z)
+    yield "tangent", lambda: dual(lambda n: loss(z, t, k, weights=n), n)
+
+
+def test_wrong_device_tensors_are_refused(device):
+    for text, call in _wrong_calls(device):
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_operands_of_another_kind_give_the_same(device):
+    g = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn(6, 40, generator=g, device=device)
+    w = torch.randn(40, generator=g, device=device)
+    # parameters that are not dense, and an integer for eps
+    y = normalization.layer_norm(x, w, w, eps=1.0)
+    apart = torch.stack([w, w], 1)[:, 0]
+    assert not apart.is_contiguous()
+    assert torch.equal(normalization.layer_norm(x, apart, apart, eps=1), y)
+    assert torch.equal(normalization.layer_norm(x.t().contiguous().t(), w, w, eps=1.0), y)
+    ids = torch.randint(0, 6, (4, 7), generator=g, device=device)
+    e = embedding.embed(ids, x, scale=2.0, padding_id=3)
+    assert torch.equal(embedding.embed(ids.t().contiguous().t(), x, scale=2, padding_id=3), e)
+    assert torch.equal(embedding.embed(ids.to(torch.int16), x.t().contiguous().t(), scale=2.0, padding_id=3), e)
+    t, k = torch.randn(6, 5, generator=g, device=device), ids[:1, :5].expand(6, 5)
+    n = torch.rand(6, generator=g, device=device)
+    loss = distillation.top_logits_loss(x, t, k.contiguous(), weights=n, temperature=2.0)
+    for other in (dict(weights=n.double()), dict(weights=torch.stack([n, n], 1)[:, 1]), dict(temperature=2)):
+        assert torch.equal(distillation.top_logits_loss(x, t, k, **{"weights": n, "temperature": 2.0, **other}),
+                           loss)
+    with torch.no_grad():  # nothing is recorded: a teacher may require what it likes
+        assert torch.equal(distillation.top_logits_loss(x, t.clone().requires_grad_(), k, weights=n,
+                                                        temperature=2.0), loss)
