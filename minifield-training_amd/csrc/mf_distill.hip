@@ -94,9 +94,9 @@ struct Teacher {
 };
 
 // Wave 0, while the row is on its way: masses, P, and the part of the loss that knows the
-// teacher alone, sum p_k log p_k.
+// teacher alone, sum p_k log p_k.  u0: entry `lane` of the teacher.
 __device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, int lane,
-                                              Teacher& t, double& P, double& kl) {
+                                              float u0, Teacher& t, double& P, double& kl) {
   const int K = a.top;
   const bool tail = a.total != nullptr;
   bool there = false, bad = false;
@@ -107,7 +107,12 @@ __device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, 
     there |= u != kNegInf;
     return u;
   };
-  const float first = entry(lane);
+  float first = kNegInf;
+  if (lane < K && t.id[lane] >= 0) {
+    first = u0;
+    bad |= !(u0 < kPosInf);
+    there |= u0 != kNegInf;
+  }
   double shift, total;  // what the entries are taken beside, and the logarithm of their sum there
   if (tail) {
     shift = 0;
@@ -202,7 +207,11 @@ void distill_kernel(DistillArgs a) {
   // return in order, and what is needed first comes first
   const int K8 = (K + 7) & ~7;
   int id0 = -1;
-  if (wave == 0 && lane < K) id0 = teacher_id(a, row * K + lane);
+  float u0 = 0.f;
+  if (wave == 0 && lane < K) {
+    id0 = teacher_id(a, row * K + lane);
+    u0 = element(a.teacher, a.teacher_f32, row * K + lane);
+  }
   const float extra = odd < V ? (float)z[odd] : kNegInf;
   fetch(raw, 0);
   float z0 = 0.f;
@@ -235,7 +244,7 @@ void distill_kernel(DistillArgs a) {
   }
   // (the other waves go on with the row; they meet wave 0 at its largest logit)
   if (wave == 0) {
-    weigh_teacher(a, row, lane, t, P, kl);
+    weigh_teacher(a, row, lane, u0, t, P, kl);
     if (lane < K) t.z[lane] = z0;
   }
   // sums beside `top`, of what is not named and what is
