@@ -121,6 +121,17 @@ void refuse_second_order(const char* what) {
               " is differentiable once: its backward pass records no graph (create_graph=True)");
 }
 
+// What was saved goes through the caller's hooks (torch.autograd.graph.saved_tensors_hooks),
+// which may lay it out anew but have to give it back.
+void restored(bool same) {
+  TORCH_CHECK(same, "a tensor saved for the backward pass came back with another shape, dtype "
+                    "or device");
+}
+
+bool on(const Tensor& t, const Tensor& like, int64_t numel) {
+  return t.device() == like.device() && t.numel() == numel;
+}
+
 // A library's refusal inside the engine's thread.
 template <typename F>
 void in_backward(F&& f) {
@@ -163,11 +174,16 @@ struct Norm : public Function<Norm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order("the norm");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+    const Tensor x = even(saved[0]), weight = saved[1].contiguous(), stats = saved[2].contiguous();
     const bool center = ctx->saved_data["center"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     const int64_t d = x.size(-1), rows = x.numel() / d;
+    const auto param = weight.scalar_type();
+    restored(x.sizes() == grads[0].sizes() && on(x, grads[0], grads[0].numel()) &&
+             x.scalar_type() == grads[0].scalar_type() && on(weight, x, d) &&
+             (param == x.scalar_type() || param == at::kFloat) && on(stats, x, 2 * rows) &&
+             stats.scalar_type() == at::kFloat);
     c10::DeviceGuard guard(x.device());
     Tensor dx, dw, db, ws;
     if (rows == 0) {
@@ -215,6 +231,8 @@ Tensor embed(const Tensor& ids, const Tensor& table, double scale, int64_t paddi
 Tensor embed_gradient(const Tensor& grad, const Tensor& ids, int64_t v, double scale,
                       int64_t padding) {
   const int64_t d = grad.size(-1), n = ids.numel();
+  restored(on(ids, grad, grad.numel() / d) &&
+           (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong));
   c10::DeviceGuard guard(grad.device());
   if (n == 0) return at::zeros({v, d}, grad.options());
   const Tensor dout = even(grad);
@@ -250,7 +268,9 @@ struct EmbedGradient : public Function<EmbedGradient> {
     return embed_gradient(grad, ids, v, scale, padding);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor ids = ctx->get_saved_variables()[0], g = even(grads[0]);
+    const Tensor ids = ctx->get_saved_variables()[0].contiguous(), g = even(grads[0]);
+    restored(ids.device() == g.device() &&
+             (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong));
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt();
     Tensor out;
@@ -263,7 +283,7 @@ struct EmbedGradient : public Function<EmbedGradient> {
 };
 
 variable_list Embed::backward(AutogradContext* ctx, variable_list grads) {
-  const Tensor ids = ctx->get_saved_variables()[0];
+  const Tensor ids = ctx->get_saved_variables()[0].contiguous();
   const int64_t v = ctx->saved_data["v"].toInt(), padding = ctx->saved_data["padding"].toInt();
   const double scale = ctx->saved_data["scale"].toDouble();
   Tensor dtable;
@@ -308,14 +328,24 @@ struct TopLogitsLoss : public Function<TopLogitsLoss> {
                                  temperature, &stats, Tensor());
     ctx->save_for_backward({logits, ids, weights, stats});
     ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["dtype"] = logits.scalar_type();
     return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order("the loss");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &ids = saved[1], &weights = saved[2], &stats = saved[3];
-    const int64_t v = logits.size(-1), k = ids.size(-1), rows = logits.numel() / v;
+    const Tensor logits = even(saved[0]), ids = saved[1].contiguous(),
+                 weights = saved[2].defined() ? saved[2].contiguous() : saved[2],
+                 stats = saved[3].contiguous();
+    const int64_t v = logits.size(-1), k = ids.size(-1), rows = grads[0].numel();
+    restored(on(logits, grads[0], rows * v) && logits.dim() == grads[0].dim() + 1 &&
+             logits.scalar_type() == ctx->saved_data["dtype"].toScalarType() &&
+             on(ids, logits, rows * k) &&
+             (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) &&
+             (!weights.defined() ||
+              (on(weights, logits, rows) && weights.scalar_type() == at::kFloat)) &&
+             on(stats, logits, rows * (k + 4)) && stats.scalar_type() == at::kFloat);
     c10::DeviceGuard guard(logits.device());
     const Tensor grad = at::empty(logits.sizes(), logits.options());
     const Tensor dloss = grads[0].contiguous();

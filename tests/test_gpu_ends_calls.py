@@ -292,3 +292,41 @@ def test_operands_of_another_kind_give_the_same(device):
     with torch.no_grad():  # nothing is recorded: a teacher may require what it likes
         assert torch.equal(distillation.top_logits_loss(x, t.clone().requires_grad_(), k, weights=n,
                                                         temperature=2.0), loss)
+
+
+def _steps(device):
+    g = torch.Generator(device=device).manual_seed(11)
+    x = torch.randn(6, 40, generator=g, device=device).requires_grad_()
+    w = torch.randn(40, generator=g, device=device).requires_grad_()
+    ids = torch.randint(0, 6, (9, 4), generator=g, device=device)
+    t, k = torch.randn(6, 4, generator=g, device=device), ids[:6].to(torch.int32)
+    n = torch.rand(6, generator=g, device=device)
+    return ((lambda: normalization.layer_norm(x, w, w), (x, w)), (lambda: embedding.embed(ids, x), (x,)),
+            (lambda: distillation.top_logits_loss(x, t, k, weights=n), (x,)))
+
+
+def _across(t):
+    """The same values, strides the other way round."""
+    return t if t.dim() < 2 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize("how", ["host", "strides"])
+def test_saved_tensors_that_were_elsewhere(how, device):
+    hooks = (torch.autograd.graph.save_on_cpu() if how == "host" else
+             torch.autograd.graph.saved_tensors_hooks(lambda t: t, _across))
+    for call, leaves in _steps(device):
+        want = torch.autograd.grad(call().sum(), leaves)
+        with hooks:
+            out = call()
+        for a, b in zip(torch.autograd.grad(out.sum(), leaves), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("other", [lambda t: t.cpu(), lambda t: t.half(), lambda t: t[:-1],
+                                   lambda t: torch.cat([t, t])], ids=["host", "half", "less", "more"])
+def test_saved_tensors_that_come_back_changed(other, device):
+    for call, leaves in _steps(device):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            out = call()
+        with pytest.raises(RuntimeError, match="came back"):
+            torch.autograd.grad(out.sum(), leaves)
