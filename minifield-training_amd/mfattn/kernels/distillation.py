@@ -78,7 +78,8 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     logits instead of three.  (A backward captured into a graph: see
     :func:`normalization.layer_norm`.)
     """
-    loss = _nodes.usual_distill(logits, teacher_logits, teacher_ids, teacher_total, weights, temperature)
+    loss = _nodes.usual_distill(logits, teacher_logits, teacher_ids, teacher_total, weights, temperature,
+                                False)
     if loss is not None:
         return loss
     teacher, ids, total, weights = _checked("top_logits_loss", logits, teacher_logits, teacher_ids,
@@ -101,6 +102,11 @@ def top_logits_loss_and_gradient(logits: torch.Tensor, teacher_logits: torch.Ten
     graph is recorded: logits that require a gradient are refused unless under
     ``torch.no_grad()``.
     """
+    if out is None:
+        both = _nodes.usual_distill(logits, teacher_logits, teacher_ids, teacher_total, weights,
+                                    temperature, True)
+        if both is not None:
+            return both
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("top_logits_loss_and_gradient records no graph; call it under "
                          "torch.no_grad(), or top_logits_loss")

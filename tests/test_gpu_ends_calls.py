@@ -250,6 +250,11 @@ def _wrong_calls(device):
     yield "temperature", lambda: loss(z, t, k, temperature=2e6)
     yield "detach", lambda: loss(z, t.clone().requires_grad_(), k)
     yield "detach", lambda: loss(z, t, k, weights=n.clone().requires_grad_())
+    both = distillation.top_logits_loss_and_gradient
+    yield "records no graph", lambda: both(z.clone().requires_grad_(), t, k)
+    yield "teacher", lambda: both(z, f(3, 3), k)
+    yield "temperature", lambda: both(z, t, k, temperature=float("nan"))
+    yield "at most", lambda: both(z, f(3, 1025), f(3, 1025, dtype=torch.int32))
 
     def dual(call, x):
         with forward_ad.dual_level():
@@ -289,6 +294,11 @@ def test_operands_of_another_kind_give_the_same(device):
     for other in (dict(weights=n.double()), dict(weights=torch.stack([n, n], 1)[:, 1]), dict(temperature=2)):
         assert torch.equal(distillation.top_logits_loss(x, t, k, **{"weights": n, "temperature": 2.0, **other}),
                            loss)
+    pair = distillation.top_logits_loss_and_gradient(x, t, k.contiguous(), weights=n, temperature=2.0)
+    for other in (dict(weights=n.double()), dict(temperature=2), dict(out=torch.empty_like(x))):
+        more = {"weights": n, "temperature": 2.0, **other}
+        for a, b in zip(distillation.top_logits_loss_and_gradient(x, t, k, **more), pair):
+            assert torch.equal(a, b) and not a.requires_grad
     with torch.no_grad():  # nothing is recorded: a teacher may require what it likes
         assert torch.equal(distillation.top_logits_loss(x, t.clone().requires_grad_(), k, weights=n,
                                                         temperature=2.0), loss)
