@@ -190,3 +190,23 @@ def test_the_gradient_differentiated(device):
     (g,) = torch.autograd.grad(embedding.embed(ids, table, scale=2.0), table, dout, create_graph=True)
     (back,) = torch.autograd.grad(g, dout, u, create_graph=True)
     assert torch.equal(back, embedding.embed(ids, u, scale=2.0))
+
+
+@pytest.mark.parametrize("v, kind", [(1003, torch.int32), (300000, torch.int64)], ids=["few", "many"])
+def test_the_most_tokens(v, kind, device):
+    """Small whole numbers: their sums are exact in any order (below 2^24 in fp32)."""
+    n = 1 << 24
+    say("embed tokens", n, v)
+    g = torch.Generator(device=device).manual_seed(3)
+    ids = torch.randint(-1, v, (n,), generator=g, device=device, dtype=kind)
+    ids[: n // 3] = 5  # one that fills many tiles
+    table = torch.zeros(v, 2, device=device, requires_grad=True)
+    dout = torch.randint(-2, 3, (n, 2), generator=g, device=device).float()
+    (got,) = torch.autograd.grad(embedding.embed(ids, table), table, dout)
+    got = got.double().cpu()
+    # (on the host: millions of atomic additions to one 64-bit address take minutes on the GPU)
+    at, d = torch.where(ids < 0, v, ids).long().cpu(), dout.double().cpu()
+    want = torch.stack([torch.bincount(at, d[:, i], minlength=v + 1)[:v] for i in (0, 1)], 1)
+    assert want.abs().max() < 1 << 24 and torch.equal(got, want)
+    with pytest.raises(ValueError, match="at most"):
+        embedding.embed(torch.cat([ids, ids[:1]]), table)
