@@ -137,16 +137,20 @@ def test_a_step_captured_and_replayed(device):
             assert torch.equal(a, b)
 
 
-def _each(device):
+# launches of few rows and tokens, and of many
+SIZES = [(300, 2000, 40), (1500, 9001, 600)]
+
+
+def _each(device, rows, tokens, logits):
     """Every operator's pass over buffers that the caller refills."""
-    x = torch.randn(300, 1024, device=device).bfloat16()
+    x = torch.randn(rows, 1024, device=device).bfloat16()
     w = torch.randn(1024, device=device).bfloat16().requires_grad_()
-    dy = torch.randn(300, 1024, device=device).bfloat16()
-    ids = torch.randint(0, 3000, (2000,), device=device)
+    dy = torch.randn(rows, 1024, device=device).bfloat16()
+    ids = torch.randint(0, 3000, (tokens,), device=device)
     table = torch.randn(3000, 136, device=device).requires_grad_()
-    dout = torch.randn(2000, 136, device=device)
-    z = torch.randn(40, 9001, device=device).bfloat16().requires_grad_()
-    t, tids = torch.randn(40, 16, device=device), torch.randint(0, 9001, (40, 16), device=device)
+    dout = torch.randn(tokens, 136, device=device)
+    z = torch.randn(logits, 9001, device=device).bfloat16().requires_grad_()
+    t, tids = torch.randn(logits, 16, device=device), torch.randint(0, 9001, (logits, 16), device=device)
     total = torch.logsumexp(t, 1) + 0.1
     leaf = x.requires_grad_()
 
@@ -166,16 +170,17 @@ def _each(device):
         with torch.no_grad():
             for b in (x, dy, dout, z, t):
                 b.normal_()
-            ids.copy_(torch.randint(0, 3000, (2000,), device=device))
-            tids.copy_(torch.randint(0, 9001, (40, 16), device=device))
+            ids.copy_(torch.randint(0, 3000, (tokens,), device=device))
+            tids.copy_(torch.randint(0, 9001, (logits, 16), device=device))
             total.copy_(torch.logsumexp(t, 1) + 0.2)
 
     return (one, two, three), refill
 
 
-def test_two_graphs_over_the_same_operands(device):
+@pytest.mark.parametrize("sizes", SIZES)
+def test_two_graphs_over_the_same_operands(sizes, device):
     """Captured one by one, replayed in turn several times: no graph lives on another's scratch."""
-    calls, refill = _each(device)
+    calls, refill = _each(device, *sizes)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -203,9 +208,10 @@ def test_two_graphs_over_the_same_operands(device):
                 assert torch.equal(a, b), i
 
 
-def test_calls_in_flight_on_two_streams(device):
-    first, _ = _each(device)
-    second, refill = _each(device)
+@pytest.mark.parametrize("sizes", SIZES)
+def test_calls_in_flight_on_two_streams(sizes, device):
+    first, _ = _each(device, *sizes)
+    second, refill = _each(device, *sizes)
     want = [[c() for c in calls] for calls in (first, second)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
