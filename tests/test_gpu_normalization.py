@@ -49,14 +49,15 @@ def _check(x, w, b, dy, center, eps=1e-5):
 @pytest.mark.parametrize("center", [True, False], ids=["layer", "rms"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", WIDTHS)
-def test_widths(dim, dtype, center, device):
-    say("norm", dim, dtype, center)
-    x, w, b, dy = _operands(dtype, 37, dim, device)
+@pytest.mark.parametrize("rows", [37, 1100], ids=["few", "many"])
+def test_widths(rows, dim, dtype, center, device):
+    say("norm", rows, dim, dtype, center)
+    x, w, b, dy = _operands(dtype, rows, dim, device)
     _check(x, w, b, dy, center)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows", [1, 2, 3, 63, 64, 65, 1023, 4097])
+@pytest.mark.parametrize("rows", [1, 2, 3, 63, 64, 65, 1023, 1024, 1025, 4097])
 @pytest.mark.parametrize("dim", [64, 1024, 4096])
 def test_rows(rows, dim, dtype, device):
     say("norm rows", rows, dim, dtype)
@@ -124,8 +125,9 @@ def test_a_row_that_is_not_finite_stays_alone(device):
 
 
 @pytest.mark.parametrize("which", [(0,), (1,), (2,), (0, 2), (1, 2)])
-def test_gradients_that_are_asked_for(which, device):
-    x, w, b, dy = _operands(torch.bfloat16, 300, 1024, device)
+@pytest.mark.parametrize("rows", [300, 1300])
+def test_gradients_that_are_asked_for(rows, which, device):
+    x, w, b, dy = _operands(torch.bfloat16, rows, 1024, device)
     leaves = [t.requires_grad_() for t in (x, w, b)]
     y = normalization.layer_norm(*leaves)
     every = torch.autograd.grad(y, leaves, dy)
