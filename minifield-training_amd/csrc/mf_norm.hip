@@ -431,7 +431,11 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* partials
   if (out) store_param(out, f32, at, s);
 }
 
-// Lanes and vectors a row by its width (in vectors).
+// Lanes and vectors a row by its width (in vectors): the fewest lanes, so that sums cross the
+// fewest, as long as a lane's vectors leave the registers for enough rows.  32768 rows of
+// bf16, forward + backward us, taken and with the next more lanes: 128 wide, 16 lanes 6.2 + 12.8,
+// 64 lanes 11.3 + 19.8; 1024 wide, 64 lanes 25.3 + 40.3, 256 lanes 35.2 + 50.6; 2048 wide, 256
+// lanes 43.3 + 82.8, 512 lanes 67.7 + 87.0.  Up to 4096 rows they differ by 3 us at most.
 struct NormShape {
   int lanes, vectors;
 };
