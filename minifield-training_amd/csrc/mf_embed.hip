@@ -436,9 +436,10 @@ static void launch_embed_e(const EmbedArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((embed_kernel<T, L, E>), dim3((a.tokens + 256 / L - 1) / (256 / L)),
                        dim3(256), 0, stream, a);
   };
-  // (32768 tokens, bf16, 16 lanes a token against 64: 128 columns 5.8 us and 9.1, 256 7.5 and
-  // 10.4, 512 12.9 and 13.8, 1024 23.4 and 23.0)
-  if (vectors <= 64)
+  // Rows that 16 lanes take at once.  (32768 tokens, bf16, 16 lanes a token against 64: 128
+  // columns 5.8 us and 9.1, 256 7.5 and 10.4, in several turns 512 12.9 and 13.8, 1024 23.4
+  // and 23.0; 5001 tokens of 129 fp32 3.4 and 3.1.)
+  if (vectors <= 2 * 16)
     go(std::integral_constant<int, 16>{});
   else
     go(std::integral_constant<int, 64>{});
