@@ -15,7 +15,6 @@ true.  ``exact`` is the operators' definition in 64 bits.
 
 from __future__ import annotations
 
-import functools
 import math
 import pathlib
 import sys
@@ -210,20 +209,13 @@ def run(state):
         case, state)
 
 
-@functools.lru_cache(maxsize=None)
-def _kernels():
-    """The framework's modules, imported once as a program does."""
+def _call(case, s):
+    """The same pass through the framework."""
     package = str(pathlib.Path(__file__).resolve().parents[1] / "minifield-training_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
     from mfattn.kernels import distillation, embedding, normalization
 
-    return distillation, embedding, normalization
-
-
-def _call(case, s):
-    """The same pass through the framework."""
-    distillation, embedding, normalization = _kernels()
     if case["kind"] == "norm":
         if case["center"]:
             y = normalization.layer_norm(s["x"], s["weight"], s["bias"], eps=_EPS)
