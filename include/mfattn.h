@@ -434,7 +434,9 @@ int mf_embed_bwd(const void* ids, int id_bytes, const void* dout,
  * Entries whose id is outside the vocabulary are not there.  A row of weight zero
  * (weights [rows] fp32, NULL: ones) has loss zero and no gradient, whatever it
  * holds, and so has one without entries (and without total).  The masses and the
- * logarithms in 64 bits, exponentials of logits and their sums in fp32.  teacher [rows, top] in
+ * logarithms in 64 bits, exponentials of logits and their sums in fp32 (those of the ids that
+ * no entry names beside a maximum of their own: a mass there that is no number in fp32 still
+ * has its logarithm and its gradient).  teacher [rows, top] in
  * teacher_dtype, teacher_ids [rows, top] of id_bytes (4 or 8) each.  Up to 1024
  * entries a row, vocabularies up to 393216, 2^35 logits, and temperatures in
  * [1e-6, 1e6].

@@ -13,8 +13,8 @@ constexpr long long kDistillMostLogits = 1ll << 35;  // (and 256 threads a part 
 constexpr double kDistillLeastTemperature = 1e-6, kDistillMostTemperature = 1e6;
 constexpr int kDistillStats = 4;                  // floats a row in front of its masses
 
-// Saved for the backward pass of each row: its largest logit, the two factors of
-// its exponentials, weight times temperature, and the mass of each entry.
+// Saved for the backward pass of each row: its largest logit and the named ones' factor, the
+// largest of the rest and the rest's factor, and the weighted mass of each entry.
 inline size_t distill_stats_bytes(int rows, int top) {
   return sizeof(float) * (size_t)rows * (kDistillStats + top);
 }

@@ -8,15 +8,19 @@
 // and with P = sum p_k, s = sum of q_j over the j that no entry names:
 //   loss = w T^2 [ sum p_k (log p_k - log q_{i_k}) + r (log r - log s) ]
 //   d loss / d z_j = w T [ q_j (P + r) - sum of p_k with i_k = j - r q_j / s [j not named] ].
-// With e_j = exp((z_j - max z) / T), S = sum e and S' = sum of e over the j that are
-// not named, every dense element is e_j times one factor of its row,
-//   w T ((P + r) / S - r / S'),
-// and the K named ones are written anew, w T (e_j (P + r) / S - p).  S' is summed by
-// itself, through one bit per logit in LDS: as a difference S - sum of named e it
-// would lose what a confident student leaves beyond the teacher's entries.
+// With L known, the logits that no entry names (the rest; one bit per logit in LDS tells) are
+// summed beside a maximum of their own: with m' = max of them, e'_j = exp((z_j - m') / T),
+// S' = sum e', f = exp((m' - max z) / T) and S = S' f + sum of exp((z_i - max z) / T) over the
+// named i, the dense elements are e'_j times one factor of their row,
+//   w T (f (P + r) / S - r / S'),
+// and the K named ones are written anew, w T (exp((z_i - max z) / T) (P + r) / S - p);
+// log s = (m' - max z) / T + log S' - log S.  A student whose logits of the entries are far
+// above all others leaves a mass beyond them that is no number in fp32 (f is zero from 87 T
+// on); its logarithm, and what its gradient says to the rest, do not need it.  Without L all
+// logits are the rest: m' = max z, f = 1, S = S'.
 //
-// Exponentials of logits and their sums are fp32 (each thread adds at most a few
-// hundred); the K masses, 1 - P and the few logarithms of a row are 64-bit, since
+// Exponentials of logits and their sums are fp32 (each thread adds at most 768: 512 of
+// them, 393216 logits); the K masses, 1 - P and the few logarithms of a row are 64-bit, since
 // they cancel: at log q = -20 and a loss of 1 the fp32 terms alone would cost 1e-6.
 //
 // Bound: memory, one read of the logits and one write of the gradient.  A workgroup
@@ -64,11 +68,11 @@ __device__ __forceinline__ float weight_of(float z, float top, float scale) {
   return fast_exp2((z - top) * scale);
 }
 
-// A named element of a row's gradient: after the dense ones.
+// A named element of a row's gradient: after the dense ones.  mass: weighted by w T.
 template <typename T>
 __device__ __forceinline__ void store_named(T* grad, int id, float z, float mass, float top,
-                                            float scale, float factor, float w) {
-  grad[id] = (T)fmaf(weight_of(z, top, scale), factor, -w * mass);
+                                            float scale, float factor) {
+  grad[id] = (T)fmaf(weight_of(z, top, scale), factor, -mass);
 }
 
 template <typename T, bool STREAM>
@@ -91,6 +95,8 @@ struct Teacher {
   double mass[kDistillMostTop];
   float whole, rest;  // P + r and r
   int none, bad;      // no entry at all; one that is NaN or +infinity
+  float top;          // the largest named logit, where the total is known
+  int twice;          // and whether an id is named more than once
 };
 
 // Wave 0, while the row is on its way: masses, P, and the part of the loss that knows the
@@ -212,7 +218,7 @@ void distill_kernel(DistillArgs a) {
     id0 = teacher_id(a, row * K + lane);
     u0 = element(a.teacher, a.teacher_f32, row * K + lane);
   }
-  const float extra = odd < V ? (float)z[odd] : kNegInf;
+  float extra = odd < V ? (float)z[odd] : kNegInf;
   fetch(raw, 0);
   float z0 = 0.f;
   if (wave == 0) {
@@ -224,8 +230,10 @@ void distill_kernel(DistillArgs a) {
       t.z[k] = id >= 0 ? (float)z[id] : 0.f;
     }
   }
-  if (tail)
+  if (tail) {
     for (int i = tid; i < (V + 31) / 32; i += THREADS) named[i] = 0;
+    if (tid == 0) t.twice = 0;
+  }
   // A vector of the row as it was loaded.  Each pass widens its values anew, one vector at
   // a time (left to itself the compiler keeps the first pass's, twice the registers in
   // bf16, and all exponentials of a pass: scratch).
@@ -238,17 +246,40 @@ void distill_kernel(DistillArgs a) {
   double P = 0, kl = 0;
   if (tail) {
     __syncthreads();
-    for (int k = tid; k < K; k += THREADS)
-      if (t.id[k] >= 0) atomicOr(&named[t.id[k] >> 5], 1u << (t.id[k] & 31));
+    for (int k = tid; k < K; k += THREADS) {
+      if (t.id[k] < 0) continue;
+      const uint32_t bit = 1u << (t.id[k] & 31);
+      if (atomicOr(&named[t.id[k] >> 5], bit) & bit) t.twice = 1;
+    }
     __syncthreads();
   }
   // (the other waves go on with the row; they meet wave 0 at its largest logit)
   if (wave == 0) {
     weigh_teacher(a, row, lane, u0, t, P, kl);
     if (lane < K) t.z[lane] = z0;
+    if (tail) {
+      float m = kNegInf;
+      for (int k = lane; k < K; k += 64) m = t.id[k] >= 0 ? fmaxf(m, t.z[k]) : m;
+      m = max64(m);
+      if (lane == 0) t.top = m;
+    }
   }
-  // sums beside `top`, of what is not named and what is
-  float top = kNegInf, rest = 0.f, held = 0.f;
+  // named logits are not the rest's
+  auto hide = [&](int first) {
+    if (!tail) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = first + u * THREADS + tid;
+      const uint32_t bits =
+          v < vectors ? (named[v * N >> 5] >> (v * N & 31)) & ((1u << N) - 1) : 0;
+      if (bits) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[u][i] = bits >> i & 1 ? (T)kNegInf : raw[u][i];
+      }
+    }
+  };
+  if (tail && odd < V && named[odd >> 5] >> (odd & 31) & 1) extra = kNegInf;
+  float top = kNegInf, rest = 0.f;  // the largest of the rest, and its sum beside that
   auto largest = [&] {
     float m = top;
 #pragma unroll
@@ -257,51 +288,33 @@ void distill_kernel(DistillArgs a) {
       for (int i = 0; i < N; ++i) m = fmaxf(m, (float)raw[u][i]);
     return m;
   };
-  auto add = [&](int first, float base) {
+  auto add = [&](float base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int v = first + u * THREADS + tid;
       const Vec<T> x = as_loaded(u);
-      float e[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = weight_of((float)x[i], base, a.scale);
-      uint32_t bits = 0;
-      if (tail && v < vectors) bits = (named[v * N >> 5] >> (v * N & 31)) & ((1u << N) - 1);
-      if (bits) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          held += bits >> i & 1 ? e[i] : 0.f;
-          e[i] = bits >> i & 1 ? 0.f : e[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) rest += e[i];
+      for (int i = 0; i < N; ++i) rest += weight_of((float)x[i], base, a.scale);
       asm volatile("" : "+v"(rest));  // (added here, not all behind the last vector)
     }
   };
-  auto add_extra = [&](float base) {
-    const float e = weight_of(extra, base, a.scale);
-    const bool is_named = tail && odd < V && named[odd >> 5] >> (odd & 31) & 1;
-    held += is_named ? e : 0.f;
-    rest += is_named ? 0.f : e;
-  };
   if constexpr (RESIDENT) {
     blank(0);
+    hide(0);
     top = fmaxf(largest(), extra);
   } else {
     top = extra;
-    add_extra(extra == kNegInf ? 0.f : extra);
+    rest = weight_of(extra, extra == kNegInf ? 0.f : extra, a.scale);
     for (int first = 0; first < vectors; first += STEP) {
       Vec<T> next[U];
       fetch(next, first + STEP);
       blank(first);
+      hide(first);
       const float m = largest();
       // (a thread whose logits are all -infinity has a sum of zero, not NaN)
-      const float base = m == kNegInf ? 0.f : m, old = weight_of(top, base, a.scale);
-      rest *= old;
-      held *= old;
+      const float base = m == kNegInf ? 0.f : m;
+      rest *= weight_of(top, base, a.scale);
       top = m;
-      add(first, base);
+      add(base);
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = next[u];
     }
@@ -309,20 +322,35 @@ void distill_kernel(DistillArgs a) {
   const float wave_top = max64(top);
   if (lane == 0) part[0][wave] = wave_top;
   __syncthreads();
-  float base = part[0][0];
+  float free = part[0][0];  // m'
 #pragma unroll
-  for (int i = 1; i < W; ++i) base = fmaxf(base, part[0][i]);
+  for (int i = 1; i < W; ++i) free = fmaxf(free, part[0][i]);
+  float base = tail ? fmaxf(free, t.top) : free;  // the largest of all
+  // (zero in the place of -infinity, so that differences to it are not NaN)
+  free = free == kNegInf ? 0.f : free;
   base = base == kNegInf ? 0.f : base;
   if constexpr (RESIDENT) {
-    add(0, base);
-    add_extra(base);
+    add(free);
+    rest += weight_of(extra, free, a.scale);
   } else {
-    const float mine = weight_of(top, base, a.scale);
-    rest *= mine;
-    held *= mine;
+    rest *= weight_of(top, free, a.scale);
+  }
+  float held = 0.f;  // the named ones' sum beside `base`, each id once
+  if (tail) {
+    for (int k = tid; k < K; k += THREADS) {
+      const int id = t.id[k];
+      bool once = id >= 0;
+      if (t.twice) {  // (the first entry of an id counts)
+        for (int j = 0; j < k; j += 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) once &= t.id[j + i] != id || j + i >= k;
+        }
+      }
+      held += once ? weight_of(t.z[k], base, a.scale) : 0.f;
+    }
+    held = sum64(held);
   }
   rest = sum64(rest);
-  if (tail) held = sum64(held);
   if (lane == 0) {
     part[1][wave] = rest;
     part[2][wave] = held;
@@ -334,12 +362,14 @@ void distill_kernel(DistillArgs a) {
     rest += part[1][i];
     held += part[2][i];
   }
-  const float sum = rest + held;
+  // f; zero where there is no rest
+  const float factor = !tail ? 1.f : rest > 0.f ? weight_of(free, base, a.scale) : 0.f;
+  const float sum = fmaf(rest, factor, held);
   // so does a logit that is NaN or +infinity, and a row of -infinity alone
   const bool none = t.none, bad = !none && (t.bad || !(sum > 0.f && sum < kPosInf));
   const float wt = (float)(w * a.temperature);
   const float one = none ? 0.f : bad ? __builtin_nanf("") : wt * (t.whole / sum);
-  const float dense = one - (rest > 0.f ? wt * (t.rest / rest) : 0.f);
+  const float dense = fmaf(one, factor, rest > 0.f ? -wt * (t.rest / rest) : 0.f);
   if constexpr (GRAD) {
     if (none) {
       no_gradient();
@@ -352,15 +382,17 @@ void distill_kernel(DistillArgs a) {
           const Vec<T> x = as_loaded(u);
           float g[N];
 #pragma unroll
-          for (int i = 0; i < N; ++i) g[i] = weight_of((float)x[i], base, a.scale) * dense;
+          for (int i = 0; i < N; ++i) g[i] = weight_of((float)x[i], free, a.scale) * dense;
           if (v < vectors) store_vec<T>(grad + (size_t)v * N, g);
         }
       }
-      if (odd < V) grad[odd] = (T)(weight_of(extra, base, a.scale) * dense);
+      if (odd < V) grad[odd] = (T)(weight_of(extra, free, a.scale) * dense);
     }
   }
-  // an element that several entries name has the mass of all of them
+  // an element that several entries name has the mass of all of them.  (Where the bits tell that
+  // none is, its own: 4096 x 65536 bf16, 64 entries, 225 us -> 207.)
   auto mass_of = [&](int k) {
+    if (tail && !t.twice) return (float)t.mass[k];
     const int id = t.id[k];
     double m = 0;
     for (int j = 0; j < K8; j += 8) {
@@ -378,17 +410,17 @@ void distill_kernel(DistillArgs a) {
     __syncthreads();
     for (int k = tid; k < K; k += THREADS)
       if (t.id[k] >= 0)
-        store_named(grad, t.id[k], t.z[k], k == tid ? mass0 : mass_of(k), base, a.scale, one, wt);
+        store_named(grad, t.id[k], t.z[k], wt * (k == tid ? mass0 : mass_of(k)), base, a.scale, one);
   }
   if (!GRAD && a.stats) {
     float* st = a.stats + row * (kDistillStats + K);
     for (int k = tid; k < K; k += THREADS)
-      st[kDistillStats + k] = t.id[k] >= 0 ? mass_of(k) : 0.f;
+      st[kDistillStats + k] = t.id[k] >= 0 ? wt * mass_of(k) : 0.f;
     if (tid == 0) {
       st[0] = base;
       st[1] = one;
-      st[2] = dense;
-      st[3] = wt;
+      st[2] = free;
+      st[3] = dense;
     }
   }
   if (wave == 0) {
@@ -397,9 +429,11 @@ void distill_kernel(DistillArgs a) {
       if (t.mass[k] > 0) kl -= t.mass[k] * (((double)t.z[k] - base) * a.per);
     kl = sum64(kl);
     if (lane == 0) {
-      const double r = tail ? fmax(0.0, 1.0 - P) : 0.0, all = (double)rest + held;
+      const double lower = tail ? ((double)free - base) * a.per : 0.0;  // (m' - max z) / T
+      const double all = (double)rest * factor + held;                  // S
+      const double r = tail ? fmax(0.0, 1.0 - P) : 0.0;
       kl += P * log(all);
-      if (r > 0) kl += r * (log(r) - log((double)rest / all));
+      if (r > 0) kl += r * (log(r) - (lower + log((double)rest)) + log(all));
       a.loss[row] = none ? 0.f
                     : bad ? __builtin_nanf("")
                           : (float)(w * a.temperature * a.temperature * kl);
@@ -442,22 +476,22 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a, int par
     for (int u = 0; u < U; ++u)
       raw[u] = load_vec<T, true>(z + (size_t)min(first + u * 256 + tid, vectors - 1) * N);
   }
-  const float base = st[0], one = st[1] * up, dense = st[2] * up, wt = st[3] * up;
+  const float base = st[0], one = st[1] * up, free = st[2], dense = st[3] * up;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float g[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = weight_of((float)raw[u][i], base, a.scale) * dense;
+    for (int i = 0; i < N; ++i) g[i] = weight_of((float)raw[u][i], free, a.scale) * dense;
     store(u, g);
   }
-  if (odd < V) grad[odd] = (T)(weight_of((float)z[odd], base, a.scale) * dense);
+  if (odd < V) grad[odd] = (T)(weight_of((float)z[odd], free, a.scale) * dense);
   drain_memory();
   __syncthreads();
   const int last = part == parts - 1 ? V : (first + SPAN) * N;
   for (int k = tid; k < K; k += 256) {
     const int id = teacher_id(a, row * K + k);
     if (id >= first * N && id < last)
-      store_named(grad, id, (float)z[id], st[kDistillStats + k], base, a.scale, one, wt);
+      store_named(grad, id, (float)z[id], st[kDistillStats + k] * up, base, a.scale, one);
   }
 }
 

@@ -73,7 +73,10 @@ def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
     hold, and so has a row without entries (where no total is given).  V up to
     393216, K up to 1024, temperatures in [1e-6, 1e6].  The teacher's masses and the
     logarithms are 64-bit, exponentials of logits and their sums float32: a loss is
-    off by some 1e-7 times ``weight * temperature ** 2``.  Differentiable in the logits, once;
+    off by some 1e-7 times ``weight * temperature ** 2``.  With a total this holds however far the
+    student's logits of the entries are above all others; the loss is infinite only where an
+    entry with mass, or every id without one while ``r`` is positive, has the logit -infinity.
+    Differentiable in the logits, once;
     :func:`top_logits_loss_and_gradient` needs half the memory and two passes over the
     logits instead of three.  (A backward captured into a graph: see
     :func:`normalization.layer_norm`.)
