@@ -157,8 +157,8 @@ __device__ __forceinline__ void weigh_teacher(const DistillArgs& a, size_t row, 
   }
 }
 
-// LOSS: the loss (and with `stats` what the backward needs); GRAD: the gradient of
-// the weighted loss.  U: vectors a thread has in flight; RESIDENT: they are the row.
+// The loss, with `stats` what the backward needs, and with GRAD the gradient of the
+// weighted loss.  U: vectors a thread has in flight; RESIDENT: they are the row.
 template <typename T, bool GRAD, int THREADS, int U, bool RESIDENT>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4)))
 void distill_kernel(DistillArgs a) {
@@ -412,7 +412,7 @@ void distill_kernel(DistillArgs a) {
       if (t.id[k] >= 0)
         store_named(grad, t.id[k], t.z[k], wt * (k == tid ? mass0 : mass_of(k)), base, a.scale, one);
   }
-  if (!GRAD && a.stats) {
+  if (a.stats) {
     float* st = a.stats + row * (kDistillStats + K);
     for (int k = tid; k < K; k += THREADS)
       st[kDistillStats + k] = t.id[k] >= 0 ? wt * mass_of(k) : 0.f;
