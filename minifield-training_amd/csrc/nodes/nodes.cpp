@@ -104,7 +104,10 @@ bool rows_even(const Tensor& x) {
   return true;
 }
 
-Tensor even(const Tensor& x) { return rows_even(x) ? x : x.contiguous(); }
+// The kernels read memory: a view whose sign stands beside it (of a conjugate's imaginary part,
+// say) is written out.
+Tensor dense(const Tensor& x) { return x.resolve_neg().contiguous(); }
+Tensor even(const Tensor& x) { return rows_even(x) ? x.resolve_neg() : dense(x); }
 
 // The C ABI takes its sizes as int.
 void fit(std::initializer_list<int64_t> sizes) {
@@ -174,7 +177,7 @@ struct Norm : public Function<Norm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order("the norm");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor x = even(saved[0]), weight = saved[1].contiguous(), stats = saved[2].contiguous();
+    const Tensor x = even(saved[0]), weight = dense(saved[1]), stats = dense(saved[2]);
     const bool center = ctx->saved_data["center"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
@@ -268,7 +271,7 @@ struct EmbedGradient : public Function<EmbedGradient> {
     return embed_gradient(grad, ids, v, scale, padding);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor ids = ctx->get_saved_variables()[0].contiguous(), g = even(grads[0]);
+    const Tensor ids = dense(ctx->get_saved_variables()[0]), g = even(grads[0]);
     restored(ids.device() == g.device() &&
              (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong));
     const double scale = ctx->saved_data["scale"].toDouble();
@@ -283,7 +286,7 @@ struct EmbedGradient : public Function<EmbedGradient> {
 };
 
 variable_list Embed::backward(AutogradContext* ctx, variable_list grads) {
-  const Tensor ids = ctx->get_saved_variables()[0].contiguous();
+  const Tensor ids = dense(ctx->get_saved_variables()[0]);
   const int64_t v = ctx->saved_data["v"].toInt(), padding = ctx->saved_data["padding"].toInt();
   const double scale = ctx->saved_data["scale"].toDouble();
   Tensor dtable;
@@ -335,9 +338,9 @@ struct TopLogitsLoss : public Function<TopLogitsLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order("the loss");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor logits = even(saved[0]), ids = saved[1].contiguous(),
-                 weights = saved[2].defined() ? saved[2].contiguous() : saved[2],
-                 stats = saved[3].contiguous();
+    const Tensor logits = even(saved[0]), ids = dense(saved[1]),
+                 weights = saved[2].defined() ? dense(saved[2]) : saved[2],
+                 stats = dense(saved[3]);
     const int64_t v = logits.size(-1), k = ids.size(-1), rows = grads[0].numel();
     restored(on(logits, grads[0], rows * v) && logits.dim() == grads[0].dim() + 1 &&
              logits.scalar_type() == ctx->saved_data["dtype"].toScalarType() &&
@@ -348,7 +351,7 @@ struct TopLogitsLoss : public Function<TopLogitsLoss> {
              on(stats, logits, rows * (k + 4)) && stats.scalar_type() == at::kFloat);
     c10::DeviceGuard guard(logits.device());
     const Tensor grad = at::empty(logits.sizes(), logits.options());
-    const Tensor dloss = grads[0].contiguous();
+    const Tensor dloss = dense(grads[0]);
     in_backward([&] {
       if (rows)
         check(lib.mf_distill_bwd(data(logits), row_step(logits), data(ids), (int)ids.element_size(),
@@ -476,17 +479,17 @@ PyObject* py_distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // Ordinary calls
 // ---------------------------------------------------------------------------
 
-// A device tensor of a dtype that the kernels have and without a tangent; one of `like`'s
-// device.
+// A device tensor of a dtype that the kernels have, without a tangent and its memory what it
+// holds; one of `like`'s device.
 bool usual(const Tensor& t, const Tensor& like) {
   const auto dtype = t.scalar_type();
   return t.is_cuda() && (dtype == at::kFloat || dtype == at::kBFloat16) &&
-         t.device() == like.device() && !t._fw_grad(0).defined();
+         t.device() == like.device() && !t.is_neg() && !t._fw_grad(0).defined();
 }
 
 bool usual_ids(const Tensor& t, const Tensor& like) {
   return t.is_cuda() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) &&
-         t.device() == like.device() && t.is_contiguous();
+         t.device() == like.device() && t.is_contiguous() && !t.is_neg();
 }
 
 // None or a tensor; false: neither.

@@ -53,10 +53,13 @@ def _checked(what, logits, teacher, ids, total, weights, temperature):
     if ids.dtype is not torch.int32 and ids.dtype is not torch.int64:
         ids = ids.to(torch.int64)
 
-    def row(t):
-        return None if t is None else t.detach().to(torch.float32).contiguous()
+    def dense(t):
+        return t.detach().resolve_neg().contiguous()
 
-    return teacher.detach().contiguous(), ids.contiguous(), row(total), row(weights)
+    def row(t):
+        return None if t is None else dense(t.to(torch.float32))
+
+    return dense(teacher), dense(ids), row(total), row(weights)
 
 
 def top_logits_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,

@@ -46,5 +46,5 @@ def _other(ids, table, scale, padding_id):
     require_device(table, ids)
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         ids = ids.to(torch.int64)
-    return _nodes.embed(ids.contiguous(), even_rows(table), scale, padding_id,
+    return _nodes.embed(ids.resolve_neg().contiguous(), even_rows(table), scale, padding_id,
                         table.requires_grad and torch.is_grad_enabled())

@@ -44,10 +44,10 @@ def _other(what, x, weight, bias, eps, center):
         require_device(x, weight)
     else:
         require_device(x, weight, bias)
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     record = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                           or (bias is not None and bias.requires_grad))
-    return _nodes.norm(even_rows(x), weight.contiguous(), bias, eps, center, record)
+    return _nodes.norm(even_rows(x), weight.resolve_neg().contiguous(), bias, eps, center, record)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,

@@ -142,8 +142,9 @@ def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 
 def even_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x [..., D]``, copied only where its last dimension is not dense or its rows are not
-    evenly spaced or overlap."""
+    """``x [..., D]``, copied only where its last dimension is not dense, its rows are not evenly
+    spaced or overlap, or its sign stands beside its memory (``torch.Tensor.is_neg``)."""
+    x = x.resolve_neg()
     return x if x.is_contiguous() or _nodes.rows_even(x) else x.contiguous()
 
 
