@@ -52,7 +52,7 @@ FLAGS = [
 # sources in which NaN operands are part of the contract (a row that holds one is NaN, its
 # neighbours are not): without the flag above, whose assumption spreads from the sums to
 # tests of their bits
-HONOR_NANS = {"mf_distill.hip"}
+HONOR_NANS = {"mf_distill.hip", "mf_embed.hip", "mf_norm.hip"}
 
 
 def _flags(src: pathlib.Path) -> list[str]:
