@@ -1,7 +1,8 @@
 """The autograd nodes of ``csrc/nodes`` (``_mfnodes.so``), bound to the loaded C ABI.
 
 Outputs, workspaces and what a backward pass needs are made there, without the
-interpreter.  Like the library it is loaded at import, and there is no fallback.
+interpreter.  Like the library it is loaded at import, and there is no fallback; modules
+that have no nodes do not import this one.
 """
 
 from __future__ import annotations
@@ -39,3 +40,10 @@ norm, embed, distill, rows_even = _module.norm, _module.embed, _module.distill, 
 # the same with the checks of ordinary operands: None to a call that has others
 usual_norm, usual_embed, usual_distill = (_module.usual_norm, _module.usual_embed,
                                           _module.usual_distill)
+
+
+def even_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x [..., D]``, copied only where its last dimension is not dense, its rows are not evenly
+    spaced or overlap, or its sign stands beside its memory (``torch.Tensor.is_neg``)."""
+    x = x.resolve_neg()
+    return x if x.is_contiguous() or rows_even(x) else x.contiguous()

@@ -5,7 +5,8 @@ package needs the library it builds) or
 ``mfattn.build.build()``.  Every ``.hip`` file under ``csrc/`` is compiled
 with ``hipcc --offload-arch=gfx950`` into an object in ``csrc/_build`` and
 linked into ``mfattn/libmfattn.so``; the autograd nodes of ``csrc/nodes`` become
-``mfattn/_mfnodes.so``.  Packed-FP32 instructions are disabled
+``mfattn/_mfnodes.so`` where the headers of torch and Python are there (without them the
+modules that have nodes do not import, and the rest does).  Packed-FP32 instructions are disabled
 (``-packed-fp32-ops``); the host pass warns that it does not know that
 feature, which is harmless.
 """
@@ -79,9 +80,20 @@ def _compile(src: pathlib.Path, obj: pathlib.Path) -> None:
 
 def _build_nodes() -> None:
     """The autograd nodes (``csrc/nodes``): host code over torch's C++ API, no GPU code."""
-    import torch
+    try:
+        import torch
 
-    root = pathlib.Path(torch.__file__).resolve().parent
+        root = pathlib.Path(torch.__file__).resolve().parent
+        needs = (root / "include/torch/csrc/autograd/custom_function.h",
+                 pathlib.Path(sysconfig.get_paths()["include"]) / "Python.h")
+        missing = [str(p) for p in needs if not p.exists()]
+    except ImportError as e:
+        missing = [str(e)]
+    if missing:
+        NODES.unlink(missing_ok=True)  # (one of another torch or another source would be loaded)
+        print("mfattn: the autograd nodes of the norms, the embedding and the distillation loss are "
+              f"not built ({', '.join(missing)})", file=sys.stderr)
+        return
     include, tmp = root / "include", NODES.with_suffix(".so.tmp")
     cmd = [_hipcc(), "-x", "c++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
@@ -105,13 +117,13 @@ def build(verbose: bool = True) -> pathlib.Path:
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as pool:
         nodes = pool.submit(_build_nodes)  # (the longest of them)
         list(pool.map(_compile, sources, objs))
+        tmp = OUT.with_suffix(".so.tmp")
+        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"link failed:\n{proc.stderr}")
+        os.replace(tmp, OUT)
         nodes.result()
-    tmp = OUT.with_suffix(".so.tmp")
-    cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"link failed:\n{proc.stderr}")
-    os.replace(tmp, OUT)
     if verbose:
         print(f"built {OUT}")
     return OUT

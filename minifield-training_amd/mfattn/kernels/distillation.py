@@ -18,7 +18,8 @@ from __future__ import annotations
 import torch
 
 from .. import _nodes
-from ..ops import dtype_code, even_rows, refuse_tangents, require_device
+from .._nodes import even_rows
+from ..ops import dtype_code, refuse_tangents, require_device
 
 
 def _checked(what, logits, teacher, ids, total, weights, temperature):

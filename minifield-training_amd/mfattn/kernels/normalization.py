@@ -14,7 +14,8 @@ import math
 import torch
 
 from .. import _nodes
-from ..ops import dtype_code, even_rows, refuse_tangents, require_device
+from .._nodes import even_rows
+from ..ops import dtype_code, refuse_tangents, require_device
 
 
 def _norm(what, x, weight, bias, eps, center):

@@ -16,7 +16,7 @@ import weakref
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib, _nodes
+from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -139,13 +139,6 @@ def token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
             and step * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0):
         return x, step
     return x.contiguous(), h * d
-
-
-def even_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x [..., D]``, copied only where its last dimension is not dense, its rows are not evenly
-    spaced or overlap, or its sign stands beside its memory (``torch.Tensor.is_neg``)."""
-    x = x.resolve_neg()
-    return x if x.is_contiguous() or _nodes.rows_even(x) else x.contiguous()
 
 
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
