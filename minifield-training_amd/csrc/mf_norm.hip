@@ -460,14 +460,18 @@ static int norm_bwd_blocks(int rows, int dim, bool f32) {
 }
 
 // Rows that are few enough for the workgroups of sum_columns to read again instead of a
-// second launch over the others' sums.  Forward and backward, us, second launch -> none:
-//   bf16  64 x 1024  19.3 ->  7.5   fp32  64 x 1024   8.5 ->  5.9
-//        512 x 1024  19.7 -> 10.4        512 x 1024   9.6 ->  7.6
-//       1024 x 1024  20.4 -> 13.7       1024 x 1024  11.3 -> 10.8
-//       1024 x 8192  35.6 -> 28.9        999 x 771   11.1 -> 12.7
-//       2048 x 1024  21.2 -> 19.9       2048 x 1024  15.5 -> 22.8
-//       2048 x  256  13.0 -> 19.0       2048 x  256  10.4 -> 15.3
-// A workgroup of theirs goes through all rows, so their time grows with the rows.
+// second launch over the others' sums.  A workgroup of theirs goes through all rows, so their
+// time grows with the rows; a second launch and its workspace cost the host 5 to 7 us a pass
+// (forward and backward through autograd, 999 x 771 fp32: 70 us, with one launch 64; in the
+// caller's thread 34 and 29; every size up to 1024 rows is as much below).  On the card, the
+// backward pass alone, us, two launches -> one:
+//              bf16 256 rows   768 rows       1024 rows      1536 rows       fp32 1024 rows
+//    256 wide    7.2 ->  4.9    7.9 ->  6.9    8.1 ->  7.8    8.8 ->  9.8     6.8 ->  5.9
+//   1024 wide    9.7 ->  5.1   10.5 ->  7.1   10.7 ->  8.1   11.5 -> 15.8     8.1 -> 10.7
+//   2048 wide    7.6 ->  5.1    9.7 -> 10.3   10.2 -> 13.9   13.2 -> 18.1    13.4 -> 12.8
+//   8192 wide   13.5 ->  7.2   18.1 -> 18.1   19.4 -> 21.5   22.7 -> 28.3    25.9 -> 28.2
+// Up to 1024 rows one launch loses at most 3.7 us there, less than it saves the host; beyond,
+// it loses more with every row.
 static bool norm_small(int rows) { return rows <= kNormFewRows; }
 
 size_t norm_bwd_workspace_bytes(int rows, int dim, bool f32) {
