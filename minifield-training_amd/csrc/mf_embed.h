@@ -15,7 +15,6 @@ constexpr long long kEmbedMostValues = 1ll << 34;  // of the output: launches st
 constexpr int kSortDigit = 9;               // bits of a key in one pass
 constexpr int kSortFewest = 5;              // (kernels are made for 5 to 9)
 constexpr int kSortBins = 1 << kSortDigit;
-constexpr int kSortTiles = 64;              // workgroups that share the tokens, at most
 constexpr int kSortWaves = 8;               // of each
 constexpr int kSortRuns = 2;                // runs of 64 tokens that a wave takes in a step
 constexpr int kSortStep = kSortWaves * kSortRuns * 64;
@@ -30,6 +29,12 @@ constexpr int kEmbedMaxChunk = 64;          // (one for each lane)
 // Waves that the chunks are made for: with twice as many the sums of 32768 tokens of 1024 columns
 // take the same 19 us and joining their pieces 6.9 instead of 4.5.
 constexpr int kEmbedWaves = 2048;
+
+// Workgroups that share the tokens, at most: every one reads the digit counts of all, and takes
+// its share step by step.  The whole gradient of 65536 x 64 bf16, us, with 64, 128 and 256: 65536
+// tokens 36.9, 38.3, 37.5; 131072 51.1, 52.8, 53.3; 180000 59.4, 57.7, 62.1; 524288 102.6, 91.8, 95.3;
+// 700000 128, 113, 112; 2^20 171, 144, 139; 2^23 1153, 877, 759.
+inline int sort_tiles(int tokens) { return tokens <= 1 << 17 ? 64 : tokens <= 1 << 19 ? 128 : 256; }
 
 // A token and the row of the table that it adds to (the vocabulary: none).
 struct SortedToken {
@@ -52,7 +57,7 @@ inline EmbedLayout embed_layout(int tokens, int vocabulary, int dim) {
   l.bits = (bits + l.passes - 1) / l.passes;
   if (l.bits < kSortFewest) l.bits = kSortFewest;
   const int steps = (tokens + kSortStep - 1) / kSortStep;
-  l.steps = (steps + kSortTiles - 1) / kSortTiles;
+  l.steps = (steps + sort_tiles(tokens) - 1) / sort_tiles(tokens);
   l.tiles = (steps + l.steps - 1) / l.steps;
   if (tokens <= kSortOne) {
     l.tiles = 1;

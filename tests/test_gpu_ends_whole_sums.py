@@ -79,7 +79,7 @@ def test_embedding_gradients_of_runs_around_a_share(d, n, dtype, device):
     assert torch.equal(got.cpu(), want.to(dtype))
 
 
-@pytest.mark.parametrize("n", [100, 1024, 5000, 8192, 8193, 70001, 300000])
+@pytest.mark.parametrize("n", [100, 1024, 5000, 8192, 8193, 70001, 300000, 700001])
 @pytest.mark.parametrize("share", [1.0, 0.5, 0.1])
 def test_embedding_gradients_of_one_frequent_id(share, n, device):
     g = torch.Generator(device=device).manual_seed(n)
