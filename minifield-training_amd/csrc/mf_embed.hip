@@ -23,7 +23,8 @@
 // the tokens count their digits, and then place their tokens.  A wave takes runs of 64;
 // lanes with one digit find each other by ballots over its bits, so that a lane's place is
 // its digit's first place, what the tiles, steps and waves before have of that digit, and
-// the lanes before it.  Few tokens are sorted by one workgroup in one launch.
+// the lanes before it.  Few tokens are sorted by one workgroup in one launch; of narrow rows, and of
+// small tables, their whole gradient is one launch (embed_few_kernel).
 //
 // Measured, 32768 tokens of 65536 x 1024 bf16, us: lookup 17 (64 MiB written, the table's
 // rows from the cache); zeroing 128 MiB beside sorting 28 (4.7 TB/s; the four launches
@@ -433,6 +434,165 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
 
 // ---------------------------------------------------------------------------
 
+struct FewArgs {
+  EmbedArgs e;
+  const void* dout;
+  long long stride;
+  int shift;  // groups of rows: 1 << shift
+};
+
+// The whole gradient of few tokens in one launch: a workgroup has every 2^shift-th row
+// of the table over kEmbedFewLanes vectors of columns.  It looks through all ids, sorts the tokens
+// of its rows by row in LDS (by one digit, stably), and its waves take equal shares of them, a
+// run at a time, four tokens in a load.  What passes a share's end stays in LDS and is added there
+// by the wave that a run begins in.
+template <typename T, Edge E>
+__global__ __launch_bounds__(1024) void embed_few_kernel(FewArgs a) {
+  constexpr int N = kVec<T>, W = kEmbedFewWaves, RUNS = kEmbedFewTokens / (W * 64);
+  constexpr int L = kEmbedFewLanes, R = 64 / L, AHEAD = 8;
+  constexpr uint32_t kToken = (1 << kEmbedFewBits) - 1;
+  __shared__ uint32_t list[kEmbedFewTokens];  // a token and, above it, its row
+  // first the places of a wave's tokens by row, then the pieces of its share's two ends
+  __shared__ union {
+    int place[W][kSortBins];
+    float piece[W][2][N][L];
+  } lds;
+  __shared__ int row_sums[kSortBins / 64];
+  __shared__ uint64_t met[kSortBins / 64];  // rows that have tokens
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  // (workgroups go to the XCDs in turn: a frequent id's columns to different ones)
+  const int group = (blockIdx.x + blockIdx.y) % gridDim.x, vec = lane % L, sub = lane / L;
+  const RowPlace<T, E> at(blockIdx.y * L + vec, a.e.dim);
+  T* out = reinterpret_cast<T*>(a.e.out);
+  auto row_at = [&](int r) { return out + (((size_t)r << a.shift) + group) * a.e.dim; };
+  const int n0 = wave * RUNS * 64 + lane;
+  uint32_t row[RUNS];
+  long long id[RUNS];
+#pragma unroll
+  for (int j = 0; j < RUNS; ++j) id[j] = id_of(a.e, min(n0 + 64 * j, a.e.tokens - 1));
+  for (int d = lane; d < kSortBins; d += 64) lds.place[wave][d] = 0;
+  int to[RUNS];
+  uint32_t live = 0;
+#pragma unroll
+  for (int j = 0; j < RUNS; ++j) {
+    const uint32_t r = row_of(a.e, id[j]);
+    const bool in = n0 + 64 * j < a.e.tokens && r < (uint32_t)a.e.vocabulary &&
+                    (int)(r & ((1u << a.shift) - 1)) == group;
+    row[j] = r >> a.shift;
+    live |= (uint32_t)in << j;
+    to[j] = 0;
+    if (__any(in)) to[j] = place_of<kSortDigit>(lds.place[wave], row[j], in, lane);
+  }
+  __syncthreads();
+  // first places: over the rows, then over a row's waves
+  int whole = 0, sum = 0;
+  if (tid < kSortBins) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int c = lds.place[i][tid];
+      lds.place[i][tid] = whole;
+      whole += c;
+    }
+    sum = whole;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int o = __shfl_up(sum, m);
+      if (lane >= m) sum += o;
+    }
+    const uint64_t some = __ballot(whole > 0);
+    if (lane == 63) row_sums[wave] = sum;
+    if (lane == 0) met[wave] = some;
+  }
+  __syncthreads();
+  if (tid < kSortBins) {
+    int start = sum - whole;
+    for (int i = 0; i < wave; ++i) start += row_sums[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) lds.place[i][tid] += start;
+  }
+  int tokens = 0;
+  for (int i = 0; i < kSortBins / 64; ++i) tokens += row_sums[i];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < RUNS; ++j)
+    if (live >> j & 1)
+      list[lds.place[wave][row[j]] + to[j]] = row[j] << kEmbedFewBits | (uint32_t)(n0 + 64 * j);
+  // rows without tokens
+  const int rows = ((a.e.vocabulary - 1 - group) >> a.shift) + 1;
+  const float zero[N] = {};
+  for (int r = wave * R + sub; r < rows; r += W * R)
+    if (!(met[r >> 6] >> (r & 63) & 1)) at.store(row_at(r), zero);
+  __syncthreads();
+  constexpr int none = kSortBins;  // (no row's number)
+  const int per = (tokens + W - 1) / W;
+  const int first = wave * per, last = min(tokens, first + per);
+  auto key_of = [&](int i) {
+    return i >= 0 && i < tokens ? uniform((int)(list[i] >> kEmbedFewBits)) : none;
+  };
+  const T* dout = reinterpret_cast<const T*>(a.dout);
+  int open = none;  // the row whose run begins in the share and goes on behind it
+  for (int i = first; i < last;) {
+    const int key = key_of(i);
+    const bool head = i == first && key_of(first - 1) == key;
+    int end = i;  // of the run, or of the share
+    for (int more = 64; more == 64 && end < last; end += more) {
+      const int k = min(end + lane, last - 1);
+      const uint64_t same = __ballot(end + lane < last && (int)(list[k] >> kEmbedFewBits) == key);
+      more = same == ~0ull ? 64 : __ffsll((long long)~same) - 1;
+    }
+    float s[N] = {};
+    auto add = [&](auto count, auto all) {  // loads at once; all: none of their tokens is behind the end
+      constexpr int C = decltype(count)::value;
+      Vec<T> x[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const uint32_t token = list[min(i + R * j + sub, end - 1)] & kToken;
+        x[j] = at.load(dout + (size_t)token * a.stride);
+      }
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          s[e] += decltype(all)::value || i + R * j + sub < end ? (float)x[j][e] : 0.f;
+      i += R * C;
+    };
+    using std::integral_constant;
+    while (i + R * AHEAD <= end) add(integral_constant<int, AHEAD>{}, std::true_type{});
+    while (i + R < end) add(integral_constant<int, AHEAD / 2>{}, std::false_type{});
+    if (i < end) add(integral_constant<int, 1>{}, std::false_type{});
+    i = end;
+    if constexpr (L == 16) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = halves_sum(rows16_sum(s[e]));
+    }
+    if (head || key_of(i) == key) {
+      if (!head) open = key;
+      if (sub == 0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) lds.piece[wave][head ? 0 : 1][e][vec] = s[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] *= a.e.scale;
+      if (sub == 0) at.store(row_at(key), s);
+    }
+  }
+  __syncthreads();
+  if (open == none) return;
+  float s[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] = lds.piece[wave][1][e][vec];
+  for (int i = wave + 1; i < W && key_of(i * per) == open; ++i) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += lds.piece[i][0][e][vec];
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] *= a.e.scale;
+  if (sub == 0) at.store(row_at(open), s);
+}
+
+// ---------------------------------------------------------------------------
+
 template <typename T, Edge E>
 static void launch_embed_e(const EmbedArgs& a, hipStream_t stream) {
   const int vectors = (a.dim + kVec<T> - 1) / kVec<T>;
@@ -487,6 +647,23 @@ static hipError_t launch_sums(SumArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T>
+static hipError_t launch_few(const FewArgs& a, hipStream_t stream) {
+  const int slabs = few_slabs(a.e.dim, kVec<T>);
+  const dim3 grid(std::min(1 << a.shift, a.e.vocabulary), slabs);
+  switch (edge_of<T>(a.e.dim)) {
+    case EDGE_WHOLE:
+      hipLaunchKernelGGL((embed_few_kernel<T, EDGE_WHOLE>), grid, dim3(64 * kEmbedFewWaves), 0, stream, a);
+      break;
+    case EDGE_CUT:
+      hipLaunchKernelGGL((embed_few_kernel<T, EDGE_CUT>), grid, dim3(64 * kEmbedFewWaves), 0, stream, a);
+      break;
+    default:
+      hipLaunchKernelGGL((embed_few_kernel<T, EDGE_SHORT>), grid, dim3(64 * kEmbedFewWaves), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
 template <typename F>
 static void with_bits(int bits, F&& f) {
   using std::integral_constant;
@@ -502,6 +679,11 @@ static void with_bits(int bits, F&& f) {
 hipError_t launch_embed_bwd(const void* ids, bool ids64, const void* dout, long long stride,
                             bool f32, int tokens, int vocabulary, int dim, long long padding,
                             float scale, void* dtable, void* workspace, hipStream_t stream) {
+  if (embed_few(tokens, vocabulary, dim, f32)) {
+    const FewArgs a{EmbedArgs{ids, nullptr, dtable, 0, padding, tokens, vocabulary, dim, scale, ids64},
+                    dout, stride, few_shift(few_slabs(dim, f32 ? 4 : 8))};
+    return f32 ? launch_few<float>(a, stream) : launch_few<bf16>(a, stream);
+  }
   const EmbedLayout l = embed_layout(tokens, vocabulary, dim);
   char* ws = reinterpret_cast<char*>(workspace);
   SortedToken* lists[2] = {reinterpret_cast<SortedToken*>(ws + l.tokens[0]),
