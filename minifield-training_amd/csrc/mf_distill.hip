@@ -27,11 +27,11 @@
 // of 256, 512 or 1024 takes a row.  Rows of up to 16 vectors of 16 bytes a thread stay in
 // registers between the maximum, the sum and the gradient; longer ones are read again.
 //
-// Measured, 4096 x 65536 bf16 (512 MiB), 64 entries a row: loss 96-101 us (5.3-5.6
-// TB/s), gradient from what it saved 172 (6.2 TB/s, a part of the logits still in the
-// cache), both in one pass 209 (5.1 TB/s; a copy of the logits, at 5.2, takes 206).  64
-// rows of 65536: loss 8.2 us.  24 rows of 131077: loss 12.9 us (one CU a row, its exponentials),
-// gradient 6.5.
+// Measured, 4096 x 65536 bf16 (512 MiB), 64 entries a row: loss 95-104 us (5.2-5.7
+// TB/s), gradient from what it saved 173 (6.2 TB/s, a part of the logits still in the
+// cache), both in one pass 207, with the teacher's total too (5.2 TB/s; a copy of the logits
+// takes 206).  64 rows of 65536: loss 8.5 us.  24 rows of 131077: loss 13.8 us (one CU a row, its
+// exponentials), gradient 6.4.
 #include <algorithm>
 
 #include "mf_distill.h"

@@ -29,7 +29,8 @@
 // Measured, 32768 tokens of 65536 x 1024 bf16, us: lookup 17 (64 MiB written, the table's
 // rows from the cache); zeroing 128 MiB beside sorting 28 (4.7 TB/s; the four launches
 // alone 18, the zeros alone 20), sums 18.6 (6 TB/s with the rows and pieces they write),
-// joining 4.5.  5001 tokens of 1003 x 129 fp32: sorting 11, sums 4.1, joining 4.7.
+// joining 4.5.  5001 tokens of 1003 x 129 fp32: in one launch 18.5 (as three, sorting 11, sums
+// 4.1 and joining 4.7).
 #include <algorithm>
 
 #include "mf_embed.h"

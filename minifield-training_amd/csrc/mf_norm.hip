@@ -21,7 +21,7 @@
 //
 // Measured, 32768 x 1024 bf16 (64 MiB a tensor, what the last pass left in the cache
 // included): forward 30 us (4.5 TB/s read and written), backward 36 (5.6), its second launch
-// 4.0; 8192 x 4096 bf16: 28, 36 and 4.1; 999 x 771 fp32: 3.8 and 10.5 (one launch).
+// 4.0; 8192 x 4096 bf16: 28, 36 and 4.1; 999 x 771 fp32: 3.8 and 10.8 (one launch).
 #include <algorithm>
 
 #include "mf_norm.h"
