@@ -15,7 +15,7 @@
 // those pieces in chunk order, a run's by one workgroup of every 256 columns: their number
 // is what a frequent id costs.  The whole gradient of 65536 x 1024 bf16, us, with even ids and
 // with an id that half of the tokens have: 8192 tokens 36 and 46, 32768 55 and 62; 2^20 tokens
-// 560, 622 with an id of a third, 749 with one id alone; 2^24 tokens of one id, 64 wide, 5.7 ms.
+// 560, 630 with an id of a third, 760 with one id alone; 2^24 tokens of one id, 64 wide, 6.0 ms.
 // The rows of ids that no token has are zeros: the launches that sort, which are a few
 // waves' work each, zero the whole table beside it, a share each.
 //
@@ -417,10 +417,16 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   // (rows of `width`, a multiple of 4; lanes beyond it read its start)
   const float* piece = a.partials + ((size_t)chunk * 2 + 1) * a.width + (col < a.width ? col : 0);
+  // (64 at a time: added in a row, 2^20 equal tokens of one id would be off by 1e-5 and more)
+  for (int c0 = from; c0 < to; c0 += 64) {
+    const int c1 = min(to, c0 + 64);
+    f32x4 some = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int c = from; c < to; ++c) {
-    // the run's first piece is its chunk's second, the others their chunks' first
-    s += *reinterpret_cast<const f32x4*>(piece + (c == 0 ? 0ll : (2ll * c - 1) * a.width));
+    for (int c = c0; c < c1; ++c) {
+      // the run's first piece is its chunk's second, the others their chunks' first
+      some += *reinterpret_cast<const f32x4*>(piece + (c == 0 ? 0ll : (2ll * c - 1) * a.width));
+    }
+    s += some;
   }
   sums[wave][lane] = s;
   __syncthreads();
