@@ -42,11 +42,10 @@ inline int few_shift(int slabs) {
   while ((2 << shift) * slabs <= kEmbedFewGroups) ++shift;
   return shift;
 }
-// Rows of one slab, and of up to four of a small table.  What it saves is launches and a
-// workspace that waits for them: 5 to 7 us of the host a pass (5001 tokens of 1003 x 129 fp32,
-// forward and backward through autograd, 69 us -> 64).  On the card, us, sorting, sums and joining in
-// launches of their own -> one launch, with ids of frequency 1 / rank, and with one id half of the
-// time:
+// Rows of one slab, and of up to four of a small table.  What it saves is two launches, 5 us of the
+// host a pass (5001 tokens of 1003 x 129 fp32, forward and backward through autograd, 69 us -> 64).
+// On the card, us, sorting, sums and joining in launches of their own -> one launch, with ids of
+// frequency 1 / rank, and with one id half of the time:
 //   bf16  64 wide:   64 tokens of   1003 rows 11.0 ->  7.9, 12.0 ->  8.5
 //                  8192 tokens of   1003 rows 22.5 -> 14.9, 31.2 -> 22.3
 //                  8192 tokens of 131072 rows 26.6 -> 19.9, 35.2 -> 27.4   (one token 7.2 -> 7.3)
