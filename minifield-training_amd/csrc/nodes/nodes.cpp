@@ -20,7 +20,6 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -116,10 +115,8 @@ void fit(std::initializer_list<int64_t> sizes) {
     if (n > INT_MAX) throw Refused{MF_ERR_SHAPE, "sizes must be below 2^31"};
 }
 
-// Memory for a call on the current stream, from the allocator that tensors have theirs from
-// (a tensor of bytes takes the host 0.7 us more).
-c10::DataPtr bytes(size_t n, const Tensor& like) {
-  return c10::GetAllocator(like.device().type())->allocate(n);
+Tensor bytes(size_t n, const Tensor& like) {
+  return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
 }
 
 void refuse_second_order(const char* what) {
@@ -191,8 +188,7 @@ struct Norm : public Function<Norm> {
              (param == x.scalar_type() || param == at::kFloat) && on(stats, x, 2 * rows) &&
              stats.scalar_type() == at::kFloat);
     c10::DeviceGuard guard(x.device());
-    Tensor dx, dw, db;
-    c10::DataPtr ws;
+    Tensor dx, dw, db, ws;
     if (rows == 0) {
       if (need_x) dx = at::zeros_like(x);
       if (need_w) dw = at::zeros_like(weight);
@@ -211,7 +207,7 @@ struct Norm : public Function<Norm> {
     in_backward([&] {
       check(lib.mf_norm_bwd(data(x), row_step(x), data(weight), data_as<float>(stats), data(dy),
                             row_step(dy), code_of(x), code_of(weight), (int)rows, (int)d, center,
-                            data(dx), data(dw), data(db), ws.get(), need, stream_of(x)));
+                            data(dx), data(dw), data(db), data(ws), need, stream_of(x)));
     });
     return {dx, dw, db, Tensor(), Tensor()};
   }
@@ -245,10 +241,10 @@ Tensor embed_gradient(const Tensor& grad, const Tensor& ids, int64_t v, double s
   const Tensor dout = even(grad);
   Tensor dtable = at::empty({v, d}, dout.options());
   const size_t need = lib.mf_embed_bwd_workspace_bytes((int)n, (int)v, (int)d);
-  const c10::DataPtr ws = bytes(need, dout);
+  const Tensor ws = bytes(need, dout);
   check(lib.mf_embed_bwd(data(ids), (int)ids.element_size(), data(dout), row_step(dout),
                          code_of(dout), (int)n, (int)v, (int)d, padding, (float)scale, data(dtable),
-                         ws.get(), need, stream_of(dout)));
+                         data(ws), need, stream_of(dout)));
   return dtable;
 }
 
